@@ -285,7 +285,7 @@ def _own_distill(s, case):
     if not case["train"]:
         return loss
     return [loss, ops.distillation_loss_backward(s["grad"], s["logits"], s["teacher"], s["classes"], s["labels"], stats,
-                                                 case["tail"], t, ALPHA)]
+                                                 t, ALPHA)]
 
 
 # ---------------------------------------------------------------------------
