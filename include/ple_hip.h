@@ -299,6 +299,157 @@ int ple_encode_plan_query(const void *output, int64_t N, int64_t F, int64_t B, i
                           int backward, ple_encode_plan_info_t *info);
 
 /*
+ * Embedding lookup with scaling (tokens, or categorical columns next to the
+ * numerical ones); no counterpart in the reference.
+ *   output[i, :] = scale * weight[row(i), :], rounded once to output_dtype
+ *   row(i) = tokens[i], or offsets[f] + tokens[i] with f = i % F for
+ *            categorical tokens [N, F] (T = N * F) of F tables in one
+ * A negative token is a missing value: its output is 0.  A token beyond its
+ * table (its column's size, or V rows) gives NaN.  Neither reads the table.
+ *   tokens     int32 or int64 (token_bytes 4 or 8) [T]
+ *   offsets    int64 [F + 1], the columns' first rows and V; or NULL (F is
+ *              not used then; pass 1)
+ *   weight     weight_dtype [V, D]
+ *   output     output_dtype [T, D]
+ * T may be 0.  T, V < 2^31 - 1, D <= 2^20 (else PLE_E_TOO_LARGE).
+ */
+int ple_lookup_launch(const void *tokens, int token_bytes, const int64_t *offsets, const void *weight, void *output,
+                      int64_t T, int64_t F, int64_t V, int64_t D, float scale, int weight_dtype, int output_dtype,
+                      void *stream);
+
+/* Scratch bytes ple_lookup_backward_launch needs for these sizes. */
+size_t ple_lookup_backward_workspace_bytes(int64_t T, int64_t V, int64_t D);
+
+/*
+ * Backward of ple_lookup_launch: every row of grad_weight is written,
+ *   grad_weight[r, :] = scale * sum_{i: row(i) = r} grad_output[i, :]
+ * summed in 32 bits in a fixed order (the tokens are sorted; no atomics on
+ * floating-point data) and rounded once to weight_dtype; 0 for rows without
+ * tokens.  Missing tokens, tokens beyond their table and tokens equal to
+ * padding_idx (>= 0; a negative one: none) have no gradient.
+ *   workspace  >= ple_lookup_backward_workspace_bytes(T, V, D) bytes, 256-byte
+ *              aligned, contents need not be initialised
+ */
+int ple_lookup_backward_launch(const void *grad_output, const void *tokens, int token_bytes, const int64_t *offsets,
+                               void *grad_weight, int64_t T, int64_t F, int64_t V, int64_t D, int64_t padding_idx,
+                               float scale, int grad_dtype, int weight_dtype, void *workspace, size_t workspace_bytes,
+                               void *stream);
+
+/*
+ * Norms after and before a block, fused with the block's gate and the residual
+ * scale; no counterpart in the reference.  For every row of the residual
+ * stream r and the block's output (the branch) y, both [N, D]:
+ *   p = post_norm(y) * post_weight + post_bias
+ *   s = residual_scale * r + h(gate) * p, stored in stream_dtype
+ *   n = pre_norm(s) * pre_weight + pre_bias, stored in branch_dtype
+ * A norm is none, rms (x / sqrt(mean(x^2) + eps)) or layer ((x - mean) /
+ * sqrt(var + eps)); the norm before the next block reads s as it is stored.
+ * h is the identity, sigmoid or tanh.  The gate has gate_rows rows, 1, N or a
+ * divisor of N: row n uses gate row n / (N / gate_rows).  Weights, biases and
+ * the gate may each be NULL (1, 0 and 1).  Sums, means and factors are 32-bit.
+ *   stream_dtype  of r and s: branch_dtype, or PLE_DTYPE_F32
+ *   branch_dtype  of y and n
+ *   param_dtype   of weights, biases and gate
+ * D <= PLE_NORM_MAX_WIDTH (else PLE_E_TOO_LARGE).
+ */
+enum {
+    PLE_NORM_NONE = 0,
+    PLE_NORM_RMS = 1,
+    PLE_NORM_LAYER = 2,
+};
+enum {
+    PLE_GATE_IDENTITY = 0,
+    PLE_GATE_SIGMOID = 1,
+    PLE_GATE_TANH = 2,
+};
+#define PLE_NORM_MAX_WIDTH 8192
+typedef struct ple_norm {
+    const void *post_weight, *post_bias;  /* [D] or NULL */
+    const void *gate;                     /* [gate_rows, D] or NULL */
+    const void *pre_weight, *pre_bias;    /* [D] or NULL */
+    int64_t gate_rows;
+    int post_norm, pre_norm;              /* PLE_NORM_* */
+    int gate_activation;                  /* PLE_GATE_* */
+    int stream_dtype, branch_dtype, param_dtype;
+    float residual_scale, eps;
+} ple_norm_t;
+
+/*
+ * Forward.  branch NULL: only the norm before a block, n = pre_norm(r) (no
+ * post norm, no gate, residual_scale 1; stream_out NULL).  pre_norm none:
+ * normed NULL.
+ *   stats   float32 [N, 4], 16-byte aligned: mean and factor of y, of s
+ */
+int ple_residual_norm_launch(const void *residual, const void *branch, const ple_norm_t *norm, void *stream_out,
+                             void *normed, float *stats, int64_t N, int64_t D, void *stream);
+
+/* Gradients that ple_residual_norm_backward_launch writes; NULL: not wanted. */
+typedef struct ple_norm_grads {
+    void *residual;                       /* stream_dtype [N, D] */
+    void *branch;                         /* branch_dtype [N, D] */
+    void *post_weight, *post_bias;        /* param_dtype [D] */
+    void *gate;                           /* param_dtype [gate_rows, D] */
+    void *pre_weight, *pre_bias;          /* param_dtype [D] */
+} ple_norm_grads_t;
+
+/* Scratch bytes the backward needs (on the current device). */
+size_t ple_residual_norm_backward_workspace_bytes(const ple_norm_t *norm, int64_t N, int64_t D);
+
+/*
+ * Backward of ple_residual_norm_launch.  grad_stream (stream_dtype) and
+ * grad_normed (branch_dtype) may be NULL (zero); stream_in is the forward's
+ * stream_out (its residual, where there was no branch).  Sums over rows are
+ * 32-bit in a fixed order, without atomics.
+ *   workspace  >= ple_residual_norm_backward_workspace_bytes() bytes, 256-byte
+ *              aligned, contents need not be initialised
+ */
+int ple_residual_norm_backward_launch(const void *grad_stream, const void *grad_normed, const void *stream_in,
+                                      const void *branch, const float *stats, const ple_norm_t *norm,
+                                      const ple_norm_grads_t *grads, int64_t N, int64_t D, void *workspace,
+                                      size_t workspace_bytes, void *stream);
+
+/*
+ * Distillation from a teacher's top logits, with optional hard labels; no
+ * counterpart in the reference.  For every row, with q = softmax(z / T) of the
+ * student's logits z [V] and p_k = exp(t_k / T - l) of the teacher's K logits:
+ *   loss = alpha T^2 (sum_k p_k (log p_k - log q_{c_k}) + rest)
+ *          + (1 - alpha) (log sum exp z - z[label])
+ * teacher_lse NULL: l is the log-sum over the row's own K logits (p sums to 1)
+ * and rest 0.  Else l = teacher_lse[n], the log-sum of exp(t / T) over the
+ * teacher's whole vocabulary, and rest = rho (log rho - log Q) with rho = 1 -
+ * sum p and Q the student's mass outside the K classes.
+ * Negative classes and labels are absent (a row without classes has only its
+ * label's term, and the other way round).  A class or label >= V makes the
+ * row's loss and gradient NaN.  A row whose logits are all -inf has loss and
+ * gradient 0.  A class may occur twice.  labels NULL: the first term alone.
+ *   logits           dtype [N, V]
+ *   teacher_logits   teacher_dtype [N, K]
+ *   teacher_classes  int32 or int64 (class_bytes 4 or 8) [N, K]
+ *   teacher_lse      float32 [N] or NULL
+ *   labels           int64 [N] or NULL
+ *   loss             float32 [N]
+ *   stats            float32 [N, PLE_DISTILL_STATS], for the backward
+ *   workspace        >= ple_distill_workspace_bytes(N, V) bytes (0 is
+ *                    possible), 256-byte aligned, need not be initialised
+ * 1e-6 < T < 1e6, 0 <= alpha <= 1 (else PLE_E_UNSUPPORTED); V <= 2^30, K <=
+ * 2^20, N <= 2^24, N * V <= 2^40 (else PLE_E_TOO_LARGE).
+ */
+#define PLE_DISTILL_STATS 8
+size_t ple_distill_workspace_bytes(int64_t N, int64_t V);
+int ple_distill_launch(const void *logits, const void *teacher_logits, const void *teacher_classes, int class_bytes,
+                       const float *teacher_lse, const int64_t *labels, float *loss, float *stats, int64_t N, int64_t V,
+                       int64_t K, float temperature, float alpha, int dtype, int teacher_dtype, void *workspace,
+                       size_t workspace_bytes, void *stream);
+
+/* Backward of ple_distill_launch: grad_logits (dtype [N, V]) = grad_loss[n] *
+ * d loss[n] / d logits[n], from the forward's stats; the teacher has no
+ * gradient. */
+int ple_distill_backward_launch(const float *grad_loss, const void *logits, const void *teacher_logits,
+                                const void *teacher_classes, int class_bytes, const int64_t *labels, const float *stats,
+                                void *grad_logits, int64_t N, int64_t V, int64_t K, float temperature, float alpha,
+                                int dtype, int teacher_dtype, void *stream);
+
+/*
  * Planner overrides, for tuning sweeps and for tests that run every kernel
  * form on the same inputs.  No counterpart in the reference (its launchers
  * have no knobs).  Each knob holds 0 -- the planner's own choice, the default

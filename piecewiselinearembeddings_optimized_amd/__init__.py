@@ -32,10 +32,15 @@ if not _running_build():
     from . import _autograd as _autograd  # noqa: F401
     from .module import CudaPiecewiseLinearEmbeddings, CudaPiecewiseLinearEncoding
     from .bins import bin_tables, compute_bins
+    from .trunk import CudaCategoricalEmbeddings, CudaDistillationLoss, CudaResidualNorm, CudaTokenEmbeddings
 
 __all__ = [
+    "CudaCategoricalEmbeddings",
+    "CudaDistillationLoss",
     "CudaPiecewiseLinearEmbeddings",
     "CudaPiecewiseLinearEncoding",
+    "CudaResidualNorm",
+    "CudaTokenEmbeddings",
     "bin_tables",
     "compute_bins",
 ]

@@ -65,7 +65,8 @@ def _hipcc() -> str:
     return p
 
 
-KERNEL_SOURCES = ("ple_capi.hip", "ple_forward.hip", "ple_backward.hip", "ple_encode.hip", "ple_noalloc.hip")
+KERNEL_SOURCES = ("ple_capi.hip", "ple_forward.hip", "ple_backward.hip", "ple_encode.hip", "ple_noalloc.hip",
+                  "ple_token_capi.hip", "ple_lookup.hip", "ple_norm.hip", "ple_distill.hip")
 
 
 def build_kernels(verbose: bool = False) -> str:
@@ -95,7 +96,7 @@ def build_extension(verbose: bool = False) -> str:
     torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     incs = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], os.path.join(ROCM, "include"), INCLUDE]
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    srcs = [os.path.join(CSRC, f) for f in ("ple_ops.cpp", "ple_autograd.cpp")]
+    srcs = [os.path.join(CSRC, f) for f in ("ple_ops.cpp", "ple_autograd.cpp", "ple_token_ops.cpp", "ple_token_autograd.cpp")]
     tmp = EXT_PATH + ".tmp"
     cmd = [
         os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-Wno-unused-function",

@@ -174,3 +174,108 @@ def _encode_backward_fake(grad_output, x, bin_edges, inv_bin_widths, n_bins, off
     torch._check(grad_output.ndim == 2 and grad_output.shape[0] == x.shape[0],
                  lambda: "grad_output must be contiguous float32 [N, total_bins]")
     return torch.empty_like(x)
+
+
+# ---------------------------------------------------------------------------
+# lookup, residual norm, distillation loss
+# ---------------------------------------------------------------------------
+
+INDEX_DTYPES = (torch.int32, torch.int64)
+NORM_MAX_WIDTH = 8192
+DISTILL_STATS = 8
+
+
+def _check_tokens(tokens, offsets) -> None:
+    torch._check(tokens.dtype in INDEX_DTYPES, lambda: "tokens must be int32 or int64")
+    if offsets is not None:
+        torch._check(offsets.ndim == 1 and offsets.dtype == torch.int64, lambda: "offsets must be int64 [F + 1]")
+        torch._check(tokens.ndim >= 1 and tokens.shape[-1] == offsets.shape[0] - 1,
+                     lambda: "the last dimension of tokens must be offsets.size(0) - 1")
+
+
+@torch.library.register_fake("rtdl_num_embeddings_cuda::lookup")
+def _lookup_fake(tokens, weight, offsets, scale, padding_idx, output_dtype):
+    _check_tokens(tokens, offsets)
+    torch._check(weight.ndim == 2, lambda: "weight must have shape [V, D]")
+    torch._check(weight.dtype in SUPPORTED_OUTPUT_DTYPES, lambda: "weight must be float32, float16, or bfloat16")
+    torch._check(output_dtype in SUPPORTED_OUTPUT_DTYPES, lambda: "output_dtype must be float32, float16, or bfloat16")
+    return weight.new_empty((*tokens.shape, weight.shape[1]), dtype=output_dtype)
+
+
+@torch.library.register_fake("rtdl_num_embeddings_cuda::lookup_backward")
+def _lookup_backward_fake(grad_output, tokens, offsets, num_rows, scale, padding_idx, grad_dtype):
+    _check_tokens(tokens, offsets)
+    torch._check(grad_output.ndim == tokens.ndim + 1,
+                 lambda: "grad_output must have the shape of tokens and one more dimension")
+    torch._check(grad_dtype in SUPPORTED_OUTPUT_DTYPES, lambda: "grad_dtype must be float32, float16, or bfloat16")
+    return grad_output.new_empty((num_rows, grad_output.shape[-1]), dtype=grad_dtype)
+
+
+@torch.library.register_fake("rtdl_num_embeddings_cuda::residual_norm")
+def _residual_norm_fake(residual, branch, post_weight, post_bias, gate, pre_weight, pre_bias, post_norm, pre_norm,
+                        gate_activation, residual_scale, eps, normed_dtype):
+    torch._check(residual.ndim >= 1, lambda: "the residual stream must have shape [..., D]")
+    torch._check(residual.dtype == torch.float32 or residual.dtype == normed_dtype,
+                 lambda: "the residual stream must be float32 or of the branch's dtype")
+    if branch is not None:
+        torch._check(branch.dtype == normed_dtype, lambda: "normed_dtype must be the branch's dtype")
+        torch._check(branch.shape == residual.shape, lambda: "branch must have the shape of the residual stream")
+    else:
+        torch._check(post_norm == 0 and gate is None and residual_scale == 1.0,
+                     lambda: "without a branch there is no post norm, no gate and no residual scale")
+        torch._check(pre_norm != 0, lambda: "without a branch there has to be a pre norm")
+    d = residual.shape[-1]
+    torch._check(d <= NORM_MAX_WIDTH, lambda: f"rows of at most {NORM_MAX_WIDTH} elements are supported, got {d}")
+    for name, t in (("post_weight", post_weight), ("post_bias", post_bias), ("pre_weight", pre_weight),
+                    ("pre_bias", pre_bias)):
+        if t is not None:
+            torch._check(t.ndim == 1 and t.shape[0] == d, lambda name=name: f"{name} must have shape [D]")
+    if gate is not None:
+        torch._check(gate.ndim == 2 and gate.shape[1] == d, lambda: "gate must have shape [G, D]")
+    stream = torch.empty_like(residual) if branch is not None else residual.new_empty((0,))
+    normed = (torch.empty_like(residual, dtype=normed_dtype) if pre_norm != 0
+              else residual.new_empty((0,), dtype=normed_dtype))
+    return stream, normed, residual.new_empty((residual.numel() // d, 4), dtype=torch.float32)
+
+
+@torch.library.register_fake("rtdl_num_embeddings_cuda::residual_norm_backward")
+def _residual_norm_backward_fake(grad_stream, grad_normed, stream, branch, stats, post_weight, post_bias, gate, pre_weight,
+                                 pre_bias, post_norm, pre_norm, gate_activation, residual_scale, output_mask):
+    if grad_stream is not None:
+        torch._check(grad_stream.shape == stream.shape and grad_stream.dtype == stream.dtype,
+                     lambda: "grad_stream must have the shape and dtype of stream")
+    if grad_normed is not None:
+        torch._check(pre_norm != 0, lambda: "grad_normed needs a pre norm")
+        torch._check(grad_normed.shape == stream.shape,
+                     lambda: "grad_normed must have the shape of stream and the branch's dtype")
+    inputs = (stream, branch, post_weight, post_bias, gate, pre_weight, pre_bias)
+    return tuple(torch.empty_like(t) if wanted and t is not None else stream.new_empty((0,))
+                 for t, wanted in zip(inputs, output_mask))
+
+
+def _check_distillation(logits, teacher_logits, teacher_classes, labels, temperature, alpha) -> None:
+    torch._check(logits.ndim == 2, lambda: "logits must have shape [N, V]")
+    torch._check(logits.dtype in SUPPORTED_OUTPUT_DTYPES, lambda: "logits must be float32, float16, or bfloat16")
+    torch._check(teacher_logits.ndim == 2 and teacher_logits.shape[0] == logits.shape[0],
+                 lambda: "teacher_logits must have shape [N, K]")
+    torch._check(teacher_classes.shape == teacher_logits.shape, lambda: "teacher_classes must have shape [N, K]")
+    torch._check(teacher_classes.dtype in INDEX_DTYPES, lambda: "teacher_classes must be int32 or int64")
+    if labels is not None:
+        torch._check(labels.ndim == 1 and labels.shape[0] == logits.shape[0] and labels.dtype == torch.int64,
+                     lambda: "labels must be int64 [N]")
+    torch._check(1e-6 < temperature < 1e6, lambda: f"temperature must be between 1e-6 and 1e6, got {temperature}")
+    torch._check(0.0 <= alpha <= 1.0, lambda: f"alpha must be between 0 and 1, got {alpha}")
+
+
+@torch.library.register_fake("rtdl_num_embeddings_cuda::distillation_loss")
+def _distillation_loss_fake(logits, teacher_logits, teacher_classes, teacher_lse, labels, temperature, alpha):
+    _check_distillation(logits, teacher_logits, teacher_classes, labels, temperature, alpha)
+    n = logits.shape[0]
+    return (logits.new_empty((n,), dtype=torch.float32), logits.new_empty((n, DISTILL_STATS), dtype=torch.float32))
+
+
+@torch.library.register_fake("rtdl_num_embeddings_cuda::distillation_loss_backward")
+def _distillation_loss_backward_fake(grad_loss, logits, teacher_logits, teacher_classes, labels, stats, temperature, alpha):
+    _check_distillation(logits, teacher_logits, teacher_classes, labels, temperature, alpha)
+    torch._check(grad_loss.ndim == 1 and grad_loss.dtype == torch.float32, lambda: "grad_loss must be float32 [N]")
+    return torch.empty_like(logits)

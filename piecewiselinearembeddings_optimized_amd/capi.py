@@ -77,6 +77,41 @@ class EncodePlanInfo(ctypes.Structure):
     ]
 
 
+class Norm(ctypes.Structure):
+    """``ple_norm_t``: the norms, gate and residual scale around a block."""
+
+    _fields_ = [
+        ("post_weight", ctypes.c_void_p),
+        ("post_bias", ctypes.c_void_p),
+        ("gate", ctypes.c_void_p),
+        ("pre_weight", ctypes.c_void_p),
+        ("pre_bias", ctypes.c_void_p),
+        ("gate_rows", ctypes.c_int64),
+        ("post_norm", ctypes.c_int),
+        ("pre_norm", ctypes.c_int),
+        ("gate_activation", ctypes.c_int),
+        ("stream_dtype", ctypes.c_int),
+        ("branch_dtype", ctypes.c_int),
+        ("param_dtype", ctypes.c_int),
+        ("residual_scale", ctypes.c_float),
+        ("eps", ctypes.c_float),
+    ]
+
+
+class NormGrads(ctypes.Structure):
+    """``ple_norm_grads_t``: the gradients a norm's backward writes."""
+
+    _fields_ = [
+        ("residual", ctypes.c_void_p),
+        ("branch", ctypes.c_void_p),
+        ("post_weight", ctypes.c_void_p),
+        ("post_bias", ctypes.c_void_p),
+        ("gate", ctypes.c_void_p),
+        ("pre_weight", ctypes.c_void_p),
+        ("pre_bias", ctypes.c_void_p),
+    ]
+
+
 class PleError(RuntimeError):
     def __init__(self, code: int, message: str):
         super().__init__(f"{message} (code {code})")
@@ -118,6 +153,24 @@ def lib() -> ctypes.CDLL:
         L.ple_encode_backward_launch.restype = i32
         L.ple_encode_plan_query.argtypes = [p, i64, i64, i64, i64, i32, ctypes.POINTER(EncodePlanInfo)]
         L.ple_encode_plan_query.restype = i32
+        f32, np_, gp = ctypes.c_float, ctypes.POINTER(Norm), ctypes.POINTER(NormGrads)
+        L.ple_lookup_launch.argtypes = [p, i32, p, p, p, i64, i64, i64, i64, f32, i32, i32, p]
+        L.ple_lookup_launch.restype = i32
+        L.ple_lookup_backward_workspace_bytes.argtypes = [i64, i64, i64]
+        L.ple_lookup_backward_workspace_bytes.restype = sz
+        L.ple_lookup_backward_launch.argtypes = [p, p, i32, p, p, i64, i64, i64, i64, i64, f32, i32, i32, p, sz, p]
+        L.ple_lookup_backward_launch.restype = i32
+        L.ple_residual_norm_launch.argtypes = [p, p, np_, p, p, p, i64, i64, p]
+        L.ple_residual_norm_launch.restype = i32
+        L.ple_residual_norm_backward_workspace_bytes.argtypes = [np_, i64, i64]
+        L.ple_residual_norm_backward_workspace_bytes.restype = sz
+        L.ple_residual_norm_backward_launch.argtypes = [p, p, p, p, p, np_, gp, i64, i64, p, sz, p]
+        L.ple_residual_norm_backward_launch.restype = i32
+        L.ple_distill_workspace_bytes.argtypes, L.ple_distill_workspace_bytes.restype = [i64, i64], sz
+        L.ple_distill_launch.argtypes = [p, p, p, i32, p, p, p, p, i64, i64, i64, f32, f32, i32, i32, p, sz, p]
+        L.ple_distill_launch.restype = i32
+        L.ple_distill_backward_launch.argtypes = [p, p, p, p, i32, p, p, p, i64, i64, i64, f32, f32, i32, i32, p]
+        L.ple_distill_backward_launch.restype = i32
         L.ple_timing_start.argtypes, L.ple_timing_start.restype = [i32], i32
         L.ple_timing_stop.argtypes, L.ple_timing_stop.restype = [], i32
         L.ple_timing_read.argtypes = [i32, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_int)]
@@ -269,3 +322,90 @@ def encode_backward(grad_output, x, bin_edges, inv_bin_widths, n_bins, offsets, 
     check(lib().ple_encode_backward_launch(
         _ptr(grad_output), _ptr(x), _ptr(bin_edges), _ptr(inv_bin_widths), _ptr(n_bins), _ptr(offsets),
         _ptr(grad_x), n, f, inv_bin_widths.shape[1], grad_output.shape[1], _stream(stream)))
+
+
+def _workspace(need: int, like):
+    return (torch.empty(need, dtype=torch.uint8, device=like.device) if need > 0 else None), need
+
+
+def lookup(tokens, weight, output, offsets=None, scale=1.0, stream=None) -> None:
+    """``ple_lookup_launch`` into a caller-provided ``output`` [*tokens.shape, D]."""
+    v, d = weight.shape
+    check(lib().ple_lookup_launch(
+        _ptr(tokens), tokens.element_size(), _ptr(offsets), _ptr(weight), _ptr(output), tokens.numel(),
+        1 if offsets is None else offsets.numel() - 1, v, d, scale, dtype_code(weight.dtype), dtype_code(output.dtype),
+        _stream(stream)))
+
+
+def lookup_backward(grad_output, tokens, grad_weight, offsets=None, scale=1.0, padding_idx=-1, workspace=None,
+                    stream=None) -> None:
+    """``ple_lookup_backward_launch`` into a caller-provided ``grad_weight`` [V, D]."""
+    v, d = grad_weight.shape
+    need = int(lib().ple_lookup_backward_workspace_bytes(tokens.numel(), v, d))
+    if workspace is None:
+        workspace, need = _workspace(need, tokens)
+    else:
+        need = workspace.numel() * workspace.element_size()
+    check(lib().ple_lookup_backward_launch(
+        _ptr(grad_output), _ptr(tokens), tokens.element_size(), _ptr(offsets), _ptr(grad_weight), tokens.numel(),
+        1 if offsets is None else offsets.numel() - 1, v, d, padding_idx, scale, dtype_code(grad_output.dtype),
+        dtype_code(grad_weight.dtype), _ptr(workspace), need, _stream(stream)))
+
+
+def norm(stream_dtype, branch_dtype, post_norm=0, pre_norm=0, post_weight=None, post_bias=None, gate=None,
+         gate_activation=0, pre_weight=None, pre_bias=None, residual_scale=1.0, eps=1e-5) -> Norm:
+    """The descriptor of a residual norm (the tensors have to outlive it)."""
+    def addr(t):
+        return None if t is None else t.data_ptr()
+
+    given = [t for t in (post_weight, post_bias, gate, pre_weight, pre_bias) if t is not None]
+    return Norm(addr(post_weight), addr(post_bias), addr(gate), addr(pre_weight), addr(pre_bias),
+                0 if gate is None else gate.shape[0], post_norm, pre_norm, gate_activation, dtype_code(stream_dtype),
+                dtype_code(branch_dtype), dtype_code(given[0].dtype) if given else DTYPE_F32, residual_scale, eps)
+
+
+def residual_norm(residual, branch, descriptor: Norm, stream_out, normed, stats, stream=None) -> None:
+    """``ple_residual_norm_launch`` into caller-provided outputs."""
+    n, d = residual.shape
+    check(lib().ple_residual_norm_launch(_ptr(residual), _ptr(branch), ctypes.byref(descriptor), _ptr(stream_out),
+                                         _ptr(normed), _ptr(stats), n, d, _stream(stream)))
+
+
+def residual_norm_backward(grad_stream, grad_normed, stream_in, branch, stats, descriptor: Norm, grads: dict,
+                           workspace=None, stream=None) -> None:
+    """``ple_residual_norm_backward_launch``; ``grads``: caller-provided tensors
+    by :class:`NormGrads`'s field names."""
+    n, d = stream_in.shape
+    if workspace is None:
+        workspace, need = _workspace(
+            int(lib().ple_residual_norm_backward_workspace_bytes(ctypes.byref(descriptor), n, d)), stream_in)
+    else:
+        need = workspace.numel() * workspace.element_size()
+    out = NormGrads(**{k: t.data_ptr() for k, t in grads.items() if t is not None})
+    check(lib().ple_residual_norm_backward_launch(
+        _ptr(grad_stream), _ptr(grad_normed), _ptr(stream_in), _ptr(branch), _ptr(stats), ctypes.byref(descriptor),
+        ctypes.byref(out), n, d, _ptr(workspace), need, _stream(stream)))
+
+
+def distill(logits, teacher_logits, teacher_classes, loss, stats, teacher_lse=None, labels=None, temperature=1.0,
+            alpha=1.0, workspace=None, stream=None) -> None:
+    """``ple_distill_launch`` into caller-provided ``loss`` [N] and ``stats`` [N, 8]."""
+    n, v = logits.shape
+    if workspace is None:
+        workspace, need = _workspace(int(lib().ple_distill_workspace_bytes(n, v)), logits)
+    else:
+        need = workspace.numel() * workspace.element_size()
+    check(lib().ple_distill_launch(
+        _ptr(logits), _ptr(teacher_logits), _ptr(teacher_classes), teacher_classes.element_size(), _ptr(teacher_lse),
+        _ptr(labels), _ptr(loss), _ptr(stats), n, v, teacher_logits.shape[1], temperature, alpha,
+        dtype_code(logits.dtype), dtype_code(teacher_logits.dtype), _ptr(workspace), need, _stream(stream)))
+
+
+def distill_backward(grad_loss, logits, teacher_logits, teacher_classes, stats, grad_logits, labels=None,
+                     temperature=1.0, alpha=1.0, stream=None) -> None:
+    """``ple_distill_backward_launch`` into a caller-provided ``grad_logits`` [N, V]."""
+    n, v = logits.shape
+    check(lib().ple_distill_backward_launch(
+        _ptr(grad_loss), _ptr(logits), _ptr(teacher_logits), _ptr(teacher_classes), teacher_classes.element_size(),
+        _ptr(labels), _ptr(stats), _ptr(grad_logits), n, v, teacher_logits.shape[1], temperature, alpha,
+        dtype_code(logits.dtype), dtype_code(teacher_logits.dtype), _stream(stream)))

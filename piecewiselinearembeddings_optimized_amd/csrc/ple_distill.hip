@@ -1,0 +1,479 @@
+// Distillation from a teacher's top logits, with optional hard labels (gfx950).
+// Row n has the student's logits z [V], the teacher's logits t [K] of the
+// classes c [K], a temperature T and the weight alpha of the teacher:
+//
+//     q = softmax(z / T),  p_k = exp(t_k / T - l)
+//     loss = alpha T^2 (sum_k p_k (log p_k - log q_{c_k}) + rest)
+//            + (1 - alpha) (lse(z) - z[label])
+//
+// l is the log-sum over the row's own K logits, or is given: the log-sum over
+// the teacher's whole vocabulary.  Then the mass it left out, rho = 1 - sum p,
+// is one more outcome: rest = rho (log rho - log Q), Q the student's mass
+// outside the K classes.  With m = sum p + rho the gradient is
+//
+//     dz_j = alpha T (m q_j - sum_{c_k = j} p_k - [j outside] rho q_j / Q)
+//            + (1 - alpha) (softmax(z)_j - [j = label])
+//
+// Bound by memory: the forward reads z once, with the running maximum and the
+// sums at both temperatures; the backward reads it once and writes dz once:
+// every class gets the formula without its sparse terms in a dense pass, and
+// the K classes and the label are then computed whole and written over it.
+// Classes outside the K are told by a bit each in LDS, so that Q is a sum of
+// its own terms and not a difference.
+//
+// A row belongs to a team of lanes (part of a wave, a wave or a workgroup);
+// where there are few rows of many classes, to several workgroups, each a range
+// of the classes, whose sums a second kernel joins.
+
+#include <algorithm>
+#include <cfloat>
+
+#include "ple_internal.h"
+#include "ple_rows.h"
+
+namespace ple {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// stats of a row (PLE_DISTILL_STATS floats)
+enum { kPeak, kLogT, kLog1, kTeacherLse, kMass, kOutside, kLabelled };
+
+struct DistillArgs {
+    const void *z, *t, *classes;
+    const float *t_lse;          // NULL: over the row's own K logits
+    const int64_t *labels;       // NULL: none
+    const float *g;
+    void *dz;
+    float *loss, *stats, *partial;   // partial: [N, splits, 4]
+    int64_t N;
+    int V, K, t_dtype, wide;     // wide: 64-bit classes
+    int splits, part;            // classes a split takes
+    int words;                   // of a team's bits in LDS
+    float inv_t, t_factor, alpha;    // 1 / T, T
+};
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+__device__ __forceinline__ int64_t class_of(const DistillArgs &a, int64_t i) {
+    return a.wide ? static_cast<const int64_t *>(a.classes)[i] : static_cast<const int32_t *>(a.classes)[i];
+}
+
+// Vectors of a row's range [c0, c1): element c0 + i is bit shift + i of the
+// team's bits, so that 16-byte vectors of z own whole groups of bits.
+template <int Z, bool VEC>
+struct Range {
+    static constexpr int kVec = VEC ? (Z == PLE_DTYPE_F32 ? 4 : 8) : 1;
+    int64_t base;                // of the row
+    int c0, c1, shift, head;     // head: elements before the first vector
+    __device__ __forceinline__ Range(const void *z, int64_t row, int v, int begin, int end) : base(row * v), c0(begin), c1(end) {
+        if constexpr (VEC) {
+            shift = static_cast<int>((reinterpret_cast<uintptr_t>(z) / elem_bytes(Z) + base + begin) % kVec);
+            head = min((kVec - shift) % kVec, end - begin);
+        } else {
+            shift = head = 0;
+        }
+    }
+    __device__ __forceinline__ int vectors() const { return (c1 - c0 - head) / kVec; }
+    __device__ __forceinline__ int at(int vec) const { return c0 + head + vec * kVec; }      // its first class
+    __device__ __forceinline__ int bit(int c) const { return c - c0 + shift; }
+    // classes beside the vectors: `head` before, the others behind
+    __device__ __forceinline__ int odd() const { return (c1 - c0) - vectors() * kVec; }
+    __device__ __forceinline__ int odd_at(int i) const { return i < head ? c0 + i : c0 + vectors() * kVec + i; }
+};
+
+// Running maximum and sums of a lane.  The maximum starts at the lowest number,
+// not at -inf: a class of -inf then adds exp(-inf) = 0 without a NaN.
+template <bool BOTH>
+struct Sums {
+    float m = -FLT_MAX, at_t = 0.0f, at_1 = 0.0f, outside = 0.0f;
+    __device__ __forceinline__ void rescale(float to, float ct) {
+        const float f = exp2_fast((m - to) * ct);
+        at_t *= f;
+        outside *= f;
+        if constexpr (BOTH) at_1 *= exp2_fast((m - to) * kLog2e);
+        m = to;
+    }
+    template <int VEC>
+    __device__ __forceinline__ void add(const float *v, uint32_t inside, float ct) {
+        float top = v[0];
+#pragma unroll
+        for (int e = 1; e < VEC; ++e) top = fmaxf(top, v[e]);
+        if (top > m) rescale(top, ct);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const float x = exp2_fast((v[e] - m) * ct);
+            at_t += x;
+            outside += (inside >> e) & 1 ? 0.0f : x;
+            if constexpr (BOTH) at_1 += exp2_fast((v[e] - m) * kLog2e);
+        }
+    }
+    template <int TEAM>
+    __device__ __forceinline__ void join(Team<TEAM> &team, float ct) {
+        rescale(team.max(m), ct);
+        team.sum2(at_t, outside);
+        if constexpr (BOTH) at_1 = team.sum(at_1);
+        else at_1 = at_t;
+    }
+};
+
+// Marks the row's classes of [c0, c1) in the team's bits, which it clears
+// first.  Returns whether one of them was there already.  (All threads of the
+// workgroup.)
+template <int TEAM, int Z, bool VEC>
+__device__ __forceinline__ bool mark_classes(Team<TEAM> &team, const DistillArgs &a, int64_t n, const Range<Z, VEC> &r,
+                                             uint32_t *bits, int *twice) {
+    for (int w = team.lane(); w < a.words; w += team.lanes()) bits[w] = 0;
+    if (team.lane() == 0) *twice = 0;
+    __syncthreads();
+    if (n < a.N)
+        for (int k = team.lane(); k < a.K; k += team.lanes()) {
+            const int64_t c = class_of(a, n * a.K + k);
+            if (c < r.c0 || c >= r.c1) continue;
+            const int b = r.bit(static_cast<int>(c));
+            if (atomicOr(&bits[b >> 5], 1u << (b & 31)) >> (b & 31) & 1) *twice = 1;
+        }
+    __syncthreads();
+    return *twice != 0;
+}
+
+template <int Z, int TEAM, bool BOTH>
+__device__ __forceinline__ void scan_row(Team<TEAM> &team, const DistillArgs &a, const Range<Z, true> &r, const uint32_t *bits,
+                                         float ct, Sums<BOTH> &s) {
+    constexpr int kVec = Range<Z, true>::kVec;
+    const auto inside = [&](int c, int n) -> uint32_t {
+        if (!a.t_lse) return 0;
+        const int b = r.bit(c);
+        return bits[b >> 5] >> (b & 31) & ((1u << n) - 1);
+    };
+    const int vectors = r.vectors();
+    for (int i = team.lane(); i < vectors; i += team.lanes()) {
+        float v[kVec];
+        load_vec<Z, kVec>(a.z, r.base + r.at(i), v);
+        s.template add<kVec>(v, inside(r.at(i), kVec), ct);
+    }
+    for (int i = team.lane(); i < r.odd(); i += team.lanes()) {
+        const float v = load_grad<Z>(a.z, r.base + r.odd_at(i));
+        s.template add<1>(&v, inside(r.odd_at(i), 1), ct);
+    }
+}
+
+// The row's loss and stats from its sums.
+template <int Z, int TEAM>
+__device__ __forceinline__ void finish_row(Team<TEAM> &team, const DistillArgs &a, int64_t n, float m, float at_t, float at_1,
+                                           float outside) {
+    const bool on = n < a.N;
+    float peak = -FLT_MAX, count = 0.0f, wrong = 0.0f;
+    for (int k = team.lane(); on && k < a.K; k += team.lanes()) {
+        const int64_t c = class_of(a, n * a.K + k);
+        if (c < 0) continue;
+        if (c >= a.V) wrong = 1.0f;
+        count = 1.0f;
+        peak = fmaxf(peak, load_any(a.t, n * a.K + k, a.t_dtype) * a.inv_t);
+    }
+    float lse = 0.0f;
+    team.sum2(count, wrong);
+    if (a.t_lse) {
+        if (on) lse = a.t_lse[n];
+    } else {
+        peak = team.max(peak);
+        float sum = 0.0f;
+        for (int k = team.lane(); on && k < a.K; k += team.lanes())
+            if (class_of(a, n * a.K + k) >= 0)
+                sum += exp2_fast((load_any(a.t, n * a.K + k, a.t_dtype) * a.inv_t - peak) * kLog2e);
+        sum = team.sum(sum);
+        if (sum == 0.0f) count = 0.0f;       // (no class has a probability)
+        lse = count != 0.0f ? peak + logf(sum) : 0.0f;
+    }
+    const float log_t = logf(at_t), log_1 = logf(at_1);
+    float kd = 0.0f, mass = 0.0f;
+    for (int k = team.lane(); on && k < a.K; k += team.lanes()) {
+        const int64_t c = class_of(a, n * a.K + k);
+        if (c < 0 || c >= a.V) continue;
+        const float log_p = load_any(a.t, n * a.K + k, a.t_dtype) * a.inv_t - lse;
+        const float p = exp2_fast(log_p * kLog2e);
+        mass += p;
+        if (p != 0.0f) kd += p * (log_p - (load_grad<Z>(a.z, n * a.V + c) - m) * a.inv_t + log_t);
+    }
+    team.sum2(kd, mass);
+    if (team.lane() != 0 || !on) return;
+    float factor = mass, labelled = 0.0f, ce = 0.0f;
+    if (a.t_lse && count > 0.0f) {
+        const float rho = fmaxf(1.0f - mass, 0.0f);
+        // (a row whose K classes are all there are has no outside)
+        if (rho > 0.0f && outside > 0.0f) {
+            kd += rho * (logf(rho) - logf(outside) + log_t);
+            mass += rho;
+            factor = mass - rho * (at_t / outside);
+        }
+    }
+    if (a.labels) {
+        const int64_t label = a.labels[n];
+        if (label >= a.V) labelled = __builtin_nanf("");
+        else if (label >= 0) labelled = 1.0f;
+        if (label >= 0 && label < a.V) ce = log_1 - (load_grad<Z>(a.z, n * a.V + label) - m);
+        else ce = labelled;
+    }
+    if (wrong > 0.0f) kd = mass = factor = __builtin_nanf("");
+    float *st = a.stats + n * PLE_DISTILL_STATS;
+    if (at_t == 0.0f) {          // every class is masked: no loss, no gradient
+        kd = ce = m = mass = factor = labelled = 0.0f;
+        st[kLogT] = st[kLog1] = 0.0f;
+    } else {
+        st[kLogT] = log_t * kLog2e;
+        st[kLog1] = log_1 * kLog2e;
+    }
+    st[kPeak] = m;
+    st[kTeacherLse] = lse;
+    st[kMass] = mass;
+    st[kOutside] = factor;
+    st[kLabelled] = labelled;
+    st[7] = 0.0f;
+    a.loss[n] = (a.alpha > 0.0f && count > 0.0f ? a.alpha * a.t_factor * a.t_factor * kd : 0.0f) +
+                (a.alpha < 1.0f && labelled != 0.0f ? (1.0f - a.alpha) * ce : 0.0f);
+}
+
+template <int Z, int TEAM, bool BOTH>
+__global__ __launch_bounds__(Team<TEAM>::kThreads) void ple_distill_forward_kernel(DistillArgs a) {
+    extern __shared__ uint32_t s_bits[];
+    __shared__ float s_sum[Team<TEAM>::kLdsFloats];
+    __shared__ int s_twice[Team<TEAM>::kThreads / (TEAM < kBlock ? TEAM : kBlock)];
+    Team<TEAM> team(s_sum);
+    const int split = blockIdx.x % a.splits;
+    const int64_t n = static_cast<int64_t>(blockIdx.x / a.splits) * team.per_block() + team.index();
+    const float ct = a.inv_t * kLog2e;
+    uint32_t *bits = s_bits + team.index() * a.words;
+    const Range<Z, true> r(a.z, n, a.V, split * a.part, min(a.V, (split + 1) * a.part));
+    Sums<BOTH> s;
+    if (a.t_lse) mark_classes(team, a, n, r, bits, &s_twice[team.index()]);
+    if (n < a.N) scan_row<Z, TEAM, BOTH>(team, a, r, bits, ct, s);
+    s.join(team, ct);
+    if (a.splits == 1) {
+        finish_row<Z>(team, a, n, s.m, s.at_t, s.at_1, s.outside);
+    } else if (team.lane() == 0 && n < a.N) {
+        reinterpret_cast<float4 *>(a.partial)[n * a.splits + split] = make_float4(s.m, s.at_t, s.at_1, s.outside);
+    }
+}
+
+// A row's sums from its splits' (one wave a row), then its loss.
+template <int Z>
+__global__ __launch_bounds__(kBlock) void ple_distill_join_kernel(DistillArgs a) {
+    Team<kWave> team(nullptr);
+    const int64_t n = static_cast<int64_t>(blockIdx.x) * team.per_block() + team.index();
+    const float ct = a.inv_t * kLog2e;
+    float m = -FLT_MAX, at_t = 0.0f, at_1 = 0.0f, outside = 0.0f;
+    for (int i = team.lane(); n < a.N && i < a.splits; i += kWave) {
+        const float4 v = reinterpret_cast<const float4 *>(a.partial)[n * a.splits + i];
+        const float to = fmaxf(m, v.x);
+        const float f = exp2_fast((m - to) * ct), g = exp2_fast((v.x - to) * ct);
+        at_t = at_t * f + v.y * g;
+        outside = outside * f + v.w * g;
+        at_1 = at_1 * exp2_fast((m - to) * kLog2e) + v.z * exp2_fast((v.x - to) * kLog2e);
+        m = to;
+    }
+    const float to = team.max(m);
+    const float f = exp2_fast((m - to) * ct);
+    at_t *= f;
+    outside *= f;
+    at_1 *= exp2_fast((m - to) * kLog2e);
+    team.sum2(at_t, outside);
+    at_1 = team.sum(at_1);
+    finish_row<Z>(team, a, n, to, at_t, at_1, outside);
+}
+
+template <int Z, int TEAM, bool VEC, bool BOTH>
+__global__ __launch_bounds__(Team<TEAM>::kThreads) void ple_distill_backward_kernel(DistillArgs a) {
+    constexpr int kVec = Range<Z, VEC>::kVec;
+    extern __shared__ uint32_t s_bits[];
+    __shared__ int s_twice[Team<TEAM>::kThreads / (TEAM < kBlock ? TEAM : kBlock)];
+    Team<TEAM> team(nullptr);
+    const int split = blockIdx.x % a.splits;
+    const int64_t n = static_cast<int64_t>(blockIdx.x / a.splits) * team.per_block() + team.index();
+    const float ct = a.inv_t * kLog2e;
+    uint32_t *bits = s_bits + team.index() * a.words;
+    const Range<Z, VEC> r(a.z, n, a.V, split * a.part, min(a.V, (split + 1) * a.part));
+    const bool twice = mark_classes(team, a, n, r, bits, &s_twice[team.index()]);
+    float peak = 0.0f, log_t = 0.0f, log_1 = 0.0f, lse = 0.0f, mass = 0.0f, w_soft = 0.0f, w_out = 0.0f, w_hard = 0.0f;
+    int64_t label = -1;
+    if (n < a.N) {
+        const float *st = a.stats + n * PLE_DISTILL_STATS;
+        const float g = a.g[n];
+        peak = st[kPeak];
+        log_t = st[kLogT];
+        log_1 = st[kLog1];
+        lse = st[kTeacherLse];
+        mass = st[kMass];
+        w_soft = a.alpha > 0.0f && mass != 0.0f ? g * a.alpha * a.t_factor : 0.0f;
+        w_out = w_soft != 0.0f ? w_soft * st[kOutside] : 0.0f;
+        w_hard = a.alpha < 1.0f && st[kLabelled] != 0.0f ? g * (1.0f - a.alpha) * st[kLabelled] : 0.0f;
+        if (a.labels && st[kLabelled] != 0.0f) label = a.labels[n];
+    }
+    const auto soft = [&](float z) { return exp2_fast((z - peak) * ct - log_t); };
+    const auto hard = [&](float z) { return exp2_fast((z - peak) * kLog2e - log_1); };
+    const auto dense = [&](float z) {
+        if constexpr (BOTH) return w_out * soft(z) + w_hard * hard(z);
+        else return (w_out + w_hard) * soft(z);
+    };
+    if (n < a.N) {
+        const int vectors = r.vectors();
+        for (int i = team.lane(); i < vectors; i += team.lanes()) {
+            float v[kVec];
+            load_vec<Z, kVec>(a.z, r.base + r.at(i), v);
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) v[e] = dense(v[e]);
+            store_vec<Z, kVec>(a.dz, r.base + r.at(i), v);
+        }
+        if constexpr (VEC)
+            for (int i = team.lane(); i < r.odd(); i += team.lanes()) {
+                const float v = dense(load_grad<Z>(a.z, r.base + r.odd_at(i)));
+                store_vec<Z, 1>(a.dz, r.base + r.odd_at(i), &v);
+            }
+    }
+    __syncthreads();
+    if (n >= a.N) return;
+    for (int k = team.lane(); k < a.K; k += team.lanes()) {
+        const int64_t c = class_of(a, n * a.K + k);
+        if (c < r.c0 || c >= r.c1) continue;
+        const auto prob = [&](int i) { return exp2_fast((load_any(a.t, n * a.K + i, a.t_dtype) * a.inv_t - lse) * kLog2e); };
+        float p = 0.0f;
+        bool mine = true;
+        if (twice) {
+            for (int i = 0; i < a.K; ++i)
+                if (class_of(a, n * a.K + i) == c) {
+                    if (i < k) mine = false;
+                    p += prob(i);
+                }
+        } else {
+            p = prob(k);
+        }
+        if (!mine) continue;
+        const float z = load_grad<Z>(a.z, r.base + c);
+        float v = w_soft != 0.0f ? w_soft * (mass * soft(z) - p) : 0.0f;
+        if (w_hard != 0.0f) v += w_hard * (hard(z) - (c == label ? 1.0f : 0.0f));
+        store_vec<Z, 1>(a.dz, r.base + c, &v);
+    }
+    if (team.lane() == 0 && label >= r.c0 && label < r.c1) {
+        const int b = r.bit(static_cast<int>(label));
+        if (!(bits[b >> 5] >> (b & 31) & 1)) {
+            const float v = dense(load_grad<Z>(a.z, r.base + label)) - w_hard;
+            store_vec<Z, 1>(a.dz, r.base + label, &v);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// plans and launches
+// ---------------------------------------------------------------------------
+
+struct DistillPlan {
+    int team, threads, per_block, splits, part, words;
+    size_t bytes, lds;
+};
+
+constexpr int kMaxPart = 1 << 18;        // classes a workgroup has bits for (32 KB)
+
+DistillPlan plan_distill(int64_t N, int64_t V) {
+    DistillPlan p{};
+    p.team = V <= 64 ? 8 : (V <= 2048 ? kWave : kBlock);
+    p.threads = kBlock;
+    p.per_block = kBlock / p.team;
+    p.splits = 1;
+    p.part = static_cast<int>(V);
+    if (p.team == kBlock) {
+        const int64_t wanted = std::max<int64_t>((4 * device_cu_count() + N - 1) / std::max<int64_t>(N, 1), (V + kMaxPart - 1) / kMaxPart);
+        const int64_t splits = std::max((V + kMaxPart - 1) / kMaxPart, std::min(wanted, V / 2048));
+        if (splits > 1) {
+            p.part = static_cast<int>(((V + splits - 1) / splits + 63) / 64 * 64);
+            p.splits = static_cast<int>((V + p.part - 1) / p.part);
+        }
+    }
+    p.words = (p.part + 8 + 31) / 32;
+    p.lds = static_cast<size_t>(p.words) * 4 * p.per_block;
+    p.bytes = p.splits > 1 ? align_up(static_cast<size_t>(N) * p.splits * 16, 256) : 0;
+    return p;
+}
+
+DistillArgs distill_args(const DistillRequest &r, const DistillPlan &p) {
+    DistillArgs a{};
+    a.z = r.logits; a.t = r.teacher; a.classes = r.classes;
+    a.t_lse = r.teacher_lse; a.labels = r.labels;
+    a.g = r.g; a.dz = r.dz; a.loss = r.loss; a.stats = r.stats;
+    a.partial = static_cast<float *>(r.workspace);
+    a.N = r.N; a.V = static_cast<int>(r.V); a.K = static_cast<int>(r.K);
+    a.t_dtype = r.teacher_dtype; a.wide = r.wide;
+    a.splits = p.splits; a.part = p.part; a.words = p.words;
+    a.inv_t = 1.0f / r.temperature; a.t_factor = r.temperature; a.alpha = r.alpha;
+    return a;
+}
+
+// f(type, team, both sums) as compile-time constants
+template <typename F>
+hipError_t with_distill(const DistillRequest &r, const DistillPlan &p, F f) {
+    const bool both = r.labels && r.temperature != 1.0f;
+    const auto by_both = [&](auto z, auto team) {
+        return both ? f(z, team, std::true_type{}) : f(z, team, std::false_type{});
+    };
+    const auto by_team = [&](auto z) {
+        switch (p.team) {
+            case 8: return by_both(z, std::integral_constant<int, 8>{});
+            case kWave: return by_both(z, std::integral_constant<int, kWave>{});
+            default: return by_both(z, std::integral_constant<int, kBlock>{});
+        }
+    };
+    switch (r.dtype) {
+        case PLE_DTYPE_F32: return by_team(std::integral_constant<int, PLE_DTYPE_F32>{});
+        case PLE_DTYPE_F16: return by_team(std::integral_constant<int, PLE_DTYPE_F16>{});
+        default: return by_team(std::integral_constant<int, PLE_DTYPE_BF16>{});
+    }
+}
+
+dim3 distill_grid(const DistillRequest &r, const DistillPlan &p) {
+    return dim3(static_cast<unsigned>((r.N + p.per_block - 1) / p.per_block * p.splits));
+}
+
+}  // namespace
+
+size_t distill_workspace_bytes(int64_t N, int64_t V) { return plan_distill(N, V).bytes; }
+
+int distill_run(const DistillRequest &r) {
+    const DistillPlan p = plan_distill(r.N, r.V);
+    if (p.bytes > 0 && (!r.workspace || r.workspace_bytes < p.bytes || reinterpret_cast<uintptr_t>(r.workspace) % 256 != 0))
+        return PLE_E_WORKSPACE;
+    const DistillArgs a = distill_args(r, p);
+    const hipError_t rc = with_distill(r, p, [&](auto z, auto team, auto both) {
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_distill_forward_kernel<decltype(z)::value, decltype(team)::value,
+                                                                      decltype(both)::value>),
+                           distill_grid(r, p), dim3(p.threads), p.lds, r.stream, a);
+        return hipGetLastError();
+    });
+    if (rc != hipSuccess || p.splits == 1) return static_cast<int>(rc);
+    const dim3 grid(static_cast<unsigned>((r.N + kWavesPerBlock - 1) / kWavesPerBlock));
+    switch (r.dtype) {
+        case PLE_DTYPE_F32:
+            hipLaunchKernelGGL(ple_distill_join_kernel<PLE_DTYPE_F32>, grid, dim3(kBlock), 0, r.stream, a);
+            break;
+        case PLE_DTYPE_F16:
+            hipLaunchKernelGGL(ple_distill_join_kernel<PLE_DTYPE_F16>, grid, dim3(kBlock), 0, r.stream, a);
+            break;
+        default: hipLaunchKernelGGL(ple_distill_join_kernel<PLE_DTYPE_BF16>, grid, dim3(kBlock), 0, r.stream, a);
+    }
+    return static_cast<int>(hipGetLastError());
+}
+
+int distill_backward_run(const DistillRequest &r) {
+    const DistillPlan p = plan_distill(r.N, r.V);
+    const DistillArgs a = distill_args(r, p);
+    // one vector for z and dz: both addresses are the same way into 16 bytes
+    const bool vec = (reinterpret_cast<uintptr_t>(r.logits) - reinterpret_cast<uintptr_t>(r.dz)) % 16 == 0;
+    return static_cast<int>(with_distill(r, p, [&](auto z, auto team, auto both) {
+        const auto launch = [&](auto v) {
+            hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_distill_backward_kernel<decltype(z)::value, decltype(team)::value,
+                                                                           decltype(v)::value, decltype(both)::value>),
+                               distill_grid(r, p), dim3(p.threads), p.lds, r.stream, a);
+            return hipGetLastError();
+        };
+        return vec ? launch(std::true_type{}) : launch(std::false_type{});
+    }));
+}
+
+}  // namespace ple

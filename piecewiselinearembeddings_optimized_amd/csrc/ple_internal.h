@@ -100,4 +100,63 @@ int encode_backward_run(const EncodeRequest &r);
 // the address of `out` counts).
 int encode_plan_info(const EncodeRequest &r, bool backward, ple_encode_plan_info_t *info);
 
+struct LookupRequest {
+    const void *tokens;
+    const int64_t *offsets = nullptr;    // categorical columns: [F + 1]
+    const void *table = nullptr;         // forward: [V, D]
+    void *out = nullptr;                 // forward: [T, D]
+    const void *grad = nullptr;          // backward: [T, D], of out_dtype
+    void *dw = nullptr;                  // backward: [V, D], of table_dtype
+    int64_t T, F, V, D, padding = -1;
+    int wide, table_dtype, out_dtype;    // wide: 64-bit tokens
+    float scale;
+    void *workspace = nullptr;
+    size_t workspace_bytes = 0;
+    hipStream_t stream;
+};
+
+int lookup_run(const LookupRequest &r);
+size_t lookup_backward_workspace_bytes(int64_t T, int64_t V, int64_t D);
+int lookup_backward_run(const LookupRequest &r);
+
+struct NormRequest {
+    const void *residual, *branch;       // backward: residual is the stored stream
+    const void *post_w, *post_b, *gate, *pre_w, *pre_b;
+    void *stream_out = nullptr, *normed = nullptr;
+    float *stats;                        // [N, 4]
+    const void *g_stream = nullptr, *g_normed = nullptr;
+    void *d_residual = nullptr, *d_branch = nullptr;
+    void *d_post_w = nullptr, *d_post_b = nullptr, *d_gate = nullptr, *d_pre_w = nullptr, *d_pre_b = nullptr;
+    int64_t N, D, groups;                // groups: rows of the gate
+    int stream_dtype, branch_dtype, param_dtype;
+    int post, pre, act;
+    float alpha, eps;
+    void *workspace = nullptr;
+    size_t workspace_bytes = 0;
+    hipStream_t stream;
+};
+
+int norm_run(const NormRequest &r);
+size_t norm_backward_workspace_bytes(const NormRequest &r);
+int norm_backward_run(const NormRequest &r);
+
+struct DistillRequest {
+    const void *logits, *teacher, *classes;
+    const float *teacher_lse;
+    const int64_t *labels;
+    const float *g = nullptr;
+    void *dz = nullptr;
+    float *loss = nullptr, *stats;
+    int64_t N, V, K;
+    int dtype, teacher_dtype, wide;      // wide: 64-bit classes
+    float temperature, alpha;
+    void *workspace = nullptr;
+    size_t workspace_bytes = 0;
+    hipStream_t stream;
+};
+
+int distill_run(const DistillRequest &r);
+size_t distill_workspace_bytes(int64_t N, int64_t V);
+int distill_backward_run(const DistillRequest &r);
+
 }  // namespace ple

@@ -1,0 +1,509 @@
+// Norms after and before a block, fused with its gate and residual scale
+// (gfx950).  For every row (stream r, branch y, both [N, D]):
+//
+//     p = post(y)                      post, pre: none, rms or layer norm
+//     s = round_R(alpha r + h(gate) p) R: the stream's type, h: identity,
+//     n = round_Y(pre(s))                 sigmoid or tanh
+//
+// The norm before the next block and the whole backward read s as it is
+// stored, so that they agree with each other.  Backward, with xh the
+// standardised row, rho its factor and m() a row's mean:
+//
+//     ds = dS + rho (dn w - [layer] m(dn w) - xh m(dn w xh))
+//     dr = alpha ds,  dp = ds h(gate),  dgate = h'(gate) sum ds p
+//     dy = the first line's right term for dp and the norm after the block
+//     dw = sum_rows dn xh,  db = sum_rows dn
+//
+// Bound by memory: forward 2 reads and 2 writes of a row, backward 4 and 2.
+// A row is held in registers by a team of lanes, 8 elements each (a part of a
+// wave, a wave, or a workgroup of up to 16 waves), so it is read once.  In the
+// backward a team walks its rows with the parameters' gradient sums in
+// registers; a workgroup adds its teams' sums and leaves them as partials in
+// 32 bits, which a second kernel adds in a fixed order.
+
+#include <algorithm>
+
+#include "ple_internal.h"
+#include "ple_rows.h"
+
+namespace ple {
+namespace {
+
+constexpr int kElems = 8;              // elements of a row a lane holds
+constexpr int kMaxD = 16 * kWave * kElems;
+
+struct NormArgs {
+    const void *residual, *branch;     // backward: residual is the stored stream
+    const void *post_w, *post_b, *gate, *pre_w, *pre_b;
+    void *stream_out, *normed;
+    float4 *stats;                     // [N]: mean and factor after the block, before the next
+    const void *g_stream, *g_normed;
+    void *d_residual, *d_branch, *d_gate;
+    float *partial;                    // [workgroups, sums, D]
+    float *gate_partial;               // [groups, pieces, D]
+    int64_t N, rows_per_gate;
+    int64_t piece_rows, pieces;        // backward: rows of a piece, pieces of a gate's rows
+    int D, param_dtype;
+    int post, pre, act, gates;         // gates: 0 none, 1 one for all rows, 2 one each for groups of rows, 3 one a row
+    int slot_pw, slot_pb, slot_g, slot_nw, slot_nb, slots;   // sums' places in a partial (-1: not wanted)
+    float alpha, eps;
+};
+
+// A lane's 8 elements of a row: adjacent where rows are 16-byte vectors (VEC),
+// else one of every `lanes` elements.
+template <bool VEC>
+struct Cols {
+    int first, step, D;
+    __device__ __forceinline__ Cols(int lane, int lanes, int d)
+        : first(VEC ? lane * kElems : lane), step(VEC ? 1 : lanes), D(d) {}
+    __device__ __forceinline__ bool on(int e) const { return VEC ? first < D : first + e * step < D; }
+    __device__ __forceinline__ int at(int e) const { return first + e * step; }
+
+    template <int T>
+    __device__ __forceinline__ void load(const void *p, int64_t row, float (&v)[kElems]) const {
+        if constexpr (VEC) {
+            if (on(0)) load_vec<T, kElems>(p, row * D + first, v);
+            else
+#pragma unroll
+                for (int e = 0; e < kElems; ++e) v[e] = 0.0f;
+        } else {
+#pragma unroll
+            for (int e = 0; e < kElems; ++e) v[e] = on(e) ? load_grad<T>(p, row * D + at(e)) : 0.0f;
+        }
+    }
+    template <int T>
+    __device__ __forceinline__ void store(void *p, int64_t row, const float (&v)[kElems]) const {
+        if constexpr (VEC) {
+            if (on(0)) store_vec<T, kElems>(p, row * D + first, v);
+        } else {
+#pragma unroll
+            for (int e = 0; e < kElems; ++e)
+                if (on(e)) store_vec<T, 1>(p, row * D + at(e), &v[e]);
+        }
+    }
+    __device__ __forceinline__ void load_param(const void *p, int64_t row, int dtype, float none, float (&v)[kElems]) const {
+#pragma unroll
+        for (int e = 0; e < kElems; ++e) v[e] = p && on(e) ? load_any(p, row * D + at(e), dtype) : none;
+    }
+};
+
+__device__ __forceinline__ float gate_value(float x, int act) {
+    if (act == PLE_GATE_SIGMOID) return 1.0f / (1.0f + expf(-x));
+    if (act == PLE_GATE_TANH) return tanhf(x);
+    return x;
+}
+
+// Derivative of gate_value, from its value.
+__device__ __forceinline__ float gate_slope(float h, int act) {
+    if (act == PLE_GATE_SIGMOID) return h * (1.0f - h);
+    if (act == PLE_GATE_TANH) return 1.0f - h * h;
+    return 1.0f;
+}
+
+// Mean (0 for an rms norm) and factor of a row.
+template <int TEAM, bool VEC>
+__device__ __forceinline__ void row_stats(Team<TEAM> &team, const Cols<VEC> &c, const float (&v)[kElems], int kind,
+                                          float eps, float &mean, float &rho) {
+    const float inv = 1.0f / static_cast<float>(c.D);
+    mean = 0.0f;
+    if (kind == PLE_NORM_LAYER) {
+        float t = 0.0f;
+#pragma unroll
+        for (int e = 0; e < kElems; ++e) t += v[e];      // (elements past the row are 0)
+        mean = team.sum(t) * inv;
+    }
+    float t = 0.0f;
+#pragma unroll
+    for (int e = 0; e < kElems; ++e) {
+        const float d = c.on(e) ? v[e] - mean : 0.0f;
+        t += d * d;
+    }
+    rho = rsqrtf(team.sum(t) * inv + eps);
+}
+
+template <int R, int Y, int TEAM, bool VEC>
+__global__ __launch_bounds__(Team<TEAM>::kThreads) void ple_norm_forward_kernel(NormArgs a) {
+    __shared__ float s_sum[Team<TEAM>::kLdsFloats];
+    Team<TEAM> team(s_sum);
+    const Cols<VEC> c(team.lane(), team.lanes(), a.D);
+    float pw[kElems], pb[kElems], nw[kElems], nb[kElems], h[kElems];
+    c.load_param(a.post_w, 0, a.param_dtype, 1.0f, pw);
+    c.load_param(a.post_b, 0, a.param_dtype, 0.0f, pb);
+    c.load_param(a.pre_w, 0, a.param_dtype, 1.0f, nw);
+    c.load_param(a.pre_b, 0, a.param_dtype, 0.0f, nb);
+    c.load_param(a.gates == 1 ? a.gate : nullptr, 0, a.param_dtype, 1.0f, h);
+    if (a.gates == 1)
+#pragma unroll
+        for (int e = 0; e < kElems; ++e) h[e] = gate_value(h[e], a.act);
+    const int64_t teams = static_cast<int64_t>(gridDim.x) * team.per_block();
+    for (int64_t n = static_cast<int64_t>(blockIdx.x) * team.per_block() + team.index(); n < a.N; n += teams) {
+        float4 st = make_float4(0.0f, 1.0f, 0.0f, 1.0f);
+        float s[kElems], v[kElems];
+        c.template load<R>(a.residual, n, s);
+        if (a.branch) {
+            c.template load<Y>(a.branch, n, v);
+            if (a.post != PLE_NORM_NONE) {
+                row_stats(team, c, v, a.post, a.eps, st.x, st.y);
+#pragma unroll
+                for (int e = 0; e < kElems; ++e) v[e] = (v[e] - st.x) * st.y * pw[e] + pb[e];
+            }
+            if (a.gates > 1) {
+                c.load_param(a.gate, n / a.rows_per_gate, a.param_dtype, 1.0f, h);
+#pragma unroll
+                for (int e = 0; e < kElems; ++e) h[e] = gate_value(h[e], a.act);
+            }
+#pragma unroll
+            for (int e = 0; e < kElems; ++e) s[e] = c.on(e) ? quant<R>(a.alpha * s[e] + h[e] * v[e]) : 0.0f;
+            c.template store<R>(a.stream_out, n, s);
+        }
+        if (a.pre != PLE_NORM_NONE) {
+            row_stats(team, c, s, a.pre, a.eps, st.z, st.w);
+#pragma unroll
+            for (int e = 0; e < kElems; ++e) v[e] = (s[e] - st.z) * st.w * nw[e] + nb[e];
+            c.template store<Y>(a.normed, n, v);
+        }
+        if (team.lane() == 0) a.stats[n] = st;
+    }
+}
+
+// d of a norm's input from d of its output (times its weight), in place.
+template <int TEAM, bool VEC>
+__device__ __forceinline__ void norm_grad(Team<TEAM> &team, const Cols<VEC> &c, float (&g)[kElems],
+                                          const float (&xh)[kElems], float rho, int kind) {
+    float proj = 0.0f, mean = 0.0f;
+#pragma unroll
+    for (int e = 0; e < kElems; ++e) {
+        proj += g[e] * xh[e];
+        mean += g[e];
+    }
+    team.sum2(proj, mean);
+    const float inv = 1.0f / static_cast<float>(c.D);
+    proj *= inv;
+    mean = kind == PLE_NORM_LAYER ? mean * inv : 0.0f;
+#pragma unroll
+    for (int e = 0; e < kElems; ++e) g[e] = rho * (g[e] - mean - xh[e] * proj);
+}
+
+template <int R, int Y, int TEAM, bool VEC>
+__global__ __launch_bounds__(Team<TEAM>::kThreads) void ple_norm_backward_kernel(NormArgs a) {
+    constexpr int kTeams = Team<TEAM>::kBlockWide ? 1 : kBlock / TEAM;
+    __shared__ float s_sum[Team<TEAM>::kLdsFloats];
+    __shared__ float s_cols[kTeams > 1 ? kBlock * kElems : 1];
+    Team<TEAM> team(s_sum);
+    const Cols<VEC> c(team.lane(), team.lanes(), a.D);
+    float pw[kElems], pb[kElems], nw[kElems], h[kElems];
+    c.load_param(a.post_w, 0, a.param_dtype, 1.0f, pw);
+    c.load_param(a.post_b, 0, a.param_dtype, 0.0f, pb);
+    c.load_param(a.pre_w, 0, a.param_dtype, 1.0f, nw);
+    c.load_param(a.gates == 1 ? a.gate : nullptr, 0, a.param_dtype, 1.0f, h);
+    if (a.gates == 1)
+#pragma unroll
+        for (int e = 0; e < kElems; ++e) h[e] = gate_value(h[e], a.act);
+    float s_pw[kElems] = {}, s_pb[kElems] = {}, s_g[kElems] = {}, s_nw[kElems] = {}, s_nb[kElems] = {};
+    const int64_t teams = static_cast<int64_t>(gridDim.x) * team.per_block();
+    const int64_t units = a.gates == 2 ? (a.N / a.rows_per_gate) * a.pieces : a.N;
+    for (int64_t u = static_cast<int64_t>(blockIdx.x) * team.per_block() + team.index(); u < units; u += teams) {
+        int64_t row = u, stop = u + 1;
+        if (a.gates == 2) {
+            const int64_t group = u / a.pieces, piece = u - group * a.pieces;
+            row = group * a.rows_per_gate + piece * a.piece_rows;
+            stop = min(row + a.piece_rows, (group + 1) * a.rows_per_gate);
+            c.load_param(a.gate, group, a.param_dtype, 1.0f, h);
+        } else if (a.gates == 3) {
+            c.load_param(a.gate, u, a.param_dtype, 1.0f, h);
+        }
+        if (a.gates > 1)
+#pragma unroll
+            for (int e = 0; e < kElems; ++e) {
+                h[e] = gate_value(h[e], a.act);
+                s_g[e] = 0.0f;
+            }
+        for (int64_t n = row; n < stop; ++n) {
+            const float4 st = a.stats[n];
+            float ds[kElems] = {}, xh[kElems], g[kElems];
+            if (a.g_stream) c.template load<R>(a.g_stream, n, ds);
+            if (a.g_normed) {
+                c.template load<Y>(a.g_normed, n, g);
+                c.template load<R>(a.residual, n, xh);
+#pragma unroll
+                for (int e = 0; e < kElems; ++e) {
+                    xh[e] = c.on(e) ? (xh[e] - st.z) * st.w : 0.0f;
+                    s_nw[e] += g[e] * xh[e];
+                    s_nb[e] += g[e];
+                    g[e] *= nw[e];
+                }
+                norm_grad(team, c, g, xh, st.w, a.pre);
+#pragma unroll
+                for (int e = 0; e < kElems; ++e) ds[e] += g[e];
+            }
+            if (a.d_residual) {
+#pragma unroll
+                for (int e = 0; e < kElems; ++e) g[e] = a.alpha * ds[e];
+                c.template store<R>(a.d_residual, n, g);
+            }
+            if (!a.branch) continue;
+            c.template load<Y>(a.branch, n, xh);
+            if (a.post != PLE_NORM_NONE) {
+#pragma unroll
+                for (int e = 0; e < kElems; ++e) {
+                    xh[e] = c.on(e) ? (xh[e] - st.x) * st.y : 0.0f;
+                    g[e] = c.on(e) ? ds[e] * h[e] : 0.0f;
+                    s_g[e] += ds[e] * (xh[e] * pw[e] + pb[e]);
+                    s_pw[e] += g[e] * xh[e];
+                    s_pb[e] += g[e];
+                    g[e] *= pw[e];
+                }
+                norm_grad(team, c, g, xh, st.y, a.post);
+            } else {
+#pragma unroll
+                for (int e = 0; e < kElems; ++e) {
+                    g[e] = ds[e] * h[e];
+                    s_g[e] += ds[e] * xh[e];
+                }
+            }
+            if (a.d_branch) c.template store<Y>(a.d_branch, n, g);
+        }
+        if (a.gates > 1 && a.d_gate) {
+#pragma unroll
+            for (int e = 0; e < kElems; ++e) {
+                if (!c.on(e)) continue;
+                const float v = s_g[e] * gate_slope(h[e], a.act);
+                if (a.gates == 3 || a.pieces == 1) store_any(a.d_gate, u * a.D + c.at(e), v, a.param_dtype);
+                else a.gate_partial[u * a.D + c.at(e)] = v;
+            }
+        }
+    }
+    if (a.gates == 1)
+#pragma unroll
+        for (int e = 0; e < kElems; ++e) s_g[e] *= gate_slope(h[e], a.act);
+    const auto leave = [&](float (&v)[kElems], int slot) {
+        if (slot < 0) return;
+        if constexpr (kTeams > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < kElems; ++e) s_cols[e * kBlock + threadIdx.x] = v[e];
+            __syncthreads();
+            if (team.index() == 0)
+                for (int t = 1; t < kTeams; ++t)
+#pragma unroll
+                    for (int e = 0; e < kElems; ++e) v[e] += s_cols[e * kBlock + t * TEAM + team.lane()];
+        }
+        if (team.index() == 0)
+            c.template store<PLE_DTYPE_F32>(a.partial, static_cast<int64_t>(blockIdx.x) * a.slots + slot, v);
+    };
+    leave(s_pw, a.slot_pw);
+    leave(s_pb, a.slot_pb);
+    leave(s_g, a.slot_g);
+    leave(s_nw, a.slot_nw);
+    leave(s_nb, a.slot_nb);
+}
+
+// out[j, d] = sum over the parts of partial[part, j, d]; 64 columns a workgroup,
+// its waves taking every fourth part each.
+constexpr int kMaxSums = 5;
+
+struct JoinArgs {
+    const float *partial;
+    void *out[kMaxSums];         // stacked: out[0] is [sums, D], else one vector a sum
+    int64_t part_stride, sum_stride;
+    int parts, D, param_dtype, stacked, colblocks;
+};
+
+__global__ __launch_bounds__(kBlock) void ple_norm_join_kernel(JoinArgs a) {
+    __shared__ float s_sum[kBlock];
+    const int wave = threadIdx.x / kWave, d = blockIdx.x % a.colblocks * kWave + threadIdx.x % kWave;
+    const int64_t j = blockIdx.x / a.colblocks;
+    float v = 0.0f;
+    if (d < a.D) {
+#pragma unroll 8
+        for (int p = wave; p < a.parts; p += kWavesPerBlock) v += a.partial[p * a.part_stride + j * a.sum_stride + d];
+    }
+    s_sum[threadIdx.x] = v;
+    __syncthreads();
+    if (wave == 0 && d < a.D) {
+        for (int w = 1; w < kWavesPerBlock; ++w) v += s_sum[w * kWave + threadIdx.x];
+        if (a.stacked) store_any(a.out[0], j * a.D + d, v, a.param_dtype);
+        else store_any(a.out[j], d, v, a.param_dtype);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// plans and launches
+// ---------------------------------------------------------------------------
+
+struct NormPlan {
+    int team, threads, per_block, vec;
+    int blocks;                          // backward workgroups
+    int64_t piece_rows, pieces;
+    int slots;
+    size_t o_gate, bytes;
+};
+
+int gate_mode(const NormRequest &r) {
+    if (!r.gate) return 0;
+    return r.groups == 1 ? 1 : (r.groups == r.N ? 3 : 2);
+}
+
+NormPlan plan_norm(const NormRequest &r) {
+    NormPlan p{};
+    if (r.N == 0) return p;
+    const int lanes = static_cast<int>((r.D + kElems - 1) / kElems);
+    p.team = lanes <= 8 ? 8 : (lanes <= 16 ? 16 : (lanes <= 32 ? 32 : (lanes <= 64 ? 64 : (lanes <= 512 ? 512 : 1024))));
+    p.threads = p.team > kWave ? (lanes + kWave - 1) / kWave * kWave : kBlock;
+    p.per_block = p.team > kWave ? 1 : kBlock / p.team;
+    p.vec = r.D % kElems == 0;
+    for (const void *q : {r.residual, r.branch, r.g_stream, r.g_normed, static_cast<const void *>(r.stream_out),
+                          static_cast<const void *>(r.normed), static_cast<const void *>(r.d_residual),
+                          static_cast<const void *>(r.d_branch)})
+        p.vec = p.vec && reinterpret_cast<uintptr_t>(q) % 16 == 0;
+    const int mode = gate_mode(r);
+    const int most = device_cu_count() * std::max(1, 1024 / p.threads);
+    const int64_t teams = static_cast<int64_t>(most) * p.per_block;
+    int64_t units = r.N;
+    p.piece_rows = p.pieces = 1;
+    if (mode == 2) {
+        const int64_t rows = r.N / r.groups;
+        p.piece_rows = std::min(rows, std::max<int64_t>(4, (r.N + 4 * teams - 1) / (4 * teams)));
+        p.pieces = (rows + p.piece_rows - 1) / p.piece_rows;
+        units = r.groups * p.pieces;
+    }
+    p.blocks = static_cast<int>(std::min<int64_t>(most, std::max<int64_t>(1, (units + p.per_block - 1) / p.per_block)));
+    p.slots = (r.post_w != nullptr) + (r.post_b != nullptr) + (mode == 1) + (r.pre_w != nullptr) + (r.pre_b != nullptr);
+    p.o_gate = align_up(static_cast<size_t>(p.blocks) * p.slots * r.D * 4, 256);
+    p.bytes = p.o_gate + (mode == 2 && p.pieces > 1 ? align_up(static_cast<size_t>(units) * r.D * 4, 256) : 0);
+    return p;
+}
+
+NormArgs norm_args(const NormRequest &r) {
+    NormArgs a{};
+    a.residual = r.residual; a.branch = r.branch;
+    a.post_w = r.post_w; a.post_b = r.post_b; a.gate = r.gate; a.pre_w = r.pre_w; a.pre_b = r.pre_b;
+    a.stream_out = r.stream_out; a.normed = r.normed;
+    a.stats = reinterpret_cast<float4 *>(r.stats);
+    a.g_stream = r.g_stream; a.g_normed = r.g_normed;
+    a.d_residual = r.d_residual; a.d_branch = r.d_branch; a.d_gate = r.d_gate;
+    a.N = r.N; a.D = static_cast<int>(r.D);
+    a.gates = gate_mode(r);
+    a.rows_per_gate = a.gates ? r.N / r.groups : r.N;
+    a.param_dtype = r.param_dtype;
+    a.post = r.post; a.pre = r.pre; a.act = r.act;
+    a.alpha = r.alpha; a.eps = r.eps;
+    return a;
+}
+
+// f(stream type, branch type, team, vectors) as compile-time constants
+template <typename F>
+hipError_t with_norm(const NormRequest &r, const NormPlan &p, F f) {
+    const auto by_vec = [&](auto st, auto br, auto team) {
+        return p.vec ? f(st, br, team, std::true_type{}) : f(st, br, team, std::false_type{});
+    };
+    const auto by_team = [&](auto st, auto br) {
+        switch (p.team) {
+            case 8: return by_vec(st, br, std::integral_constant<int, 8>{});
+            case 16: return by_vec(st, br, std::integral_constant<int, 16>{});
+            case 32: return by_vec(st, br, std::integral_constant<int, 32>{});
+            case 64: return by_vec(st, br, std::integral_constant<int, 64>{});
+            case 512: return by_vec(st, br, std::integral_constant<int, 512>{});
+            default: return by_vec(st, br, std::integral_constant<int, 1024>{});
+        }
+    };
+    using F32 = std::integral_constant<int, PLE_DTYPE_F32>;
+    using F16 = std::integral_constant<int, PLE_DTYPE_F16>;
+    using BF16 = std::integral_constant<int, PLE_DTYPE_BF16>;
+    if (r.stream_dtype == PLE_DTYPE_BF16) return by_team(BF16{}, BF16{});
+    if (r.stream_dtype == PLE_DTYPE_F16) return by_team(F16{}, F16{});
+    if (r.branch_dtype == PLE_DTYPE_BF16) return by_team(F32{}, BF16{});
+    if (r.branch_dtype == PLE_DTYPE_F16) return by_team(F32{}, F16{});
+    return by_team(F32{}, F32{});
+}
+
+// An empty batch: the parameters' gradients are 0.
+int norm_zero_gradients(const NormRequest &r) {
+    JoinArgs j{};
+    j.D = static_cast<int>(r.D);
+    j.param_dtype = r.param_dtype;
+    j.colblocks = (j.D + kWave - 1) / kWave;
+    int sums = 0;
+    for (void *p : {r.d_post_w, r.d_post_b, r.d_pre_w, r.d_pre_b})
+        if (p) j.out[sums++] = p;
+    if (sums > 0) hipLaunchKernelGGL(ple_norm_join_kernel, dim3(j.colblocks * sums), dim3(kBlock), 0, r.stream, j);
+    if (r.d_gate) {
+        j.out[0] = r.d_gate;
+        j.stacked = 1;
+        hipLaunchKernelGGL(ple_norm_join_kernel, dim3(static_cast<unsigned>(j.colblocks * r.groups)), dim3(kBlock), 0,
+                           r.stream, j);
+    }
+    return static_cast<int>(hipGetLastError());
+}
+
+}  // namespace
+
+int norm_run(const NormRequest &r) {
+    if (r.D > kMaxD) return PLE_E_TOO_LARGE;
+    const NormPlan p = plan_norm(r);
+    const NormArgs a = norm_args(r);
+    const int64_t most = static_cast<int64_t>(device_cu_count()) * std::max(1, 2048 / p.threads);
+    const dim3 grid(static_cast<unsigned>(std::min(most, (r.N + p.per_block - 1) / p.per_block)));
+    return static_cast<int>(with_norm(r, p, [&](auto st, auto br, auto team, auto vec) {
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_norm_forward_kernel<decltype(st)::value, decltype(br)::value,
+                                                                   decltype(team)::value, decltype(vec)::value>),
+                           grid, dim3(p.threads), 0, r.stream, a);
+        return hipGetLastError();
+    }));
+}
+
+size_t norm_backward_workspace_bytes(const NormRequest &r) { return r.D > kMaxD ? 0 : plan_norm(r).bytes; }
+
+int norm_backward_run(const NormRequest &r) {
+    if (r.D > kMaxD) return PLE_E_TOO_LARGE;
+    const NormPlan p = plan_norm(r);
+    if (r.N == 0) return norm_zero_gradients(r);
+    if (p.bytes > 0 && (!r.workspace || r.workspace_bytes < p.bytes || reinterpret_cast<uintptr_t>(r.workspace) % 256 != 0))
+        return PLE_E_WORKSPACE;
+    NormArgs a = norm_args(r);
+    a.piece_rows = p.piece_rows;
+    a.pieces = p.pieces;
+    a.partial = static_cast<float *>(r.workspace);
+    a.gate_partial = reinterpret_cast<float *>(static_cast<char *>(r.workspace) + p.o_gate);
+    JoinArgs j{};
+    const auto slot = [&](const void *param, void *grad) {
+        if (!param || !grad) return -1;
+        j.out[a.slots] = grad;
+        return a.slots++;
+    };
+    a.slot_pw = slot(r.post_w, r.d_post_w);
+    a.slot_pb = slot(r.post_b, r.d_post_b);
+    a.slot_g = slot(a.gates == 1 ? r.gate : nullptr, r.d_gate);
+    a.slot_nw = slot(r.pre_w, r.d_pre_w);
+    a.slot_nb = slot(r.pre_b, r.d_pre_b);
+    const hipError_t rc = with_norm(r, p, [&](auto st, auto br, auto team, auto vec) {
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_norm_backward_kernel<decltype(st)::value, decltype(br)::value,
+                                                                    decltype(team)::value, decltype(vec)::value>),
+                           dim3(p.blocks), dim3(p.threads), 0, r.stream, a);
+        return hipGetLastError();
+    });
+    if (rc != hipSuccess) return static_cast<int>(rc);
+    j.D = a.D;
+    j.param_dtype = a.param_dtype;
+    j.colblocks = (a.D + kWave - 1) / kWave;
+    if (a.slots > 0) {
+        j.partial = a.partial;
+        j.part_stride = static_cast<int64_t>(a.slots) * a.D;
+        j.sum_stride = a.D;
+        j.parts = p.blocks;
+        hipLaunchKernelGGL(ple_norm_join_kernel, dim3(j.colblocks * a.slots), dim3(kBlock), 0, r.stream, j);
+    }
+    if (a.gates == 2 && a.d_gate && p.pieces > 1) {
+        j.partial = a.gate_partial;
+        j.part_stride = a.D;
+        j.sum_stride = p.pieces * a.D;
+        j.parts = static_cast<int>(p.pieces);
+        j.out[0] = r.d_gate;
+        j.stacked = 1;
+        hipLaunchKernelGGL(ple_norm_join_kernel, dim3(static_cast<unsigned>(j.colblocks * r.groups)), dim3(kBlock), 0,
+                           r.stream, j);
+    }
+    return static_cast<int>(hipGetLastError());
+}
+
+}  // namespace ple

@@ -1,0 +1,99 @@
+// Device-side helpers of the row operators (lookup, residual norm,
+// distillation loss): element vectors of any of the three types, parameters
+// whose type is known at run time, and sums over the lanes that share a row.
+#pragma once
+
+#include "ple_device.h"
+
+namespace ple {
+
+__host__ __device__ constexpr int elem_bytes(int dtype) { return dtype == PLE_DTYPE_F32 ? 4 : 2; }
+
+// VEC consecutive elements of type T from element i (aligned for the access:
+// VEC elements, 16 bytes at most), as floats.  VEC in {1, 2, 4, 8}.
+template <int T, int VEC>
+__device__ __forceinline__ void load_vec(const void *p, int64_t i, float *v) {
+    load_grad_vec<T, VEC>(p, i, v);
+}
+
+// VEC consecutive floats rounded to type T and stored from element i.  NT: past
+// the caches.
+template <int T, int VEC, bool NT = false>
+__device__ __forceinline__ void store_vec(void *p, int64_t i, const float *v) {
+    if constexpr (T == PLE_DTYPE_F32 && VEC == 8) {
+        store_out<T, 4, NT>(p, i, v);
+        store_out<T, 4, NT>(p, i + 4, v + 4);
+    } else {
+        store_out<T, VEC, NT>(p, i, v);
+    }
+}
+
+// One element of a type known at run time (the same for the whole launch).
+__device__ __forceinline__ float load_any(const void *p, int64_t i, int dtype) {
+    if (dtype == PLE_DTYPE_F32) return static_cast<const float *>(p)[i];
+    const uint16_t h = static_cast<const uint16_t *>(p)[i];
+    return dtype == PLE_DTYPE_BF16 ? bf16_to_float(h) : f16_to_float(h);
+}
+
+__device__ __forceinline__ void store_any(void *p, int64_t i, float v, int dtype) {
+    if (dtype == PLE_DTYPE_F32) static_cast<float *>(p)[i] = v;
+    else static_cast<uint16_t *>(p)[i] = dtype == PLE_DTYPE_BF16 ? bf16_bits(v) : f16_bits(v);
+}
+
+// The lanes that share a row.  TEAM: 8, 16, 32 or 64 lanes inside a wave, or
+// (more than 64) a workgroup of at most that many threads.
+template <int TEAM>
+struct Team {
+    static constexpr bool kBlockWide = TEAM > kWave;
+    static constexpr int kThreads = kBlockWide ? TEAM : kBlock;
+    static constexpr int kLdsFloats = kBlockWide ? 4 * TEAM / kWave : 1;
+    float *lds;                  // kLdsFloats floats
+    int turn = 0;
+    __device__ __forceinline__ explicit Team(float *s) : lds(s) {}
+    __device__ __forceinline__ int lane() const { return kBlockWide ? threadIdx.x : threadIdx.x % TEAM; }
+    __device__ __forceinline__ int lanes() const { return kBlockWide ? blockDim.x : TEAM; }
+    __device__ __forceinline__ int index() const { return kBlockWide ? 0 : threadIdx.x / TEAM; }
+    __device__ __forceinline__ int per_block() const { return kBlockWide ? 1 : kBlock / TEAM; }
+
+    // sums of two values over the team's lanes, to all of them
+    __device__ __forceinline__ void sum2(float &a, float &b) {
+        if constexpr (!kBlockWide) {
+            a = group_sum<TEAM>(a);
+            b = group_sum<TEAM>(b);
+        } else {
+            a = group_sum<kWave>(a);
+            b = group_sum<kWave>(b);
+            // (two buffers in turn: a wave can be one sum ahead of another)
+            float2 *buf = reinterpret_cast<float2 *>(lds) + (turn ^= 1) * (TEAM / kWave);
+            const int waves = blockDim.x / kWave;
+            if (threadIdx.x % kWave == 0) buf[threadIdx.x / kWave] = make_float2(a, b);
+            __syncthreads();
+            a = b = 0.0f;
+            for (int w = 0; w < waves; ++w) {
+                const float2 v = buf[w];
+                a += v.x;
+                b += v.y;
+            }
+        }
+    }
+    __device__ __forceinline__ float sum(float a) {
+        float b = 0.0f;
+        sum2(a, b);
+        return a;
+    }
+    // maximum over the team's lanes (NaN is passed over), to all of them
+    __device__ __forceinline__ float max(float a) {
+#pragma unroll
+        for (int o = (kBlockWide ? kWave : TEAM) / 2; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor(a, o));
+        if constexpr (kBlockWide) {
+            float2 *buf = reinterpret_cast<float2 *>(lds) + (turn ^= 1) * (TEAM / kWave);
+            const int waves = blockDim.x / kWave;
+            if (threadIdx.x % kWave == 0) buf[threadIdx.x / kWave].x = a;
+            __syncthreads();
+            for (int w = 0; w < waves; ++w) a = fmaxf(a, buf[w].x);
+        }
+        return a;
+    }
+};
+
+}  // namespace ple
