@@ -24,9 +24,16 @@ namespace {
 
 constexpr int kSortBlock = 512;
 constexpr int kSortWaves = kSortBlock / kWave;
+constexpr int kSortRounds = 4;         // tokens a lane ranks at a time
+constexpr int kSortStep = kSortBlock * kSortRounds;
 constexpr int kMaxDigitBits = 10;
 constexpr int kMaxTiles = 256;
-constexpr int kMinTile = 1024;         // tokens a sorting workgroup takes at least
+// One workgroup sorts up to this many tokens by itself, in LDS: its 16 waves
+// hold up to 8 of them a lane.
+constexpr int kLocalBlock = 1024;
+constexpr int kLocalWaves = kLocalBlock / kWave;
+constexpr int kLocalRounds = 8;
+constexpr int64_t kLocalTokens = kLocalBlock * kLocalRounds;
 
 struct TokenArgs {
     const void *tokens;
@@ -74,30 +81,37 @@ struct GatherArgs {
 
 constexpr int kGatherUnroll = 4;
 
-template <int W, int O, int VEC>
+// A group of lanes has kGatherUnroll vectors in flight: of one token's row
+// where it is long enough, else of as many tokens' rows (TOKENS).
+template <int W, int O, int VEC, bool TOKENS>
 __global__ __launch_bounds__(kBlock) void ple_lookup_kernel(GatherArgs a) {
     const int lanes = 1 << a.lg;
-    const int64_t i = (static_cast<int64_t>(blockIdx.x) << (8 - a.lg)) + (threadIdx.x >> a.lg);
-    if (i >= a.t.T) return;
-    const int64_t row = token_row(a.t, static_cast<uint32_t>(i));
-    const int64_t col0 = (static_cast<int64_t>(blockIdx.y) * kGatherUnroll * lanes + (threadIdx.x & (lanes - 1))) * VEC;
+    const int64_t per_block = kBlock >> a.lg;
+    const int64_t i0 = static_cast<int64_t>(blockIdx.x) * per_block * (TOKENS ? kGatherUnroll : 1) + (threadIdx.x >> a.lg);
+    const int64_t col0 = (static_cast<int64_t>(blockIdx.y) * (TOKENS ? 1 : kGatherUnroll) * lanes +
+                          (threadIdx.x & (lanes - 1))) * VEC;
+    const auto token = [&](int u) { return i0 + (TOKENS ? u * per_block : 0); };
+    const auto column = [&](int u) { return col0 + (TOKENS ? 0 : static_cast<int64_t>(u) * lanes * VEC); };
+    int64_t row[kGatherUnroll];
+#pragma unroll
+    for (int u = 0; u < kGatherUnroll; ++u)
+        row[u] = TOKENS || u == 0 ? (token(u) < a.t.T ? token_row(a.t, static_cast<uint32_t>(token(u))) : kMissing) : row[0];
     float v[kGatherUnroll][VEC];
 #pragma unroll
     for (int u = 0; u < kGatherUnroll; ++u) {
-        const int64_t col = col0 + static_cast<int64_t>(u) * lanes * VEC;
-        if (row >= 0 && col < a.D) {
-            load_vec<W, VEC>(a.weight, row * a.D + col, v[u]);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) v[u][e] *= a.scale;
+        if (row[u] >= 0 && column(u) < a.D) {
+            load_vec<W, VEC>(a.weight, row[u] * a.D + column(u), v[u]);
         } else {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) v[u][e] = row == kBeyond ? __builtin_nanf("") : 0.0f;
+            for (int e = 0; e < VEC; ++e) v[u][e] = row[u] == kBeyond ? __builtin_nanf("") : 0.0f;
         }
     }
 #pragma unroll
     for (int u = 0; u < kGatherUnroll; ++u) {
-        const int64_t col = col0 + static_cast<int64_t>(u) * lanes * VEC;
-        if (col < a.D) store_vec<O, VEC>(a.out, i * a.D + col, v[u]);
+        if (token(u) >= a.t.T || column(u) >= a.D) continue;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[u][e] *= a.scale;
+        store_vec<O, VEC, true>(a.out, token(u) * a.D + column(u), v[u]);
     }
 }
 
@@ -112,7 +126,7 @@ struct SortArgs {
     uint32_t *counts;                    // [tiles, 1 << bits]
     uint8_t *present;                    // [V]: rows that have tokens
     uint32_t tile;                       // tokens a workgroup takes
-    int tiles, shift, bits;
+    int tiles, shift, bits, passes;
 };
 
 template <bool FIRST>
@@ -121,62 +135,42 @@ __device__ __forceinline__ uint32_t sort_key(const SortArgs &a, uint32_t i) {
     else return a.keys_in[i];
 }
 
-template <bool FIRST>
-__global__ __launch_bounds__(kSortBlock) void ple_lookup_count_kernel(SortArgs a) {
-    __shared__ uint32_t hist[1 << kMaxDigitBits];
-    const uint32_t digits = 1u << a.bits;
-    for (uint32_t d = threadIdx.x; d < digits; d += kSortBlock) hist[d] = 0;
-    if constexpr (FIRST)
-        for (int64_t r = static_cast<int64_t>(blockIdx.x) * kSortBlock + threadIdx.x; r < a.t.V;
-             r += static_cast<int64_t>(gridDim.x) * kSortBlock)
-            a.present[r] = 0;
-    __syncthreads();
-    const uint64_t begin = static_cast<uint64_t>(blockIdx.x) * a.tile;
-    const uint64_t end = begin + a.tile < a.t.T ? begin + a.tile : a.t.T;
-    for (uint64_t i = begin + threadIdx.x; i < end; i += kSortBlock)
-        atomicAdd(&hist[(sort_key<FIRST>(a, static_cast<uint32_t>(i)) >> a.shift) & (digits - 1)], 1u);
-    __syncthreads();
-    for (uint32_t d = threadIdx.x; d < digits; d += kSortBlock)
-        a.counts[static_cast<size_t>(blockIdx.x) * digits + d] = hist[d];
+// The lanes of the wave that are `on` and have this lane's digit, of at most
+// BITS bits: a ballot for each bit, whose mask or its complement every lane
+// keeps by its own bit.  (Bits above the digit are 0 for all and keep all.)
+template <int BITS>
+__device__ __forceinline__ uint64_t same_digit(uint32_t digit, bool on) {
+    const uint64_t all = __ballot(on);
+    uint32_t lo = static_cast<uint32_t>(all), hi = static_cast<uint32_t>(all >> 32);
+#pragma unroll
+    for (int b = 0; b < BITS; ++b) {
+        const uint32_t mine = static_cast<uint32_t>(static_cast<int32_t>(digit << (31 - b)) >> 31);   // all ones: bit set
+        const uint64_t set = __ballot(mine != 0);
+        lo &= ~(static_cast<uint32_t>(set) ^ mine);
+        hi &= ~(static_cast<uint32_t>(set >> 32) ^ mine);
+    }
+    return (static_cast<uint64_t>(hi) << 32) | lo;
 }
 
-// Each wave takes a contiguous part of the workgroup's tile, 64 tokens at a
-// time: the lanes with the same digit find each other by ballots, and their
-// places are the wave's running offset of that digit plus their rank.
-template <bool FIRST, bool LAST>
-__global__ __launch_bounds__(kSortBlock) void ple_lookup_scatter_kernel(SortArgs a) {
-    extern __shared__ uint32_t s_off[];      // [kSortWaves][digits]
-    __shared__ uint32_t s_wave[kSortWaves];
-    const uint32_t digits = 1u << a.bits;
-    const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
-    for (uint32_t d = tid; d < kSortWaves * digits; d += kSortBlock) s_off[d] = 0;
-    __syncthreads();
-    const uint64_t begin = static_cast<uint64_t>(blockIdx.x) * a.tile;
-    const uint64_t end = begin + a.tile < a.t.T ? begin + a.tile : a.t.T;
-    const uint32_t part = a.tile / kSortWaves;      // (a multiple of 64)
-    const uint64_t w0 = begin + static_cast<uint64_t>(wave) * part;
-    const uint64_t w1 = w0 + part < end ? w0 + part : end;
-    uint32_t *mine = s_off + wave * digits;
-    for (uint64_t i = w0 + lane; i < w1; i += kWave)
-        atomicAdd(&mine[(sort_key<FIRST>(a, static_cast<uint32_t>(i)) >> a.shift) & (digits - 1)], 1u);
+// Rank of this lane's token among the wave's tokens of its digit so far, whose
+// number `seen` holds (in LDS, the wave's own).
+template <int BITS, typename Count>
+__device__ __forceinline__ uint32_t rank_token(volatile Count *seen, uint32_t digit, bool on) {
+    const uint32_t prior = seen[digit];
+    const uint64_t same = same_digit<BITS>(digit, on);
+    const uint32_t below = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(same >> 32),
+                                                     __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(same), 0));
+    __builtin_amdgcn_wave_barrier();
+    if (on && below == 0) seen[digit] = static_cast<Count>(prior + __popcll(same));
+    __builtin_amdgcn_wave_barrier();
+    return prior + below;
+}
 
-    // the digits of this thread: `per` adjacent ones
-    const uint32_t per = digits > kSortBlock ? digits / kSortBlock : 1;
-    uint32_t before[4] = {0, 0, 0, 0}, total[4] = {0, 0, 0, 0}, sum = 0;
-    if (tid * per < digits) {
-        for (int t = 0; t < a.tiles; ++t)
-#pragma unroll
-            for (uint32_t k = 0; k < 4; ++k)
-                if (k < per) {
-                    const uint32_t c = a.counts[static_cast<size_t>(t) * digits + tid * per + k];
-                    total[k] += c;
-                    if (t < static_cast<int>(blockIdx.x)) before[k] += c;
-                }
-#pragma unroll
-        for (uint32_t k = 0; k < 4; ++k) sum += total[k];
-    }
-    // tokens of smaller digits: exclusive sum over the threads
-    uint32_t incl = sum;
+// Exclusive sums over the workgroup's threads of one value each.
+template <int THREADS>
+__device__ __forceinline__ uint32_t exclusive_sum(uint32_t v, uint32_t *s_wave) {
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    uint32_t incl = v;
 #pragma unroll
     for (int o = 1; o < kWave; o <<= 1) {
         const uint32_t up = __shfl_up(incl, o);
@@ -184,47 +178,216 @@ __global__ __launch_bounds__(kSortBlock) void ple_lookup_scatter_kernel(SortArgs
     }
     if (lane == kWave - 1) s_wave[wave] = incl;
     __syncthreads();
-    uint32_t base = incl - sum;
+    uint32_t base = incl - v;
     for (int w = 0; w < wave; ++w) base += s_wave[w];
-    if (tid * per < digits) {
+    return base;
+}
+
+template <bool FIRST>
+__global__ __launch_bounds__(kSortBlock) void ple_lookup_count_kernel(SortArgs a) {
+    __shared__ uint32_t hist[1 << kMaxDigitBits];
+    const uint32_t digits = 1u << a.bits;
+    for (uint32_t d = threadIdx.x; d < digits; d += kSortBlock) hist[d] = 0;
+    if constexpr (FIRST)
+        // (`present` is rounded up to 16 bytes)
+        for (int64_t r = static_cast<int64_t>(blockIdx.x) * kSortBlock + threadIdx.x; r < (a.t.V + 15) / 16;
+             r += static_cast<int64_t>(gridDim.x) * kSortBlock)
+            reinterpret_cast<uint4 *>(a.present)[r] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    const uint64_t begin = static_cast<uint64_t>(blockIdx.x) * a.tile;
+    const uint64_t end = begin + a.tile < a.t.T ? begin + a.tile : a.t.T;
+    for (uint64_t i0 = begin + threadIdx.x; i0 < end; i0 += kSortStep) {
+        uint32_t key[kSortRounds];
 #pragma unroll
-        for (uint32_t k = 0; k < 4; ++k)
-            if (k < per) {
-                uint32_t at = base + before[k];
-                for (int w = 0; w < kSortWaves; ++w) {
-                    uint32_t *p = &s_off[w * digits + tid * per + k];
-                    const uint32_t c = *p;
-                    *p = at;
-                    at += c;
-                }
-                base += total[k];
-            }
+        for (int r = 0; r < kSortRounds; ++r) {
+            const uint64_t i = i0 + r * kSortBlock;
+            key[r] = sort_key<FIRST>(a, static_cast<uint32_t>(i < end ? i : end - 1));
+        }
+#pragma unroll
+        for (int r = 0; r < kSortRounds; ++r)
+            if (i0 + r * kSortBlock < end) atomicAdd(&hist[(key[r] >> a.shift) & (digits - 1)], 1u);
     }
     __syncthreads();
+    for (uint32_t d = threadIdx.x; d < digits; d += kSortBlock)
+        a.counts[static_cast<size_t>(blockIdx.x) * digits + d] = hist[d];
+}
 
-    volatile uint32_t *off = mine;
-    for (uint64_t i0 = w0; i0 < w1; i0 += kWave) {
-        const uint64_t i = i0 + lane;
-        const bool on = i < w1;
-        const uint32_t key = on ? sort_key<FIRST>(a, static_cast<uint32_t>(i)) : 0;
-        const uint32_t digit = (key >> a.shift) & (digits - 1);
-        uint64_t same = __ballot(on);
-        for (int b = 0; b < a.bits; ++b) {
-            const bool bit = (digit >> b) & 1;
-            const uint64_t set = __ballot(bit);
-            same &= bit ? set : ~set;
+// The workgroup's first place of every digit comes from all workgroups' counts
+// (each reads them all, 16 bytes a load and the loads in parallel: a kernel of
+// its own for these sums costs more than the reads up to 256 workgroups).  Then
+// it walks its tokens in steps: each wave takes a contiguous part of a step and
+// ranks its tokens per digit, the waves' numbers give each wave its place.
+template <bool FIRST, bool LAST, int BITS>
+__global__ __launch_bounds__(kSortBlock) void ple_lookup_scatter_kernel(SortArgs a) {
+    extern __shared__ uint32_t s_dyn[];
+    __shared__ uint32_t s_wave[kSortWaves];
+    const uint32_t digits = 1u << a.bits;
+    uint32_t *s_place = s_dyn, *s_total = s_dyn + digits, *s_seen = s_dyn + 2 * digits;   // seen: [waves, digits]
+    const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
+    const uint64_t begin = static_cast<uint64_t>(blockIdx.x) * a.tile;
+    const uint64_t end = begin + a.tile < a.t.T ? begin + a.tile : a.t.T;
+    uint32_t key[kSortRounds], pos[kSortRounds], rank[kSortRounds];
+    uint64_t i0 = begin + wave * (kWave * kSortRounds) + lane;
+    const auto load = [&] {
+#pragma unroll
+        for (int r = 0; r < kSortRounds; ++r) {
+            const uint64_t i = i0 + r * kWave < end ? i0 + r * kWave : end - 1;
+            key[r] = sort_key<FIRST>(a, static_cast<uint32_t>(i));
+            pos[r] = FIRST ? static_cast<uint32_t>(i) : a.pos_in[i];
         }
-        const uint32_t rank = __popcll(same & ((uint64_t{1} << lane) - 1));
-        uint32_t dst = 0;
-        if (on) dst = off[digit] + rank;
-        __builtin_amdgcn_wave_barrier();
-        if (on && rank == 0) off[digit] = dst + __popcll(same);
-        __builtin_amdgcn_wave_barrier();
-        if (on) {
-            a.keys_out[dst] = key;
-            a.pos_out[dst] = FIRST ? static_cast<uint32_t>(i) : a.pos_in[i];
-            if (LAST && key < static_cast<uint64_t>(a.t.V)) a.present[key] = 1;
+    };
+    load();
+    for (uint32_t d = tid; d < (2 + kSortWaves) * digits; d += kSortBlock) s_dyn[d] = 0;
+    __syncthreads();
+    {
+        const uint32_t wide = digits / 4;            // (at least 1: bits >= 2)
+        const uint32_t groups = kSortBlock / wide;
+        const uint32_t group = tid / wide, at = tid % wide;
+        uint32_t before[4] = {0, 0, 0, 0}, total[4] = {0, 0, 0, 0};
+#pragma unroll 8
+        for (uint32_t t = group; t < static_cast<uint32_t>(a.tiles); t += groups) {
+            const uint4 c = reinterpret_cast<const uint4 *>(a.counts)[static_cast<size_t>(t) * wide + at];
+            const uint32_t mine = t < blockIdx.x ? ~0u : 0u;
+            total[0] += c.x; total[1] += c.y; total[2] += c.z; total[3] += c.w;
+            before[0] += c.x & mine; before[1] += c.y & mine; before[2] += c.z & mine; before[3] += c.w & mine;
         }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            atomicAdd(&s_place[4 * at + k], before[k]);
+            atomicAdd(&s_total[4 * at + k], total[k]);
+        }
+    }
+    uint32_t *mine = s_seen + wave * digits;
+    const auto rank_step = [&] {
+#pragma unroll
+        for (int r = 0; r < kSortRounds; ++r)
+            rank[r] = rank_token<BITS, uint32_t>(mine, (key[r] >> a.shift) & (digits - 1), i0 + r * kWave < end);
+    };
+    rank_step();
+    __syncthreads();
+    {
+        constexpr int kPer = (1 << kMaxDigitBits) / kSortBlock;
+        uint32_t total[kPer], sum = 0;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            const uint32_t d = tid * kPer + k;
+            total[k] = d < digits ? s_total[d] : 0;
+            sum += total[k];
+        }
+        uint32_t base = exclusive_sum<kSortBlock>(sum, s_wave);
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            const uint32_t d = tid * kPer + k;
+            if (d < digits) s_place[d] += base;
+            base += total[k];
+        }
+    }
+    for (uint64_t step = begin;;) {
+        __syncthreads();
+        for (uint32_t d = tid; d < digits; d += kSortBlock) {
+            uint32_t at = s_place[d];
+#pragma unroll
+            for (int w = 0; w < kSortWaves; ++w) {
+                const uint32_t c = s_seen[w * digits + d];
+                s_seen[w * digits + d] = at;
+                at += c;
+            }
+            s_place[d] = at;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < kSortRounds; ++r)
+            if (i0 + r * kWave < end) {
+                const uint32_t dst = mine[(key[r] >> a.shift) & (digits - 1)] + rank[r];
+                a.keys_out[dst] = key[r];
+                a.pos_out[dst] = pos[r];
+                if (LAST && key[r] < static_cast<uint64_t>(a.t.V)) a.present[key[r]] = 1;
+            }
+        step += kSortStep;
+        if (step >= end) break;
+        i0 += kSortStep;
+        load();
+        __syncthreads();       // (the places of the step before are used)
+        for (uint32_t d = tid; d < kSortWaves * digits; d += kSortBlock) s_seen[d] = 0;
+        __syncthreads();
+        rank_step();
+    }
+}
+
+// All passes for up to kLocalTokens tokens in one workgroup: keys and positions
+// go through LDS between the passes, ranks as above.
+template <int ROUNDS, int BITS>
+__global__ __launch_bounds__(kLocalBlock) void ple_lookup_sort_kernel(SortArgs a) {
+    extern __shared__ uint32_t s_dyn[];
+    __shared__ uint32_t s_wave[kLocalWaves];
+    const uint32_t digits = 1u << a.bits, T = a.t.T;
+    uint32_t *s_key = s_dyn;                                             // [rounded T]
+    const uint32_t room = (T + kLocalBlock - 1) / kLocalBlock * kLocalBlock;
+    uint16_t *s_pos = reinterpret_cast<uint16_t *>(s_key + room);        // [rounded T]
+    uint16_t *s_seen = s_pos + room;                                     // [waves, digits]
+    const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
+    const int rounds = static_cast<int>(room / kLocalBlock);             // (at most ROUNDS)
+    const uint32_t i0 = wave * rounds * kWave + lane;
+    uint32_t key[ROUNDS], pos[ROUNDS];
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r)
+        if (r < rounds) {
+            const uint32_t i = i0 + r * kWave < T ? i0 + r * kWave : T - 1;
+            key[r] = token_key(a.t, i);
+            pos[r] = i;
+        }
+    // (`present` is rounded up to 16 bytes)
+    for (int64_t r = tid; r < (a.t.V + 15) / 16; r += kLocalBlock) reinterpret_cast<uint4 *>(a.present)[r] = make_uint4(0, 0, 0, 0);
+    uint16_t *mine = s_seen + wave * digits;
+    for (int pass = 0; pass < a.passes; ++pass) {
+        const int shift = pass * a.bits;
+        for (uint32_t d = tid; d < kLocalWaves * digits / 2; d += kLocalBlock) reinterpret_cast<uint32_t *>(s_seen)[d] = 0;
+        __syncthreads();
+        uint32_t rank[ROUNDS];
+#pragma unroll
+        for (int r = 0; r < ROUNDS; ++r)
+            if (r < rounds)
+                rank[r] = rank_token<BITS, uint16_t>(mine, (key[r] >> shift) & (digits - 1), i0 + r * kWave < T);
+        __syncthreads();
+        // (digits <= kLocalBlock: one a thread)
+        uint32_t seen[kLocalWaves], sum = 0;
+        if (tid < static_cast<int>(digits))
+#pragma unroll
+            for (int w = 0; w < kLocalWaves; ++w) {
+                seen[w] = s_seen[w * digits + tid];
+                sum += seen[w];
+            }
+        uint32_t at = exclusive_sum<kLocalBlock>(sum, s_wave);
+        if (tid < static_cast<int>(digits))
+#pragma unroll
+            for (int w = 0; w < kLocalWaves; ++w) {
+                s_seen[w * digits + tid] = static_cast<uint16_t>(at);
+                at += seen[w];
+            }
+        __syncthreads();
+        const bool last = pass + 1 == a.passes;
+#pragma unroll
+        for (int r = 0; r < ROUNDS; ++r)
+            if (r < rounds && i0 + r * kWave < T) {
+                const uint32_t dst = mine[(key[r] >> shift) & (digits - 1)] + rank[r];
+                s_key[dst] = key[r];
+                s_pos[dst] = static_cast<uint16_t>(pos[r]);
+            }
+        __syncthreads();
+        if (!last) {
+#pragma unroll
+            for (int r = 0; r < ROUNDS; ++r)
+                if (r < rounds && i0 + r * kWave < T) {
+                    key[r] = s_key[i0 + r * kWave];
+                    pos[r] = s_pos[i0 + r * kWave];
+                }
+        }
+    }
+    for (uint32_t i = tid; i < T; i += kLocalBlock) {
+        const uint32_t k = s_key[i];
+        a.keys_out[i] = k;
+        a.pos_out[i] = s_pos[i];
+        if (k < static_cast<uint64_t>(a.t.V)) a.present[k] = 1;
     }
 }
 
@@ -236,10 +399,10 @@ struct SumArgs {
     const void *g;
     const uint32_t *keys, *pos;
     const uint8_t *present;              // NULL: no row has tokens
-    float *partial;                      // [chunks, 2, D]
+    float *partial;                      // [blocks, 2, D]: a run from the block before, a run into the next
     void *dw;
     int64_t D, V;
-    uint32_t T, S, chunks;
+    uint32_t T, S, block, blocks;        // tokens a group of lanes, a workgroup takes; workgroups (a block of columns)
     int lg, colblocks;
     uint32_t sum_blocks, zero_rows;      // workgroups that sum; rows a zeroing one looks at
     float scale;
@@ -255,6 +418,15 @@ __device__ __forceinline__ void store_row(const SumArgs &a, uint32_t row, int64_
     store_vec<O, VEC>(a.dw, static_cast<int64_t>(row) * a.D + col, v);
 }
 
+template <int VEC>
+__device__ __forceinline__ void store_partial(const SumArgs &a, uint32_t block, int slot, int64_t col, const float *acc) {
+    store_vec<PLE_DTYPE_F32, VEC>(a.partial, (static_cast<int64_t>(block) * 2 + slot) * a.D + col, acc);
+}
+
+// A group of lanes adds up its S tokens' runs in registers.  A run inside them is
+// finished; the sums of one that came from the group before (the head) and of
+// one that goes on in the next (the tail) meet in LDS, and those that cross the
+// workgroup's border become partials.
 template <int G, int O, int VEC>
 __global__ __launch_bounds__(kBlock) void ple_lookup_sum_kernel(SumArgs a) {
     if (blockIdx.x >= a.sum_blocks) {
@@ -270,96 +442,189 @@ __global__ __launch_bounds__(kBlock) void ple_lookup_sum_kernel(SumArgs a) {
         }
         return;
     }
-    const int lanes = 1 << a.lg;
-    const uint32_t unit = (blockIdx.x << (8 - a.lg)) + (threadIdx.x >> a.lg);
-    const uint32_t chunk = unit / a.colblocks;
-    const int64_t col = (static_cast<int64_t>(unit % a.colblocks) * lanes + (threadIdx.x & (lanes - 1))) * VEC;
-    if (chunk >= a.chunks || col >= a.D) return;
-    const uint32_t begin = chunk * a.S;
-    const uint32_t end = a.T - begin < a.S ? a.T : begin + a.S;
-    uint32_t cur = a.keys[begin];
-    bool first = true, joined = begin > 0 && a.keys[begin - 1] == cur;
+    enum { kHead = 1, kThrough = 2, kTail = 4 };     // through: the head goes on into the next group
+    __shared__ float s_head[kBlock * VEC];
+    __shared__ int s_has[kBlock];
+    const int lanes = 1 << a.lg, teams = kBlock >> a.lg;
+    const int team = threadIdx.x >> a.lg, lane = threadIdx.x & (lanes - 1);
+    const uint32_t block = blockIdx.x / a.colblocks;
+    const int64_t col = (static_cast<int64_t>(blockIdx.x % a.colblocks) * lanes + lane) * VEC;
+    const uint64_t begin = static_cast<uint64_t>(block) * a.block + static_cast<uint64_t>(team) * a.S;
+    const uint64_t end = begin + a.S < a.T ? begin + a.S : a.T;
     float acc[VEC] = {};
-    const auto flush = [&](bool ended) {
-        if (cur >= static_cast<uint64_t>(a.V)) return;
-        if (!joined && ended) store_row<O, VEC>(a, cur, col, acc);
-        else store_vec<PLE_DTYPE_F32, VEC>(a.partial, (static_cast<int64_t>(chunk) * 2 + (first ? 0 : 1)) * a.D + col, acc);
-    };
-    for (uint32_t i = begin; i < end; i += kSumUnroll) {
-        uint32_t key[kSumUnroll];
-        float v[kSumUnroll][VEC];
+    uint32_t cur = 0;
+    int has = 0;
+    if (begin < a.T && col < a.D) {
+        cur = a.keys[begin];
+        bool joined = begin > 0 && a.keys[begin - 1] == cur;
+        const auto end_run = [&] {
+            if (cur < static_cast<uint64_t>(a.V)) {
+                if (joined) {
+                    has |= kHead;
 #pragma unroll
-        for (int u = 0; u < kSumUnroll; ++u) {
-            const uint32_t at = i + u < end ? i + u : end - 1;
-            key[u] = a.keys[at];
-            load_vec<G, VEC>(a.g, static_cast<int64_t>(a.pos[at]) * a.D + col, v[u]);
-        }
+                    for (int e = 0; e < VEC; ++e) s_head[e * kBlock + threadIdx.x] = acc[e];
+                } else {
+                    store_row<O, VEC>(a, cur, col, acc);
+                }
+            }
+        };
+        for (uint64_t i = begin; i < end; i += kSumUnroll) {
+            uint32_t key[kSumUnroll];
+            float v[kSumUnroll][VEC];
 #pragma unroll
-        for (int u = 0; u < kSumUnroll; ++u) {
-            if (i + u >= end) break;
-            if (key[u] != cur) {
-                flush(true);
-                cur = key[u];
-                first = joined = false;
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) acc[e] = 0.0f;
+            for (int u = 0; u < kSumUnroll; ++u) {
+                const uint64_t at = i + u < end ? i + u : end - 1;
+                key[u] = a.keys[at];
+                load_vec<G, VEC>(a.g, static_cast<int64_t>(a.pos[at]) * a.D + col, v[u]);
             }
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) acc[e] += v[u][e];
+            for (int u = 0; u < kSumUnroll; ++u) {
+                if (i + u >= end) break;
+                if (key[u] != cur) {
+                    end_run();
+                    cur = key[u];
+                    joined = false;
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) acc[e] = 0.0f;
+                }
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) acc[e] += v[u][e];
+            }
+        }
+        if (end < a.T && a.keys[end] == cur) {
+            if (cur < static_cast<uint64_t>(a.V)) {
+                if (joined) {
+                    end_run();
+                    has |= kThrough;
+                } else {
+                    has |= kTail;
+                }
+            }
+        } else {
+            end_run();
         }
     }
-    flush(!(end < a.T && a.keys[end] == cur));
+    // head[t] += head[t + 1] for as long as the run goes through, by doubling: then
+    // a head has the whole rest of its run, and kThrough says that it leaves the
+    // workgroup
+    if (lane == 0) s_has[team] = has;        // (lane 0's columns exist)
+    const int through = __syncthreads_or(has & kThrough);
+    for (int d = 1; through && d < teams; d *= 2) {
+        const bool on = (s_has[team] & kThrough) && team + d < teams;
+        const int other = on ? s_has[team + d] : 0;
+        float v[VEC];
+        if (on)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[e] = s_head[e * kBlock + threadIdx.x] + s_head[e * kBlock + threadIdx.x + d * lanes];
+        __syncthreads();
+        if (on) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) s_head[e * kBlock + threadIdx.x] = v[e];
+            if (lane == 0 && !(other & kThrough)) s_has[team] &= ~kThrough;
+        }
+        __syncthreads();
+    }
+    if (col >= a.D) return;
+    if (has & kTail) {
+        bool leaves = true;
+        if (team + 1 < teams) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) acc[e] += s_head[e * kBlock + threadIdx.x + lanes];
+            leaves = s_has[team + 1] & kThrough;
+        }
+        if (leaves) store_partial<VEC>(a, block, 1, col, acc);
+        else store_row<O, VEC>(a, cur, col, acc);
+    }
+    if (team == 0 && (has & kHead)) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) acc[e] = s_head[e * kBlock + lane];
+        store_partial<VEC>(a, block, 0, col, acc);
+    }
 }
 
-// Runs that cross a chunk's border: the workgroup of the chunk where the run
-// starts adds its partials, the groups of lanes a contiguous part each.
+// Runs that cross a block's border.  A group of lanes looks at one block: a run
+// that starts there and goes on in up to kShortRun blocks it adds itself.  A
+// longer one the workgroup adds, its groups a contiguous part each; it looks at
+// no more than kShortRun blocks, so it has one of those at most.
+constexpr int kShortRun = 8;
+
 template <int O, int VEC>
 __global__ __launch_bounds__(kBlock) void ple_lookup_join_kernel(SumArgs a) {
     __shared__ float s_sum[kBlock * VEC];
-    const uint32_t chunk = blockIdx.x / a.colblocks;
-    const uint32_t begin = chunk * a.S;
-    if (a.T - begin <= a.S) return;      // (the last chunk: nothing follows)
-    const uint32_t end = begin + a.S;
-    const uint32_t key = a.keys[end];
-    if (key >= static_cast<uint64_t>(a.V) || a.keys[end - 1] != key) return;
-    const bool whole = a.keys[begin] == key;
-    if (whole && begin > 0 && a.keys[begin - 1] == key) return;     // it started before
-    // chunks that begin inside the run: chunk + 1 .. last
-    uint32_t stop = chunk + 1;
+    __shared__ uint32_t s_long;              // the long run's block
+    const int lanes = 1 << a.lg, teams = kBlock >> a.lg;
+    const int team = threadIdx.x >> a.lg, lane = threadIdx.x & (lanes - 1);
+    const int looking = teams < kShortRun ? teams : kShortRun;
+    const uint32_t block = blockIdx.x / a.colblocks * looking + team;
+    const int64_t col = (static_cast<int64_t>(blockIdx.x % a.colblocks) * lanes + lane) * VEC;
+    const auto first_key = [&](uint32_t b) { return a.keys[static_cast<uint64_t>(b) * a.block]; };
+    uint32_t n = 0, key = 0;                 // n: partials of the run that starts here
+    if (team < looking && block + 1 < a.blocks) {    // (the last block has nothing behind it)
+        const uint64_t begin = static_cast<uint64_t>(block) * a.block;
+        uint32_t ahead[kShortRun + 1];
+#pragma unroll
+        for (uint32_t j = 0; j <= kShortRun; ++j)
+            ahead[j] = first_key(block + 1 + j < a.blocks ? block + 1 + j : a.blocks - 1);
+        const uint32_t last = a.keys[begin + a.block - 1], first = a.keys[begin];
+        const uint32_t prior = begin > 0 ? a.keys[begin - 1] : ~0u;      // (no key is ~0)
+        key = ahead[0];
+        if (key < static_cast<uint64_t>(a.V) && last == key && !(first == key && prior == key)) {
+            n = 2;
+#pragma unroll
+            for (uint32_t j = 1; j <= kShortRun; ++j)
+                if (n == j + 1 && block + 1 + j < a.blocks && ahead[j] == key) n = j + 2;
+        }
+    }
+    const bool more = n > kShortRun + 1;
+    if (n > 0 && !more && col < a.D) {
+        float acc[VEC];
+        load_vec<PLE_DTYPE_F32, VEC>(a.partial, (static_cast<int64_t>(block) * 2 + 1) * a.D + col, acc);
+#pragma unroll
+        for (uint32_t p = 1; p <= kShortRun; ++p)
+            if (p < n) {
+                float v[VEC];
+                load_vec<PLE_DTYPE_F32, VEC>(a.partial, static_cast<int64_t>(block + p) * 2 * a.D + col, v);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) acc[e] += v[e];
+            }
+        store_row<O, VEC>(a, key, col, acc);
+    }
+    if (more && lane == 0) s_long = block;
+    if (!__syncthreads_or(more)) return;
+    const uint32_t at = s_long, k = first_key(at + 1);
+    // blocks that begin inside the run: at + 1 .. stop - 1
+    uint32_t stop = at + kShortRun + 1;
     for (;;) {
-        const uint32_t c = stop + threadIdx.x % kWave;
-        const uint64_t out = __ballot(!(c < a.chunks && a.keys[c * a.S] == key));
+        const uint32_t b = stop + threadIdx.x % kWave;
+        const uint64_t out = __ballot(!(b < a.blocks && first_key(b) == k));
         if (out) {
             stop += __builtin_ctzll(out);
             break;
         }
         stop += kWave;
     }
-    const int lanes = 1 << a.lg, teams = kBlock >> a.lg;
-    const int team = threadIdx.x >> a.lg, lane = threadIdx.x & (lanes - 1);
-    const int64_t col = (static_cast<int64_t>(blockIdx.x % a.colblocks) * lanes + lane) * VEC;
-    const uint32_t n = stop - chunk, per = (n + teams - 1) / teams;
+    const uint32_t parts = stop - at, per = (parts + teams - 1) / teams;
     float acc[VEC] = {};
     if (col < a.D) {
-        const uint32_t p1 = (team + 1) * per < n ? (team + 1) * per : n;
-#pragma unroll 4
+        const uint32_t p1 = (team + 1) * per < parts ? (team + 1) * per : parts;
+#pragma unroll 8
         for (uint32_t p = team * per; p < p1; ++p) {
             float v[VEC];
-            const int64_t slot = static_cast<int64_t>(chunk + p) * 2 + (p == 0 && !whole ? 1 : 0);
-            load_vec<PLE_DTYPE_F32, VEC>(a.partial, slot * a.D + col, v);
+            load_vec<PLE_DTYPE_F32, VEC>(a.partial, (static_cast<int64_t>(at + p) * 2 + (p == 0 ? 1 : 0)) * a.D + col, v);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) acc[e] += v[e];
         }
     }
+    for (int half = teams / 2; half > 0; half /= 2) {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) s_sum[e * kBlock + threadIdx.x] = acc[e];
-    __syncthreads();
-    if (team == 0 && col < a.D) {
-        for (int t = 1; t < teams; ++t)
+        for (int e = 0; e < VEC; ++e) s_sum[e * kBlock + threadIdx.x] = acc[e];
+        __syncthreads();
+        if (team < half)
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) acc[e] += s_sum[e * kBlock + t * lanes + lane];
-        store_row<O, VEC>(a, key, col, acc);
+            for (int e = 0; e < VEC; ++e) acc[e] += s_sum[e * kBlock + threadIdx.x + half * lanes];
+        __syncthreads();
     }
+    if (team == 0 && col < a.D) store_row<O, VEC>(a, k, col, acc);
 }
 
 // ---------------------------------------------------------------------------
@@ -382,7 +647,7 @@ int row_vec(int64_t D, std::initializer_list<std::pair<const void *, int>> ptrs)
 
 struct SumPlan {
     int passes, bits, tiles, lg, colblocks;
-    uint32_t tile, S, chunks;
+    uint32_t tile, S, block, blocks;     // block: tokens a summing workgroup takes
     size_t o_pos, o_keys2, o_pos2, o_counts, o_present, o_partial, bytes;
 };
 
@@ -391,14 +656,23 @@ SumPlan plan_sum(int64_t T, int64_t V, int64_t D, int vec) {
     const int key_bits = std::max(1, bits_of(static_cast<uint64_t>(V)));
     p.passes = (key_bits + kMaxDigitBits - 1) / kMaxDigitBits;
     p.bits = (key_bits + p.passes - 1) / p.passes;
+    p.bits = std::max(2, p.bits);        // (counts are read four digits at a time)
     const int64_t per = (T + kMaxTiles - 1) / kMaxTiles;
-    p.tile = static_cast<uint32_t>(std::max<int64_t>(kMinTile, (per + kSortBlock - 1) / kSortBlock * kSortBlock));
+    p.tile = static_cast<uint32_t>(std::max<int64_t>(1, (per + kSortStep - 1) / kSortStep) * kSortStep);
     p.tiles = static_cast<int>((T + p.tile - 1) / p.tile);
     const int64_t vecs = (D + vec - 1) / vec;
     p.lg = std::min(6, vecs <= 1 ? 0 : bits_of(static_cast<uint64_t>(vecs - 1)));
     p.colblocks = static_cast<int>((vecs + (int64_t{1} << p.lg) - 1) >> p.lg);
-    p.S = 32;
-    p.chunks = static_cast<uint32_t>((T + p.S - 1) / p.S);
+    // tokens a chunk: enough waves for the GPU (16 a CU, 8 elements a lane), chunks
+    // long enough for their partials to be few.  (By T and D alone, which size the
+    // workspace.)
+    const int64_t waves = T * D / (8 * kWave);
+    p.S = 8;
+    while (p.S < 128 && waves / p.S > 16 * 256) p.S *= 2;
+    p.block = p.S * (kBlock >> p.lg);
+    p.blocks = static_cast<uint32_t>((T + p.block - 1) / p.block);
+    // (partials: by the fewest tokens a block has, those of rows of 64 lanes)
+    const size_t most_blocks = static_cast<size_t>((T + p.S * kWavesPerBlock - 1) / (p.S * kWavesPerBlock));
     const size_t list = align_up(static_cast<size_t>(T) * 4, 256);
     size_t at = list;
     const auto take = [&](size_t n) {
@@ -411,7 +685,7 @@ SumPlan plan_sum(int64_t T, int64_t V, int64_t D, int vec) {
     p.o_pos2 = take(p.passes > 1 ? list : 0);
     p.o_counts = take(static_cast<size_t>(p.tiles) * 4 << p.bits);
     p.o_present = take(static_cast<size_t>(V));
-    p.o_partial = take(static_cast<size_t>(p.chunks) * 2 * D * 4);
+    p.o_partial = take(most_blocks * 2 * D * 4);
     p.bytes = at;
     return p;
 }
@@ -420,25 +694,30 @@ template <int W, int O, int VEC>
 hipError_t launch_gather(GatherArgs a, hipStream_t s) {
     const int64_t vecs = a.D / VEC;
     a.lg = std::min(6, vecs <= 1 ? 0 : bits_of(static_cast<uint64_t>(vecs - 1)));
-    const int64_t per_block = kBlock >> a.lg, cols = (int64_t{1} << a.lg) * kGatherUnroll;
-    const dim3 grid(static_cast<unsigned>((a.t.T + per_block - 1) / per_block),
-                    static_cast<unsigned>((vecs + cols - 1) / cols));
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_lookup_kernel<W, O, VEC>), grid, dim3(kBlock), 0, s, a);
+    const int64_t per_block = kBlock >> a.lg, lanes = int64_t{1} << a.lg;
+    const auto blocks = [](int64_t n, int64_t per) { return static_cast<unsigned>((n + per - 1) / per); };
+    if (vecs <= lanes)
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_lookup_kernel<W, O, VEC, true>), dim3(blocks(a.t.T, per_block * kGatherUnroll)),
+                           dim3(kBlock), 0, s, a);
+    else
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_lookup_kernel<W, O, VEC, false>),
+                           dim3(blocks(a.t.T, per_block), blocks(vecs, lanes * kGatherUnroll)), dim3(kBlock), 0, s, a);
     return hipGetLastError();
 }
 
 template <int G, int O, int VEC>
 hipError_t launch_sum(SumArgs a, hipStream_t s) {
-    const uint64_t units = static_cast<uint64_t>(a.chunks) * a.colblocks, per_block = kBlock >> a.lg;
-    a.sum_blocks = static_cast<uint32_t>((units + per_block - 1) / per_block);
+    a.sum_blocks = a.blocks * a.colblocks;
     const int64_t row_bytes = a.D * elem_bytes(O);
     a.zero_rows = static_cast<uint32_t>(std::max<int64_t>(1, 32768 / row_bytes));
     const uint64_t zero_blocks = (a.V + a.zero_rows - 1) / a.zero_rows;
     hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_lookup_sum_kernel<G, O, VEC>),
                        dim3(static_cast<unsigned>(a.sum_blocks + zero_blocks)), dim3(kBlock), 0, s, a);
-    if (a.chunks > 1)
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_lookup_join_kernel<O, VEC>), dim3(a.chunks * a.colblocks), dim3(kBlock),
-                           0, s, a);
+    if (a.blocks > 1) {
+        const uint32_t looking = std::min(kBlock >> a.lg, kShortRun);
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_lookup_join_kernel<O, VEC>), dim3((a.blocks + looking - 1) / looking * a.colblocks),
+                           dim3(kBlock), 0, s, a);
+    }
     return hipGetLastError();
 }
 
@@ -460,6 +739,33 @@ hipError_t with_vec(int vec, F f) {
         case 2: return f(std::integral_constant<int, 2>{});
         default: return f(std::integral_constant<int, 1>{});
     }
+}
+
+template <int BITS>
+void launch_local_sort(const SortArgs &s, hipStream_t stream) {
+    const size_t room = align_up(s.t.T, kLocalBlock);
+    const size_t lds = room * 6 + (static_cast<size_t>(kLocalWaves) * 2 << s.bits);
+    if (room <= 2 * kLocalBlock)
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_lookup_sort_kernel<2, BITS>), dim3(1), dim3(kLocalBlock), lds, stream, s);
+    else
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_lookup_sort_kernel<kLocalRounds, BITS>), dim3(1), dim3(kLocalBlock), lds,
+                           stream, s);
+}
+
+template <int BITS>
+void launch_sort_pass(const SortArgs &s, bool first, bool last, hipStream_t stream) {
+    const size_t lds = static_cast<size_t>(2 + kSortWaves) * 4 << s.bits;
+    const dim3 grid(s.tiles), block(kSortBlock);
+    if (first) hipLaunchKernelGGL(ple_lookup_count_kernel<true>, grid, block, 0, stream, s);
+    else hipLaunchKernelGGL(ple_lookup_count_kernel<false>, grid, block, 0, stream, s);
+    const auto scatter = [&](auto f, auto l) {
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_lookup_scatter_kernel<decltype(f)::value, decltype(l)::value, BITS>), grid,
+                           block, lds, stream, s);
+    };
+    if (first && last) scatter(std::true_type{}, std::true_type{});
+    else if (first) scatter(std::true_type{}, std::false_type{});
+    else if (last) scatter(std::false_type{}, std::true_type{});
+    else scatter(std::false_type{}, std::false_type{});
 }
 
 TokenArgs token_args(const LookupRequest &r) {
@@ -513,23 +819,21 @@ int lookup_backward_run(const LookupRequest &r) {
         s.present = reinterpret_cast<uint8_t *>(ws + p.o_present);
         uint32_t *keys[2] = {list(0), p.passes > 1 ? list(p.o_keys2) : nullptr};
         uint32_t *pos[2] = {list(p.o_pos), p.passes > 1 ? list(p.o_pos2) : nullptr};
-        const size_t lds = static_cast<size_t>(kSortWaves) * 4 << p.bits;
-        const dim3 grid(p.tiles), block(kSortBlock);
-        for (int k = 0; k < p.passes; ++k) {
-            s.shift = k * p.bits;
-            s.keys_in = keys[(k + 1) & 1];
-            s.pos_in = pos[(k + 1) & 1];
-            s.keys_out = keys[k & 1];
-            s.pos_out = pos[k & 1];
-            const bool last = k + 1 == p.passes;
-            if (k == 0) {
-                hipLaunchKernelGGL(ple_lookup_count_kernel<true>, grid, block, 0, r.stream, s);
-                if (last) hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_lookup_scatter_kernel<true, true>), grid, block, lds, r.stream, s);
-                else hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_lookup_scatter_kernel<true, false>), grid, block, lds, r.stream, s);
-            } else {
-                hipLaunchKernelGGL(ple_lookup_count_kernel<false>, grid, block, 0, r.stream, s);
-                if (last) hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_lookup_scatter_kernel<false, true>), grid, block, lds, r.stream, s);
-                else hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_lookup_scatter_kernel<false, false>), grid, block, lds, r.stream, s);
+        s.passes = p.passes;
+        if (r.T <= kLocalTokens) {
+            s.keys_out = keys[0];
+            s.pos_out = pos[0];
+            if (p.bits <= 8) launch_local_sort<8>(s, r.stream);
+            else launch_local_sort<kMaxDigitBits>(s, r.stream);
+        } else {
+            for (int k = 0; k < p.passes; ++k) {
+                s.shift = k * p.bits;
+                s.keys_in = keys[(k + 1) & 1];
+                s.pos_in = pos[(k + 1) & 1];
+                s.keys_out = keys[k & 1];
+                s.pos_out = pos[k & 1];
+                if (p.bits <= 8) launch_sort_pass<8>(s, k == 0, k + 1 == p.passes, r.stream);
+                else launch_sort_pass<kMaxDigitBits>(s, k == 0, k + 1 == p.passes, r.stream);
             }
         }
         a.keys = s.keys_out;
@@ -543,7 +847,8 @@ int lookup_backward_run(const LookupRequest &r) {
     a.V = r.V;
     a.T = static_cast<uint32_t>(r.T);
     a.S = p.S;
-    a.chunks = p.chunks;
+    a.block = p.block;
+    a.blocks = p.blocks;
     a.lg = p.lg;
     a.colblocks = p.colblocks;
     a.scale = r.scale;

@@ -305,3 +305,14 @@ def test_c_abi(ops):
     assert torch.equal(dw, ops.lookup_backward(g, tokens, None, 70, 0.5, -1, F32))
     with pytest.raises(capi.PleError, match="workspace"):
         capi.lookup_backward(g, tokens, dw, workspace=torch.empty(64, dtype=torch.uint8, device=DEV))
+
+
+@pytest.mark.parametrize("t,d,dtype", [(20_000, 512, BF16), (20_000, 500, BF16), (9000, 1001, F32), (300_000, 16, F32),
+                                       (600_000, 4, F32), (1_100_000, 2, BF16)])
+def test_workspace_and_steps(ops, t, d, dtype):
+    """Chunk lengths above the smallest, and sorts of several steps a workgroup; one workspace size for every layout."""
+    gen = torch.Generator().manual_seed(t)
+    v = 5001
+    tokens = (torch.rand(t, generator=gen) ** 4 * v).long()
+    g = torch.randn(t, d, generator=gen).to(dtype)
+    _check_backward(ops, tokens, g, v, 1.0, dtype)
