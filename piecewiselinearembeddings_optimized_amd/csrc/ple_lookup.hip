@@ -119,21 +119,44 @@ __global__ __launch_bounds__(kBlock) void ple_lookup_kernel(GatherArgs a) {
 // backward: the sort
 // ---------------------------------------------------------------------------
 
+// Rows without tokens are written by workgroups of their own beside the sort's,
+// which leave the memory idle: `present` tells them which rows those are, or
+// (NULL) every row is cleared and the rows with tokens are written again.
+struct ZeroArgs {
+    char *dw;
+    const uint8_t *present;
+    int64_t begin, end;          // rows
+    uint32_t units, rows;        // units of a row; rows a workgroup looks at
+    int unit;                    // bytes: 16, 4 or 2
+};
+
+// (Stored past the caches: beside a gradient of more than the memory-side cache,
+// plain stores of the rows and of the zeros took 288 us where these take 251,
+// 65536 tokens x 2048 over 131072 rows; smaller ones are as fast either way.)
+__device__ __forceinline__ void zero_rows(const ZeroArgs &z, int64_t block) {
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    const int64_t r0 = z.begin + block * z.rows;
+    const uint32_t rows = static_cast<uint32_t>(z.end - r0 < z.rows ? z.end - r0 : z.rows);
+    for (uint32_t j = threadIdx.x; j < rows * z.units; j += blockDim.x) {
+        if (z.present && z.present[r0 + j / z.units]) continue;
+        char *p = z.dw + (r0 * z.units + j) * z.unit;
+        if (z.unit == 16) __builtin_nontemporal_store(u32x4{0, 0, 0, 0}, reinterpret_cast<u32x4 *>(p));
+        else if (z.unit == 4) *reinterpret_cast<uint32_t *>(p) = 0;
+        else *reinterpret_cast<uint16_t *>(p) = 0;
+    }
+}
+
 struct SortArgs {
     TokenArgs t;
-    const uint32_t *keys_in, *pos_in;    // the first pass makes them from the tokens
+    ZeroArgs z;                          // of the launch's workgroups past `tiles`
+    uint32_t *keys_in;                   // the first pass's count kernel makes them from the tokens
+    const uint32_t *pos_in;              // first pass: the tokens' own order
     uint32_t *keys_out, *pos_out;
     uint32_t *counts;                    // [tiles, 1 << bits]
     uint8_t *present;                    // [V]: rows that have tokens
     uint32_t tile;                       // tokens a workgroup takes
     int tiles, shift, bits, passes;
 };
-
-template <bool FIRST>
-__device__ __forceinline__ uint32_t sort_key(const SortArgs &a, uint32_t i) {
-    if constexpr (FIRST) return token_key(a.t, i);
-    else return a.keys_in[i];
-}
 
 // The lanes of the wave that are `on` and have this lane's digit, of at most
 // BITS bits: a ballot for each bit, whose mask or its complement every lane
@@ -186,12 +209,16 @@ __device__ __forceinline__ uint32_t exclusive_sum(uint32_t v, uint32_t *s_wave) 
 template <bool FIRST>
 __global__ __launch_bounds__(kSortBlock) void ple_lookup_count_kernel(SortArgs a) {
     __shared__ uint32_t hist[1 << kMaxDigitBits];
+    if (static_cast<int>(blockIdx.x) >= a.tiles) {
+        zero_rows(a.z, blockIdx.x - a.tiles);
+        return;
+    }
     const uint32_t digits = 1u << a.bits;
     for (uint32_t d = threadIdx.x; d < digits; d += kSortBlock) hist[d] = 0;
     if constexpr (FIRST)
         // (`present` is rounded up to 16 bytes)
         for (int64_t r = static_cast<int64_t>(blockIdx.x) * kSortBlock + threadIdx.x; r < (a.t.V + 15) / 16;
-             r += static_cast<int64_t>(gridDim.x) * kSortBlock)
+             r += static_cast<int64_t>(a.tiles) * kSortBlock)
             reinterpret_cast<uint4 *>(a.present)[r] = make_uint4(0, 0, 0, 0);
     __syncthreads();
     const uint64_t begin = static_cast<uint64_t>(blockIdx.x) * a.tile;
@@ -201,11 +228,15 @@ __global__ __launch_bounds__(kSortBlock) void ple_lookup_count_kernel(SortArgs a
 #pragma unroll
         for (int r = 0; r < kSortRounds; ++r) {
             const uint64_t i = i0 + r * kSortBlock;
-            key[r] = sort_key<FIRST>(a, static_cast<uint32_t>(i < end ? i : end - 1));
+            if constexpr (FIRST) key[r] = token_key(a.t, static_cast<uint32_t>(i < end ? i : end - 1));
+            else key[r] = a.keys_in[i < end ? i : end - 1];
         }
 #pragma unroll
         for (int r = 0; r < kSortRounds; ++r)
-            if (i0 + r * kSortBlock < end) atomicAdd(&hist[(key[r] >> a.shift) & (digits - 1)], 1u);
+            if (i0 + r * kSortBlock < end) {
+                if constexpr (FIRST) a.keys_in[i0 + r * kSortBlock] = key[r];
+                atomicAdd(&hist[(key[r] >> a.shift) & (digits - 1)], 1u);
+            }
     }
     __syncthreads();
     for (uint32_t d = threadIdx.x; d < digits; d += kSortBlock)
@@ -217,10 +248,14 @@ __global__ __launch_bounds__(kSortBlock) void ple_lookup_count_kernel(SortArgs a
 // its own for these sums costs more than the reads up to 256 workgroups).  Then
 // it walks its tokens in steps: each wave takes a contiguous part of a step and
 // ranks its tokens per digit, the waves' numbers give each wave its place.
-template <bool FIRST, bool LAST, int BITS>
+template <bool FIRST, int BITS>
 __global__ __launch_bounds__(kSortBlock) void ple_lookup_scatter_kernel(SortArgs a) {
     extern __shared__ uint32_t s_dyn[];
     __shared__ uint32_t s_wave[kSortWaves];
+    if (static_cast<int>(blockIdx.x) >= a.tiles) {
+        zero_rows(a.z, blockIdx.x - a.tiles);
+        return;
+    }
     const uint32_t digits = 1u << a.bits;
     uint32_t *s_place = s_dyn, *s_total = s_dyn + digits, *s_seen = s_dyn + 2 * digits;   // seen: [waves, digits]
     const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
@@ -232,7 +267,7 @@ __global__ __launch_bounds__(kSortBlock) void ple_lookup_scatter_kernel(SortArgs
 #pragma unroll
         for (int r = 0; r < kSortRounds; ++r) {
             const uint64_t i = i0 + r * kWave < end ? i0 + r * kWave : end - 1;
-            key[r] = sort_key<FIRST>(a, static_cast<uint32_t>(i));
+            key[r] = a.keys_in[i];
             pos[r] = FIRST ? static_cast<uint32_t>(i) : a.pos_in[i];
         }
     };
@@ -301,7 +336,7 @@ __global__ __launch_bounds__(kSortBlock) void ple_lookup_scatter_kernel(SortArgs
                 const uint32_t dst = mine[(key[r] >> a.shift) & (digits - 1)] + rank[r];
                 a.keys_out[dst] = key[r];
                 a.pos_out[dst] = pos[r];
-                if (LAST && key[r] < static_cast<uint64_t>(a.t.V)) a.present[key[r]] = 1;
+                if (FIRST && key[r] < static_cast<uint64_t>(a.t.V)) a.present[key[r]] = 1;
             }
         step += kSortStep;
         if (step >= end) break;
@@ -320,6 +355,10 @@ template <int ROUNDS, int BITS>
 __global__ __launch_bounds__(kLocalBlock) void ple_lookup_sort_kernel(SortArgs a) {
     extern __shared__ uint32_t s_dyn[];
     __shared__ uint32_t s_wave[kLocalWaves];
+    if (blockIdx.x > 0) {
+        zero_rows(a.z, blockIdx.x - 1);
+        return;
+    }
     const uint32_t digits = 1u << a.bits, T = a.t.T;
     uint32_t *s_key = s_dyn;                                             // [rounded T]
     const uint32_t room = (T + kLocalBlock - 1) / kLocalBlock * kLocalBlock;
@@ -336,8 +375,9 @@ __global__ __launch_bounds__(kLocalBlock) void ple_lookup_sort_kernel(SortArgs a
             key[r] = token_key(a.t, i);
             pos[r] = i;
         }
-    // (`present` is rounded up to 16 bytes)
-    for (int64_t r = tid; r < (a.t.V + 15) / 16; r += kLocalBlock) reinterpret_cast<uint4 *>(a.present)[r] = make_uint4(0, 0, 0, 0);
+    // (`present` is rounded up to 16 bytes; NULL: this launch clears all rows)
+    for (int64_t r = tid; a.present && r < (a.t.V + 15) / 16; r += kLocalBlock)
+        reinterpret_cast<uint4 *>(a.present)[r] = make_uint4(0, 0, 0, 0);
     uint16_t *mine = s_seen + wave * digits;
     for (int pass = 0; pass < a.passes; ++pass) {
         const int shift = pass * a.bits;
@@ -387,7 +427,7 @@ __global__ __launch_bounds__(kLocalBlock) void ple_lookup_sort_kernel(SortArgs a
         const uint32_t k = s_key[i];
         a.keys_out[i] = k;
         a.pos_out[i] = s_pos[i];
-        if (k < static_cast<uint64_t>(a.t.V)) a.present[k] = 1;
+        if (a.present && k < static_cast<uint64_t>(a.t.V)) a.present[k] = 1;
     }
 }
 
@@ -398,13 +438,13 @@ __global__ __launch_bounds__(kLocalBlock) void ple_lookup_sort_kernel(SortArgs a
 struct SumArgs {
     const void *g;
     const uint32_t *keys, *pos;
-    const uint8_t *present;              // NULL: no row has tokens
+    ZeroArgs z;                          // of the launch's workgroups past `sum_blocks`
     float *partial;                      // [blocks, 2, D]: a run from the block before, a run into the next
     void *dw;
     int64_t D, V;
     uint32_t T, S, block, blocks;        // tokens a group of lanes, a workgroup takes; workgroups (a block of columns)
     int lg, colblocks;
-    uint32_t sum_blocks, zero_rows;      // workgroups that sum; rows a zeroing one looks at
+    uint32_t sum_blocks;                 // workgroups that sum
     float scale;
 };
 
@@ -415,7 +455,7 @@ __device__ __forceinline__ void store_row(const SumArgs &a, uint32_t row, int64_
     float v[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) v[e] = acc[e] * a.scale;
-    store_vec<O, VEC>(a.dw, static_cast<int64_t>(row) * a.D + col, v);
+    store_vec<O, VEC, true>(a.dw, static_cast<int64_t>(row) * a.D + col, v);
 }
 
 template <int VEC>
@@ -430,16 +470,7 @@ __device__ __forceinline__ void store_partial(const SumArgs &a, uint32_t block, 
 template <int G, int O, int VEC>
 __global__ __launch_bounds__(kBlock) void ple_lookup_sum_kernel(SumArgs a) {
     if (blockIdx.x >= a.sum_blocks) {
-        // rows without tokens
-        const int64_t r0 = static_cast<int64_t>(blockIdx.x - a.sum_blocks) * a.zero_rows;
-        const uint32_t rows = static_cast<uint32_t>(a.V - r0 < a.zero_rows ? a.V - r0 : a.zero_rows);
-        const uint32_t vecs = static_cast<uint32_t>(a.D / VEC);
-        const float zero[VEC] = {};
-        for (uint32_t j = threadIdx.x; j < rows * vecs; j += kBlock) {
-            const uint32_t r = j / vecs;
-            if (!a.present || !a.present[r0 + r])
-                store_vec<O, VEC>(a.dw, (r0 + r) * a.D + static_cast<int64_t>(j - r * vecs) * VEC, zero);
-        }
+        zero_rows(a.z, blockIdx.x - a.sum_blocks);
         return;
     }
     enum { kHead = 1, kThrough = 2, kTail = 4 };     // through: the head goes on into the next group
@@ -681,13 +712,17 @@ SumPlan plan_sum(int64_t T, int64_t V, int64_t D, int vec) {
         return o;
     };
     p.o_pos = take(list);
-    p.o_keys2 = take(p.passes > 1 ? list : 0);
+    p.o_keys2 = take(list);
     p.o_pos2 = take(p.passes > 1 ? list : 0);
     p.o_counts = take(static_cast<size_t>(p.tiles) * 4 << p.bits);
     p.o_present = take(static_cast<size_t>(V));
     p.o_partial = take(most_blocks * 2 * D * 4);
     p.bytes = at;
     return p;
+}
+
+uint32_t zero_blocks(const ZeroArgs &z) {
+    return z.end > z.begin ? static_cast<uint32_t>((z.end - z.begin + z.rows - 1) / z.rows) : 0;
 }
 
 template <int W, int O, int VEC>
@@ -708,11 +743,8 @@ hipError_t launch_gather(GatherArgs a, hipStream_t s) {
 template <int G, int O, int VEC>
 hipError_t launch_sum(SumArgs a, hipStream_t s) {
     a.sum_blocks = a.blocks * a.colblocks;
-    const int64_t row_bytes = a.D * elem_bytes(O);
-    a.zero_rows = static_cast<uint32_t>(std::max<int64_t>(1, 32768 / row_bytes));
-    const uint64_t zero_blocks = (a.V + a.zero_rows - 1) / a.zero_rows;
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_lookup_sum_kernel<G, O, VEC>),
-                       dim3(static_cast<unsigned>(a.sum_blocks + zero_blocks)), dim3(kBlock), 0, s, a);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_lookup_sum_kernel<G, O, VEC>), dim3(a.sum_blocks + zero_blocks(a.z)), dim3(kBlock), 0,
+                       s, a);
     if (a.blocks > 1) {
         const uint32_t looking = std::min(kBlock >> a.lg, kShortRun);
         hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_lookup_join_kernel<O, VEC>), dim3((a.blocks + looking - 1) / looking * a.colblocks),
@@ -745,27 +777,28 @@ template <int BITS>
 void launch_local_sort(const SortArgs &s, hipStream_t stream) {
     const size_t room = align_up(s.t.T, kLocalBlock);
     const size_t lds = room * 6 + (static_cast<size_t>(kLocalWaves) * 2 << s.bits);
+    const dim3 grid(1 + zero_blocks(s.z)), block(kLocalBlock);
     if (room <= 2 * kLocalBlock)
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_lookup_sort_kernel<2, BITS>), dim3(1), dim3(kLocalBlock), lds, stream, s);
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_lookup_sort_kernel<2, BITS>), grid, block, lds, stream, s);
     else
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_lookup_sort_kernel<kLocalRounds, BITS>), dim3(1), dim3(kLocalBlock), lds,
-                           stream, s);
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_lookup_sort_kernel<kLocalRounds, BITS>), grid, block, lds, stream, s);
 }
 
+// One pass; the second one's two kernels clear a third and two thirds of `rows`
+// rows (their own times are about as 1 to 2).
 template <int BITS>
-void launch_sort_pass(const SortArgs &s, bool first, bool last, hipStream_t stream) {
+void launch_sort_pass(SortArgs s, int pass, int64_t rows, hipStream_t stream) {
     const size_t lds = static_cast<size_t>(2 + kSortWaves) * 4 << s.bits;
-    const dim3 grid(s.tiles), block(kSortBlock);
-    if (first) hipLaunchKernelGGL(ple_lookup_count_kernel<true>, grid, block, 0, stream, s);
-    else hipLaunchKernelGGL(ple_lookup_count_kernel<false>, grid, block, 0, stream, s);
-    const auto scatter = [&](auto f, auto l) {
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_lookup_scatter_kernel<decltype(f)::value, decltype(l)::value, BITS>), grid,
-                           block, lds, stream, s);
-    };
-    if (first && last) scatter(std::true_type{}, std::true_type{});
-    else if (first) scatter(std::true_type{}, std::false_type{});
-    else if (last) scatter(std::false_type{}, std::true_type{});
-    else scatter(std::false_type{}, std::false_type{});
+    const dim3 block(kSortBlock);
+    s.z.begin = 0;
+    s.z.end = pass == 1 ? rows / 3 : 0;
+    const auto grid = [&] { return dim3(s.tiles + zero_blocks(s.z)); };
+    if (pass == 0) hipLaunchKernelGGL(ple_lookup_count_kernel<true>, grid(), block, 0, stream, s);
+    else hipLaunchKernelGGL(ple_lookup_count_kernel<false>, grid(), block, 0, stream, s);
+    s.z.begin = s.z.end;
+    s.z.end = pass == 1 ? rows : 0;
+    if (pass == 0) hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_lookup_scatter_kernel<true, BITS>), grid(), block, lds, stream, s);
+    else hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_lookup_scatter_kernel<false, BITS>), grid(), block, lds, stream, s);
 }
 
 TokenArgs token_args(const LookupRequest &r) {
@@ -814,31 +847,50 @@ int lookup_backward_run(const LookupRequest &r) {
     s.tiles = p.tiles;
     s.bits = p.bits;
     SumArgs a{};
+    const int64_t row_bytes = r.D * elem_bytes(r.table_dtype);
+    ZeroArgs z{};
+    z.dw = static_cast<char *>(r.dw);
+    z.unit = reinterpret_cast<uintptr_t>(r.dw) % 16 == 0 && row_bytes % 16 == 0 ? 16 : elem_bytes(r.table_dtype);
+    z.units = static_cast<uint32_t>(row_bytes / z.unit);
+    z.rows = static_cast<uint32_t>(std::max<int64_t>(1, 32768 / row_bytes));
+    z.end = r.V;
+    a.z = z;
     if (r.T > 0) {
         s.counts = list(p.o_counts);
         s.present = reinterpret_cast<uint8_t *>(ws + p.o_present);
-        uint32_t *keys[2] = {list(0), p.passes > 1 ? list(p.o_keys2) : nullptr};
+        a.z.present = s.present;
+        uint32_t *keys[2] = {list(0), list(p.o_keys2)};
         uint32_t *pos[2] = {list(p.o_pos), p.passes > 1 ? list(p.o_pos2) : nullptr};
         s.passes = p.passes;
+        s.z = z;
         if (r.T <= kLocalTokens) {
             s.keys_out = keys[0];
             s.pos_out = pos[0];
+            // the sort of one workgroup takes as long as clearing some 100 MB; clearing
+            // rows that have tokens too is little where they are few
+            if (r.V >= 4 * r.T) {
+                s.present = nullptr;
+                a.z.end = 0;
+            } else {
+                s.z.end = 0;
+            }
             if (p.bits <= 8) launch_local_sort<8>(s, r.stream);
             else launch_local_sort<kMaxDigitBits>(s, r.stream);
         } else {
+            s.z.present = s.present;
+            if (p.passes > 1) a.z.end = 0;
             for (int k = 0; k < p.passes; ++k) {
                 s.shift = k * p.bits;
                 s.keys_in = keys[(k + 1) & 1];
                 s.pos_in = pos[(k + 1) & 1];
                 s.keys_out = keys[k & 1];
                 s.pos_out = pos[k & 1];
-                if (p.bits <= 8) launch_sort_pass<8>(s, k == 0, k + 1 == p.passes, r.stream);
-                else launch_sort_pass<kMaxDigitBits>(s, k == 0, k + 1 == p.passes, r.stream);
+                if (p.bits <= 8) launch_sort_pass<8>(s, k, r.V, r.stream);
+                else launch_sort_pass<kMaxDigitBits>(s, k, r.V, r.stream);
             }
         }
         a.keys = s.keys_out;
         a.pos = s.pos_out;
-        a.present = s.present;
         a.partial = reinterpret_cast<float *>(ws + p.o_partial);
     }
     a.g = r.grad;
