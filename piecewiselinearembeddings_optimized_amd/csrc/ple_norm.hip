@@ -42,6 +42,7 @@ struct NormArgs {
     float *partial;                    // [workgroups, sums, D]
     float *gate_partial;               // [groups, pieces, D]
     int64_t N, rows_per_gate;
+    int64_t block_rows;                // forward: rows of a workgroup
     int64_t piece_rows, pieces;        // backward: rows of a piece, pieces of a gate's rows
     int D, param_dtype;
     int post, pre, act, gates;         // gates: 0 none, 1 one for all rows, 2 one each for groups of rows, 3 one a row
@@ -81,9 +82,47 @@ struct Cols {
                 if (on(e)) store_vec<T, 1>(p, row * D + at(e), &v[e]);
         }
     }
-    __device__ __forceinline__ void load_param(const void *p, int64_t row, int dtype, float none, float (&v)[kElems]) const {
+    // a row as loaded, widened at use (grad_elem), so that the next row's can be
+    // in flight while this one's is used
+    template <int T>
+    __device__ __forceinline__ void load_raw(const void *p, int64_t row, uint32_t (&w)[grad_words<T, kElems>()]) const {
+        constexpr int W = grad_words<T, kElems>();
+        if constexpr (VEC) {
+            if (on(0)) {
+                const uint4 *q = reinterpret_cast<const uint4 *>(static_cast<const char *>(p) + (row * D + first) * elem_bytes(T));
 #pragma unroll
-        for (int e = 0; e < kElems; ++e) v[e] = p && on(e) ? load_any(p, row * D + at(e), dtype) : none;
+                for (int k = 0; k < W / 4; ++k) {
+                    const uint4 v = q[k];
+                    w[4 * k] = v.x; w[4 * k + 1] = v.y; w[4 * k + 2] = v.z; w[4 * k + 3] = v.w;
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < W; ++k) w[k] = 0;
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < W; ++k) w[k] = 0;
+#pragma unroll
+            for (int e = 0; e < kElems; ++e) {
+                if (!on(e)) continue;
+                if constexpr (T == PLE_DTYPE_F32) w[e] = static_cast<const uint32_t *>(p)[row * D + at(e)];
+                else w[e / 2] |= static_cast<uint32_t>(static_cast<const uint16_t *>(p)[row * D + at(e)]) << (16 * (e % 2));
+            }
+        }
+    }
+    // a parameter row of a type known at run time (`none` where there is none)
+    __device__ __forceinline__ void load_param(const void *p, int64_t row, int dtype, float none, float (&v)[kElems]) const {
+        if (p && dtype == PLE_DTYPE_F32) load<PLE_DTYPE_F32>(p, row, v);
+        else if (p && dtype == PLE_DTYPE_BF16) load<PLE_DTYPE_BF16>(p, row, v);
+        else if (p) load<PLE_DTYPE_F16>(p, row, v);
+        else
+#pragma unroll
+            for (int e = 0; e < kElems; ++e) v[e] = none;
+    }
+    __device__ __forceinline__ void store_param(void *p, int64_t row, int dtype, const float (&v)[kElems]) const {
+        if (dtype == PLE_DTYPE_F32) store<PLE_DTYPE_F32>(p, row, v);
+        else if (dtype == PLE_DTYPE_BF16) store<PLE_DTYPE_BF16>(p, row, v);
+        else store<PLE_DTYPE_F16>(p, row, v);
     }
 };
 
@@ -121,36 +160,50 @@ __device__ __forceinline__ void row_stats(Team<TEAM> &team, const Cols<VEC> &c, 
     rho = rsqrtf(team.sum(t) * inv + eps);
 }
 
+// A workgroup takes a contiguous range of rows, its teams every so many of them.
 template <int R, int Y, int TEAM, bool VEC>
 __global__ __launch_bounds__(Team<TEAM>::kThreads) void ple_norm_forward_kernel(NormArgs a) {
     __shared__ float s_sum[Team<TEAM>::kLdsFloats];
     Team<TEAM> team(s_sum);
     const Cols<VEC> c(team.lane(), team.lanes(), a.D);
+    const int64_t begin = static_cast<int64_t>(blockIdx.x) * a.block_rows + team.index();
+    const int64_t end = min(a.N, static_cast<int64_t>(blockIdx.x + 1) * a.block_rows);
+    if (begin >= end) return;        // (a whole team)
+    uint32_t raw_s[grad_words<R, kElems>()], raw_y[grad_words<Y, kElems>()] = {};
+    c.template load_raw<R>(a.residual, begin, raw_s);
+    if (a.branch) c.template load_raw<Y>(a.branch, begin, raw_y);
     float pw[kElems], pb[kElems], nw[kElems], nb[kElems], h[kElems];
     c.load_param(a.post_w, 0, a.param_dtype, 1.0f, pw);
     c.load_param(a.post_b, 0, a.param_dtype, 0.0f, pb);
     c.load_param(a.pre_w, 0, a.param_dtype, 1.0f, nw);
     c.load_param(a.pre_b, 0, a.param_dtype, 0.0f, nb);
-    c.load_param(a.gates == 1 ? a.gate : nullptr, 0, a.param_dtype, 1.0f, h);
-    if (a.gates == 1)
-#pragma unroll
-        for (int e = 0; e < kElems; ++e) h[e] = gate_value(h[e], a.act);
-    const int64_t teams = static_cast<int64_t>(gridDim.x) * team.per_block();
-    for (int64_t n = static_cast<int64_t>(blockIdx.x) * team.per_block() + team.index(); n < a.N; n += teams) {
+    c.load_param(nullptr, 0, a.param_dtype, 1.0f, h);
+    int64_t gate_end = a.gates ? 0 : a.N;        // rows up to here have the gate row in h
+    for (int64_t n = begin; n < end; n += team.per_block()) {
+        uint32_t next_s[grad_words<R, kElems>()] = {}, next_y[grad_words<Y, kElems>()] = {};
+        if (n + team.per_block() < end) {
+            c.template load_raw<R>(a.residual, n + team.per_block(), next_s);
+            if (a.branch) c.template load_raw<Y>(a.branch, n + team.per_block(), next_y);
+        }
         float4 st = make_float4(0.0f, 1.0f, 0.0f, 1.0f);
         float s[kElems], v[kElems];
-        c.template load<R>(a.residual, n, s);
+#pragma unroll
+        for (int e = 0; e < kElems; ++e) {
+            s[e] = grad_elem<R>(raw_s, e);
+            v[e] = grad_elem<Y>(raw_y, e);
+        }
         if (a.branch) {
-            c.template load<Y>(a.branch, n, v);
+            if (n >= gate_end) {
+                const int64_t row = n / a.rows_per_gate;
+                gate_end = (row + 1) * a.rows_per_gate;
+                c.load_param(a.gate, row, a.param_dtype, 1.0f, h);
+#pragma unroll
+                for (int e = 0; e < kElems; ++e) h[e] = gate_value(h[e], a.act);
+            }
             if (a.post != PLE_NORM_NONE) {
                 row_stats(team, c, v, a.post, a.eps, st.x, st.y);
 #pragma unroll
                 for (int e = 0; e < kElems; ++e) v[e] = (v[e] - st.x) * st.y * pw[e] + pb[e];
-            }
-            if (a.gates > 1) {
-                c.load_param(a.gate, n / a.rows_per_gate, a.param_dtype, 1.0f, h);
-#pragma unroll
-                for (int e = 0; e < kElems; ++e) h[e] = gate_value(h[e], a.act);
             }
 #pragma unroll
             for (int e = 0; e < kElems; ++e) s[e] = c.on(e) ? quant<R>(a.alpha * s[e] + h[e] * v[e]) : 0.0f;
@@ -163,6 +216,10 @@ __global__ __launch_bounds__(Team<TEAM>::kThreads) void ple_norm_forward_kernel(
             c.template store<Y>(a.normed, n, v);
         }
         if (team.lane() == 0) a.stats[n] = st;
+#pragma unroll
+        for (int k = 0; k < grad_words<R, kElems>(); ++k) raw_s[k] = next_s[k];
+#pragma unroll
+        for (int k = 0; k < grad_words<Y, kElems>(); ++k) raw_y[k] = next_y[k];
     }
 }
 
@@ -184,6 +241,26 @@ __device__ __forceinline__ void norm_grad(Team<TEAM> &team, const Cols<VEC> &c, 
     for (int e = 0; e < kElems; ++e) g[e] = rho * (g[e] - mean - xh[e] * proj);
 }
 
+// A row's inputs of the backward, as loaded.
+template <int R, int Y>
+struct BackRow {
+    uint32_t ds[grad_words<R, kElems>()], x[grad_words<R, kElems>()];
+    uint32_t gn[grad_words<Y, kElems>()], y[grad_words<Y, kElems>()];
+    float4 st;
+    template <bool VEC>
+    __device__ __forceinline__ void load(const NormArgs &a, const Cols<VEC> &c, int64_t n) {
+        if (a.g_stream) c.template load_raw<R>(a.g_stream, n, ds);
+        if (a.g_normed) {
+            c.template load_raw<Y>(a.g_normed, n, gn);
+            c.template load_raw<R>(a.residual, n, x);
+        }
+        if (a.branch) c.template load_raw<Y>(a.branch, n, y);
+        st = a.stats[n];
+    }
+};
+
+// Teams walk units of rows: a row each, or a piece of the rows of one gate, whose
+// sum is finished with the piece.
 template <int R, int Y, int TEAM, bool VEC>
 __global__ __launch_bounds__(Team<TEAM>::kThreads) void ple_norm_backward_kernel(NormArgs a) {
     constexpr int kTeams = Team<TEAM>::kBlockWide ? 1 : kBlock / TEAM;
@@ -191,43 +268,61 @@ __global__ __launch_bounds__(Team<TEAM>::kThreads) void ple_norm_backward_kernel
     __shared__ float s_cols[kTeams > 1 ? kBlock * kElems : 1];
     Team<TEAM> team(s_sum);
     const Cols<VEC> c(team.lane(), team.lanes(), a.D);
+    const int64_t teams = static_cast<int64_t>(gridDim.x) * team.per_block();
+    const int64_t units = a.gates == 2 ? (a.N / a.rows_per_gate) * a.pieces : a.N;
+    int64_t u = static_cast<int64_t>(blockIdx.x) * team.per_block() + team.index(), n = 0, stop = 0;
+    const auto enter = [&] {         // the rows of unit u
+        if (a.gates == 2) {
+            const int64_t group = u / a.pieces, piece = u - group * a.pieces;
+            n = group * a.rows_per_gate + piece * a.piece_rows;
+            stop = min(n + a.piece_rows, (group + 1) * a.rows_per_gate);
+        } else {
+            n = u;
+            stop = u + 1;
+        }
+    };
+    BackRow<R, Y> now{}, next{};
+    if (u < units) {
+        enter();
+        now.load(a, c, n);
+    }
     float pw[kElems], pb[kElems], nw[kElems], h[kElems];
     c.load_param(a.post_w, 0, a.param_dtype, 1.0f, pw);
     c.load_param(a.post_b, 0, a.param_dtype, 0.0f, pb);
     c.load_param(a.pre_w, 0, a.param_dtype, 1.0f, nw);
-    c.load_param(a.gates == 1 ? a.gate : nullptr, 0, a.param_dtype, 1.0f, h);
-    if (a.gates == 1)
+    const auto load_gate = [&](int64_t row) {
+        c.load_param(a.gate, row, a.param_dtype, 1.0f, h);
 #pragma unroll
         for (int e = 0; e < kElems; ++e) h[e] = gate_value(h[e], a.act);
+    };
+    if (a.gates < 2) {
+        if (a.gates == 1) load_gate(0);
+        else c.load_param(nullptr, 0, a.param_dtype, 1.0f, h);
+    }
     float s_pw[kElems] = {}, s_pb[kElems] = {}, s_g[kElems] = {}, s_nw[kElems] = {}, s_nb[kElems] = {};
-    const int64_t teams = static_cast<int64_t>(gridDim.x) * team.per_block();
-    const int64_t units = a.gates == 2 ? (a.N / a.rows_per_gate) * a.pieces : a.N;
-    for (int64_t u = static_cast<int64_t>(blockIdx.x) * team.per_block() + team.index(); u < units; u += teams) {
-        int64_t row = u, stop = u + 1;
-        if (a.gates == 2) {
-            const int64_t group = u / a.pieces, piece = u - group * a.pieces;
-            row = group * a.rows_per_gate + piece * a.piece_rows;
-            stop = min(row + a.piece_rows, (group + 1) * a.rows_per_gate);
-            c.load_param(a.gate, group, a.param_dtype, 1.0f, h);
-        } else if (a.gates == 3) {
-            c.load_param(a.gate, u, a.param_dtype, 1.0f, h);
-        }
-        if (a.gates > 1)
+    while (u < units) {
+        const int64_t unit = u;
+        if (a.gates > 1) {
+            load_gate(a.gates == 2 ? unit / a.pieces : unit);
 #pragma unroll
-            for (int e = 0; e < kElems; ++e) {
-                h[e] = gate_value(h[e], a.act);
-                s_g[e] = 0.0f;
+            for (int e = 0; e < kElems; ++e) s_g[e] = 0.0f;
+        }
+        do {
+            const int64_t row = n;
+            if (++n == stop) {
+                u += teams;
+                if (u < units) enter();
             }
-        for (int64_t n = row; n < stop; ++n) {
-            const float4 st = a.stats[n];
-            float ds[kElems] = {}, xh[kElems], g[kElems];
-            if (a.g_stream) c.template load<R>(a.g_stream, n, ds);
+            if (u < units) next.load(a, c, n);
+            const float4 st = now.st;
+            float ds[kElems], xh[kElems], g[kElems];
+#pragma unroll
+            for (int e = 0; e < kElems; ++e) ds[e] = grad_elem<R>(now.ds, e);
             if (a.g_normed) {
-                c.template load<Y>(a.g_normed, n, g);
-                c.template load<R>(a.residual, n, xh);
 #pragma unroll
                 for (int e = 0; e < kElems; ++e) {
-                    xh[e] = c.on(e) ? (xh[e] - st.z) * st.w : 0.0f;
+                    g[e] = grad_elem<Y>(now.gn, e);
+                    xh[e] = c.on(e) ? (grad_elem<R>(now.x, e) - st.z) * st.w : 0.0f;
                     s_nw[e] += g[e] * xh[e];
                     s_nb[e] += g[e];
                     g[e] *= nw[e];
@@ -239,38 +334,39 @@ __global__ __launch_bounds__(Team<TEAM>::kThreads) void ple_norm_backward_kernel
             if (a.d_residual) {
 #pragma unroll
                 for (int e = 0; e < kElems; ++e) g[e] = a.alpha * ds[e];
-                c.template store<R>(a.d_residual, n, g);
+                c.template store<R>(a.d_residual, row, g);
             }
-            if (!a.branch) continue;
-            c.template load<Y>(a.branch, n, xh);
-            if (a.post != PLE_NORM_NONE) {
+            if (a.branch) {
 #pragma unroll
-                for (int e = 0; e < kElems; ++e) {
-                    xh[e] = c.on(e) ? (xh[e] - st.x) * st.y : 0.0f;
-                    g[e] = c.on(e) ? ds[e] * h[e] : 0.0f;
-                    s_g[e] += ds[e] * (xh[e] * pw[e] + pb[e]);
-                    s_pw[e] += g[e] * xh[e];
-                    s_pb[e] += g[e];
-                    g[e] *= pw[e];
-                }
-                norm_grad(team, c, g, xh, st.y, a.post);
-            } else {
+                for (int e = 0; e < kElems; ++e) xh[e] = grad_elem<Y>(now.y, e);
+                if (a.post != PLE_NORM_NONE) {
 #pragma unroll
-                for (int e = 0; e < kElems; ++e) {
-                    g[e] = ds[e] * h[e];
-                    s_g[e] += ds[e] * xh[e];
+                    for (int e = 0; e < kElems; ++e) {
+                        xh[e] = c.on(e) ? (xh[e] - st.x) * st.y : 0.0f;
+                        g[e] = c.on(e) ? ds[e] * h[e] : 0.0f;
+                        s_g[e] += ds[e] * (xh[e] * pw[e] + pb[e]);
+                        s_pw[e] += g[e] * xh[e];
+                        s_pb[e] += g[e];
+                        g[e] *= pw[e];
+                    }
+                    norm_grad(team, c, g, xh, st.y, a.post);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < kElems; ++e) {
+                        g[e] = ds[e] * h[e];
+                        s_g[e] += ds[e] * xh[e];
+                    }
                 }
+                if (a.d_branch) c.template store<Y>(a.d_branch, row, g);
             }
-            if (a.d_branch) c.template store<Y>(a.d_branch, n, g);
-        }
+            now = next;
+        } while (u == unit);
         if (a.gates > 1 && a.d_gate) {
+            float v[kElems];
 #pragma unroll
-            for (int e = 0; e < kElems; ++e) {
-                if (!c.on(e)) continue;
-                const float v = s_g[e] * gate_slope(h[e], a.act);
-                if (a.gates == 3 || a.pieces == 1) store_any(a.d_gate, u * a.D + c.at(e), v, a.param_dtype);
-                else a.gate_partial[u * a.D + c.at(e)] = v;
-            }
+            for (int e = 0; e < kElems; ++e) v[e] = s_g[e] * gate_slope(h[e], a.act);
+            if (a.gates == 3 || a.pieces == 1) c.store_param(a.d_gate, unit, a.param_dtype, v);
+            else c.template store<PLE_DTYPE_F32>(a.gate_partial, unit, v);
         }
     }
     if (a.gates == 1)
@@ -299,7 +395,8 @@ __global__ __launch_bounds__(Team<TEAM>::kThreads) void ple_norm_backward_kernel
 }
 
 // out[j, d] = sum over the parts of partial[part, j, d]; 64 columns a workgroup,
-// its waves taking every fourth part each.
+// its waves a part each in turn.
+constexpr int kJoinWaves = 16;
 constexpr int kMaxSums = 5;
 
 struct JoinArgs {
@@ -309,19 +406,19 @@ struct JoinArgs {
     int parts, D, param_dtype, stacked, colblocks;
 };
 
-__global__ __launch_bounds__(kBlock) void ple_norm_join_kernel(JoinArgs a) {
-    __shared__ float s_sum[kBlock];
+__global__ __launch_bounds__(kJoinWaves * kWave) void ple_norm_join_kernel(JoinArgs a) {
+    __shared__ float s_sum[kJoinWaves * kWave];
     const int wave = threadIdx.x / kWave, d = blockIdx.x % a.colblocks * kWave + threadIdx.x % kWave;
     const int64_t j = blockIdx.x / a.colblocks;
     float v = 0.0f;
     if (d < a.D) {
 #pragma unroll 8
-        for (int p = wave; p < a.parts; p += kWavesPerBlock) v += a.partial[p * a.part_stride + j * a.sum_stride + d];
+        for (int p = wave; p < a.parts; p += kJoinWaves) v += a.partial[p * a.part_stride + j * a.sum_stride + d];
     }
     s_sum[threadIdx.x] = v;
     __syncthreads();
     if (wave == 0 && d < a.D) {
-        for (int w = 1; w < kWavesPerBlock; ++w) v += s_sum[w * kWave + threadIdx.x];
+        for (int w = 1; w < kJoinWaves; ++w) v += s_sum[w * kWave + threadIdx.x];
         if (a.stacked) store_any(a.out[0], j * a.D + d, v, a.param_dtype);
         else store_any(a.out[j], d, v, a.param_dtype);
     }
@@ -354,7 +451,8 @@ NormPlan plan_norm(const NormRequest &r) {
     p.vec = r.D % kElems == 0;
     for (const void *q : {r.residual, r.branch, r.g_stream, r.g_normed, static_cast<const void *>(r.stream_out),
                           static_cast<const void *>(r.normed), static_cast<const void *>(r.d_residual),
-                          static_cast<const void *>(r.d_branch)})
+                          static_cast<const void *>(r.d_branch), r.post_w, r.post_b, r.gate, r.pre_w, r.pre_b,
+                          static_cast<const void *>(r.d_gate)})
         p.vec = p.vec && reinterpret_cast<uintptr_t>(q) % 16 == 0;
     const int mode = gate_mode(r);
     const int most = device_cu_count() * std::max(1, 1024 / p.threads);
@@ -426,11 +524,11 @@ int norm_zero_gradients(const NormRequest &r) {
     int sums = 0;
     for (void *p : {r.d_post_w, r.d_post_b, r.d_pre_w, r.d_pre_b})
         if (p) j.out[sums++] = p;
-    if (sums > 0) hipLaunchKernelGGL(ple_norm_join_kernel, dim3(j.colblocks * sums), dim3(kBlock), 0, r.stream, j);
+    if (sums > 0) hipLaunchKernelGGL(ple_norm_join_kernel, dim3(j.colblocks * sums), dim3(kJoinWaves * kWave), 0, r.stream, j);
     if (r.d_gate) {
         j.out[0] = r.d_gate;
         j.stacked = 1;
-        hipLaunchKernelGGL(ple_norm_join_kernel, dim3(static_cast<unsigned>(j.colblocks * r.groups)), dim3(kBlock), 0,
+        hipLaunchKernelGGL(ple_norm_join_kernel, dim3(static_cast<unsigned>(j.colblocks * r.groups)), dim3(kJoinWaves * kWave), 0,
                            r.stream, j);
     }
     return static_cast<int>(hipGetLastError());
@@ -441,9 +539,11 @@ int norm_zero_gradients(const NormRequest &r) {
 int norm_run(const NormRequest &r) {
     if (r.D > kMaxD) return PLE_E_TOO_LARGE;
     const NormPlan p = plan_norm(r);
-    const NormArgs a = norm_args(r);
+    NormArgs a = norm_args(r);
     const int64_t most = static_cast<int64_t>(device_cu_count()) * std::max(1, 2048 / p.threads);
-    const dim3 grid(static_cast<unsigned>(std::min(most, (r.N + p.per_block - 1) / p.per_block)));
+    const int64_t steps = (r.N + p.per_block - 1) / p.per_block;
+    a.block_rows = (steps + most - 1) / most * p.per_block;
+    const dim3 grid(static_cast<unsigned>((r.N + a.block_rows - 1) / a.block_rows));
     return static_cast<int>(with_norm(r, p, [&](auto st, auto br, auto team, auto vec) {
         hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_norm_forward_kernel<decltype(st)::value, decltype(br)::value,
                                                                    decltype(team)::value, decltype(vec)::value>),
@@ -491,7 +591,7 @@ int norm_backward_run(const NormRequest &r) {
         j.part_stride = static_cast<int64_t>(a.slots) * a.D;
         j.sum_stride = a.D;
         j.parts = p.blocks;
-        hipLaunchKernelGGL(ple_norm_join_kernel, dim3(j.colblocks * a.slots), dim3(kBlock), 0, r.stream, j);
+        hipLaunchKernelGGL(ple_norm_join_kernel, dim3(j.colblocks * a.slots), dim3(kJoinWaves * kWave), 0, r.stream, j);
     }
     if (a.gates == 2 && a.d_gate && p.pieces > 1) {
         j.partial = a.gate_partial;
@@ -500,7 +600,7 @@ int norm_backward_run(const NormRequest &r) {
         j.parts = static_cast<int>(p.pieces);
         j.out[0] = r.d_gate;
         j.stacked = 1;
-        hipLaunchKernelGGL(ple_norm_join_kernel, dim3(static_cast<unsigned>(j.colblocks * r.groups)), dim3(kBlock), 0,
+        hipLaunchKernelGGL(ple_norm_join_kernel, dim3(static_cast<unsigned>(j.colblocks * r.groups)), dim3(kJoinWaves * kWave), 0,
                            r.stream, j);
     }
     return static_cast<int>(hipGetLastError());
