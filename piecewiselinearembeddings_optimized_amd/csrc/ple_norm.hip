@@ -259,13 +259,57 @@ struct BackRow {
     }
 };
 
+// A lane's elements of a parameter row over all of its rows: in registers, or
+// (LDS) in a place of its own in LDS, two 16-byte reads a use.  The registers of
+// wide teams are what keeps a second workgroup off the CU.
+template <bool LDS>
+struct Held {
+    float v[LDS ? 1 : kElems];
+    float none = 0.0f;
+    float4 *place = nullptr;
+    __device__ __forceinline__ void set(const float (&from)[kElems], float *&lds, bool given, float otherwise) {
+        if constexpr (LDS) {
+            none = otherwise;
+            if (!given) return;
+            place = reinterpret_cast<float4 *>(lds) + threadIdx.x;
+            lds += blockDim.x * kElems;
+            place[0] = make_float4(from[0], from[1], from[2], from[3]);
+            place[blockDim.x] = make_float4(from[4], from[5], from[6], from[7]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < kElems; ++e) v[e] = from[e];
+        }
+    }
+    __device__ __forceinline__ void get(float (&to)[kElems]) const {
+        if constexpr (LDS) {
+            if (place) {
+                const float4 a = place[0], b = place[blockDim.x];
+                to[0] = a.x; to[1] = a.y; to[2] = a.z; to[3] = a.w;
+                to[4] = b.x; to[5] = b.y; to[6] = b.z; to[7] = b.w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < kElems; ++e) to[e] = none;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < kElems; ++e) to[e] = v[e];
+        }
+    }
+};
+
+// Waves a SIMD the backward of wide rows is compiled for (its registers: 128, 168
+// or 256).
+constexpr int backward_waves(bool vec, bool bias) { return !vec ? 2 : bias ? 3 : 4; }
+
 // Teams walk units of rows: a row each, or a piece of the rows of one gate, whose
-// sum is finished with the piece.
-template <int R, int Y, int TEAM, bool VEC>
-__global__ __launch_bounds__(Team<TEAM>::kThreads) void ple_norm_backward_kernel(NormArgs a) {
+// sum is finished with the piece.  BIAS: the norms may have biases.  OWN: rows or
+// groups of them have gates of their own.
+template <int R, int Y, int TEAM, bool VEC, bool BIAS, bool OWN>
+__global__ __launch_bounds__(Team<TEAM>::kThreads, TEAM == 512 ? backward_waves(VEC, BIAS) : 1) void ple_norm_backward_kernel(NormArgs a) {
     constexpr int kTeams = Team<TEAM>::kBlockWide ? 1 : kBlock / TEAM;
     __shared__ float s_sum[Team<TEAM>::kLdsFloats];
     __shared__ float s_cols[kTeams > 1 ? kBlock * kElems : 1];
+    extern __shared__ float s_params[];
     Team<TEAM> team(s_sum);
     const Cols<VEC> c(team.lane(), team.lanes(), a.D);
     const int64_t teams = static_cast<int64_t>(gridDim.x) * team.per_block();
@@ -286,26 +330,37 @@ __global__ __launch_bounds__(Team<TEAM>::kThreads) void ple_norm_backward_kernel
         enter();
         now.load(a, c, n);
     }
-    float pw[kElems], pb[kElems], nw[kElems], h[kElems];
-    c.load_param(a.post_w, 0, a.param_dtype, 1.0f, pw);
-    c.load_param(a.post_b, 0, a.param_dtype, 0.0f, pb);
-    c.load_param(a.pre_w, 0, a.param_dtype, 1.0f, nw);
-    const auto load_gate = [&](int64_t row) {
-        c.load_param(a.gate, row, a.param_dtype, 1.0f, h);
+    Held<Team<TEAM>::kBlockWide> post_w, post_b, pre_w, gate;
+    float h[kElems];                 // OWN: of the unit's rows
+    {
+        float *lds = s_params, v[kElems];
+        c.load_param(a.post_w, 0, a.param_dtype, 1.0f, v);
+        post_w.set(v, lds, a.post_w != nullptr, 1.0f);
+        if constexpr (BIAS) {
+            c.load_param(a.post_b, 0, a.param_dtype, 0.0f, v);
+            post_b.set(v, lds, a.post_b != nullptr, 0.0f);
+        }
+        c.load_param(a.pre_w, 0, a.param_dtype, 1.0f, v);
+        pre_w.set(v, lds, a.pre_w != nullptr, 1.0f);
+        if constexpr (!OWN) {
+            c.load_param(a.gate, 0, a.param_dtype, 1.0f, v);
+            if (a.gates)
 #pragma unroll
-        for (int e = 0; e < kElems; ++e) h[e] = gate_value(h[e], a.act);
-    };
-    if (a.gates < 2) {
-        if (a.gates == 1) load_gate(0);
-        else c.load_param(nullptr, 0, a.param_dtype, 1.0f, h);
+                for (int e = 0; e < kElems; ++e) v[e] = gate_value(v[e], a.act);
+            gate.set(v, lds, a.gates != 0, 1.0f);
+        }
     }
-    float s_pw[kElems] = {}, s_pb[kElems] = {}, s_g[kElems] = {}, s_nw[kElems] = {}, s_nb[kElems] = {};
+    float s_pw[kElems] = {}, s_g[kElems] = {}, s_nw[kElems] = {};
+    float s_pb[BIAS ? kElems : 1] = {}, s_nb[BIAS ? kElems : 1] = {};
     while (u < units) {
         const int64_t unit = u;
-        if (a.gates > 1) {
-            load_gate(a.gates == 2 ? unit / a.pieces : unit);
+        if constexpr (OWN) {
+            c.load_param(a.gate, a.gates == 2 ? unit / a.pieces : unit, a.param_dtype, 1.0f, h);
 #pragma unroll
-            for (int e = 0; e < kElems; ++e) s_g[e] = 0.0f;
+            for (int e = 0; e < kElems; ++e) {
+                h[e] = gate_value(h[e], a.act);
+                s_g[e] = 0.0f;
+            }
         }
         do {
             const int64_t row = n;
@@ -319,13 +374,15 @@ __global__ __launch_bounds__(Team<TEAM>::kThreads) void ple_norm_backward_kernel
 #pragma unroll
             for (int e = 0; e < kElems; ++e) ds[e] = grad_elem<R>(now.ds, e);
             if (a.g_normed) {
+                float w[kElems];
+                pre_w.get(w);
 #pragma unroll
                 for (int e = 0; e < kElems; ++e) {
                     g[e] = grad_elem<Y>(now.gn, e);
                     xh[e] = c.on(e) ? (grad_elem<R>(now.x, e) - st.z) * st.w : 0.0f;
                     s_nw[e] += g[e] * xh[e];
-                    s_nb[e] += g[e];
-                    g[e] *= nw[e];
+                    if constexpr (BIAS) s_nb[e] += g[e];
+                    g[e] *= w[e];
                 }
                 norm_grad(team, c, g, xh, st.w, a.pre);
 #pragma unroll
@@ -337,17 +394,21 @@ __global__ __launch_bounds__(Team<TEAM>::kThreads) void ple_norm_backward_kernel
                 c.template store<R>(a.d_residual, row, g);
             }
             if (a.branch) {
+                if constexpr (!OWN) gate.get(h);
 #pragma unroll
                 for (int e = 0; e < kElems; ++e) xh[e] = grad_elem<Y>(now.y, e);
                 if (a.post != PLE_NORM_NONE) {
+                    float w[kElems], b[kElems];
+                    post_w.get(w);
+                    if constexpr (BIAS) post_b.get(b);
 #pragma unroll
                     for (int e = 0; e < kElems; ++e) {
                         xh[e] = c.on(e) ? (xh[e] - st.x) * st.y : 0.0f;
                         g[e] = c.on(e) ? ds[e] * h[e] : 0.0f;
-                        s_g[e] += ds[e] * (xh[e] * pw[e] + pb[e]);
+                        s_g[e] += ds[e] * (BIAS ? xh[e] * w[e] + b[e] : xh[e] * w[e]);
                         s_pw[e] += g[e] * xh[e];
-                        s_pb[e] += g[e];
-                        g[e] *= pw[e];
+                        if constexpr (BIAS) s_pb[e] += g[e];
+                        g[e] *= w[e];
                     }
                     norm_grad(team, c, g, xh, st.y, a.post);
                 } else {
@@ -361,7 +422,8 @@ __global__ __launch_bounds__(Team<TEAM>::kThreads) void ple_norm_backward_kernel
             }
             now = next;
         } while (u == unit);
-        if (a.gates > 1 && a.d_gate) {
+        if constexpr (OWN) {
+            if (!a.d_gate) continue;
             float v[kElems];
 #pragma unroll
             for (int e = 0; e < kElems; ++e) v[e] = s_g[e] * gate_slope(h[e], a.act);
@@ -369,9 +431,11 @@ __global__ __launch_bounds__(Team<TEAM>::kThreads) void ple_norm_backward_kernel
             else c.template store<PLE_DTYPE_F32>(a.gate_partial, unit, v);
         }
     }
-    if (a.gates == 1)
+    if constexpr (!OWN) {
+        gate.get(h);
 #pragma unroll
         for (int e = 0; e < kElems; ++e) s_g[e] *= gate_slope(h[e], a.act);
+    }
     const auto leave = [&](float (&v)[kElems], int slot) {
         if (slot < 0) return;
         if constexpr (kTeams > 1) {
@@ -388,10 +452,12 @@ __global__ __launch_bounds__(Team<TEAM>::kThreads) void ple_norm_backward_kernel
             c.template store<PLE_DTYPE_F32>(a.partial, static_cast<int64_t>(blockIdx.x) * a.slots + slot, v);
     };
     leave(s_pw, a.slot_pw);
-    leave(s_pb, a.slot_pb);
-    leave(s_g, a.slot_g);
     leave(s_nw, a.slot_nw);
-    leave(s_nb, a.slot_nb);
+    if constexpr (!OWN) leave(s_g, a.slot_g);
+    if constexpr (BIAS) {
+        leave(s_pb, a.slot_pb);
+        leave(s_nb, a.slot_nb);
+    }
 }
 
 // out[j, d] = sum over the parts of partial[part, j, d]; 64 columns a workgroup,
@@ -433,7 +499,7 @@ struct NormPlan {
     int blocks;                          // backward workgroups
     int64_t piece_rows, pieces;
     int slots;
-    size_t o_gate, bytes;
+    size_t lds, o_gate, bytes;
 };
 
 int gate_mode(const NormRequest &r) {
@@ -455,14 +521,37 @@ NormPlan plan_norm(const NormRequest &r) {
                           static_cast<const void *>(r.d_gate)})
         p.vec = p.vec && reinterpret_cast<uintptr_t>(q) % 16 == 0;
     const int mode = gate_mode(r);
-    const int most = device_cu_count() * std::max(1, 1024 / p.threads);
+    // as many backward workgroups as run at once (a few more leave most of the GPU
+    // idle at the end): by the waves a SIMD has registers for, where workgroups of
+    // an odd number of waves fill the four SIMDs as the next multiple of four does
+    // (3 waves of 168 registers: 768 workgroups took 175 us where 1024 took 228,
+    // 32800 x 1152), and by LDS
+    const bool bias = r.post_b || r.pre_b;
+    const int simd_waves = p.team == 1024 ? 4 : p.team < 512 ? (bias ? 2 : 3) : backward_waves(p.vec, bias);
+    const int block_waves = p.threads / kWave;
+    const int filled = block_waves <= 2 ? block_waves : (block_waves + 3) / 4 * 4;
+    p.lds = p.team > kWave ? static_cast<size_t>((r.post_w != nullptr) + (r.post_b != nullptr) + (r.pre_w != nullptr) +
+                                                 (mode == 1)) * p.threads * kElems * 4 : 0;
+    const int by_lds = p.lds > 0 ? static_cast<int>(kLdsMax / (p.lds + 1024)) : 8;
+    const int most = device_cu_count() * std::max(1, std::min(4 * simd_waves / filled, by_lds));
     const int64_t teams = static_cast<int64_t>(most) * p.per_block;
     int64_t units = r.N;
     p.piece_rows = p.pieces = 1;
     if (mode == 2) {
         const int64_t rows = r.N / r.groups;
-        p.piece_rows = std::min(rows, std::max<int64_t>(4, (r.N + 4 * teams - 1) / (4 * teams)));
-        p.pieces = (rows + p.piece_rows - 1) / p.piece_rows;
+        // pieces of a gate's rows such that the teams have about one to four each,
+        // the most rows a team gets being the fewest
+        int64_t best = INT64_MAX;
+        for (int64_t k = 1; k <= 4; ++k) {
+            const int64_t want = std::min(rows, std::max<int64_t>(1, k * teams / r.groups));
+            const int64_t size = (rows + want - 1) / want, pieces = (rows + size - 1) / size;
+            const int64_t cost = (r.groups * pieces + teams - 1) / teams * (size + 1);
+            if (cost < best) {
+                best = cost;
+                p.piece_rows = size;
+                p.pieces = pieces;
+            }
+        }
         units = r.groups * p.pieces;
     }
     p.blocks = static_cast<int>(std::min<int64_t>(most, std::max<int64_t>(1, (units + p.per_block - 1) / p.per_block)));
@@ -576,11 +665,17 @@ int norm_backward_run(const NormRequest &r) {
     a.slot_g = slot(a.gates == 1 ? r.gate : nullptr, r.d_gate);
     a.slot_nw = slot(r.pre_w, r.d_pre_w);
     a.slot_nb = slot(r.pre_b, r.d_pre_b);
+    const bool bias = r.post_b || r.pre_b, own = a.gates > 1;
     const hipError_t rc = with_norm(r, p, [&](auto st, auto br, auto team, auto vec) {
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_norm_backward_kernel<decltype(st)::value, decltype(br)::value,
-                                                                    decltype(team)::value, decltype(vec)::value>),
-                           dim3(p.blocks), dim3(p.threads), 0, r.stream, a);
-        return hipGetLastError();
+        const auto launch = [&](auto has_bias, auto has_own) {
+            hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_norm_backward_kernel<decltype(st)::value, decltype(br)::value,
+                                                                        decltype(team)::value, decltype(vec)::value,
+                                                                        decltype(has_bias)::value, decltype(has_own)::value>),
+                               dim3(p.blocks), dim3(p.threads), p.lds, r.stream, a);
+            return hipGetLastError();
+        };
+        if (bias) return own ? launch(std::true_type{}, std::true_type{}) : launch(std::true_type{}, std::false_type{});
+        return own ? launch(std::false_type{}, std::true_type{}) : launch(std::false_type{}, std::false_type{});
     });
     if (rc != hipSuccess) return static_cast<int>(rc);
     j.D = a.D;
