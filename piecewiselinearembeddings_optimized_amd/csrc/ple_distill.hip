@@ -18,8 +18,13 @@
 // sums at both temperatures; the backward reads it once and writes dz once:
 // every class gets the formula without its sparse terms in a dense pass, and
 // the K classes and the label are then computed whole and written over it.
-// Classes outside the K are told by a bit each in LDS, so that Q is a sum of
-// its own terms and not a difference.
+// With a given l the dense sums leave the K classes out, by a bit for each class
+// in LDS, and their own K terms are added: Q is a sum of its own terms and not a
+// difference.
+//
+// At T = 2 and T = 4 the exponentials of both temperatures are one: exp(x) is
+// exp(x / T) squared once or twice.  (One exponential a class less, at a
+// quarter of the rate of other operations.)
 //
 // A row belongs to a team of lanes (part of a wave, a wave or a workgroup);
 // where there are few rows of many classes, to several workgroups, each a range
@@ -82,38 +87,86 @@ struct Range {
     __device__ __forceinline__ int odd_at(int i) const { return i < head ? c0 + i : c0 + vectors() * kVec + i; }
 };
 
+// Vectors of z that a lane has in flight.
+constexpr int kUnroll = 4;
+
+// A vector of z as loaded: VEC elements of type Z.
+template <int Z, int VEC>
+struct Words {
+    uint32_t w[grad_words<Z, VEC>()];
+    __device__ __forceinline__ void load(const void *z, int64_t i) {
+        if constexpr (VEC == 1) {
+            if constexpr (Z == PLE_DTYPE_F32) w[0] = static_cast<const uint32_t *>(z)[i];
+            else w[0] = static_cast<const uint16_t *>(z)[i];
+        } else {
+            const uint4 v = *reinterpret_cast<const uint4 *>(static_cast<const char *>(z) + i * elem_bytes(Z));
+            w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+        }
+    }
+    __device__ __forceinline__ float at(int e) const { return grad_elem<Z>(w, e); }
+};
+
+// The sums of a row: at T alone, at 1 too, or at 1 by squaring those at T.
+enum { kOneSum, kTwoSums, kOneSquare, kTwoSquares };
+
+template <int SUMS>
+__device__ __forceinline__ float at_one(float x) {       // exp(v - m) from exp((v - m) / T)
+    x *= x;
+    return SUMS == kTwoSquares ? x * x : x;
+}
+
 // Running maximum and sums of a lane.  The maximum starts at the lowest number,
 // not at -inf: a class of -inf then adds exp(-inf) = 0 without a NaN.
-template <bool BOTH>
+template <int SUMS>
 struct Sums {
-    float m = -FLT_MAX, at_t = 0.0f, at_1 = 0.0f, outside = 0.0f;
+    float m = -FLT_MAX, at_t = 0.0f, at_1 = 0.0f;
     __device__ __forceinline__ void rescale(float to, float ct) {
-        const float f = exp2_fast((m - to) * ct);
-        at_t *= f;
-        outside *= f;
-        if constexpr (BOTH) at_1 *= exp2_fast((m - to) * kLog2e);
+        at_t *= exp2_fast((m - to) * ct);
+        if constexpr (SUMS != kOneSum) at_1 *= exp2_fast((m - to) * kLog2e);
         m = to;
     }
-    template <int VEC>
-    __device__ __forceinline__ void add(const float *v, uint32_t inside, float ct) {
-        float top = v[0];
+    // adds N vectors without the classes of `skip` (bit e: element e)
+    template <int N, int Z, int VEC>
+    __device__ __forceinline__ void add(const Words<Z, VEC> (&w)[N], const uint32_t (&skip)[N], float ct) {
+        float v[N][VEC], top = w[0].at(0);
 #pragma unroll
-        for (int e = 1; e < VEC; ++e) top = fmaxf(top, v[e]);
+        for (int k = 0; k < N; ++k)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                v[k][e] = w[k].at(e);
+                top = fmaxf(top, v[k][e]);
+            }
         if (top > m) rescale(top, ct);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const float x = exp2_fast((v[e] - m) * ct);
-            at_t += x;
-            outside += (inside >> e) & 1 ? 0.0f : x;
-            if constexpr (BOTH) at_1 += exp2_fast((v[e] - m) * kLog2e);
+        for (int k = 0; k < N; ++k)
+            if (skip[k])
+#pragma unroll
+                for (int e = 0; e < VEC; ++e)
+                    if ((skip[k] >> e) & 1) v[k][e] = -__builtin_inff();
+        // (a sum of its own for every vector: their additions overlap)
+        float part[N], part_1[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            part[k] = part_1[k] = 0.0f;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float d = v[k][e] - m, x = exp2_fast(d * ct);
+                part[k] += x;
+                if constexpr (SUMS == kTwoSums) part_1[k] += exp2_fast(d * kLog2e);
+                else if constexpr (SUMS != kOneSum) part_1[k] += at_one<SUMS>(x);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            at_t += part[k];
+            at_1 += part_1[k];
         }
     }
     template <int TEAM>
     __device__ __forceinline__ void join(Team<TEAM> &team, float ct) {
         rescale(team.max(m), ct);
-        team.sum2(at_t, outside);
-        if constexpr (BOTH) at_1 = team.sum(at_1);
-        else at_1 = at_t;
+        team.sum2(at_t, at_1);
+        if constexpr (SUMS == kOneSum) at_1 = at_t;
     }
 };
 
@@ -137,68 +190,114 @@ __device__ __forceinline__ bool mark_classes(Team<TEAM> &team, const DistillArgs
     return *twice != 0;
 }
 
-template <int Z, int TEAM, bool BOTH>
+template <int Z, int TEAM, int SUMS>
 __device__ __forceinline__ void scan_row(Team<TEAM> &team, const DistillArgs &a, const Range<Z, true> &r, const uint32_t *bits,
-                                         float ct, Sums<BOTH> &s) {
+                                         float ct, Sums<SUMS> &s) {
     constexpr int kVec = Range<Z, true>::kVec;
     const auto inside = [&](int c, int n) -> uint32_t {
         if (!a.t_lse) return 0;
         const int b = r.bit(c);
         return bits[b >> 5] >> (b & 31) & ((1u << n) - 1);
     };
-    const int vectors = r.vectors();
-    for (int i = team.lane(); i < vectors; i += team.lanes()) {
-        float v[kVec];
-        load_vec<Z, kVec>(a.z, r.base + r.at(i), v);
-        s.template add<kVec>(v, inside(r.at(i), kVec), ct);
+    const int vectors = r.vectors(), lanes = team.lanes();
+    int i = team.lane();
+    for (; i + (kUnroll - 1) * lanes < vectors; i += kUnroll * lanes) {
+        Words<Z, kVec> v[kUnroll];
+        uint32_t in[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) v[u].load(a.z, r.base + r.at(i + u * lanes));
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) in[u] = inside(r.at(i + u * lanes), kVec);
+        s.add(v, in, ct);
     }
-    for (int i = team.lane(); i < r.odd(); i += team.lanes()) {
-        const float v = load_grad<Z>(a.z, r.base + r.odd_at(i));
-        s.template add<1>(&v, inside(r.odd_at(i), 1), ct);
+    for (; i < vectors; i += lanes) {
+        Words<Z, kVec> v[1];
+        v[0].load(a.z, r.base + r.at(i));
+        const uint32_t in[1] = {inside(r.at(i), kVec)};
+        s.add(v, in, ct);
+    }
+    for (i = team.lane(); i < r.odd(); i += lanes) {
+        Words<Z, 1> v[1];
+        v[0].load(a.z, r.base + r.odd_at(i));
+        const uint32_t in[1] = {inside(r.odd_at(i), 1)};
+        s.add(v, in, ct);
     }
 }
 
-// The row's loss and stats from its sums.
+// An entry of the teacher's.
+struct Entry {
+    int64_t c;
+    float t, z;                  // t / T; the student's logit (of a class in [0, V))
+};
+
+template <int Z>
+__device__ __forceinline__ Entry load_entry(const DistillArgs &a, int64_t n, int k) {
+    Entry e{-1, 0.0f, 0.0f};
+    if (n >= a.N || k >= a.K) return e;
+    e.c = class_of(a, n * a.K + k);
+    e.t = load_any(a.t, n * a.K + k, a.t_dtype) * a.inv_t;
+    if (e.c >= 0 && e.c < a.V) e.z = load_grad<Z>(a.z, n * a.V + e.c);
+    return e;
+}
+
+// The row's loss and stats from its sums.  mine: this lane's first entry; outside:
+// with a given l, the sums leave out the K classes, which may occur `twice`.
 template <int Z, int TEAM>
-__device__ __forceinline__ void finish_row(Team<TEAM> &team, const DistillArgs &a, int64_t n, float m, float at_t, float at_1,
-                                           float outside) {
-    const bool on = n < a.N;
-    float peak = -FLT_MAX, count = 0.0f, wrong = 0.0f;
-    for (int k = team.lane(); on && k < a.K; k += team.lanes()) {
-        const int64_t c = class_of(a, n * a.K + k);
-        if (c < 0) continue;
-        if (c >= a.V) wrong = 1.0f;
+__device__ __forceinline__ void finish_row(Team<TEAM> &team, const DistillArgs &a, int64_t n, const Entry &mine, float m,
+                                           float at_t, float at_1, bool twice) {
+    const bool on = n < a.N, tail = a.t_lse != nullptr;
+    const float ct = a.inv_t * kLog2e, outside = at_t;
+    const auto each = [&](auto f) {
+        for (int k = team.lane(); on && k < a.K; k += team.lanes()) f(k, k == team.lane() ? mine : load_entry<Z>(a, n, k));
+    };
+    float peak = -FLT_MAX, count = 0.0f, wrong = 0.0f, in_t = 0.0f, in_1 = 0.0f;
+    each([&](int k, const Entry &e) {
+        if (e.c < 0) return;
         count = 1.0f;
-        peak = fmaxf(peak, load_any(a.t, n * a.K + k, a.t_dtype) * a.inv_t);
+        peak = fmaxf(peak, e.t);
+        if (e.c >= a.V) {
+            wrong = 1.0f;
+            return;
+        }
+        if (!tail) return;
+        bool first = true;
+        if (twice)
+            for (int i = 0; i < k; ++i) first = first && class_of(a, n * a.K + i) != e.c;
+        if (!first) return;
+        in_t += exp2_fast((e.z - m) * ct);
+        in_1 += exp2_fast((e.z - m) * kLog2e);
+    });
+    team.sum2(count, wrong);
+    if (tail) {
+        team.sum2(in_t, in_1);
+        at_t += in_t;
+        at_1 += in_1;
     }
     float lse = 0.0f;
-    team.sum2(count, wrong);
-    if (a.t_lse) {
+    if (tail) {
         if (on) lse = a.t_lse[n];
     } else {
         peak = team.max(peak);
         float sum = 0.0f;
-        for (int k = team.lane(); on && k < a.K; k += team.lanes())
-            if (class_of(a, n * a.K + k) >= 0)
-                sum += exp2_fast((load_any(a.t, n * a.K + k, a.t_dtype) * a.inv_t - peak) * kLog2e);
+        each([&](int, const Entry &e) {
+            if (e.c >= 0) sum += exp2_fast((e.t - peak) * kLog2e);
+        });
         sum = team.sum(sum);
         if (sum == 0.0f) count = 0.0f;       // (no class has a probability)
         lse = count != 0.0f ? peak + logf(sum) : 0.0f;
     }
     const float log_t = logf(at_t), log_1 = logf(at_1);
     float kd = 0.0f, mass = 0.0f;
-    for (int k = team.lane(); on && k < a.K; k += team.lanes()) {
-        const int64_t c = class_of(a, n * a.K + k);
-        if (c < 0 || c >= a.V) continue;
-        const float log_p = load_any(a.t, n * a.K + k, a.t_dtype) * a.inv_t - lse;
-        const float p = exp2_fast(log_p * kLog2e);
+    each([&](int, const Entry &e) {
+        if (e.c < 0 || e.c >= a.V) return;
+        const float log_p = e.t - lse, p = exp2_fast(log_p * kLog2e);
         mass += p;
-        if (p != 0.0f) kd += p * (log_p - (load_grad<Z>(a.z, n * a.V + c) - m) * a.inv_t + log_t);
-    }
+        if (p != 0.0f) kd += p * (log_p - (e.z - m) * a.inv_t + log_t);
+    });
     team.sum2(kd, mass);
     if (team.lane() != 0 || !on) return;
     float factor = mass, labelled = 0.0f, ce = 0.0f;
-    if (a.t_lse && count > 0.0f) {
+    if (tail && count > 0.0f) {
         const float rho = fmaxf(1.0f - mass, 0.0f);
         // (a row whose K classes are all there are has no outside)
         if (rho > 0.0f && outside > 0.0f) {
@@ -233,7 +332,7 @@ __device__ __forceinline__ void finish_row(Team<TEAM> &team, const DistillArgs &
                 (a.alpha < 1.0f && labelled != 0.0f ? (1.0f - a.alpha) * ce : 0.0f);
 }
 
-template <int Z, int TEAM, bool BOTH>
+template <int Z, int TEAM, int SUMS>
 __global__ __launch_bounds__(Team<TEAM>::kThreads) void ple_distill_forward_kernel(DistillArgs a) {
     extern __shared__ uint32_t s_bits[];
     __shared__ float s_sum[Team<TEAM>::kLdsFloats];
@@ -244,14 +343,16 @@ __global__ __launch_bounds__(Team<TEAM>::kThreads) void ple_distill_forward_kern
     const float ct = a.inv_t * kLog2e;
     uint32_t *bits = s_bits + team.index() * a.words;
     const Range<Z, true> r(a.z, n, a.V, split * a.part, min(a.V, (split + 1) * a.part));
-    Sums<BOTH> s;
-    if (a.t_lse) mark_classes(team, a, n, r, bits, &s_twice[team.index()]);
-    if (n < a.N) scan_row<Z, TEAM, BOTH>(team, a, r, bits, ct, s);
+    Entry mine{-1, 0.0f, 0.0f};
+    if (a.splits == 1) mine = load_entry<Z>(a, n, team.lane());
+    Sums<SUMS> s;
+    const bool twice = a.t_lse && mark_classes(team, a, n, r, bits, &s_twice[team.index()]);
+    if (n < a.N) scan_row<Z, TEAM, SUMS>(team, a, r, bits, ct, s);
     s.join(team, ct);
     if (a.splits == 1) {
-        finish_row<Z>(team, a, n, s.m, s.at_t, s.at_1, s.outside);
+        finish_row<Z>(team, a, n, mine, s.m, s.at_t, s.at_1, twice);
     } else if (team.lane() == 0 && n < a.N) {
-        reinterpret_cast<float4 *>(a.partial)[n * a.splits + split] = make_float4(s.m, s.at_t, s.at_1, s.outside);
+        reinterpret_cast<float4 *>(a.partial)[n * a.splits + split] = make_float4(s.m, s.at_t, s.at_1, twice ? 1.0f : 0.0f);
     }
 }
 
@@ -261,34 +362,33 @@ __global__ __launch_bounds__(kBlock) void ple_distill_join_kernel(DistillArgs a)
     Team<kWave> team(nullptr);
     const int64_t n = static_cast<int64_t>(blockIdx.x) * team.per_block() + team.index();
     const float ct = a.inv_t * kLog2e;
-    float m = -FLT_MAX, at_t = 0.0f, at_1 = 0.0f, outside = 0.0f;
+    const Entry mine = load_entry<Z>(a, n, team.lane());
+    float m = -FLT_MAX, at_t = 0.0f, at_1 = 0.0f, twice = 0.0f;
     for (int i = team.lane(); n < a.N && i < a.splits; i += kWave) {
         const float4 v = reinterpret_cast<const float4 *>(a.partial)[n * a.splits + i];
         const float to = fmaxf(m, v.x);
-        const float f = exp2_fast((m - to) * ct), g = exp2_fast((v.x - to) * ct);
-        at_t = at_t * f + v.y * g;
-        outside = outside * f + v.w * g;
+        at_t = at_t * exp2_fast((m - to) * ct) + v.y * exp2_fast((v.x - to) * ct);
         at_1 = at_1 * exp2_fast((m - to) * kLog2e) + v.z * exp2_fast((v.x - to) * kLog2e);
+        twice += v.w;
         m = to;
     }
     const float to = team.max(m);
-    const float f = exp2_fast((m - to) * ct);
-    at_t *= f;
-    outside *= f;
+    at_t *= exp2_fast((m - to) * ct);
     at_1 *= exp2_fast((m - to) * kLog2e);
-    team.sum2(at_t, outside);
-    at_1 = team.sum(at_1);
-    finish_row<Z>(team, a, n, to, at_t, at_1, outside);
+    team.sum2(at_t, at_1);
+    finish_row<Z>(team, a, n, mine, to, at_t, at_1, team.sum(twice) > 0.0f);
 }
 
-template <int Z, int TEAM, bool VEC, bool BOTH>
+template <int Z, int TEAM, bool VEC, int SUMS>
 __global__ __launch_bounds__(Team<TEAM>::kThreads) void ple_distill_backward_kernel(DistillArgs a) {
     constexpr int kVec = Range<Z, VEC>::kVec;
     extern __shared__ uint32_t s_bits[];
     __shared__ int s_twice[Team<TEAM>::kThreads / (TEAM < kBlock ? TEAM : kBlock)];
     Team<TEAM> team(nullptr);
-    const int split = blockIdx.x % a.splits;
-    const int64_t n = static_cast<int64_t>(blockIdx.x / a.splits) * team.per_block() + team.index();
+    // the last rows first: the forward left them in the memory-side cache
+    const unsigned block = gridDim.x - 1 - blockIdx.x;
+    const int split = block % a.splits;
+    const int64_t n = static_cast<int64_t>(block / a.splits) * team.per_block() + team.index();
     const float ct = a.inv_t * kLog2e;
     uint32_t *bits = s_bits + team.index() * a.words;
     const Range<Z, VEC> r(a.z, n, a.V, split * a.part, min(a.V, (split + 1) * a.part));
@@ -310,18 +410,34 @@ __global__ __launch_bounds__(Team<TEAM>::kThreads) void ple_distill_backward_ker
     }
     const auto soft = [&](float z) { return exp2_fast((z - peak) * ct - log_t); };
     const auto hard = [&](float z) { return exp2_fast((z - peak) * kLog2e - log_1); };
+    // the dense terms, with the sums' logarithms taken into the weights
+    const float w_t = (SUMS == kOneSum ? w_out + w_hard : w_out) * exp2_fast(-log_t), w_1 = w_hard * exp2_fast(-log_1);
     const auto dense = [&](float z) {
-        if constexpr (BOTH) return w_out * soft(z) + w_hard * hard(z);
-        else return (w_out + w_hard) * soft(z);
+        const float d = z - peak, x = exp2_fast(d * ct);
+        if constexpr (SUMS == kOneSum) return w_t * x;
+        else if constexpr (SUMS == kTwoSums) return w_t * x + w_1 * exp2_fast(d * kLog2e);
+        else return w_t * x + w_1 * at_one<SUMS>(x);
     };
     if (n < a.N) {
-        const int vectors = r.vectors();
-        for (int i = team.lane(); i < vectors; i += team.lanes()) {
+        const int vectors = r.vectors(), lanes = team.lanes();
+        const auto put = [&](const Words<Z, kVec> &w, int64_t at) {
             float v[kVec];
-            load_vec<Z, kVec>(a.z, r.base + r.at(i), v);
 #pragma unroll
-            for (int e = 0; e < kVec; ++e) v[e] = dense(v[e]);
-            store_vec<Z, kVec>(a.dz, r.base + r.at(i), v);
+            for (int e = 0; e < kVec; ++e) v[e] = dense(w.at(e));
+            store_vec<Z, kVec>(a.dz, at, v);
+        };
+        int i = team.lane();
+        for (; i + (kUnroll - 1) * lanes < vectors; i += kUnroll * lanes) {
+            Words<Z, kVec> w[kUnroll];
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) w[u].load(a.z, r.base + r.at(i + u * lanes));
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) put(w[u], r.base + r.at(i + u * lanes));
+        }
+        for (; i < vectors; i += lanes) {
+            Words<Z, kVec> w;
+            w.load(a.z, r.base + r.at(i));
+            put(w, r.base + r.at(i));
         }
         if constexpr (VEC)
             for (int i = team.lane(); i < r.odd(); i += team.lanes()) {
@@ -406,18 +522,20 @@ DistillArgs distill_args(const DistillRequest &r, const DistillPlan &p) {
     return a;
 }
 
-// f(type, team, both sums) as compile-time constants
+// f(type, team, sums) as compile-time constants
 template <typename F>
 hipError_t with_distill(const DistillRequest &r, const DistillPlan &p, F f) {
-    const bool both = r.labels && r.temperature != 1.0f;
-    const auto by_both = [&](auto z, auto team) {
-        return both ? f(z, team, std::true_type{}) : f(z, team, std::false_type{});
+    const auto by_sums = [&](auto z, auto team) {
+        if (!r.labels || r.temperature == 1.0f) return f(z, team, std::integral_constant<int, kOneSum>{});
+        if (r.temperature == 2.0f) return f(z, team, std::integral_constant<int, kOneSquare>{});
+        if (r.temperature == 4.0f) return f(z, team, std::integral_constant<int, kTwoSquares>{});
+        return f(z, team, std::integral_constant<int, kTwoSums>{});
     };
     const auto by_team = [&](auto z) {
         switch (p.team) {
-            case 8: return by_both(z, std::integral_constant<int, 8>{});
-            case kWave: return by_both(z, std::integral_constant<int, kWave>{});
-            default: return by_both(z, std::integral_constant<int, kBlock>{});
+            case 8: return by_sums(z, std::integral_constant<int, 8>{});
+            case kWave: return by_sums(z, std::integral_constant<int, kWave>{});
+            default: return by_sums(z, std::integral_constant<int, kBlock>{});
         }
     };
     switch (r.dtype) {
@@ -440,9 +558,9 @@ int distill_run(const DistillRequest &r) {
     if (p.bytes > 0 && (!r.workspace || r.workspace_bytes < p.bytes || reinterpret_cast<uintptr_t>(r.workspace) % 256 != 0))
         return PLE_E_WORKSPACE;
     const DistillArgs a = distill_args(r, p);
-    const hipError_t rc = with_distill(r, p, [&](auto z, auto team, auto both) {
+    const hipError_t rc = with_distill(r, p, [&](auto z, auto team, auto sums) {
         hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_distill_forward_kernel<decltype(z)::value, decltype(team)::value,
-                                                                      decltype(both)::value>),
+                                                                      decltype(sums)::value>),
                            distill_grid(r, p), dim3(p.threads), p.lds, r.stream, a);
         return hipGetLastError();
     });
@@ -465,10 +583,10 @@ int distill_backward_run(const DistillRequest &r) {
     const DistillArgs a = distill_args(r, p);
     // one vector for z and dz: both addresses are the same way into 16 bytes
     const bool vec = (reinterpret_cast<uintptr_t>(r.logits) - reinterpret_cast<uintptr_t>(r.dz)) % 16 == 0;
-    return static_cast<int>(with_distill(r, p, [&](auto z, auto team, auto both) {
+    return static_cast<int>(with_distill(r, p, [&](auto z, auto team, auto sums) {
         const auto launch = [&](auto v) {
             hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_distill_backward_kernel<decltype(z)::value, decltype(team)::value,
-                                                                           decltype(v)::value, decltype(both)::value>),
+                                                                           decltype(v)::value, decltype(sums)::value>),
                                distill_grid(r, p), dim3(p.threads), p.lds, r.stream, a);
             return hipGetLastError();
         };
