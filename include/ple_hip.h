@@ -428,7 +428,8 @@ int ple_residual_norm_backward_launch(const void *grad_stream, const void *grad_
  *   teacher_lse      float32 [N] or NULL
  *   labels           int64 [N] or NULL
  *   loss             float32 [N]
- *   stats            float32 [N, PLE_DISTILL_STATS], for the backward
+ *   stats            float32 [N, PLE_DISTILL_STATS], 16-byte aligned, for the
+ *                    backward
  *   workspace        >= ple_distill_workspace_bytes(N, V) bytes (0 is
  *                    possible), 256-byte aligned, need not be initialised
  * 1e-6 < T < 1e6, 0 <= alpha <= 1 (else PLE_E_UNSUPPORTED); V <= 2^30, K <=

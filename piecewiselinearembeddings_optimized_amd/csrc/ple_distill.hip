@@ -162,31 +162,49 @@ struct Sums {
             at_1 += part_1[k];
         }
     }
-    template <int TEAM>
-    __device__ __forceinline__ void join(Team<TEAM> &team, float ct) {
-        rescale(team.max(m), ct);
-        team.sum2(at_t, at_1);
-        if constexpr (SUMS == kOneSum) at_1 = at_t;
-    }
 };
 
-// Marks the row's classes of [c0, c1) in the team's bits, which it clears
-// first.  Returns whether one of them was there already.  (All threads of the
-// workgroup.)
+// An entry of the teacher's, or the label.
+struct Entry {
+    int64_t c = -1;
+    float t = 0.0f, z = 0.0f;    // t / T; the student's logit (of a class in [0, V))
+};
+
+template <int Z>
+__device__ __forceinline__ Entry load_entry(const DistillArgs &a, int64_t n, int k) {
+    Entry e;
+    if (n >= a.N || k >= a.K) return e;
+    e.c = class_of(a, n * a.K + k);
+    e.t = load_any(a.t, n * a.K + k, a.t_dtype) * a.inv_t;
+    if (e.c >= 0 && e.c < a.V) e.z = load_grad<Z>(a.z, n * a.V + e.c);
+    return e;
+}
+
+template <int Z>
+__device__ __forceinline__ Entry load_label(const DistillArgs &a, int64_t n) {
+    Entry e;
+    if (n >= a.N || !a.labels) return e;
+    e.c = a.labels[n];
+    if (e.c >= 0 && e.c < a.V) e.z = load_grad<Z>(a.z, n * a.V + e.c);
+    return e;
+}
+
+// Marks the row's classes of [c0, c1) in the team's bits, which it clears first;
+// mine: this lane's first entry.  Returns whether one of them was there already.
 template <int TEAM, int Z, bool VEC>
-__device__ __forceinline__ bool mark_classes(Team<TEAM> &team, const DistillArgs &a, int64_t n, const Range<Z, VEC> &r,
-                                             uint32_t *bits, int *twice) {
+__device__ __forceinline__ bool mark_classes(Team<TEAM> &team, const DistillArgs &a, int64_t n, const Entry &mine,
+                                             const Range<Z, VEC> &r, uint32_t *bits, int *twice) {
     for (int w = team.lane(); w < a.words; w += team.lanes()) bits[w] = 0;
     if (team.lane() == 0) *twice = 0;
-    __syncthreads();
+    team.sync();
     if (n < a.N)
         for (int k = team.lane(); k < a.K; k += team.lanes()) {
-            const int64_t c = class_of(a, n * a.K + k);
+            const int64_t c = k == team.lane() ? mine.c : class_of(a, n * a.K + k);
             if (c < r.c0 || c >= r.c1) continue;
             const int b = r.bit(static_cast<int>(c));
             if (atomicOr(&bits[b >> 5], 1u << (b & 31)) >> (b & 31) & 1) *twice = 1;
         }
-    __syncthreads();
+    team.sync();
     return *twice != 0;
 }
 
@@ -224,80 +242,78 @@ __device__ __forceinline__ void scan_row(Team<TEAM> &team, const DistillArgs &a,
     }
 }
 
-// An entry of the teacher's.
-struct Entry {
-    int64_t c;
-    float t, z;                  // t / T; the student's logit (of a class in [0, V))
-};
-
-template <int Z>
-__device__ __forceinline__ Entry load_entry(const DistillArgs &a, int64_t n, int k) {
-    Entry e{-1, 0.0f, 0.0f};
-    if (n >= a.N || k >= a.K) return e;
-    e.c = class_of(a, n * a.K + k);
-    e.t = load_any(a.t, n * a.K + k, a.t_dtype) * a.inv_t;
-    if (e.c >= 0 && e.c < a.V) e.z = load_grad<Z>(a.z, n * a.V + e.c);
-    return e;
-}
-
-// The row's loss and stats from its sums.  mine: this lane's first entry; outside:
-// with a given l, the sums leave out the K classes, which may occur `twice`.
-template <int Z, int TEAM>
-__device__ __forceinline__ void finish_row(Team<TEAM> &team, const DistillArgs &a, int64_t n, const Entry &mine, float m,
-                                           float at_t, float at_1, bool twice) {
+// The row's loss and stats from its lanes' sums.  mine: this lane's first entry.
+// With a given l the sums leave out the K classes, which may occur `twice`.
+template <int Z, int TEAM, int SUMS>
+__device__ __forceinline__ void finish_row(Team<TEAM> &team, const DistillArgs &a, int64_t n, const Entry &mine,
+                                           const Entry &label, Sums<SUMS> &s, bool twice) {
     const bool on = n < a.N, tail = a.t_lse != nullptr;
-    const float ct = a.inv_t * kLog2e, outside = at_t;
+    const float ct = a.inv_t * kLog2e;
     const auto each = [&](auto f) {
         for (int k = team.lane(); on && k < a.K; k += team.lanes()) f(k, k == team.lane() ? mine : load_entry<Z>(a, n, k));
     };
-    float peak = -FLT_MAX, count = 0.0f, wrong = 0.0f, in_t = 0.0f, in_1 = 0.0f;
+    const auto in_range = [&](const Entry &e) { return e.c >= 0 && e.c < a.V; };
+    float top[2] = {s.m, -FLT_MAX};
+    if (!tail)
+        each([&](int, const Entry &e) {
+            if (e.c >= 0) top[1] = fmaxf(top[1], e.t);
+        });
+    team.maxima(top);
+    s.rescale(top[0], ct);
+    // sums: at T, at 1; of the K classes at T, at 1 (given l), else the teacher's; its
+    // mass and cross terms (given l); entries, with 2^12 for one beyond V
+    enum { kSumT, kSum1, kInT, kIn1, kMassP, kCross, kCount, kValues };
+    constexpr float kWrong = 4096.0f;
+    float v[kValues] = {s.at_t, s.at_1, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    float lse = tail && on ? a.t_lse[n] : 0.0f;
+    bool some = false, wrong = false;
     each([&](int k, const Entry &e) {
         if (e.c < 0) return;
-        count = 1.0f;
-        peak = fmaxf(peak, e.t);
-        if (e.c >= a.V) {
-            wrong = 1.0f;
+        some = true;
+        wrong = wrong || e.c >= a.V;
+        if (!tail) {
+            v[kInT] += exp2_fast((e.t - top[1]) * kLog2e);
             return;
         }
-        if (!tail) return;
+        if (!in_range(e)) return;
         bool first = true;
         if (twice)
             for (int i = 0; i < k; ++i) first = first && class_of(a, n * a.K + i) != e.c;
-        if (!first) return;
-        in_t += exp2_fast((e.z - m) * ct);
-        in_1 += exp2_fast((e.z - m) * kLog2e);
+        if (first) {
+            v[kInT] += exp2_fast((e.z - s.m) * ct);
+            v[kIn1] += exp2_fast((e.z - s.m) * kLog2e);
+        }
+        const float log_p = e.t - lse, p = exp2_fast(log_p * kLog2e);
+        v[kMassP] += p;
+        if (p != 0.0f) v[kCross] += p * (log_p - (e.z - s.m) * a.inv_t);
     });
-    team.sum2(count, wrong);
+    v[kCount] = (some ? 1.0f : 0.0f) + (wrong ? kWrong : 0.0f);      // (exact: at most 256 lanes)
+    team.sums(v);
+    bool taught = v[kCount] != 0.0f;
+    wrong = v[kCount] >= kWrong;
+    const float outside = v[kSumT];
+    float at_t = outside, at_1 = SUMS == kOneSum ? v[kSumT] : v[kSum1], kd = v[kCross], mass = v[kMassP];
     if (tail) {
-        team.sum2(in_t, in_1);
-        at_t += in_t;
-        at_1 += in_1;
-    }
-    float lse = 0.0f;
-    if (tail) {
-        if (on) lse = a.t_lse[n];
-    } else {
-        peak = team.max(peak);
-        float sum = 0.0f;
-        each([&](int, const Entry &e) {
-            if (e.c >= 0) sum += exp2_fast((e.t - peak) * kLog2e);
-        });
-        sum = team.sum(sum);
-        if (sum == 0.0f) count = 0.0f;       // (no class has a probability)
-        lse = count != 0.0f ? peak + logf(sum) : 0.0f;
+        at_t += v[kInT];
+        at_1 += SUMS == kOneSum ? v[kInT] : v[kIn1];
     }
     const float log_t = logf(at_t), log_1 = logf(at_1);
-    float kd = 0.0f, mass = 0.0f;
-    each([&](int, const Entry &e) {
-        if (e.c < 0 || e.c >= a.V) return;
-        const float log_p = e.t - lse, p = exp2_fast(log_p * kLog2e);
-        mass += p;
-        if (p != 0.0f) kd += p * (log_p - (e.z - m) * a.inv_t + log_t);
-    });
-    team.sum2(kd, mass);
+    if (tail) {
+        kd += mass * log_t;
+    } else {
+        if (v[kInT] == 0.0f) taught = false;     // (no class has a probability)
+        lse = taught ? top[1] + logf(v[kInT]) : 0.0f;
+        each([&](int, const Entry &e) {
+            if (!in_range(e)) return;
+            const float log_p = e.t - lse, p = exp2_fast(log_p * kLog2e);
+            mass += p;
+            if (p != 0.0f) kd += p * (log_p - (e.z - s.m) * a.inv_t + log_t);
+        });
+        team.sum2(kd, mass);
+    }
     if (team.lane() != 0 || !on) return;
-    float factor = mass, labelled = 0.0f, ce = 0.0f;
-    if (tail && count > 0.0f) {
+    float factor = mass, labelled = 0.0f, ce = 0.0f, m = s.m;
+    if (tail && taught) {
         const float rho = fmaxf(1.0f - mass, 0.0f);
         // (a row whose K classes are all there are has no outside)
         if (rho > 0.0f && outside > 0.0f) {
@@ -306,29 +322,18 @@ __device__ __forceinline__ void finish_row(Team<TEAM> &team, const DistillArgs &
             factor = mass - rho * (at_t / outside);
         }
     }
-    if (a.labels) {
-        const int64_t label = a.labels[n];
-        if (label >= a.V) labelled = __builtin_nanf("");
-        else if (label >= 0) labelled = 1.0f;
-        if (label >= 0 && label < a.V) ce = log_1 - (load_grad<Z>(a.z, n * a.V + label) - m);
-        else ce = labelled;
+    if (label.c >= a.V) labelled = ce = __builtin_nanf("");
+    else if (label.c >= 0) {
+        labelled = 1.0f;
+        ce = log_1 - (label.z - m);
     }
-    if (wrong > 0.0f) kd = mass = factor = __builtin_nanf("");
-    float *st = a.stats + n * PLE_DISTILL_STATS;
-    if (at_t == 0.0f) {          // every class is masked: no loss, no gradient
-        kd = ce = m = mass = factor = labelled = 0.0f;
-        st[kLogT] = st[kLog1] = 0.0f;
-    } else {
-        st[kLogT] = log_t * kLog2e;
-        st[kLog1] = log_1 * kLog2e;
-    }
-    st[kPeak] = m;
-    st[kTeacherLse] = lse;
-    st[kMass] = mass;
-    st[kOutside] = factor;
-    st[kLabelled] = labelled;
-    st[7] = 0.0f;
-    a.loss[n] = (a.alpha > 0.0f && count > 0.0f ? a.alpha * a.t_factor * a.t_factor * kd : 0.0f) +
+    if (wrong) kd = mass = factor = __builtin_nanf("");
+    const bool live = at_t != 0.0f;      // else every class is masked: no loss, no gradient
+    if (!live) kd = ce = m = mass = factor = labelled = 0.0f;
+    float4 *st = reinterpret_cast<float4 *>(a.stats + n * PLE_DISTILL_STATS);
+    st[0] = make_float4(m, live ? log_t * kLog2e : 0.0f, live ? log_1 * kLog2e : 0.0f, lse);
+    st[1] = make_float4(mass, factor, labelled, 0.0f);
+    a.loss[n] = (a.alpha > 0.0f && taught ? a.alpha * a.t_factor * a.t_factor * kd : 0.0f) +
                 (a.alpha < 1.0f && labelled != 0.0f ? (1.0f - a.alpha) * ce : 0.0f);
 }
 
@@ -343,43 +348,47 @@ __global__ __launch_bounds__(Team<TEAM>::kThreads) void ple_distill_forward_kern
     const float ct = a.inv_t * kLog2e;
     uint32_t *bits = s_bits + team.index() * a.words;
     const Range<Z, true> r(a.z, n, a.V, split * a.part, min(a.V, (split + 1) * a.part));
-    Entry mine{-1, 0.0f, 0.0f};
-    if (a.splits == 1) mine = load_entry<Z>(a, n, team.lane());
+    const Entry mine = load_entry<Z>(a, n, team.lane()), label = load_label<Z>(a, n);
     Sums<SUMS> s;
-    const bool twice = a.t_lse && mark_classes(team, a, n, r, bits, &s_twice[team.index()]);
+    const bool twice = a.t_lse && mark_classes(team, a, n, mine, r, bits, &s_twice[team.index()]);
     if (n < a.N) scan_row<Z, TEAM, SUMS>(team, a, r, bits, ct, s);
-    s.join(team, ct);
     if (a.splits == 1) {
-        finish_row<Z>(team, a, n, mine, s.m, s.at_t, s.at_1, twice);
-    } else if (team.lane() == 0 && n < a.N) {
-        reinterpret_cast<float4 *>(a.partial)[n * a.splits + split] = make_float4(s.m, s.at_t, s.at_1, twice ? 1.0f : 0.0f);
+        finish_row<Z>(team, a, n, mine, label, s, twice);
+        return;
     }
+    float top[1] = {s.m};
+    team.maxima(top);
+    s.rescale(top[0], ct);
+    team.sum2(s.at_t, s.at_1);
+    if (team.lane() == 0 && n < a.N)
+        reinterpret_cast<float4 *>(a.partial)[n * a.splits + split] = make_float4(s.m, s.at_t, s.at_1, twice ? 1.0f : 0.0f);
 }
 
 // A row's sums from its splits' (one wave a row), then its loss.
-template <int Z>
+template <int Z, int SUMS>
 __global__ __launch_bounds__(kBlock) void ple_distill_join_kernel(DistillArgs a) {
     Team<kWave> team(nullptr);
     const int64_t n = static_cast<int64_t>(blockIdx.x) * team.per_block() + team.index();
-    const float ct = a.inv_t * kLog2e;
-    const Entry mine = load_entry<Z>(a, n, team.lane());
-    float m = -FLT_MAX, at_t = 0.0f, at_1 = 0.0f, twice = 0.0f;
+    const Entry mine = load_entry<Z>(a, n, team.lane()), label = load_label<Z>(a, n);
+    Sums<SUMS> s;
+    bool twice = false;
     for (int i = team.lane(); n < a.N && i < a.splits; i += kWave) {
         const float4 v = reinterpret_cast<const float4 *>(a.partial)[n * a.splits + i];
-        const float to = fmaxf(m, v.x);
-        at_t = at_t * exp2_fast((m - to) * ct) + v.y * exp2_fast((v.x - to) * ct);
-        at_1 = at_1 * exp2_fast((m - to) * kLog2e) + v.z * exp2_fast((v.x - to) * kLog2e);
-        twice += v.w;
-        m = to;
+        Sums<SUMS> part;
+        part.m = v.x;
+        part.at_t = v.y;
+        part.at_1 = v.z;
+        const float to = fmaxf(s.m, part.m);
+        s.rescale(to, a.inv_t * kLog2e);
+        part.rescale(to, a.inv_t * kLog2e);
+        s.at_t += part.at_t;
+        s.at_1 += part.at_1;
+        twice = twice || v.w != 0.0f;
     }
-    const float to = team.max(m);
-    at_t *= exp2_fast((m - to) * ct);
-    at_1 *= exp2_fast((m - to) * kLog2e);
-    team.sum2(at_t, at_1);
-    finish_row<Z>(team, a, n, mine, to, at_t, at_1, team.sum(twice) > 0.0f);
+    finish_row<Z>(team, a, n, mine, label, s, __any(twice));
 }
 
-template <int Z, int TEAM, bool VEC, int SUMS>
+template <int Z, int TEAM, bool VEC, int SUMS, bool NT>
 __global__ __launch_bounds__(Team<TEAM>::kThreads) void ple_distill_backward_kernel(DistillArgs a) {
     constexpr int kVec = Range<Z, VEC>::kVec;
     extern __shared__ uint32_t s_bits[];
@@ -392,22 +401,22 @@ __global__ __launch_bounds__(Team<TEAM>::kThreads) void ple_distill_backward_ker
     const float ct = a.inv_t * kLog2e;
     uint32_t *bits = s_bits + team.index() * a.words;
     const Range<Z, VEC> r(a.z, n, a.V, split * a.part, min(a.V, (split + 1) * a.part));
-    const bool twice = mark_classes(team, a, n, r, bits, &s_twice[team.index()]);
-    float peak = 0.0f, log_t = 0.0f, log_1 = 0.0f, lse = 0.0f, mass = 0.0f, w_soft = 0.0f, w_out = 0.0f, w_hard = 0.0f;
-    int64_t label = -1;
+    const Entry mine = load_entry<Z>(a, n, team.lane());
+    Entry label = load_label<Z>(a, n);
+    float4 st0 = make_float4(0.0f, 0.0f, 0.0f, 0.0f), st1 = st0;
+    float g = 0.0f;
     if (n < a.N) {
-        const float *st = a.stats + n * PLE_DISTILL_STATS;
-        const float g = a.g[n];
-        peak = st[kPeak];
-        log_t = st[kLogT];
-        log_1 = st[kLog1];
-        lse = st[kTeacherLse];
-        mass = st[kMass];
-        w_soft = a.alpha > 0.0f && mass != 0.0f ? g * a.alpha * a.t_factor : 0.0f;
-        w_out = w_soft != 0.0f ? w_soft * st[kOutside] : 0.0f;
-        w_hard = a.alpha < 1.0f && st[kLabelled] != 0.0f ? g * (1.0f - a.alpha) * st[kLabelled] : 0.0f;
-        if (a.labels && st[kLabelled] != 0.0f) label = a.labels[n];
+        const float4 *st = reinterpret_cast<const float4 *>(a.stats + n * PLE_DISTILL_STATS);
+        st0 = st[0];
+        st1 = st[1];
+        g = a.g[n];
     }
+    const bool twice = mark_classes(team, a, n, mine, r, bits, &s_twice[team.index()]);
+    const float peak = st0.x, log_t = st0.y, log_1 = st0.z, lse = st0.w, mass = st1.x;
+    const float w_soft = a.alpha > 0.0f && mass != 0.0f ? g * a.alpha * a.t_factor : 0.0f;
+    const float w_out = w_soft != 0.0f ? w_soft * st1.y : 0.0f;
+    const float w_hard = a.alpha < 1.0f && st1.z != 0.0f ? g * (1.0f - a.alpha) * st1.z : 0.0f;
+    if (st1.z == 0.0f) label.c = -1;
     const auto soft = [&](float z) { return exp2_fast((z - peak) * ct - log_t); };
     const auto hard = [&](float z) { return exp2_fast((z - peak) * kLog2e - log_1); };
     // the dense terms, with the sums' logarithms taken into the weights
@@ -424,7 +433,7 @@ __global__ __launch_bounds__(Team<TEAM>::kThreads) void ple_distill_backward_ker
             float v[kVec];
 #pragma unroll
             for (int e = 0; e < kVec; ++e) v[e] = dense(w.at(e));
-            store_vec<Z, kVec>(a.dz, at, v);
+            store_vec<Z, kVec, NT>(a.dz, at, v);
         };
         int i = team.lane();
         for (; i + (kUnroll - 1) * lanes < vectors; i += kUnroll * lanes) {
@@ -445,34 +454,33 @@ __global__ __launch_bounds__(Team<TEAM>::kThreads) void ple_distill_backward_ker
                 store_vec<Z, 1>(a.dz, r.base + r.odd_at(i), &v);
             }
     }
-    __syncthreads();
+    team.sync();
     if (n >= a.N) return;
+    const auto prob = [&](float t) { return exp2_fast((t - lse) * kLog2e); };
     for (int k = team.lane(); k < a.K; k += team.lanes()) {
-        const int64_t c = class_of(a, n * a.K + k);
-        if (c < r.c0 || c >= r.c1) continue;
-        const auto prob = [&](int i) { return exp2_fast((load_any(a.t, n * a.K + i, a.t_dtype) * a.inv_t - lse) * kLog2e); };
+        const Entry e = k == team.lane() ? mine : load_entry<Z>(a, n, k);
+        if (e.c < r.c0 || e.c >= r.c1) continue;
         float p = 0.0f;
-        bool mine = true;
+        bool first = true;
         if (twice) {
             for (int i = 0; i < a.K; ++i)
-                if (class_of(a, n * a.K + i) == c) {
-                    if (i < k) mine = false;
-                    p += prob(i);
+                if (class_of(a, n * a.K + i) == e.c) {
+                    first = first && i >= k;
+                    p += prob(load_any(a.t, n * a.K + i, a.t_dtype) * a.inv_t);
                 }
         } else {
-            p = prob(k);
+            p = prob(e.t);
         }
-        if (!mine) continue;
-        const float z = load_grad<Z>(a.z, r.base + c);
-        float v = w_soft != 0.0f ? w_soft * (mass * soft(z) - p) : 0.0f;
-        if (w_hard != 0.0f) v += w_hard * (hard(z) - (c == label ? 1.0f : 0.0f));
-        store_vec<Z, 1>(a.dz, r.base + c, &v);
+        if (!first) continue;
+        float v = w_soft != 0.0f ? w_soft * (mass * soft(e.z) - p) : 0.0f;
+        if (w_hard != 0.0f) v += w_hard * (hard(e.z) - (e.c == label.c ? 1.0f : 0.0f));
+        store_vec<Z, 1>(a.dz, r.base + e.c, &v);
     }
-    if (team.lane() == 0 && label >= r.c0 && label < r.c1) {
-        const int b = r.bit(static_cast<int>(label));
+    if (team.lane() == 0 && label.c >= r.c0 && label.c < r.c1) {
+        const int b = r.bit(static_cast<int>(label.c));
         if (!(bits[b >> 5] >> (b & 31) & 1)) {
-            const float v = dense(load_grad<Z>(a.z, r.base + label)) - w_hard;
-            store_vec<Z, 1>(a.dz, r.base + label, &v);
+            const float v = dense(label.z) - w_hard;
+            store_vec<Z, 1>(a.dz, r.base + label.c, &v);
         }
     }
 }
@@ -490,7 +498,7 @@ constexpr int kMaxPart = 1 << 18;        // classes a workgroup has bits for (32
 
 DistillPlan plan_distill(int64_t N, int64_t V) {
     DistillPlan p{};
-    p.team = V <= 64 ? 8 : (V <= 2048 ? kWave : kBlock);
+    p.team = V <= 64 ? 8 : (V <= 128 ? 16 : (V <= 2048 ? kWave : kBlock));
     p.threads = kBlock;
     p.per_block = kBlock / p.team;
     p.splits = 1;
@@ -534,6 +542,7 @@ hipError_t with_distill(const DistillRequest &r, const DistillPlan &p, F f) {
     const auto by_team = [&](auto z) {
         switch (p.team) {
             case 8: return by_sums(z, std::integral_constant<int, 8>{});
+            case 16: return by_sums(z, std::integral_constant<int, 16>{});
             case kWave: return by_sums(z, std::integral_constant<int, kWave>{});
             default: return by_sums(z, std::integral_constant<int, kBlock>{});
         }
@@ -566,16 +575,11 @@ int distill_run(const DistillRequest &r) {
     });
     if (rc != hipSuccess || p.splits == 1) return static_cast<int>(rc);
     const dim3 grid(static_cast<unsigned>((r.N + kWavesPerBlock - 1) / kWavesPerBlock));
-    switch (r.dtype) {
-        case PLE_DTYPE_F32:
-            hipLaunchKernelGGL(ple_distill_join_kernel<PLE_DTYPE_F32>, grid, dim3(kBlock), 0, r.stream, a);
-            break;
-        case PLE_DTYPE_F16:
-            hipLaunchKernelGGL(ple_distill_join_kernel<PLE_DTYPE_F16>, grid, dim3(kBlock), 0, r.stream, a);
-            break;
-        default: hipLaunchKernelGGL(ple_distill_join_kernel<PLE_DTYPE_BF16>, grid, dim3(kBlock), 0, r.stream, a);
-    }
-    return static_cast<int>(hipGetLastError());
+    return static_cast<int>(with_distill(r, p, [&](auto z, auto, auto sums) {
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_distill_join_kernel<decltype(z)::value, decltype(sums)::value>), grid, dim3(kBlock),
+                           0, r.stream, a);
+        return hipGetLastError();
+    }));
 }
 
 int distill_backward_run(const DistillRequest &r) {
@@ -583,14 +587,23 @@ int distill_backward_run(const DistillRequest &r) {
     const DistillArgs a = distill_args(r, p);
     // one vector for z and dz: both addresses are the same way into 16 bytes
     const bool vec = (reinterpret_cast<uintptr_t>(r.logits) - reinterpret_cast<uintptr_t>(r.dz)) % 16 == 0;
+    // Long rows' gradients of 64 MB on are stored past the caches, which the logits
+    // need (50257 classes, both kernels: 2560 rows 178 -> 145 us, 1024 73 -> 62, 512
+    // and fewer as fast either way; short rows, of parts of lines, are 3 to 5%
+    // slower so at any size).
+    const bool stream = p.team == kBlock && r.N * r.V * elem_bytes(r.dtype) >= (int64_t{64} << 20);
     return static_cast<int>(with_distill(r, p, [&](auto z, auto team, auto sums) {
-        const auto launch = [&](auto v) {
+        const auto launch = [&](auto v, auto nt) {
             hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_distill_backward_kernel<decltype(z)::value, decltype(team)::value,
-                                                                           decltype(v)::value, decltype(sums)::value>),
+                                                                           decltype(v)::value, decltype(sums)::value,
+                                                                           decltype(nt)::value>),
                                distill_grid(r, p), dim3(p.threads), p.lds, r.stream, a);
             return hipGetLastError();
         };
-        return vec ? launch(std::true_type{}) : launch(std::false_type{});
+        if (!vec) return launch(std::false_type{}, std::false_type{});
+        if constexpr (decltype(team)::value == kBlock)
+            if (stream) return launch(std::true_type{}, std::true_type{});
+        return launch(std::true_type{}, std::false_type{});
     }));
 }
 

@@ -60,7 +60,8 @@ template <int TEAM>
 struct Team {
     static constexpr bool kBlockWide = TEAM > kWave;
     static constexpr int kThreads = kBlockWide ? TEAM : kBlock;
-    static constexpr int kLdsFloats = kBlockWide ? 4 * TEAM / kWave : 1;
+    static constexpr int kMost = 8;              // values of one sum or maximum
+    static constexpr int kLdsFloats = kBlockWide ? 2 * kMost * TEAM / kWave : 1;
     float *lds;                  // kLdsFloats floats
     int turn = 0;
     __device__ __forceinline__ explicit Team(float *s) : lds(s) {}
@@ -69,44 +70,60 @@ struct Team {
     __device__ __forceinline__ int index() const { return kBlockWide ? 0 : threadIdx.x / TEAM; }
     __device__ __forceinline__ int per_block() const { return kBlockWide ? 1 : kBlock / TEAM; }
 
-    // sums of two values over the team's lanes, to all of them
-    __device__ __forceinline__ void sum2(float &a, float &b) {
-        if constexpr (!kBlockWide) {
-            a = group_sum<TEAM>(a);
-            b = group_sum<TEAM>(b);
-        } else {
-            a = group_sum<kWave>(a);
-            b = group_sum<kWave>(b);
-            // (two buffers in turn: a wave can be one sum ahead of another)
-            float2 *buf = reinterpret_cast<float2 *>(lds) + (turn ^= 1) * (TEAM / kWave);
-            const int waves = blockDim.x / kWave;
-            if (threadIdx.x % kWave == 0) buf[threadIdx.x / kWave] = make_float2(a, b);
+    // Orders the team's LDS and global accesses before it with those after it.
+    __device__ __forceinline__ void sync() const {
+        if constexpr (kBlockWide) {
             __syncthreads();
-            a = b = 0.0f;
-            for (int w = 0; w < waves; ++w) {
-                const float2 v = buf[w];
-                a += v.x;
-                b += v.y;
-            }
+        } else {
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
         }
+    }
+
+    // N values joined over the workgroup's waves (`v`: a wave's), in a fixed order
+    template <int N, typename F>
+    __device__ __forceinline__ void over_waves(float (&v)[N], F join) {
+        static_assert(N <= kMost, "values");
+        // (two buffers in turn: a wave can be one ahead of another)
+        float *buf = lds + (turn ^= 1) * (kMost * TEAM / kWave);
+        const int waves = blockDim.x / kWave;
+        if (threadIdx.x % kWave == 0)
+#pragma unroll
+            for (int i = 0; i < N; ++i) buf[threadIdx.x / kWave * N + i] = v[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = buf[i];
+        for (int w = 1; w < waves; ++w)
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = join(v[i], buf[w * N + i]);
+    }
+    // sums of N values over the team's lanes, to all of them
+    template <int N>
+    __device__ __forceinline__ void sums(float (&v)[N]) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = group_sum<kBlockWide ? kWave : TEAM>(v[i]);
+        if constexpr (kBlockWide) over_waves(v, [](float a, float b) { return a + b; });
+    }
+    __device__ __forceinline__ void sum2(float &a, float &b) {
+        float v[2] = {a, b};
+        sums(v);
+        a = v[0];
+        b = v[1];
     }
     __device__ __forceinline__ float sum(float a) {
-        float b = 0.0f;
-        sum2(a, b);
-        return a;
+        float v[1] = {a};
+        sums(v);
+        return v[0];
     }
-    // maximum over the team's lanes (NaN is passed over), to all of them
-    __device__ __forceinline__ float max(float a) {
+    // maxima (NaN is passed over), to all lanes
+    template <int N>
+    __device__ __forceinline__ void maxima(float (&v)[N]) {
 #pragma unroll
-        for (int o = (kBlockWide ? kWave : TEAM) / 2; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor(a, o));
-        if constexpr (kBlockWide) {
-            float2 *buf = reinterpret_cast<float2 *>(lds) + (turn ^= 1) * (TEAM / kWave);
-            const int waves = blockDim.x / kWave;
-            if (threadIdx.x % kWave == 0) buf[threadIdx.x / kWave].x = a;
-            __syncthreads();
-            for (int w = 0; w < waves; ++w) a = fmaxf(a, buf[w].x);
-        }
-        return a;
+        for (int o = (kBlockWide ? kWave : TEAM) / 2; o > 0; o >>= 1)
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = fmaxf(v[i], __shfl_xor(v[i], o));
+        if constexpr (kBlockWide) over_waves(v, [](float a, float b) { return fmaxf(a, b); });
     }
 };
 

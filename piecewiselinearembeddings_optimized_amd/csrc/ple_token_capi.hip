@@ -194,7 +194,7 @@ int ple_distill_launch(const void *logits, const void *teacher_logits, const voi
     if (!logits || !teacher_logits || !teacher_classes || !loss || !stats) return PLE_E_NULL_POINTER;
     if (!ple::aligned_for(logits, dtype) || !ple::aligned_for(teacher_logits, teacher_dtype) ||
         !ple::aligned(teacher_classes, class_bytes) || !ple::aligned(teacher_lse, 4) || !ple::aligned(labels, 8) ||
-        !ple::aligned(loss, 4) || !ple::aligned(stats, 4))
+        !ple::aligned(loss, 4) || !ple::aligned(stats, 16))
         return PLE_E_MISALIGNED;
     ple::DistillRequest r{};
     r.logits = logits; r.teacher = teacher_logits; r.classes = teacher_classes;
@@ -217,7 +217,7 @@ int ple_distill_backward_launch(const float *grad_loss, const void *logits, cons
     if (!grad_loss || !logits || !teacher_logits || !teacher_classes || !stats || !grad_logits) return PLE_E_NULL_POINTER;
     if (!ple::aligned_for(logits, dtype) || !ple::aligned_for(grad_logits, dtype) ||
         !ple::aligned_for(teacher_logits, teacher_dtype) || !ple::aligned(teacher_classes, class_bytes) ||
-        !ple::aligned(labels, 8) || !ple::aligned(grad_loss, 4) || !ple::aligned(stats, 4))
+        !ple::aligned(labels, 8) || !ple::aligned(grad_loss, 4) || !ple::aligned(stats, 16))
         return PLE_E_MISALIGNED;
     ple::DistillRequest r{};
     r.logits = logits; r.teacher = teacher_logits; r.classes = teacher_classes; r.labels = labels;
