@@ -7,6 +7,10 @@ operators, FakeTensor and autograd registrations, and the
 gfx950 (``csrc/ple_forward.hip``, ``csrc/ple_backward.hip``) behind the C ABI
 of ``include/ple_hip.h`` (``csrc/ple_capi.hip``).
 
+Around it, with no counterpart in the reference: embeddings of tokens and
+categorical columns, the norms of a residual trunk and a distillation loss
+(``trunk.py``; operators ``lookup``, ``residual_norm``, ``distillation_loss``).
+
 Import order follows the reference (``__init__.py:3-7`` there): the native
 registrations first, then the fake kernels, then autograd, then the module.
 """

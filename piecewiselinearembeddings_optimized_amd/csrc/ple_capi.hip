@@ -114,7 +114,7 @@ int check_common(int64_t N, int64_t F, int64_t B, int64_t D) {
 
 extern "C" {
 
-int ple_abi_version(void) { return (1 << 16) | 5; }
+int ple_abi_version(void) { return (1 << 16) | 6; }
 
 int ple_bin_index_bytes(int64_t max_n_bins) { return ple::idx_bytes_for(max_n_bins); }
 
@@ -178,12 +178,12 @@ const char *ple_error_string(int code) {
     switch (code) {
         case PLE_OK: return "success";
         case PLE_E_NULL_POINTER: return "a required pointer is NULL";
-        case PLE_E_BAD_SHAPE: return "invalid shape (need N >= 0 and F, B, D >= 1)";
+        case PLE_E_BAD_SHAPE: return "invalid shape (need N >= 0 and F, B, D >= 1; the entry point's own sizes)";
         case PLE_E_BAD_DTYPE: return "invalid dtype code";
         case PLE_E_BAD_INDEX_WIDTH: return "invalid bin index width";
         case PLE_E_TOO_LARGE:
             return "sizes exceed the supported range (max_n_bins <= 2^24, F * max_n_bins * D < 2^30; "
-                   "module epilogues with ReLU or linear0: D <= 64)";
+                   "module epilogues with ReLU or linear0: D <= 64; other operators: their own limits)";
         case PLE_E_WORKSPACE: return "workspace is NULL, too small or not 256-byte aligned";
         case PLE_E_UNSUPPORTED: return "combination not supported (dtype or epilogue pairing)";
         case PLE_E_MISALIGNED: return "pointer misaligned for its element type";

@@ -20,6 +20,14 @@
 // backward a team walks its rows with the parameters' gradient sums in
 // registers; a workgroup adds its teams' sums and leaves them as partials in
 // 32 bits, which a second kernel adds in a fixed order.
+//
+// Measured (one MI355X; forward, backward and joins; the copy's rate is 5.2
+// TB/s): 16384 x 4096 bf16 112 + 166 + 6 us (4.8 and 4.9 TB/s), 51200 x 192 fp32
+// 34 + 42 + 5 us (4.7 and 5.7, the tensors partly in the memory-side cache),
+// 32800 x 1152 fp32 stream with a bf16 branch and a gate a sample 100 + 173 + 5
+// us (4.5 and 3.9: 144 of 192 lanes, and the biases' sums leave three waves a
+// SIMD).  Loads of the next row while this one is used: 445 -> 332 us for the
+// first, a second workgroup a CU 332 -> 281.
 
 #include <algorithm>
 

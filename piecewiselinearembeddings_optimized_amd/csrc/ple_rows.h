@@ -10,24 +10,10 @@ namespace ple {
 __host__ __device__ constexpr int elem_bytes(int dtype) { return dtype == PLE_DTYPE_F32 ? 4 : 2; }
 
 // VEC consecutive elements of type T from element i (aligned for the access:
-// VEC elements, 16 bytes at most), as floats.  VEC in {1, 2, 4, 8}.  NT: 16-byte
-// accesses pass the caches by.
-template <int T, int VEC, bool NT = false>
+// VEC elements, 16 bytes at most), as floats.  VEC in {1, 2, 4, 8}.
+template <int T, int VEC>
 __device__ __forceinline__ void load_vec(const void *p, int64_t i, float *v) {
-    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-    if constexpr (NT && VEC * elem_bytes(T) >= 16) {
-        const u32x4 *q = reinterpret_cast<const u32x4 *>(static_cast<const char *>(p) + i * elem_bytes(T));
-#pragma unroll
-        for (int k = 0; k < VEC * elem_bytes(T) / 16; ++k) {
-            const u32x4 w = __builtin_nontemporal_load(q + k);
-            constexpr int kPer = 16 / elem_bytes(T);
-            const uint32_t words[4] = {w[0], w[1], w[2], w[3]};
-#pragma unroll
-            for (int e = 0; e < kPer; ++e) v[k * kPer + e] = grad_elem<T>(words, e);
-        }
-    } else {
-        load_grad_vec<T, VEC>(p, i, v);
-    }
+    load_grad_vec<T, VEC>(p, i, v);
 }
 
 // VEC consecutive floats rounded to type T and stored from element i.  NT: past
