@@ -40,6 +40,19 @@ __device__ __forceinline__ void store_any(void *p, int64_t i, float v, int dtype
     else static_cast<uint16_t *>(p)[i] = dtype == PLE_DTYPE_BF16 ? bf16_bits(v) : f16_bits(v);
 }
 
+// Maximum over aligned groups of W lanes (a power of two), to all of them; NaN is
+// passed over.  As group_sum.
+template <int W>
+__device__ __forceinline__ float group_max(float v) {
+    if constexpr (W >= 2) v = fmaxf(v, dpp_f32<0xB1>(v));
+    if constexpr (W >= 4) v = fmaxf(v, dpp_f32<0x4E>(v));
+    if constexpr (W >= 8) v = fmaxf(v, dpp_f32<0x141>(v));
+    if constexpr (W >= 16) v = fmaxf(v, dpp_f32<0x140>(v));
+    if constexpr (W >= 32) v = fmaxf(v, __shfl_xor(v, 16));
+    if constexpr (W >= 64) v = fmaxf(v, __shfl_xor(v, 32));
+    return v;
+}
+
 // The lanes that share a row.  TEAM: 8, 16, 32 or 64 lanes inside a wave, or
 // (more than 64) a workgroup of at most that many threads.
 template <int TEAM>
@@ -67,29 +80,32 @@ struct Team {
         }
     }
 
-    // N values joined over the workgroup's waves (`v`: a wave's), in a fixed order
-    template <int N, typename F>
-    __device__ __forceinline__ void over_waves(float (&v)[N], F join) {
+    // N values of each wave to all lanes, a wave's a lane (`none` past the last):
+    // every aligned group of kWaves lanes has them all, to be joined by DPP
+    static constexpr int kWaves = kBlockWide ? TEAM / kWave : 1;
+    template <int N>
+    __device__ __forceinline__ void spread(float (&v)[N], float none) {
         static_assert(N <= kMost, "values");
         // (two buffers in turn: a wave can be one ahead of another)
-        float *buf = lds + (turn ^= 1) * (kMost * TEAM / kWave);
-        const int waves = blockDim.x / kWave;
+        float *buf = lds + (turn ^= 1) * (kMost * kWaves);
         if (threadIdx.x % kWave == 0)
 #pragma unroll
             for (int i = 0; i < N; ++i) buf[threadIdx.x / kWave * N + i] = v[i];
         __syncthreads();
+        const int w = threadIdx.x % kWaves;
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = buf[i];
-        for (int w = 1; w < waves; ++w)
-#pragma unroll
-            for (int i = 0; i < N; ++i) v[i] = join(v[i], buf[w * N + i]);
+        for (int i = 0; i < N; ++i) v[i] = w < static_cast<int>(blockDim.x) / kWave ? buf[w * N + i] : none;
     }
     // sums of N values over the team's lanes, to all of them
     template <int N>
     __device__ __forceinline__ void sums(float (&v)[N]) {
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = group_sum<kBlockWide ? kWave : TEAM>(v[i]);
-        if constexpr (kBlockWide) over_waves(v, [](float a, float b) { return a + b; });
+        if constexpr (kBlockWide) {
+            spread(v, 0.0f);
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = group_sum<kWaves>(v[i]);
+        }
     }
     __device__ __forceinline__ void sum2(float &a, float &b) {
         float v[2] = {a, b};
@@ -106,10 +122,12 @@ struct Team {
     template <int N>
     __device__ __forceinline__ void maxima(float (&v)[N]) {
 #pragma unroll
-        for (int o = (kBlockWide ? kWave : TEAM) / 2; o > 0; o >>= 1)
+        for (int i = 0; i < N; ++i) v[i] = group_max<kBlockWide ? kWave : TEAM>(v[i]);
+        if constexpr (kBlockWide) {
+            spread(v, -__builtin_inff());
 #pragma unroll
-            for (int i = 0; i < N; ++i) v[i] = fmaxf(v[i], __shfl_xor(v[i], o));
-        if constexpr (kBlockWide) over_waves(v, [](float a, float b) { return fmaxf(a, b); });
+            for (int i = 0; i < N; ++i) v[i] = group_max<kWaves>(v[i]);
+        }
     }
 };
 
