@@ -307,8 +307,8 @@ int ple_encode_plan_query(const void *output, int64_t N, int64_t F, int64_t B, i
  * A negative token is a missing value: its output is 0.  A token beyond its
  * table (its column's size, or V rows) gives NaN.  Neither reads the table.
  *   tokens     int32 or int64 (token_bytes 4 or 8) [T]
- *   offsets    int64 [F + 1], the columns' first rows and V; or NULL (F is
- *              not used then; pass 1)
+ *   offsets    int64 [F + 1], the columns' first rows and V, not decreasing;
+ *              or NULL (F is not used then; pass 1)
  *   weight     weight_dtype [V, D]
  *   output     output_dtype [T, D]
  * T may be 0.  T, V < 2^31 - 1, D <= 2^20 (else PLE_E_TOO_LARGE).
