@@ -500,13 +500,15 @@ struct DistillPlan {
 
 constexpr int kMaxPart = 1 << 18;        // classes a workgroup has bits for, about (32 KB)
 
-DistillPlan plan_distill(int64_t N, int64_t V) {
-    // Lanes a row: 8 elements or more for each (16 lanes for 100 classes: 4.8 us
-    // where a wave took 5.8, 4096 rows fp32), a workgroup beyond 2048 classes.
+DistillPlan plan_distill(int64_t N, int64_t V, int vec = 8) {
+    // Lanes a row: a few vectors for each, of `vec` classes (65536 rows bf16: 200
+    // classes by waves 82 us, by 16 lanes 40; 500 classes 101 and 80; 500 fp32, 125
+    // vectors, 54 and 63), a workgroup beyond 4096 classes (2100 classes by
+    // workgroups 104 us, by waves 63; 4096 60 and 55; 8192 48.5 and 51).
     // Splits: four workgroups a CU where the rows are fewer, 2048 classes each at
     // least.
     DistillPlan p{};
-    p.team = V <= 64 ? 8 : (V <= 128 ? 16 : (V <= 2048 ? kWave : kBlock));
+    p.team = V <= 8 * vec ? 8 : (V <= 64 * vec ? 16 : (V <= 4096 ? kWave : kBlock));
     p.threads = kBlock;
     p.per_block = kBlock / p.team;
     p.splits = 1;
@@ -568,10 +570,11 @@ dim3 distill_grid(const DistillRequest &r, const DistillPlan &p) {
 
 }  // namespace
 
+// (rows that are split are a workgroup's whatever the type)
 size_t distill_workspace_bytes(int64_t N, int64_t V) { return plan_distill(N, V).bytes; }
 
 int distill_run(const DistillRequest &r) {
-    const DistillPlan p = plan_distill(r.N, r.V);
+    const DistillPlan p = plan_distill(r.N, r.V, 16 / elem_bytes(r.dtype));
     if (p.bytes > 0 && (!r.workspace || r.workspace_bytes < p.bytes || reinterpret_cast<uintptr_t>(r.workspace) % 256 != 0))
         return PLE_E_WORKSPACE;
     const DistillArgs a = distill_args(r, p);
@@ -591,7 +594,7 @@ int distill_run(const DistillRequest &r) {
 }
 
 int distill_backward_run(const DistillRequest &r) {
-    const DistillPlan p = plan_distill(r.N, r.V);
+    const DistillPlan p = plan_distill(r.N, r.V, 16 / elem_bytes(r.dtype));
     const DistillArgs a = distill_args(r, p);
     // one vector for z and dz: both addresses are the same way into 16 bytes
     const bool vec = (reinterpret_cast<uintptr_t>(r.logits) - reinterpret_cast<uintptr_t>(r.dz)) % 16 == 0;

@@ -306,14 +306,16 @@ struct Held {
 };
 
 // Waves a SIMD the backward of wide rows is compiled for (its registers: 128, 168
-// or 256).
+// or 256).  Workgroups of up to 768 threads have 168, of more than that 128, which
+// with biases are too few (9000 x 5120 layer norms with biases: 547 us with 128,
+// 232 with 168).
 constexpr int backward_waves(bool vec, bool bias) { return !vec ? 2 : bias ? 3 : 4; }
 
 // Teams walk units of rows: a row each, or a piece of the rows of one gate, whose
 // sum is finished with the piece.  BIAS: the norms may have biases.  OWN: rows or
 // groups of them have gates of their own.
 template <int R, int Y, int TEAM, bool VEC, bool BIAS, bool OWN>
-__global__ __launch_bounds__(Team<TEAM>::kThreads, TEAM == 512 ? backward_waves(VEC, BIAS) : 1) void ple_norm_backward_kernel(NormArgs a) {
+__global__ __launch_bounds__(Team<TEAM>::kThreads, TEAM == 512 ? backward_waves(VEC, BIAS) : TEAM == 768 ? 3 : 1) void ple_norm_backward_kernel(NormArgs a) {
     constexpr int kTeams = Team<TEAM>::kBlockWide ? 1 : kBlock / TEAM;
     __shared__ float s_sum[Team<TEAM>::kLdsFloats];
     __shared__ float s_cols[kTeams > 1 ? kBlock * kElems : 1];
@@ -519,7 +521,7 @@ NormPlan plan_norm(const NormRequest &r) {
     NormPlan p{};
     if (r.N == 0) return p;
     const int lanes = static_cast<int>((r.D + kElems - 1) / kElems);
-    p.team = lanes <= 8 ? 8 : (lanes <= 16 ? 16 : (lanes <= 32 ? 32 : (lanes <= 64 ? 64 : (lanes <= 512 ? 512 : 1024))));
+    p.team = lanes <= 8 ? 8 : (lanes <= 16 ? 16 : (lanes <= 32 ? 32 : (lanes <= 64 ? 64 : (lanes <= 512 ? 512 : (lanes <= 768 ? 768 : 1024)))));
     p.threads = p.team > kWave ? (lanes + kWave - 1) / kWave * kWave : kBlock;
     p.per_block = p.team > kWave ? 1 : kBlock / p.team;
     p.vec = r.D % kElems == 0;
@@ -535,7 +537,7 @@ NormPlan plan_norm(const NormRequest &r) {
     // (3 waves of 168 registers: 768 workgroups took 175 us where 1024 took 228,
     // 32800 x 1152), and by LDS
     const bool bias = r.post_b || r.pre_b;
-    const int simd_waves = p.team == 1024 ? 4 : p.team < 512 ? (bias ? 2 : 3) : backward_waves(p.vec, bias);
+    const int simd_waves = p.team == 1024 ? 4 : p.team == 768 ? 3 : p.team < 512 ? (bias ? 2 : 3) : backward_waves(p.vec, bias);
     const int block_waves = p.threads / kWave;
     const int filled = block_waves <= 2 ? block_waves : (block_waves + 3) / 4 * 4;
     p.lds = p.team > kWave ? static_cast<size_t>((r.post_w != nullptr) + (r.post_b != nullptr) + (r.pre_w != nullptr) +
@@ -599,6 +601,7 @@ hipError_t with_norm(const NormRequest &r, const NormPlan &p, F f) {
             case 32: return by_vec(st, br, std::integral_constant<int, 32>{});
             case 64: return by_vec(st, br, std::integral_constant<int, 64>{});
             case 512: return by_vec(st, br, std::integral_constant<int, 512>{});
+            case 768: return by_vec(st, br, std::integral_constant<int, 768>{});
             default: return by_vec(st, br, std::integral_constant<int, 1024>{});
         }
     };

@@ -59,8 +59,9 @@ template <int TEAM>
 struct Team {
     static constexpr bool kBlockWide = TEAM > kWave;
     static constexpr int kThreads = kBlockWide ? TEAM : kBlock;
+    static constexpr int kWaves = !kBlockWide ? 1 : TEAM <= 256 ? 4 : TEAM <= 512 ? 8 : 16;      // at most
     static constexpr int kMost = 8;              // values of one sum or maximum
-    static constexpr int kLdsFloats = kBlockWide ? 2 * kMost * TEAM / kWave : 1;
+    static constexpr int kLdsFloats = kBlockWide ? 2 * kMost * kWaves : 1;
     float *lds;                  // kLdsFloats floats
     int turn = 0;
     __device__ __forceinline__ explicit Team(float *s) : lds(s) {}
@@ -82,7 +83,6 @@ struct Team {
 
     // N values of each wave to all lanes, a wave's a lane (`none` past the last):
     // every aligned group of kWaves lanes has them all, to be joined by DPP
-    static constexpr int kWaves = kBlockWide ? TEAM / kWave : 1;
     template <int N>
     __device__ __forceinline__ void spread(float (&v)[N], float none) {
         static_assert(N <= kMost, "values");
