@@ -53,7 +53,7 @@ struct DistillArgs {
     const float *g;
     void *dz;
     float *loss;
-    float *stats;                // a row: maximum, log2 of the sums at T and 1, l; m, factor outside, labelled
+    float *stats;                // a row: maximum, log2 of the sums at T and 1, l; m, factor outside, labelled, its base
     float *partial;              // [N, splits, 4]
     int64_t N;
     int V, K, t_dtype, wide;     // wide: 64-bit classes
@@ -129,24 +129,26 @@ struct Sums {
         if constexpr (SUMS != kOneSum) at_1 *= exp2_fast((m - to) * kLog2e);
         m = to;
     }
-    // adds N vectors without the classes of `skip` (bit e: element e)
+    // adds N vectors without the classes of `skip` (bit e: element e), of which the
+    // maximum is not either
     template <int N, int Z, int VEC>
     __device__ __forceinline__ void add(const Words<Z, VEC> (&w)[N], const uint32_t (&skip)[N], float ct) {
-        float v[N][VEC], top = w[0].at(0);
+        float v[N][VEC];
 #pragma unroll
-        for (int k = 0; k < N; ++k)
+        for (int k = 0; k < N; ++k) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                v[k][e] = w[k].at(e);
-                top = fmaxf(top, v[k][e]);
-            }
-        if (top > m) rescale(top, ct);
-#pragma unroll
-        for (int k = 0; k < N; ++k)
+            for (int e = 0; e < VEC; ++e) v[k][e] = w[k].at(e);
             if (skip[k])
 #pragma unroll
                 for (int e = 0; e < VEC; ++e)
                     if ((skip[k] >> e) & 1) v[k][e] = -__builtin_inff();
+        }
+        float top = v[0][0];
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) top = fmaxf(top, v[k][e]);
+        if (top > m) rescale(top, ct);
         // (a sum of its own for every vector: their additions overlap)
         float part[N], part_1[N];
 #pragma unroll
@@ -247,7 +249,9 @@ __device__ __forceinline__ void scan_row(Team<TEAM> &team, const DistillArgs &a,
 }
 
 // The row's loss and stats from its lanes' sums.  mine: this lane's first entry.
-// With a given l the sums leave out the K classes, which may occur `twice`.
+// With a given l the sums and their maximum leave out the K classes, which may
+// occur `twice`: the outside mass keeps its own scale, however far below the
+// row's maximum it is.
 template <int Z, int TEAM, int SUMS>
 __device__ __forceinline__ void finish_row(Team<TEAM> &team, const DistillArgs &a, int64_t n, const Entry &mine,
                                            const Entry &label, Sums<SUMS> &s, bool twice) {
@@ -257,13 +261,13 @@ __device__ __forceinline__ void finish_row(Team<TEAM> &team, const DistillArgs &
         for (int k = team.lane(); on && k < a.K; k += team.lanes()) f(k, k == team.lane() ? mine : load_entry<Z>(a, n, k));
     };
     const auto in_range = [&](const Entry &e) { return e.c >= 0 && e.c < a.V; };
-    float top[2] = {s.m, -FLT_MAX};
-    if (!tail)
-        each([&](int, const Entry &e) {
-            if (e.c >= 0) top[1] = fmaxf(top[1], e.t);
-        });
+    float top[2] = {s.m, -FLT_MAX};      // of the sums; of the K classes (given l), else the teacher's
+    each([&](int, const Entry &e) {
+        if (tail ? in_range(e) : e.c >= 0) top[1] = fmaxf(top[1], tail ? e.z : e.t);
+    });
     team.maxima(top);
     s.rescale(top[0], ct);
+    const float peak = tail ? fmaxf(s.m, top[1]) : s.m;
     // sums: at T, at 1; of the K classes at T, at 1 (given l), else the teacher's; its
     // mass and cross terms (given l); entries, with 2^12 for one beyond V
     enum { kSumT, kSum1, kInT, kIn1, kMassP, kCross, kCount, kValues };
@@ -284,12 +288,12 @@ __device__ __forceinline__ void finish_row(Team<TEAM> &team, const DistillArgs &
         if (twice)
             for (int i = 0; i < k; ++i) first = first && class_of(a, n * a.K + i) != e.c;
         if (first) {
-            v[kInT] += exp2_fast((e.z - s.m) * ct);
-            v[kIn1] += exp2_fast((e.z - s.m) * kLog2e);
+            v[kInT] += exp2_fast((e.z - peak) * ct);
+            v[kIn1] += exp2_fast((e.z - peak) * kLog2e);
         }
         const float log_p = e.t - lse, p = exp2_fast(log_p * kLog2e);
         v[kMassP] += p;
-        if (p != 0.0f) v[kCross] += p * (log_p - (e.z - s.m) * a.inv_t);
+        if (p != 0.0f) v[kCross] += p * (log_p - (e.z - peak) * a.inv_t);
     });
     v[kCount] = (some ? 1.0f : 0.0f) + (wrong ? kWrong : 0.0f);      // (exact: at most 256 lanes)
     team.sums(v);
@@ -297,9 +301,10 @@ __device__ __forceinline__ void finish_row(Team<TEAM> &team, const DistillArgs &
     wrong = v[kCount] >= kWrong;
     const float outside = v[kSumT];
     float at_t = outside, at_1 = SUMS == kOneSum ? v[kSumT] : v[kSum1], kd = v[kCross], mass = v[kMassP];
+    const float down = tail ? exp2_fast((s.m - peak) * ct) : 1.0f;       // from the sums' scale to the row's
     if (tail) {
-        at_t += v[kInT];
-        at_1 += SUMS == kOneSum ? v[kInT] : v[kIn1];
+        at_t = outside * down + v[kInT];
+        at_1 = SUMS == kOneSum ? at_t : at_1 * exp2_fast((s.m - peak) * kLog2e) + v[kIn1];
     }
     const float log_t = logf(at_t), log_1 = logf(at_1);
     if (tail) {
@@ -311,19 +316,22 @@ __device__ __forceinline__ void finish_row(Team<TEAM> &team, const DistillArgs &
             if (!in_range(e)) return;
             const float log_p = e.t - lse, p = exp2_fast(log_p * kLog2e);
             mass += p;
-            if (p != 0.0f) kd += p * (log_p - (e.z - s.m) * a.inv_t + log_t);
+            if (p != 0.0f) kd += p * (log_p - (e.z - peak) * a.inv_t + log_t);
         });
         team.sum2(kd, mass);
     }
     if (team.lane() != 0 || !on) return;
-    float factor = mass, labelled = 0.0f, ce = 0.0f, m = s.m;
+    // factor: what a class without sparse terms has its exp((z - base) / T) times
+    float factor = mass / at_t, base = peak, labelled = 0.0f, ce = 0.0f, m = peak;
     if (tail && taught) {
-        const float rho = fmaxf(1.0f - mass, 0.0f);
-        // (a row whose K classes are all there are has no outside)
-        if (rho > 0.0f && outside > 0.0f) {
-            kd += rho * (logf(rho) - logf(outside) + log_t);
+        const float rho = fmaxf(1.0f - mass, 0.0f), gap = (s.m - peak) * a.inv_t;
+        // (a row whose K classes are all there are has no outside; nor has one whose
+        // others are at the type's lowest value: a mass below what 64 bits hold is none)
+        if (rho > 0.0f && outside > 0.0f && gap > -700.0f) {
+            kd += rho * (logf(rho) - (logf(outside) + gap) + log_t);
             mass += rho;
-            factor = mass - rho * (at_t / outside);
+            factor = mass * down / at_t - rho / outside;
+            base = s.m;
         }
     }
     if (label.c >= a.V) labelled = ce = __builtin_nanf("");
@@ -333,10 +341,10 @@ __device__ __forceinline__ void finish_row(Team<TEAM> &team, const DistillArgs &
     }
     if (wrong) kd = mass = factor = __builtin_nanf("");
     const bool live = at_t != 0.0f;      // else every class is masked: no loss, no gradient
-    if (!live) kd = ce = m = mass = factor = labelled = 0.0f;
+    if (!live) kd = ce = m = mass = factor = base = labelled = 0.0f;
     float4 *st = reinterpret_cast<float4 *>(a.stats + n * PLE_DISTILL_STATS);
     st[0] = make_float4(m, live ? log_t * kLog2e : 0.0f, live ? log_1 * kLog2e : 0.0f, lse);
-    st[1] = make_float4(mass, factor, labelled, 0.0f);
+    st[1] = make_float4(mass, factor, labelled, base);
     a.loss[n] = (a.alpha > 0.0f && taught ? a.alpha * a.t_factor * a.t_factor * kd : 0.0f) +
                 (a.alpha < 1.0f && labelled != 0.0f ? (1.0f - a.alpha) * ce : 0.0f);
 }
@@ -416,17 +424,18 @@ __global__ __launch_bounds__(Team<TEAM>::kThreads) void ple_distill_backward_ker
         g = a.g[n];
     }
     const bool twice = mark_classes(team, a, n, mine, r, bits, &s_twice[team.index()]);
-    const float peak = st0.x, log_t = st0.y, log_1 = st0.z, lse = st0.w, mass = st1.x;
+    const float peak = st0.x, log_t = st0.y, log_1 = st0.z, lse = st0.w, mass = st1.x, base = st1.w;
     const float w_soft = a.alpha > 0.0f && mass != 0.0f ? g * a.alpha * a.t_factor : 0.0f;
     const float w_out = w_soft != 0.0f ? w_soft * st1.y : 0.0f;
     const float w_hard = a.alpha < 1.0f && st1.z != 0.0f ? g * (1.0f - a.alpha) * st1.z : 0.0f;
     if (st1.z == 0.0f) label.c = -1;
     const auto soft = [&](float z) { return exp2_fast((z - peak) * ct - log_t); };
     const auto hard = [&](float z) { return exp2_fast((z - peak) * kLog2e - log_1); };
-    // the dense terms, with the sums' logarithms taken into the weights
-    const float w_t = (SUMS == kOneSum ? w_out + w_hard : w_out) * exp2_fast(-log_t), w_1 = w_hard * exp2_fast(-log_1);
+    // The dense terms, from the outside classes' own scale; of the K classes they may
+    // overflow, and are written over.
+    const float w_1 = w_hard * exp2_fast((base - peak) * kLog2e - log_1), w_t = SUMS == kOneSum ? w_out + w_1 : w_out;
     const auto dense = [&](float z) {
-        const float d = z - peak, x = exp2_fast(d * ct);
+        const float d = z - base, x = exp2_fast(d * ct);
         if constexpr (SUMS == kOneSum) return w_t * x;
         else if constexpr (SUMS == kTwoSums) return w_t * x + w_1 * exp2_fast(d * kLog2e);
         else return w_t * x + w_1 * at_one<SUMS>(x);

@@ -256,10 +256,11 @@ def _distill_cpu(logits, teacher_logits, classes, teacher_lse, labels, temperatu
     if teacher_lse is not None:
         inside = torch.zeros(n, v, dtype=torch.int32)
         inside.scatter_add_(1, c, known.int())
-        outside = (log_q.exp() * (inside == 0)).sum(-1)
+        # (in logarithms: a student's outside mass may be below what 32 bits hold)
+        log_outside = torch.logsumexp(log_q.masked_fill(inside != 0, -torch.inf), -1)
         rho = (1 - p.sum(-1)).clamp_min(0)
-        some = taught & (rho > 0) & (outside > 0)
-        kd = kd + torch.where(some, rho * (torch.where(some, rho, 1.0).log() - torch.where(some, outside, 1.0).log()), 0.0)
+        some = taught & (rho > 0) & (log_outside > -700)
+        kd = kd + torch.where(some, rho * (torch.where(some, rho, 1.0).log() - torch.where(some, log_outside, 0.0)), 0.0)
     kd = torch.where(taught, kd, 0.0)
     kd = torch.where((classes >= v).any(-1), torch.nan, kd)
     loss = alpha * temperature ** 2 * kd if alpha > 0 else torch.zeros(n)

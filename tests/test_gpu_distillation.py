@@ -194,6 +194,22 @@ def test_masked_classes(ops, v, dtype):
     _check(ops, {k: t[keep] for k, t in x.items()})
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=lambda d: str(d)[6:])
+@pytest.mark.parametrize("v", [14, 90, 3000, 40_000])
+@pytest.mark.parametrize("temperature", [1.0, 1.5, 2.0])
+def test_outside_mass_below_32_bits(ops, v, dtype, temperature):
+    """A student that is sure of the teacher's classes: the mass outside them has no
+    number in 32 bits, its logarithm and the outside classes' shares of it do."""
+    x = _inputs(6, v, 8, F32, True)
+    near = torch.zeros(6, v).scatter_(1, x["c"], 1.0)
+    x["z"] = (x["z"] - 300 * (1 - near)).to(dtype)
+    x["lse"] = torch.logsumexp(x["t"] / temperature, -1) + 0.3
+    loss, _ = _run(ops, x, temperature, 0.6)
+    assert bool((loss > 10).all())
+    _check(ops, x, temperature)
+    _check(ops, dict(x, labels=None), temperature, 1.0)
+
+
 def test_large_and_non_finite_logits(ops):
     x = _inputs(10, 400, 8, tail=True)
     x["z"][0] *= 1e4

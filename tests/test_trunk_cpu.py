@@ -215,6 +215,23 @@ def test_module_loss_on_cpu():
     torch.testing.assert_close(a, b, rtol=1e-5, atol=1e-5)
 
 
+def test_module_loss_outside_mass_below_32_bits():
+    """A student whose mass outside the teacher's classes has no number in 32 bits."""
+    gen = torch.Generator().manual_seed(3)
+    z, t = torch.randn(5, 20, generator=gen), torch.randn(5, 4, generator=gen)
+    c = torch.arange(4).expand(5, 4).contiguous()
+    z[:, 4:] -= 300
+    z.requires_grad_()
+    lse = torch.logsumexp(t, -1) + 0.3
+    got = pkg.CudaDistillationLoss(1.0, 1.0, "sum")(z, t, c, lse)
+    zd = z.detach().double().requires_grad_()
+    log_q, log_p = torch.log_softmax(zd, -1), t.double() - lse.double()[:, None]
+    rho = 1 - log_p.exp().sum(-1)
+    want = ((log_p.exp() * (log_p - log_q[:, :4])).sum(-1) + rho * (rho.log() - torch.logsumexp(log_q[:, 4:], -1))).sum()
+    torch.testing.assert_close(got.double(), want, rtol=1e-5, atol=0)
+    torch.testing.assert_close(torch.autograd.grad(got, z)[0].double(), torch.autograd.grad(want, zd)[0], rtol=1e-4, atol=1e-5)
+
+
 @pytest.mark.parametrize("call,match", [
     (lambda: pkg.CudaTokenEmbeddings(0, 3), "positive"),
     (lambda: pkg.CudaTokenEmbeddings(4, 3, padding_idx=4), "padding_idx"),
