@@ -83,12 +83,13 @@ struct GatherArgs {
     TokenArgs t;
     const void *weight;
     void *out;
-    int64_t D;
+    int64_t D, first;            // first: the launch's first token
     float scale;
     int lg;                      // log2 of the lanes that share a token
 };
 
 constexpr int kGatherUnroll = 4;
+constexpr int64_t kGatherBlocks = 1 << 23;       // of a launch: a grid holds fewer than 2^32 threads a dimension
 
 // A group of lanes has kGatherUnroll vectors in flight: of one token's row
 // where it is long enough, else of as many tokens' rows (TOKENS).  The output is
@@ -99,7 +100,8 @@ template <int W, int O, int VEC, bool TOKENS>
 __global__ __launch_bounds__(kBlock) void ple_lookup_kernel(GatherArgs a) {
     const int lanes = 1 << a.lg;
     const int64_t per_block = kBlock >> a.lg;
-    const int64_t i0 = static_cast<int64_t>(blockIdx.x) * per_block * (TOKENS ? kGatherUnroll : 1) + (threadIdx.x >> a.lg);
+    const int64_t i0 = a.first + static_cast<int64_t>(blockIdx.x) * per_block * (TOKENS ? kGatherUnroll : 1) +
+                       (threadIdx.x >> a.lg);
     const int64_t col0 = (static_cast<int64_t>(blockIdx.y) * (TOKENS ? 1 : kGatherUnroll) * lanes +
                           (threadIdx.x & (lanes - 1))) * VEC;
     const auto token = [&](int u) { return i0 + (TOKENS ? u * per_block : 0); };
@@ -743,12 +745,15 @@ hipError_t launch_gather(GatherArgs a, hipStream_t s) {
     a.lg = std::min(6, vecs <= 1 ? 0 : bits_of(static_cast<uint64_t>(vecs - 1)));
     const int64_t per_block = kBlock >> a.lg, lanes = int64_t{1} << a.lg;
     const auto blocks = [](int64_t n, int64_t per) { return static_cast<unsigned>((n + per - 1) / per); };
-    if (vecs <= lanes)
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_lookup_kernel<W, O, VEC, true>), dim3(blocks(a.t.T, per_block * kGatherUnroll)),
-                           dim3(kBlock), 0, s, a);
-    else
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_lookup_kernel<W, O, VEC, false>),
-                           dim3(blocks(a.t.T, per_block), blocks(vecs, lanes * kGatherUnroll)), dim3(kBlock), 0, s, a);
+    const int64_t per = vecs <= lanes ? per_block * kGatherUnroll : per_block;
+    for (a.first = 0; a.first < a.t.T; a.first += kGatherBlocks * per) {
+        const unsigned n = static_cast<unsigned>(std::min(kGatherBlocks, (a.t.T - a.first + per - 1) / per));
+        if (vecs <= lanes)
+            hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_lookup_kernel<W, O, VEC, true>), dim3(n), dim3(kBlock), 0, s, a);
+        else
+            hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_lookup_kernel<W, O, VEC, false>), dim3(n, blocks(vecs, lanes * kGatherUnroll)),
+                               dim3(kBlock), 0, s, a);
+    }
     return hipGetLastError();
 }
 

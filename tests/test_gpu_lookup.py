@@ -316,3 +316,15 @@ def test_workspace_and_steps(ops, t, d, dtype):
     tokens = (torch.rand(t, generator=gen) ** 4 * v).long()
     g = torch.randn(t, d, generator=gen).to(dtype)
     _check_backward(ops, tokens, g, v, 1.0, dtype)
+
+
+def test_more_blocks_than_one_grid(ops):
+    """70 million tokens of odd rows beyond one wave: their lanes pass 32 bits."""
+    n, d = 70_000_000, 65
+    weight = torch.arange(3 * d, dtype=F32).reshape(3, d).to(F16).to(DEV)
+    tokens = (torch.arange(n, device=DEV, dtype=torch.int32) * 7) % 3
+    tokens[-1] = -1
+    out = ops.lookup(tokens, weight, None, 1.0, -1, F16)
+    assert not bool(out[-1].any())
+    at = torch.cat([torch.arange(0, n - 1, 997), torch.arange(33_554_000, 33_555_000), torch.arange(n - 3000, n - 1)]).to(DEV)
+    assert torch.equal(out[at], weight[tokens[at].long()])
