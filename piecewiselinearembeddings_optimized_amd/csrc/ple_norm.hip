@@ -517,19 +517,15 @@ int gate_mode(const NormRequest &r) {
     return r.groups == 1 ? 1 : (r.groups == r.N ? 3 : 2);
 }
 
-NormPlan plan_norm(const NormRequest &r) {
+// aligned: whether every tensor's rows can be read as vectors.
+NormPlan plan_norm(const NormRequest &r, bool aligned) {
     NormPlan p{};
     if (r.N == 0) return p;
     const int lanes = static_cast<int>((r.D + kElems - 1) / kElems);
     p.team = lanes <= 8 ? 8 : (lanes <= 16 ? 16 : (lanes <= 32 ? 32 : (lanes <= 64 ? 64 : (lanes <= 512 ? 512 : (lanes <= 768 ? 768 : 1024)))));
     p.threads = p.team > kWave ? (lanes + kWave - 1) / kWave * kWave : kBlock;
     p.per_block = p.team > kWave ? 1 : kBlock / p.team;
-    p.vec = r.D % kElems == 0;
-    for (const void *q : {r.residual, r.branch, r.g_stream, r.g_normed, static_cast<const void *>(r.stream_out),
-                          static_cast<const void *>(r.normed), static_cast<const void *>(r.d_residual),
-                          static_cast<const void *>(r.d_branch), r.post_w, r.post_b, r.gate, r.pre_w, r.pre_b,
-                          static_cast<const void *>(r.d_gate)})
-        p.vec = p.vec && reinterpret_cast<uintptr_t>(q) % 16 == 0;
+    p.vec = aligned && r.D % kElems == 0;
     const int mode = gate_mode(r);
     // as many backward workgroups as run at once (a few more leave most of the GPU
     // idle at the end): by the waves a SIMD has registers for, where workgroups of
@@ -569,6 +565,16 @@ NormPlan plan_norm(const NormRequest &r) {
     p.o_gate = align_up(static_cast<size_t>(p.blocks) * p.slots * r.D * 4, 256);
     p.bytes = p.o_gate + (mode == 2 && p.pieces > 1 ? align_up(static_cast<size_t>(units) * r.D * 4, 256) : 0);
     return p;
+}
+
+NormPlan plan_norm(const NormRequest &r) {
+    bool aligned = true;
+    for (const void *q : {r.residual, r.branch, r.g_stream, r.g_normed, static_cast<const void *>(r.stream_out),
+                          static_cast<const void *>(r.normed), static_cast<const void *>(r.d_residual),
+                          static_cast<const void *>(r.d_branch), r.post_w, r.post_b, r.gate, r.pre_w, r.pre_b,
+                          static_cast<const void *>(r.d_gate)})
+        aligned = aligned && reinterpret_cast<uintptr_t>(q) % 16 == 0;
+    return plan_norm(r, aligned);
 }
 
 NormArgs norm_args(const NormRequest &r) {
@@ -652,7 +658,12 @@ int norm_run(const NormRequest &r) {
     }));
 }
 
-size_t norm_backward_workspace_bytes(const NormRequest &r) { return r.D > kMaxD ? 0 : plan_norm(r).bytes; }
+// (Before the call's addresses are known.  The pieces of gates' rows follow the
+// number of workgroups, which is another where vectors are not aligned: either may
+// need more.)
+size_t norm_backward_workspace_bytes(const NormRequest &r) {
+    return r.D > kMaxD ? 0 : std::max(plan_norm(r, true).bytes, plan_norm(r, false).bytes);
+}
 
 int norm_backward_run(const NormRequest &r) {
     if (r.D > kMaxD) return PLE_E_TOO_LARGE;

@@ -279,6 +279,24 @@ def test_unaligned_rows(ops, d):
         torch.testing.assert_close(a, b, rtol=2e-2, atol=2e-2)
 
 
+def test_unaligned_rows_with_gates_of_groups(ops):
+    """Their workspace is asked for before the addresses are known."""
+    x = _inputs(2570, 1152, BF16, BF16, BF16, gates=257)
+    x["post_weight"] = x["pre_weight"] = None
+    want = _run(ops, x, RMS, RMS, 0, 1.0)
+    dev = {k: None if v is None else v.to(DEV) for k, v in x.items()}
+    for k in ("residual", "branch", "g_stream", "g_normed"):
+        base = torch.zeros(dev[k].numel() + 1, dtype=BF16, device=DEV)
+        base[1:] = dev[k].reshape(-1)
+        dev[k] = base[1:].view(dev[k].shape)
+    params = [dev[k] for k in NAMES]
+    stream, normed, stats = ops.residual_norm(dev["residual"], dev["branch"], *params, RMS, RMS, 0, 1.0, EPS, BF16)
+    grads = ops.residual_norm_backward(dev["g_stream"], dev["g_normed"], stream, dev["branch"], stats, *params, RMS, RMS, 0,
+                                       1.0, [True] * 7)
+    for a, b in zip((stream, normed, *grads), (*want[:2], *want[2])):
+        torch.testing.assert_close(a, b, rtol=2e-2, atol=2e-2)
+
+
 def test_empty(ops):
     x = _inputs(0, 32, gates=3, bias=True)
     stream, normed, grads = _run(ops, x, RMS, LAYER, 0, 1.0)
