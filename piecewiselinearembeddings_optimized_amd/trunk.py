@@ -190,7 +190,9 @@ class CudaResidualNorm(nn.Module):
                 raise ValueError(f"gate of shape {tuple(gate.shape)} does not broadcast over rows of shape "
                                  f"{tuple(residual.shape)} in groups of consecutive rows")
             shared = True
-        return gate.reshape(-1, self.d)
+        weight = self.post_weight if self.pre_weight is None else self.pre_weight
+        # (under autocast a gate has the autocast dtype, the weights theirs)
+        return (gate if weight is None else gate.to(weight.dtype)).reshape(-1, self.d).contiguous()
 
     def forward(self, residual: Tensor, branch: Tensor | None = None, gate: Tensor | None = None) -> tuple[Tensor, Tensor]:
         if residual.shape[-1:] != (self.d,):

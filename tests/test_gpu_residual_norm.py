@@ -389,6 +389,29 @@ def test_module_gradients(ops, gate):
     assert abs(slope - along) < 0.02 * max(1.0, sum(float((a * s).abs().sum()) for a, s in zip(got, step)) ** 0.5 * 5)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=lambda d: str(d)[6:])
+def test_gate_of_another_layout_and_dtype(ops, dtype):
+    """A gate as a model makes it: a part of a wider tensor, in the autocast dtype."""
+    from piecewiselinearembeddings_optimized_amd import CudaResidualNorm
+
+    gen = torch.Generator().manual_seed(2)
+    m = CudaResidualNorm(24, post_norm="rms", pre_norm="layer", gate_activation="sigmoid")
+    res, br = torch.randn(6, 5, 24, generator=gen), torch.randn(6, 5, 24, generator=gen)
+    wide = torch.randn(6, 1, 72, generator=gen).to(dtype)
+    up = torch.randn(2, 6, 5, 24, generator=gen)
+
+    def grads(m, dev):
+        w = wide.to(dev).requires_grad_()
+        s, n = m(res.to(dev), br.to(dev), w.chunk(3, -1)[1])
+        return s, n, torch.autograd.grad((s * up[0].to(dev)).sum() + (n * up[1].to(dev)).sum(), w)[0]
+
+    want = grads(m, "cpu")
+    got = grads(m.to(DEV), DEV)
+    assert got[2].dtype == dtype
+    for a, b, tol in zip(got, want, (1e-5, 1e-5, 1e-4 if dtype == F32 else 2e-2)):
+        torch.testing.assert_close(a.cpu(), b, rtol=tol, atol=tol)
+
+
 def test_stream_used_twice(ops):
     """Both outputs and the residual's reuse: gradients add up as in plain autograd."""
     from piecewiselinearembeddings_optimized_amd import CudaResidualNorm
