@@ -17,9 +17,9 @@
 // Measured (one MI355X): 65536 tokens x 2048 bf16 over 131072 rows, 1.17 GB in
 // all, 251 us: forward 78 us (its reads and stores, 4.7 TB/s), sort 30 us of
 // which 14 beside the rows that are cleared, clearing and sums 150 us (805 MB,
-// 5.4 TB/s), joins 5 us.  196608 categories x 32 fp32: 55 us, of which the sort's
-// four launches 32 (each a chain of loads, ranks and barriers of 4 to 13 us, on
-// few workgroups) and the sums 15.
+// 5.4 TB/s), joins 5 us.  196608 categories x 32 fp32: 52 us, of which the sort's
+// four launches 29 (each a chain of loads, ranks and barriers, on few workgroups)
+// and the sums 15.
 
 #include <algorithm>
 
@@ -29,12 +29,22 @@
 namespace ple {
 namespace {
 
-constexpr int kSortBlock = 512;
-constexpr int kSortWaves = kSortBlock / kWave;
-constexpr int kSortRounds = 4;         // tokens a lane ranks at a time
-constexpr int kSortStep = kSortBlock * kSortRounds;
 constexpr int kMaxDigitBits = 10;
 constexpr int kMaxTiles = 256;
+
+// A sorting workgroup by its digits' bits (8 or 10 at most).  Up to 8 bits 16 waves
+// rank a token a lane at a time, the shortest chain (by 8 waves of 4 tokens 55.0
+// against 52.5 us, 196608 x 32, and 53.6 against 50.6, 16384 x 1024: whole
+// backwards with their forwards); beyond, every wave's counts are 4 KB, and 8 waves
+// leave room for the workgroups that clear rows beside them (65536 x 2048: 251.8
+// against 254.5 us).
+template <int BITS>
+struct Sort {
+    static constexpr int kBlock = BITS <= 8 ? 1024 : 512;
+    static constexpr int kWaves = kBlock / kWave;
+    static constexpr int kRounds = BITS <= 8 ? 1 : 4;    // tokens a lane ranks at a time
+    static constexpr int kStep = kBlock * kRounds;
+};
 // One workgroup sorts up to this many tokens by itself, in LDS: its 16 waves
 // hold up to 8 of them a lane (one launch for four: 1024 tokens 6 us, 4096 12,
 // 8192 19; by several workgroups 20 to 24 at any of these sizes, 16384 tokens by
@@ -220,9 +230,10 @@ __device__ __forceinline__ uint32_t exclusive_sum(uint32_t v, uint32_t *s_wave) 
     return base;
 }
 
-template <bool FIRST>
-__global__ __launch_bounds__(kSortBlock) void ple_lookup_count_kernel(SortArgs a) {
-    __shared__ uint32_t hist[1 << kMaxDigitBits];
+template <bool FIRST, int BITS>
+__global__ __launch_bounds__(Sort<BITS>::kBlock) void ple_lookup_count_kernel(SortArgs a) {
+    constexpr int kSortBlock = Sort<BITS>::kBlock, kSortRounds = Sort<BITS>::kRounds, kSortStep = Sort<BITS>::kStep;
+    __shared__ uint32_t hist[1 << BITS];
     if (static_cast<int>(blockIdx.x) >= a.tiles) {
         zero_rows(a.z, blockIdx.x - a.tiles);
         return;
@@ -263,7 +274,9 @@ __global__ __launch_bounds__(kSortBlock) void ple_lookup_count_kernel(SortArgs a
 // it walks its tokens in steps: each wave takes a contiguous part of a step and
 // ranks its tokens per digit, the waves' numbers give each wave its place.
 template <bool FIRST, int BITS>
-__global__ __launch_bounds__(kSortBlock) void ple_lookup_scatter_kernel(SortArgs a) {
+__global__ __launch_bounds__(Sort<BITS>::kBlock) void ple_lookup_scatter_kernel(SortArgs a) {
+    constexpr int kSortBlock = Sort<BITS>::kBlock, kSortWaves = Sort<BITS>::kWaves, kSortRounds = Sort<BITS>::kRounds;
+    constexpr int kSortStep = Sort<BITS>::kStep;
     extern __shared__ uint32_t s_dyn[];
     __shared__ uint32_t s_wave[kSortWaves];
     if (static_cast<int>(blockIdx.x) >= a.tiles) {
@@ -315,7 +328,7 @@ __global__ __launch_bounds__(kSortBlock) void ple_lookup_scatter_kernel(SortArgs
     rank_step();
     __syncthreads();
     {
-        constexpr int kPer = (1 << kMaxDigitBits) / kSortBlock;
+        constexpr int kPer = ((1 << BITS) + kSortBlock - 1) / kSortBlock;
         uint32_t total[kPer], sum = 0;
 #pragma unroll
         for (int k = 0; k < kPer; ++k) {
@@ -702,8 +715,8 @@ SumPlan plan_sum(int64_t T, int64_t V, int64_t D, int vec) {
     p.passes = (key_bits + kMaxDigitBits - 1) / kMaxDigitBits;
     p.bits = (key_bits + p.passes - 1) / p.passes;
     p.bits = std::max(2, p.bits);        // (counts are read four digits at a time)
-    const int64_t per = (T + kMaxTiles - 1) / kMaxTiles;
-    p.tile = static_cast<uint32_t>(std::max<int64_t>(1, (per + kSortStep - 1) / kSortStep) * kSortStep);
+    const int64_t per = (T + kMaxTiles - 1) / kMaxTiles, step = p.bits <= 8 ? Sort<8>::kStep : Sort<kMaxDigitBits>::kStep;
+    p.tile = static_cast<uint32_t>(std::max<int64_t>(1, (per + step - 1) / step) * step);
     p.tiles = static_cast<int>((T + p.tile - 1) / p.tile);
     const int64_t vecs = (D + vec - 1) / vec;
     p.lg = std::min(6, vecs <= 1 ? 0 : bits_of(static_cast<uint64_t>(vecs - 1)));
@@ -805,13 +818,13 @@ void launch_local_sort(const SortArgs &s, hipStream_t stream) {
 // rows (their own times are about as 1 to 2).
 template <int BITS>
 void launch_sort_pass(SortArgs s, int pass, int64_t rows, hipStream_t stream) {
-    const size_t lds = static_cast<size_t>(2 + kSortWaves) * 4 << s.bits;
-    const dim3 block(kSortBlock);
+    const size_t lds = static_cast<size_t>(2 + Sort<BITS>::kWaves) * 4 << s.bits;
+    const dim3 block(Sort<BITS>::kBlock);
     s.z.begin = 0;
     s.z.end = pass == 1 ? rows / 3 : 0;
     const auto grid = [&] { return dim3(s.tiles + zero_blocks(s.z)); };
-    if (pass == 0) hipLaunchKernelGGL(ple_lookup_count_kernel<true>, grid(), block, 0, stream, s);
-    else hipLaunchKernelGGL(ple_lookup_count_kernel<false>, grid(), block, 0, stream, s);
+    if (pass == 0) hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_lookup_count_kernel<true, BITS>), grid(), block, 0, stream, s);
+    else hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_lookup_count_kernel<false, BITS>), grid(), block, 0, stream, s);
     s.z.begin = s.z.end;
     s.z.end = pass == 1 ? rows : 0;
     if (pass == 0) hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_lookup_scatter_kernel<true, BITS>), grid(), block, lds, stream, s);
