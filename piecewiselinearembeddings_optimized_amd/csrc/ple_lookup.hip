@@ -46,9 +46,10 @@ struct Sort {
     static constexpr int kStep = kBlock * kRounds;
 };
 // One workgroup sorts up to this many tokens by itself, in LDS: its 16 waves
-// hold up to 8 of them a lane (one launch for four: 1024 tokens 6 us, 4096 12,
-// 8192 19; by several workgroups 20 to 24 at any of these sizes, 16384 tokens by
-// one workgroup 38).
+// hold up to 8 of them a lane (one launch for four; whole backwards of rows of 64:
+// 1500 tokens 14.5 us, by several workgroups 22.8; 4096 19.3 and 23.6; 8000 25.3 and
+// 24.4 to 25.6, and 27.9 against 32.9 where it clears 100000 rows of 256 meanwhile;
+// 16384 tokens' sort alone takes one workgroup 38).
 constexpr int kLocalBlock = 1024;
 constexpr int kLocalWaves = kLocalBlock / kWave;
 constexpr int kLocalRounds = 8;
