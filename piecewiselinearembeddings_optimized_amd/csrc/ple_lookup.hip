@@ -18,8 +18,8 @@
 // all, 251 us: forward 78 us (its reads and stores, 4.7 TB/s), sort 30 us of
 // which 14 beside the rows that are cleared, clearing and sums 150 us (805 MB,
 // 5.4 TB/s), joins 5 us.  196608 categories x 32 fp32: 52 us, of which the sort's
-// four launches 29 (each a chain of loads, ranks and barriers, on few workgroups)
-// and the sums 15.
+// four launches 31 (each a chain of loads, ranks and barriers, on few workgroups)
+// and the sums 14.
 
 #include <algorithm>
 
