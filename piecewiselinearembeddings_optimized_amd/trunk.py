@@ -258,8 +258,12 @@ def _distill_cpu(logits, teacher_logits, classes, teacher_lse, labels, temperatu
     if teacher_lse is not None:
         inside = torch.zeros(n, v, dtype=torch.int32)
         inside.scatter_add_(1, c, known.int())
-        # (in logarithms: a student's outside mass may be below what 32 bits hold)
-        log_outside = torch.logsumexp(log_q.masked_fill(inside != 0, -torch.inf), -1)
+        # (in logarithms: a student's outside mass may be below what 32 bits hold; a row
+        # whose other classes are all masked has none, and the log-sum of nothing has a
+        # gradient of NaN)
+        outside = log_q.masked_fill(inside != 0, -torch.inf)
+        none = torch.isneginf(outside).all(-1)
+        log_outside = torch.where(none, -torch.inf, torch.logsumexp(torch.where(none[:, None], 0.0, outside), -1))
         rho = (1 - p.sum(-1)).clamp_min(0)
         some = taught & (rho > 0) & (log_outside > -700)
         kd = kd + torch.where(some, rho * (torch.where(some, rho, 1.0).log() - torch.where(some, log_outside, 0.0)), 0.0)

@@ -210,6 +210,28 @@ def test_outside_mass_below_32_bits(ops, v, dtype, temperature):
     _check(ops, dict(x, labels=None), temperature, 1.0)
 
 
+@pytest.mark.parametrize("v", [9, 70, 3000, 9000])
+@pytest.mark.parametrize("temperature", [1.0, 1.5, 2.0])
+def test_rows_without_an_outside(ops, v, temperature):
+    """All classes beside the teacher's are masked: no outside, as on the CPU."""
+    from piecewiselinearembeddings_optimized_amd import CudaDistillationLoss
+
+    x = _inputs(6, v, 5, tail=True)
+    named = torch.zeros(6, v, dtype=torch.bool).scatter_(1, x["c"], True)
+    x["z"][:3][~named[:3]] = -INF
+    x["z"][3][~named[3]] = torch.finfo(F32).min
+    x["labels"] = x["c"][:, 2].clone()
+    x["lse"] = torch.logsumexp(x["t"] / temperature, -1) + 0.3
+    _check(ops, x, temperature)
+    m = CudaDistillationLoss(temperature, 0.6, "sum")
+    grads = []
+    for dev in ("cpu", DEV):
+        z = x["z"].to(dev).requires_grad_()
+        grads.append(torch.autograd.grad(m(z, *(x[k].to(dev) for k in ("t", "c", "lse", "labels"))), z)[0].cpu())
+    assert bool(torch.isfinite(grads[0]).all())
+    torch.testing.assert_close(grads[1], grads[0], rtol=1e-4, atol=1e-5)
+
+
 def test_large_and_non_finite_logits(ops):
     x = _inputs(10, 400, 8, tail=True)
     x["z"][0] *= 1e4

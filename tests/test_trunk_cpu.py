@@ -232,6 +232,31 @@ def test_module_loss_outside_mass_below_32_bits():
     torch.testing.assert_close(torch.autograd.grad(got, z)[0].double(), torch.autograd.grad(want, zd)[0], rtol=1e-4, atol=1e-5)
 
 
+@pytest.mark.parametrize("labels", [False, True])
+def test_module_loss_without_an_outside(labels):
+    """Rows whose classes beside the teacher's are all masked: no outside, and a finite gradient."""
+    gen = torch.Generator().manual_seed(4)
+    z, t = torch.randn(4, 9, generator=gen), torch.randn(4, 5, generator=gen)
+    c = torch.arange(5).expand(4, 5).contiguous()
+    z[:2, 5:] = -torch.inf                          # every class that is left is the teacher's
+    z[2, 5:] = torch.finfo(F32).min
+    label = torch.tensor([0, 3, 4, 7]) if labels else None
+    lse = torch.logsumexp(t / 2, -1) + 0.3
+    z.requires_grad_()
+    got = pkg.CudaDistillationLoss(2.0, 0.7, "none")(z, t, c, lse, label)
+    zd = z.detach().double().requires_grad_()
+    log_q, log_p = torch.log_softmax(zd / 2, -1)[:, :5], t.double() / 2 - lse.double()[:, None]
+    kd = (log_p.exp() * (log_p - log_q)).sum(-1)
+    rho = 1 - log_p[3].exp().sum()
+    rest = rho * (rho.log() - torch.logsumexp(torch.log_softmax(zd[3] / 2, -1)[5:], -1))
+    want = 0.7 * 4 * (kd + torch.cat([torch.zeros(3, dtype=torch.float64), rest[None]]))
+    if labels:
+        want = want - 0.3 * torch.log_softmax(zd, -1)[torch.arange(4), label]
+    torch.testing.assert_close(got.double(), want, rtol=1e-5, atol=1e-6)
+    torch.testing.assert_close(torch.autograd.grad(got.sum(), z)[0].double(), torch.autograd.grad(want.sum(), zd)[0],
+                               rtol=1e-4, atol=1e-6)
+
+
 @pytest.mark.parametrize("call,match", [
     (lambda: pkg.CudaTokenEmbeddings(0, 3), "positive"),
     (lambda: pkg.CudaTokenEmbeddings(4, 3, padding_idx=4), "padding_idx"),
