@@ -268,11 +268,12 @@ def _distill_cpu(logits, teacher_logits, classes, teacher_lse, labels, temperatu
         some = taught & (rho > 0) & (log_outside > -700)
         kd = kd + torch.where(some, rho * (torch.where(some, rho, 1.0).log() - torch.where(some, log_outside, 0.0)), 0.0)
     kd = torch.where(taught, kd, 0.0)
-    kd = torch.where((classes >= v).any(-1), torch.nan, kd)
+    # (a product: the gradient is NaN too)
+    kd = kd * torch.where((classes >= v).any(-1), torch.nan, 1.0)
     loss = alpha * temperature ** 2 * kd if alpha > 0 else torch.zeros(n)
     if labels is not None and alpha < 1:
         ce = -torch.log_softmax(z, -1).gather(1, labels.clamp(0, v - 1)[:, None])[:, 0]
-        loss = loss + (1 - alpha) * torch.where(labels >= v, torch.nan, torch.where(labels >= 0, ce, 0.0))
+        loss = loss + (1 - alpha) * torch.where(labels >= 0, ce, 0.0) * torch.where(labels >= v, torch.nan, 1.0)
     return torch.where(live, loss, 0.0)
 
 

@@ -266,6 +266,24 @@ def test_classes_and_labels_beyond(ops):
     _check(ops, {k: None if t is None else t[~bad] for k, t in x.items()})
 
 
+@pytest.mark.parametrize("alpha", [0.0, 0.5, 1.0])
+def test_classes_and_labels_beyond_as_on_the_cpu(ops, alpha):
+    from piecewiselinearembeddings_optimized_amd import CudaDistillationLoss
+
+    x = _inputs(9, 40, 4, tail=True)
+    x["c"][1, 2] = 40
+    x["c"][4, 0], x["z"][4] = 90, -INF              # nothing left: no loss
+    x["labels"][2], x["labels"][6] = 40, -100
+    m = CudaDistillationLoss(2.0, alpha, "none")
+    out = []
+    for dev in ("cpu", DEV):
+        z = x["z"].to(dev).requires_grad_()
+        loss = m(z, *(x[k].to(dev) for k in ("t", "c", "lse", "labels")))
+        out.append((loss.detach().cpu(), torch.autograd.grad(loss.sum(), z)[0].cpu()))
+    for a, b in zip(*out):
+        torch.testing.assert_close(a, b, rtol=1e-4, atol=1e-5, equal_nan=True)
+
+
 def test_more_entries_than_classes(ops):
     _check(ops, _inputs(4, 5, 200, repeat=True))
     _check(ops, _inputs(2, 3000, 2500, tail=True))

@@ -232,6 +232,25 @@ def test_module_loss_outside_mass_below_32_bits():
     torch.testing.assert_close(torch.autograd.grad(got, z)[0].double(), torch.autograd.grad(want, zd)[0], rtol=1e-4, atol=1e-5)
 
 
+@pytest.mark.parametrize("tail", [False, True])
+def test_module_loss_of_classes_and_labels_beyond(tail):
+    """A class or label beyond the logits': the row's loss and its whole gradient are NaN, no other row's."""
+    gen = torch.Generator().manual_seed(5)
+    z, t, c = torch.randn(6, 7, generator=gen), torch.randn(6, 3, generator=gen), torch.arange(3).repeat(6, 1)
+    c[1, 2] = 7
+    c[4, 0], z[4] = 9, -torch.inf                   # (a row without any class left has no loss)
+    label = torch.tensor([0, 1, 7, -100, 2, 6])
+    z.requires_grad_()
+    for alpha, bad in ((0.5, [1, 2]), (1.0, [1]), (0.0, [2])):
+        loss = pkg.CudaDistillationLoss(2.0, alpha, "none")(z, t, c, torch.full((6,), 2.0) if tail else None, label)
+        grad = torch.autograd.grad(loss.sum(), z)[0]
+        want = torch.zeros(6, dtype=torch.bool)
+        want[bad] = True
+        assert torch.equal(torch.isnan(loss), want)
+        assert torch.equal(torch.isnan(grad).all(1), want) and torch.equal(torch.isnan(grad).any(1), want)
+        assert loss[4] == 0 and not bool(grad[4].any())
+
+
 @pytest.mark.parametrize("labels", [False, True])
 def test_module_loss_without_an_outside(labels):
     """Rows whose classes beside the teacher's are all masked: no outside, and a finite gradient."""
