@@ -250,7 +250,7 @@ def _distill_cpu(logits, teacher_logits, classes, teacher_lse, labels, temperatu
         taught = taught & ~torch.isneginf(t).all(-1)
         lse = torch.where(taught, torch.logsumexp(torch.where(taught[:, None], t, 0.0), -1), 0.0)
     else:
-        lse = teacher_lse.float()
+        lse = teacher_lse.detach().float()
     log_p = t - lse[:, None]
     p = log_p.exp()
     q_at = log_q.gather(1, c)

@@ -232,6 +232,13 @@ def test_module_loss_outside_mass_below_32_bits():
     torch.testing.assert_close(torch.autograd.grad(got, z)[0].double(), torch.autograd.grad(want, zd)[0], rtol=1e-4, atol=1e-5)
 
 
+def test_module_loss_teacher_has_no_gradient():
+    z, t, lse = torch.randn(3, 6).requires_grad_(), torch.randn(3, 2).requires_grad_(), torch.ones(3).requires_grad_()
+    loss = pkg.CudaDistillationLoss(2.0)(z, t, torch.arange(2).repeat(3, 1), lse)
+    grads = torch.autograd.grad(loss, (z, t, lse), allow_unused=True)
+    assert grads[0] is not None and grads[1:] == (None, None)
+
+
 @pytest.mark.parametrize("tail", [False, True])
 def test_module_loss_of_classes_and_labels_beyond(tail):
     """A class or label beyond the logits': the row's loss and its whole gradient are NaN, no other row's."""
