@@ -3,9 +3,10 @@ categorical columns, the norms of a residual trunk, and the loss of a student
 that learns from a larger teacher's top logits.
 
 On a HIP device the modules run the operators ``lookup``, ``residual_norm`` and
-``distillation_loss`` of ``torch.ops.rtdl_num_embeddings_cuda`` (one kernel each
-way, sums over rows in a fixed order); on the CPU the same formulas run as
-ordinary PyTorch operations.  First-order autograd and
+``distillation_loss`` of ``torch.ops.rtdl_num_embeddings_cuda`` (sums over rows in
+a fixed order); on the CPU the same formulas run as ordinary PyTorch operations.
+Tensors are float32, float16 or bfloat16, computed in 32 bits; on the CPU float64
+too, computed in 64 bits (a device refuses it).  First-order autograd and
 ``torch.compile(fullgraph=True)`` work; double backward is not implemented.
 """
 
@@ -32,6 +33,11 @@ def _compute_dtype(t: Tensor) -> torch.dtype:
     return t.dtype
 
 
+def _wide(t: Tensor) -> Tensor:
+    """``t`` in the type the CPU computes in."""
+    return t if t.dtype == torch.float64 else t.float()
+
+
 # ---------------------------------------------------------------------------
 # lookup
 # ---------------------------------------------------------------------------
@@ -42,7 +48,7 @@ def _lookup_cpu(tokens: Tensor, weight: Tensor, offsets: Tensor | None, scale: f
     sizes = weight.shape[0] if offsets is None else offsets.diff()
     row = tokens if offsets is None else tokens + offsets[:-1]
     missing, beyond = tokens < 0, tokens >= sizes
-    out = weight[torch.where(missing | beyond, 0, row)].float() * scale
+    out = _wide(weight[torch.where(missing | beyond, 0, row)]) * scale
     if padding_idx >= 0:
         out = torch.where((tokens == padding_idx)[..., None], out.detach(), out)
     out = torch.where(missing[..., None], 0.0, torch.where(beyond[..., None], float("nan"), out))
@@ -125,8 +131,8 @@ def _norm_cpu(x: Tensor, kind: str, weight: Tensor | None, bias: Tensor | None, 
         x = x - x.mean(-1, keepdim=True)
     x = x * torch.rsqrt(x.square().mean(-1, keepdim=True) + eps)
     if weight is not None:
-        x = x * weight.float()
-    return x if bias is None else x + bias.float()
+        x = x * _wide(weight)
+    return x if bias is None else x + _wide(bias)
 
 
 class CudaResidualNorm(nn.Module):
@@ -213,17 +219,17 @@ class CudaResidualNorm(nn.Module):
         if residual.device.type != "cuda":
             stream = residual
             if branch is not None:
-                p = branch.float()
+                p = _wide(branch)
                 if after:
                     p = _norm_cpu(p, post_norm, *post, self.eps)
                 if gate is not None:
-                    h = {None: lambda t: t, "sigmoid": torch.sigmoid, "tanh": torch.tanh}[self.gate_activation](gate.float())
+                    h = {None: lambda t: t, "sigmoid": torch.sigmoid, "tanh": torch.tanh}[self.gate_activation](_wide(gate))
                     groups = max(1, gate.shape[0])
                     p = (p.reshape(groups, -1, self.d) * h[:, None]).reshape(p.shape)
-                stream = (residual_scale * residual.float() + p).to(residual.dtype)
+                stream = (residual_scale * _wide(residual) + p).to(residual.dtype)
             if self.pre_norm is None:
                 return stream, None
-            return stream, _norm_cpu(stream.float(), self.pre_norm, self.pre_weight, self.pre_bias, self.eps).to(dtype)
+            return stream, _norm_cpu(_wide(stream), self.pre_norm, self.pre_weight, self.pre_bias, self.eps).to(dtype)
         stream, normed, _ = _ops.residual_norm(
             residual.contiguous(), None if branch is None else branch.contiguous(), *post, gate, self.pre_weight,
             self.pre_bias, _NORMS[post_norm], _NORMS[self.pre_norm], _ACTIVATIONS[self.gate_activation], residual_scale,
@@ -236,7 +242,7 @@ class CudaResidualNorm(nn.Module):
 # ---------------------------------------------------------------------------
 
 def _distill_cpu(logits, teacher_logits, classes, teacher_lse, labels, temperature, alpha) -> Tensor:
-    z = logits.float()
+    z = _wide(logits)
     n, v = z.shape
     live = ~torch.isneginf(z).all(-1)
     z = torch.where(live[:, None], z, 0.0)
@@ -244,13 +250,13 @@ def _distill_cpu(logits, teacher_logits, classes, teacher_lse, labels, temperatu
     known = (classes >= 0) & (classes < v)
     c = torch.where(known, classes, 0)
     log_q = torch.log_softmax(z / temperature, -1)
-    t = torch.where(classes >= 0, teacher_logits.detach().float() / temperature, -torch.inf)
+    t = torch.where(classes >= 0, teacher_logits.detach().to(z.dtype) / temperature, -torch.inf)
     taught = (classes >= 0).any(-1)
     if teacher_lse is None:
         taught = taught & ~torch.isneginf(t).all(-1)
         lse = torch.where(taught, torch.logsumexp(torch.where(taught[:, None], t, 0.0), -1), 0.0)
     else:
-        lse = teacher_lse.detach().float()
+        lse = teacher_lse.detach().to(z.dtype)
     log_p = t - lse[:, None]
     p = log_p.exp()
     q_at = log_q.gather(1, c)
@@ -270,7 +276,7 @@ def _distill_cpu(logits, teacher_logits, classes, teacher_lse, labels, temperatu
     kd = torch.where(taught, kd, 0.0)
     # (a product: the gradient is NaN too)
     kd = kd * torch.where((classes >= v).any(-1), torch.nan, 1.0)
-    loss = alpha * temperature ** 2 * kd if alpha > 0 else torch.zeros(n)
+    loss = alpha * temperature ** 2 * kd if alpha > 0 else z.new_zeros(n)
     if labels is not None and alpha < 1:
         ce = -torch.log_softmax(z, -1).gather(1, labels.clamp(0, v - 1)[:, None])[:, 0]
         loss = loss + (1 - alpha) * torch.where(labels >= 0, ce, 0.0) * torch.where(labels >= v, torch.nan, 1.0)

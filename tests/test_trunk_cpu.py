@@ -283,6 +283,28 @@ def test_module_loss_without_an_outside(labels):
                                rtol=1e-4, atol=1e-6)
 
 
+def test_modules_in_64_bits_on_cpu():
+    """float64 inputs are computed in 64 bits: differences of 1e-5 give the gradient to 1e-8."""
+    torch.manual_seed(6)
+    F64 = torch.float64
+    e = pkg.CudaTokenEmbeddings(5, 3, scale=1 / 3).double()
+    assert torch.equal(e(torch.tensor([2])), e.weight[2:3] * (1 / 3))
+    m = pkg.CudaResidualNorm(6, post_norm="layer", pre_norm="rms", bias=True, gate="learned", gate_activation="tanh").double()
+    r, b = torch.randn(4, 6, dtype=F64), torch.randn(4, 6, dtype=F64)
+    s, n = m(r, b)
+    ref = r + torch.tanh(m.gate) * torch.nn.functional.layer_norm(b, (6,), eps=1e-5)
+    assert s.dtype == n.dtype == F64
+    torch.testing.assert_close(s, ref, rtol=1e-13, atol=1e-13)
+    torch.testing.assert_close(n, ref * (ref.square().mean(-1, keepdim=True) + 1e-5).rsqrt(), rtol=1e-13, atol=1e-13)
+    z, t, c = torch.randn(3, 8, dtype=F64).requires_grad_(), torch.randn(3, 4, dtype=F64), torch.arange(4).repeat(3, 1)
+    loss = pkg.CudaDistillationLoss(2.0, 0.6)
+    value = lambda z: loss(z, t, c, torch.logsumexp(t / 2, -1) + 0.2, torch.tensor([1, 5, -1]))  # noqa: E731
+    assert value(z).dtype == F64
+    step = torch.randn_like(z)
+    slope = (value(z + 1e-5 * step) - value(z - 1e-5 * step)) / 2e-5
+    assert abs(float(slope - (torch.autograd.grad(value(z), z)[0] * step).sum())) < 1e-8
+
+
 @pytest.mark.parametrize("call,match", [
     (lambda: pkg.CudaTokenEmbeddings(0, 3), "positive"),
     (lambda: pkg.CudaTokenEmbeddings(4, 3, padding_idx=4), "padding_idx"),
