@@ -7,7 +7,9 @@
 // norms' parameters from one `residual_norm_backward`, which reads the stored
 // stream (an output of the forward; the residual itself where there is no
 // branch), the branch and the rows' statistics.  An output without a gradient
-// is a zero gradient that is not read.
+// is a zero gradient that is not read.  Statistics (the loss's too), and the empty
+// output of a call that does not make it, are returned detached (compiled autograd
+// refuses functions that mark outputs as not differentiable).
 //
 // `distillation_loss`: the gradient of the student's logits; the teacher is
 // not learned, and a teacher that requires a gradient gets none.
@@ -139,7 +141,8 @@ Tensors3 residual_norm(DispatchKeySet ks, const Tensor &residual, const OptTenso
     }
     auto r = ResidualNorm::apply(ks, residual, branch, post_weight, post_bias, gate, pre_weight, pre_bias, post_norm,
                                  pre_norm, gate_activation, residual_scale, eps, normed_dtype);
-    return {r[0], r[1], r[2]};
+    const bool has_branch = branch.has_value() && branch->defined();
+    return {has_branch ? r[0] : r[0].detach(), pre_norm != 0 ? r[1] : r[1].detach(), r[2].detach()};
 }
 
 struct DistillationLoss : torch::autograd::Function<DistillationLoss> {
@@ -176,7 +179,7 @@ Tensors2 distillation_loss(DispatchKeySet ks, const Tensor &logits, const Tensor
                                                  temperature, alpha);
     }
     auto r = DistillationLoss::apply(ks, logits, teacher_logits, teacher_classes, teacher_lse, labels, temperature, alpha);
-    return {r[0], r[1]};
+    return {r[0], r[1].detach()};
 }
 
 }  // namespace

@@ -135,6 +135,21 @@ def test_autograd_formulas(op):
     assert [g.shape for g in torch.autograd.grad(out.sum(), wrt)] == [t.shape for t in wrt]
 
 
+def test_statistics_are_not_differentiable():
+    r, b, w = _meta(4, 8).requires_grad_(), _meta(4, 8).requires_grad_(), _meta(8).requires_grad_()
+
+    def norm(branch, post, pre):
+        out = _ops.residual_norm(r, branch, w if post else None, None, None, w if pre else None, None, post, pre, 0, 1.0, 1e-5, F32)
+        return [t.requires_grad for t in out]
+
+    assert norm(b, 1, 2) == [True, True, False]
+    assert norm(b, 1, 0) == [True, False, False]            # no norm before a block: an empty output
+    assert norm(None, 0, 2) == [False, True, False]         # no branch: an empty stream
+    loss, stats = _ops.distillation_loss(_meta(6, 20).requires_grad_(), _meta(6, 3), _meta(6, 3, dtype=torch.int64), None, None,
+                                         2.0, 0.5)
+    assert loss.requires_grad and not stats.requires_grad
+
+
 @pytest.mark.parametrize("op", OPS)
 def test_compiled_autograd(op):
     from torch._dynamo import compiled_autograd
