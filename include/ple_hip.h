@@ -336,6 +336,33 @@ int ple_lookup_backward_launch(const void *grad_output, const void *tokens, int 
                                void *stream);
 
 /*
+ * The launch plan of ple_lookup_backward_launch for a shape, without launching.
+ * `grad_output` and `grad_weight` may be NULL (then taken as aligned).  Returns
+ * the error the launch would return for the sizes (PLE_E_TOO_LARGE too where the
+ * sums' grid would pass 2^32 threads, a gradient larger than a device's memory),
+ * else fills `info`.
+ *   one_workgroup    1: one workgroup sorts, in LDS; 0: several, pass by pass
+ *   passes           passes of the sort, each of digit_bits bits of the row
+ *   sort_workgroups  workgroups that sort
+ *   sum_workgroups   workgroups that add up runs of equal rows
+ *   clear_rows       rows without tokens a clearing workgroup looks at
+ *   most_threads     threads of the largest launch, below 2^32
+ *   workspace_bytes  as ple_lookup_backward_workspace_bytes
+ */
+typedef struct ple_lookup_plan_info {
+    int one_workgroup;
+    int passes;
+    int digit_bits;
+    int sort_workgroups;
+    int64_t sum_workgroups;
+    int64_t clear_rows;
+    int64_t most_threads;
+    size_t workspace_bytes;
+} ple_lookup_plan_info_t;
+int ple_lookup_backward_plan_query(const void *grad_output, const void *grad_weight, int64_t T, int64_t V, int64_t D,
+                                   int grad_dtype, int weight_dtype, ple_lookup_plan_info_t *info);
+
+/*
  * Norms after and before a block, fused with the block's gate and the residual
  * scale; no counterpart in the reference.  For every row of the residual
  * stream r and the block's output (the branch) y, both [N, D]:

@@ -77,6 +77,21 @@ class EncodePlanInfo(ctypes.Structure):
     ]
 
 
+class LookupPlanInfo(ctypes.Structure):
+    """``ple_lookup_plan_info_t``: the lookup backward's launch plan for a shape."""
+
+    _fields_ = [
+        ("one_workgroup", ctypes.c_int),
+        ("passes", ctypes.c_int),
+        ("digit_bits", ctypes.c_int),
+        ("sort_workgroups", ctypes.c_int),
+        ("sum_workgroups", ctypes.c_int64),
+        ("clear_rows", ctypes.c_int64),
+        ("most_threads", ctypes.c_int64),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 class Norm(ctypes.Structure):
     """``ple_norm_t``: the norms, gate and residual scale around a block."""
 
@@ -160,6 +175,8 @@ def lib() -> ctypes.CDLL:
         L.ple_lookup_backward_workspace_bytes.restype = sz
         L.ple_lookup_backward_launch.argtypes = [p, p, i32, p, p, i64, i64, i64, i64, i64, f32, i32, i32, p, sz, p]
         L.ple_lookup_backward_launch.restype = i32
+        L.ple_lookup_backward_plan_query.argtypes = [p, p, i64, i64, i64, i32, i32, ctypes.POINTER(LookupPlanInfo)]
+        L.ple_lookup_backward_plan_query.restype = i32
         L.ple_residual_norm_launch.argtypes = [p, p, np_, p, p, p, i64, i64, p]
         L.ple_residual_norm_launch.restype = i32
         L.ple_residual_norm_backward_workspace_bytes.argtypes = [np_, i64, i64]
@@ -350,6 +367,17 @@ def lookup_backward(grad_output, tokens, grad_weight, offsets=None, scale=1.0, p
         _ptr(grad_output), _ptr(tokens), tokens.element_size(), _ptr(offsets), _ptr(grad_weight), tokens.numel(),
         1 if offsets is None else offsets.numel() - 1, v, d, padding_idx, scale, dtype_code(grad_output.dtype),
         dtype_code(grad_weight.dtype), _ptr(workspace), need, _stream(stream)))
+
+
+def lookup_backward_plan(t: int, v: int, d: int, grad_dtype=torch.float32, weight_dtype=None, grad_output=None,
+                         grad_weight=None) -> dict:
+    """``ple_lookup_backward_plan_query``: the plan a gradient of ``t`` tokens'
+    rows of a table [v, d] takes, as a dict of :class:`LookupPlanInfo`'s fields."""
+    info = LookupPlanInfo()
+    check(lib().ple_lookup_backward_plan_query(_ptr(grad_output), _ptr(grad_weight), t, v, d, dtype_code(grad_dtype),
+                                               dtype_code(grad_dtype if weight_dtype is None else weight_dtype),
+                                               ctypes.byref(info)))
+    return {name: getattr(info, name) for name, _ in LookupPlanInfo._fields_}
 
 
 def norm(stream_dtype, branch_dtype, post_norm=0, pre_norm=0, post_weight=None, post_bias=None, gate=None,

@@ -118,6 +118,9 @@ struct LookupRequest {
 int lookup_run(const LookupRequest &r);
 size_t lookup_backward_workspace_bytes(int64_t T, int64_t V, int64_t D);
 int lookup_backward_run(const LookupRequest &r);
+// The plan lookup_backward_run would take (of the pointers only the addresses of
+// `grad` and `dw` count).
+int lookup_backward_plan_info(const LookupRequest &r, ple_lookup_plan_info_t *info);
 
 struct NormRequest {
     const void *residual, *branch;       // backward: residual is the stored stream

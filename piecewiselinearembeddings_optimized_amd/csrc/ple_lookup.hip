@@ -784,6 +784,36 @@ hipError_t launch_sum(SumArgs a, hipStream_t s) {
     return hipGetLastError();
 }
 
+constexpr int64_t kClearBlocks = 1 << 21;        // of a launch, beside its others: a grid holds fewer than 2^32 threads
+
+struct ClearPlan {
+    uint32_t rows;                       // a workgroup looks at
+    bool local;                          // one workgroup sorts
+    bool all;                            // rows with tokens too
+    bool in_sort;                        // by the sort's launches, else by the sum's
+};
+
+ClearPlan plan_clear(const SumPlan &p, int64_t T, int64_t V, int64_t row_bytes) {
+    ClearPlan c{};
+    // 32 KB a workgroup, or as many rows as keep a launch's workgroups few enough
+    c.rows = static_cast<uint32_t>(std::max<int64_t>({1, 32768 / row_bytes, (V + kClearBlocks - 1) / kClearBlocks}));
+    c.local = T > 0 && T <= kLocalTokens;
+    // the sort of one workgroup takes as long as clearing some 100 MB; clearing
+    // rows that have tokens too is little where they are few
+    c.all = c.local && V >= 4 * T;
+    c.in_sort = c.local ? c.all : T > 0 && p.passes > 1;
+    return c;
+}
+
+// Threads of the largest grid of a backward's launches.
+int64_t most_threads(const SumPlan &p, const ClearPlan &c, int64_t T, int64_t V) {
+    const int64_t clear = (V + c.rows - 1) / c.rows;
+    const int64_t sort = T == 0 ? 0 : (c.local ? 1 : p.tiles) + (c.in_sort ? clear : 0);
+    const int64_t sum = static_cast<int64_t>(p.blocks) * p.colblocks + (c.in_sort ? 0 : clear);
+    const int block = c.local ? kLocalBlock : p.bits <= 8 ? Sort<8>::kBlock : Sort<kMaxDigitBits>::kBlock;
+    return std::max(sort * block, sum * kBlock);
+}
+
 // f(integral_constant<int, dtype>) for a dtype known at run time
 template <typename F>
 hipError_t with_dtype(int dtype, F f) {
@@ -805,7 +835,7 @@ hipError_t with_vec(int vec, F f) {
 }
 
 template <int BITS>
-void launch_local_sort(const SortArgs &s, hipStream_t stream) {
+hipError_t launch_local_sort(const SortArgs &s, hipStream_t stream) {
     const size_t room = align_up(s.t.T, kLocalBlock);
     const size_t lds = room * 6 + (static_cast<size_t>(kLocalWaves) * 2 << s.bits);
     const dim3 grid(1 + zero_blocks(s.z)), block(kLocalBlock);
@@ -813,12 +843,13 @@ void launch_local_sort(const SortArgs &s, hipStream_t stream) {
         hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_lookup_sort_kernel<2, BITS>), grid, block, lds, stream, s);
     else
         hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_lookup_sort_kernel<kLocalRounds, BITS>), grid, block, lds, stream, s);
+    return hipGetLastError();
 }
 
 // One pass; the second one's two kernels clear a third and two thirds of `rows`
 // rows (their own times are about as 1 to 2).
 template <int BITS>
-void launch_sort_pass(SortArgs s, int pass, int64_t rows, hipStream_t stream) {
+hipError_t launch_sort_pass(SortArgs s, int pass, int64_t rows, hipStream_t stream) {
     const size_t lds = static_cast<size_t>(2 + Sort<BITS>::kWaves) * 4 << s.bits;
     const dim3 block(Sort<BITS>::kBlock);
     s.z.begin = 0;
@@ -826,10 +857,13 @@ void launch_sort_pass(SortArgs s, int pass, int64_t rows, hipStream_t stream) {
     const auto grid = [&] { return dim3(s.tiles + zero_blocks(s.z)); };
     if (pass == 0) hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_lookup_count_kernel<true, BITS>), grid(), block, 0, stream, s);
     else hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_lookup_count_kernel<false, BITS>), grid(), block, 0, stream, s);
+    const hipError_t rc = hipGetLastError();
+    if (rc != hipSuccess) return rc;
     s.z.begin = s.z.end;
     s.z.end = pass == 1 ? rows : 0;
     if (pass == 0) hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_lookup_scatter_kernel<true, BITS>), grid(), block, lds, stream, s);
     else hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_lookup_scatter_kernel<false, BITS>), grid(), block, lds, stream, s);
+    return hipGetLastError();
 }
 
 TokenArgs token_args(const LookupRequest &r) {
@@ -865,11 +899,33 @@ int lookup_run(const LookupRequest &r) {
 
 size_t lookup_backward_workspace_bytes(int64_t T, int64_t V, int64_t D) { return T == 0 ? 0 : plan_sum(T, V, D, 1).bytes; }
 
+int lookup_backward_plan_info(const LookupRequest &r, ple_lookup_plan_info_t *info) {
+    const int vec = row_vec(r.D, {{r.grad, r.out_dtype}, {r.dw, r.table_dtype}});
+    const SumPlan p = plan_sum(r.T, r.V, r.D, vec);
+    const ClearPlan c = plan_clear(p, r.T, r.V, r.D * elem_bytes(r.table_dtype));
+    const int64_t most = most_threads(p, c, r.T, r.V);
+    if (most >= int64_t{1} << 32) return PLE_E_TOO_LARGE;
+    *info = ple_lookup_plan_info_t{};
+    info->one_workgroup = c.local;
+    info->passes = r.T > 0 ? p.passes : 0;
+    info->digit_bits = r.T > 0 ? p.bits : 0;
+    info->sort_workgroups = r.T == 0 ? 0 : c.local ? 1 : p.tiles;
+    info->sum_workgroups = static_cast<int64_t>(p.blocks) * p.colblocks;
+    info->clear_rows = c.rows;
+    info->most_threads = most;
+    info->workspace_bytes = r.T > 0 ? p.bytes : 0;
+    return PLE_OK;
+}
+
 int lookup_backward_run(const LookupRequest &r) {
     const int vec = row_vec(r.D, {{r.grad, r.out_dtype}, {r.dw, r.table_dtype}});
-    const SumPlan p = plan_sum(std::max<int64_t>(r.T, 0), r.V, r.D, vec);
+    const SumPlan p = plan_sum(r.T, r.V, r.D, vec);
     if (r.T > 0 && (!r.workspace || r.workspace_bytes < p.bytes || reinterpret_cast<uintptr_t>(r.workspace) % 256 != 0))
         return PLE_E_WORKSPACE;
+    const int64_t row_bytes = r.D * elem_bytes(r.table_dtype);
+    const ClearPlan clear = plan_clear(p, r.T, r.V, row_bytes);
+    // (beyond the memory of any device: the sums' threads are fewer than a gradient's elements)
+    if (most_threads(p, clear, r.T, r.V) >= int64_t{1} << 32) return PLE_E_TOO_LARGE;
     char *ws = static_cast<char *>(r.workspace);
     const auto list = [&](size_t o) { return reinterpret_cast<uint32_t *>(ws + o); };
     SortArgs s{};
@@ -878,14 +934,14 @@ int lookup_backward_run(const LookupRequest &r) {
     s.tiles = p.tiles;
     s.bits = p.bits;
     SumArgs a{};
-    const int64_t row_bytes = r.D * elem_bytes(r.table_dtype);
     ZeroArgs z{};
     z.dw = static_cast<char *>(r.dw);
     z.unit = reinterpret_cast<uintptr_t>(r.dw) % 16 == 0 && row_bytes % 16 == 0 ? 16 : elem_bytes(r.table_dtype);
     z.units = static_cast<uint32_t>(row_bytes / z.unit);
-    z.rows = static_cast<uint32_t>(std::max<int64_t>(1, 32768 / row_bytes));
+    z.rows = clear.rows;
     z.end = r.V;
     a.z = z;
+    if (clear.in_sort) a.z.end = 0;
     if (r.T > 0) {
         s.counts = list(p.o_counts);
         s.present = reinterpret_cast<uint8_t *>(ws + p.o_present);
@@ -894,32 +950,26 @@ int lookup_backward_run(const LookupRequest &r) {
         uint32_t *pos[2] = {list(p.o_pos), p.passes > 1 ? list(p.o_pos2) : nullptr};
         s.passes = p.passes;
         s.z = z;
-        if (r.T <= kLocalTokens) {
+        // (the sums read what the sort wrote: nothing follows a sort that was not launched)
+        hipError_t rc = hipSuccess;
+        if (clear.local) {
             s.keys_out = keys[0];
             s.pos_out = pos[0];
-            // the sort of one workgroup takes as long as clearing some 100 MB; clearing
-            // rows that have tokens too is little where they are few
-            if (r.V >= 4 * r.T) {
-                s.present = nullptr;
-                a.z.end = 0;
-            } else {
-                s.z.end = 0;
-            }
-            if (p.bits <= 8) launch_local_sort<8>(s, r.stream);
-            else launch_local_sort<kMaxDigitBits>(s, r.stream);
+            if (clear.all) s.present = nullptr;
+            else s.z.end = 0;
+            rc = p.bits <= 8 ? launch_local_sort<8>(s, r.stream) : launch_local_sort<kMaxDigitBits>(s, r.stream);
         } else {
             s.z.present = s.present;
-            if (p.passes > 1) a.z.end = 0;
-            for (int k = 0; k < p.passes; ++k) {
+            for (int k = 0; k < p.passes && rc == hipSuccess; ++k) {
                 s.shift = k * p.bits;
                 s.keys_in = keys[(k + 1) & 1];
                 s.pos_in = pos[(k + 1) & 1];
                 s.keys_out = keys[k & 1];
                 s.pos_out = pos[k & 1];
-                if (p.bits <= 8) launch_sort_pass<8>(s, k, r.V, r.stream);
-                else launch_sort_pass<kMaxDigitBits>(s, k, r.V, r.stream);
+                rc = p.bits <= 8 ? launch_sort_pass<8>(s, k, r.V, r.stream) : launch_sort_pass<kMaxDigitBits>(s, k, r.V, r.stream);
             }
         }
+        if (rc != hipSuccess) return static_cast<int>(rc);
         a.keys = s.keys_out;
         a.pos = s.pos_out;
         a.partial = reinterpret_cast<float *>(ws + p.o_partial);

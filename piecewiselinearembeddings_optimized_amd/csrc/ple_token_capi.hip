@@ -121,6 +121,19 @@ int ple_lookup_backward_launch(const void *grad_output, const void *tokens, int 
     return ple::lookup_backward_run(r);
 }
 
+int ple_lookup_backward_plan_query(const void *grad_output, const void *grad_weight, int64_t T, int64_t V, int64_t D,
+                                   int grad_dtype, int weight_dtype, ple_lookup_plan_info_t *info) {
+    const int rc = ple::check_lookup(T, 1, V, D, false);
+    if (rc != PLE_OK) return rc;
+    if (!ple::valid_dtype(grad_dtype) || !ple::valid_dtype(weight_dtype)) return PLE_E_BAD_DTYPE;
+    if (!info) return PLE_E_NULL_POINTER;
+    ple::LookupRequest r{};
+    r.grad = grad_output; r.dw = const_cast<void *>(grad_weight);
+    r.T = T; r.F = 1; r.V = V; r.D = D;
+    r.table_dtype = weight_dtype; r.out_dtype = grad_dtype;
+    return ple::lookup_backward_plan_info(r, info);
+}
+
 int ple_residual_norm_launch(const void *residual, const void *branch, const ple_norm_t *norm, void *stream_out,
                              void *normed, float *stats, int64_t N, int64_t D, void *stream) {
     const int rc = ple::check_norm(norm, N, D);

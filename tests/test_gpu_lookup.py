@@ -193,6 +193,25 @@ def test_offsets_beyond_32_bits(ops):
     assert not bool(dw.any())
 
 
+@pytest.mark.parametrize("t", [4000, 20_000])
+def test_clearing_wide_rows_of_a_large_table(ops, t):
+    """More rows of over 16 KB than a launch has workgroups to clear them: several rows a workgroup."""
+    v, d = 2_100_001, 8200
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB of device memory")
+    gen = torch.Generator().manual_seed(t)
+    rows = torch.randint(0, v, (600,), generator=gen)
+    rows[:2] = torch.tensor([0, v - 1])
+    tokens = rows[torch.randint(0, 600, (t,), generator=gen)].to(DEV)
+    g = torch.randint(-3, 4, (t, d), generator=gen).to(BF16).to(DEV)
+    dw = ops.lookup_backward(g, tokens, None, v, 1.0, -1, BF16)
+    seen, where = tokens.unique(return_inverse=True)
+    want = torch.zeros(len(seen), d, device=DEV).index_add_(0, where, g.float())        # (whole numbers: exact)
+    assert torch.equal(dw[seen], want.to(BF16))
+    dw[seen] = 0
+    assert not any(bool(dw[a:a + 300_000].any()) for a in range(0, v, 300_000))
+
+
 def test_other_stream(ops):
     tokens = torch.randint(0, 100, (5000,), device=DEV)
     weight = torch.randn(100, 64, device=DEV)

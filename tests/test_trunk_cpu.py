@@ -38,6 +38,35 @@ def test_c_abi_refuses_lookups():
     assert lib.ple_lookup_backward_workspace_bytes(1000, 50, 32) > 8000
 
 
+def test_lookup_backward_grids():
+    """Every launch of a gradient that a device can hold has fewer than 2^32 threads, however many rows are cleared."""
+    most = 0
+    for v in (1, 1000, 65_536, 1 << 20, 2_097_153, 4_194_303, 4_300_000, 6_300_000, 9_000_001, 1 << 24, 500_000_000, (1 << 31) - 2):
+        for d in (1, 2, 7, 64, 1000, 4096, 8200, 8192, 12_288, 16_384, 100_000, 1 << 20):
+            for t in (0, 1, 8192, 8193, 65_536, 3_000_000, (1 << 31) - 2):
+                for g, w in ((F32, F32), (BF16, BF16), (BF16, F32)):
+                    size = 4 if w == F32 else 2
+                    fits = v * d * size + t * d * (4 if g == F32 else 2) < 288 << 30
+                    try:
+                        plan = capi.lookup_backward_plan(t, v, d, g, w)
+                    except capi.PleError as e:
+                        assert e.code == -5 and not fits, (t, v, d)
+                        continue
+                    assert plan["most_threads"] < 1 << 32
+                    assert plan["clear_rows"] == max(1, 32768 // (d * size), -(-v // (1 << 21)))
+                    assert plan["one_workgroup"] == (0 < t <= 8192)
+                    assert plan["workspace_bytes"] == capi.lib().ple_lookup_backward_workspace_bytes(t, v, d)
+                    if fits:
+                        most = max(most, plan["most_threads"])
+    assert most > 1 << 30
+    assert capi.lookup_backward_plan(65_536, 131_072, 2048, BF16) | {"workspace_bytes": 0, "most_threads": 0} == {
+        "one_workgroup": 0, "passes": 2, "digit_bits": 9, "sort_workgroups": 32, "sum_workgroups": 1024, "clear_rows": 8,
+        "most_threads": 0, "workspace_bytes": 0}
+    for bad in ((-1, 5, 3), (4, 0, 3), (4, 5, 0)):
+        with pytest.raises(capi.PleError, match="shape"):
+            capi.lookup_backward_plan(*bad)
+
+
 def test_c_abi_refuses_norms():
     lib = capi.lib()
 
