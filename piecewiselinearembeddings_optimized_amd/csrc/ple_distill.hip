@@ -37,6 +37,7 @@
 
 #include <algorithm>
 #include <cfloat>
+#include <type_traits>
 
 #include "ple_internal.h"
 #include "ple_rows.h"
@@ -573,8 +574,32 @@ hipError_t with_distill(const DistillRequest &r, const DistillPlan &p, F f) {
     }
 }
 
-dim3 distill_grid(const DistillRequest &r, const DistillPlan &p) {
-    return dim3(static_cast<unsigned>((r.N + p.per_block - 1) / p.per_block * p.splits));
+constexpr int64_t kMaxBlocks = 1 << 23;  // of a launch: a grid holds fewer than 2^32 threads
+
+// f(arguments, grid) for the rows of one launch after another.
+template <typename F>
+hipError_t for_rows(const DistillRequest &r, const DistillPlan &p, const DistillArgs &a, F f) {
+    const int64_t most = std::max<int64_t>(1, kMaxBlocks / p.splits) * p.per_block;
+    for (int64_t n = 0; n < r.N; n += most) {
+        DistillArgs b = a;
+        const auto skip = [n](auto *&q, int64_t elems, int bytes) {
+            if (q) q = reinterpret_cast<std::remove_reference_t<decltype(q)>>(reinterpret_cast<uintptr_t>(q) + n * elems * bytes);
+        };
+        b.N = std::min(most, r.N - n);
+        skip(b.z, r.V, elem_bytes(r.dtype));
+        skip(b.dz, r.V, elem_bytes(r.dtype));
+        skip(b.t, r.K, elem_bytes(r.teacher_dtype));
+        skip(b.classes, r.K, r.wide ? 8 : 4);
+        skip(b.t_lse, 1, 4);
+        skip(b.labels, 1, 8);
+        skip(b.g, 1, 4);
+        skip(b.loss, 1, 4);
+        skip(b.stats, PLE_DISTILL_STATS, 4);
+        skip(b.partial, 4 * p.splits, 4);
+        const hipError_t rc = f(b, dim3(static_cast<unsigned>((b.N + p.per_block - 1) / p.per_block * p.splits)));
+        if (rc != hipSuccess) return rc;
+    }
+    return hipSuccess;
 }
 
 }  // namespace
@@ -586,25 +611,25 @@ int distill_run(const DistillRequest &r) {
     const DistillPlan p = plan_distill(r.N, r.V, 16 / elem_bytes(r.dtype));
     if (p.bytes > 0 && (!r.workspace || r.workspace_bytes < p.bytes || reinterpret_cast<uintptr_t>(r.workspace) % 256 != 0))
         return PLE_E_WORKSPACE;
-    const DistillArgs a = distill_args(r, p);
-    const hipError_t rc = with_distill(r, p, [&](auto z, auto team, auto sums) {
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_distill_forward_kernel<decltype(z)::value, decltype(team)::value,
-                                                                      decltype(sums)::value>),
-                           distill_grid(r, p), dim3(p.threads), p.lds, r.stream, a);
-        return hipGetLastError();
-    });
-    if (rc != hipSuccess || p.splits == 1) return static_cast<int>(rc);
-    const dim3 grid(static_cast<unsigned>((r.N + kWavesPerBlock - 1) / kWavesPerBlock));
-    return static_cast<int>(with_distill(r, p, [&](auto z, auto, auto sums) {
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_distill_join_kernel<decltype(z)::value, decltype(sums)::value>), grid, dim3(kBlock),
-                           0, r.stream, a);
-        return hipGetLastError();
+    return static_cast<int>(for_rows(r, p, distill_args(r, p), [&](const DistillArgs &a, dim3 grid) {
+        const hipError_t rc = with_distill(r, p, [&](auto z, auto team, auto sums) {
+            hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_distill_forward_kernel<decltype(z)::value, decltype(team)::value,
+                                                                          decltype(sums)::value>),
+                               grid, dim3(p.threads), p.lds, r.stream, a);
+            return hipGetLastError();
+        });
+        if (rc != hipSuccess || p.splits == 1) return rc;
+        const dim3 rows(static_cast<unsigned>((a.N + kWavesPerBlock - 1) / kWavesPerBlock));
+        return with_distill(r, p, [&](auto z, auto, auto sums) {
+            hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_distill_join_kernel<decltype(z)::value, decltype(sums)::value>), rows,
+                               dim3(kBlock), 0, r.stream, a);
+            return hipGetLastError();
+        });
     }));
 }
 
 int distill_backward_run(const DistillRequest &r) {
     const DistillPlan p = plan_distill(r.N, r.V, 16 / elem_bytes(r.dtype));
-    const DistillArgs a = distill_args(r, p);
     // one vector for z and dz: both addresses are the same way into 16 bytes
     const bool vec = (reinterpret_cast<uintptr_t>(r.logits) - reinterpret_cast<uintptr_t>(r.dz)) % 16 == 0;
     // Long rows' gradients of 64 MB on are stored past the caches, which the logits
@@ -612,18 +637,20 @@ int distill_backward_run(const DistillRequest &r) {
     // and fewer as fast either way; short rows, of parts of lines, are 3 to 5%
     // slower so at any size).
     const bool stream = p.team == kBlock && r.N * r.V * elem_bytes(r.dtype) >= (int64_t{64} << 20);
-    return static_cast<int>(with_distill(r, p, [&](auto z, auto team, auto sums) {
-        const auto launch = [&](auto v, auto nt) {
-            hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_distill_backward_kernel<decltype(z)::value, decltype(team)::value,
-                                                                           decltype(v)::value, decltype(sums)::value,
-                                                                           decltype(nt)::value>),
-                               distill_grid(r, p), dim3(p.threads), p.lds, r.stream, a);
-            return hipGetLastError();
-        };
-        if (!vec) return launch(std::false_type{}, std::false_type{});
-        if constexpr (decltype(team)::value == kBlock)
-            if (stream) return launch(std::true_type{}, std::true_type{});
-        return launch(std::true_type{}, std::false_type{});
+    return static_cast<int>(for_rows(r, p, distill_args(r, p), [&](const DistillArgs &a, dim3 grid) {
+        return with_distill(r, p, [&](auto z, auto team, auto sums) {
+            const auto launch = [&](auto v, auto nt) {
+                hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_distill_backward_kernel<decltype(z)::value, decltype(team)::value,
+                                                                               decltype(v)::value, decltype(sums)::value,
+                                                                               decltype(nt)::value>),
+                                   grid, dim3(p.threads), p.lds, r.stream, a);
+                return hipGetLastError();
+            };
+            if (!vec) return launch(std::false_type{}, std::false_type{});
+            if constexpr (decltype(team)::value == kBlock)
+                if (stream) return launch(std::true_type{}, std::true_type{});
+            return launch(std::true_type{}, std::false_type{});
+        });
     }));
 }
 

@@ -9,6 +9,8 @@ it is made of, plus half a unit of the stored type.
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -308,6 +310,24 @@ def test_unaligned_rows(ops, dtype, v):
 def test_very_many_classes(ops):
     """More classes than one workgroup has bits for."""
     _check(ops, _inputs(2, 600_011, 40, BF16, True))
+
+
+def test_more_rows_than_one_grid(ops):
+    """2^24 rows by workgroups: 2^32 threads, in two launches."""
+    n, v = 1 << 24, 4100
+    if torch.cuda.mem_get_info()[0] < 150 << 30:
+        pytest.skip("needs 150 GB of device memory")
+    z = torch.zeros(n, v, dtype=F16, device=DEV)
+    c = (torch.arange(n, device=DEV, dtype=torch.int32) % v).reshape(n, 1)
+    at = torch.tensor([0, 77, (1 << 23) - 1, 1 << 23, (1 << 23) + 5, n - 1], device=DEV)
+    z[at, c[at, 0].long()] = 5.0
+    loss, stats = ops.distillation_loss(z, torch.ones(n, 1, device=DEV), c, None, None, 1.0, 1.0)
+    del z
+    far = torch.ones(n, dtype=torch.bool, device=DEV)
+    far[at] = False
+    torch.testing.assert_close(loss[far], torch.full_like(loss[far], math.log(v)), rtol=1e-5, atol=0)
+    torch.testing.assert_close(loss[at].cpu(), torch.full((6,), math.log(v - 1 + math.exp(5.0)) - 5.0), rtol=1e-5, atol=0)
+    assert stats.shape == (n, 8)
 
 
 def test_empty(ops):
