@@ -621,6 +621,22 @@ hipError_t with_norm(const NormRequest &r, const NormPlan &p, F f) {
     return by_team(F32{}, F32{});
 }
 
+// The gates' joins, of as many gate rows a launch as keep it below 2^32 threads (an
+// empty batch can have any number of gate rows).
+hipError_t join_gates(const NormRequest &r, JoinArgs j) {
+    const int64_t most = (int64_t{1} << 21) / j.colblocks;
+    j.stacked = 1;
+    for (int64_t g = 0; g < r.groups; g += most) {
+        j.out[0] = static_cast<char *>(r.d_gate) + g * r.D * elem_bytes(r.param_dtype);
+        hipLaunchKernelGGL(ple_norm_join_kernel, dim3(static_cast<unsigned>(j.colblocks * std::min(most, r.groups - g))),
+                           dim3(kJoinWaves * kWave), 0, r.stream, j);
+        const hipError_t rc = hipGetLastError();
+        if (rc != hipSuccess) return rc;
+        j.partial += most * j.sum_stride;
+    }
+    return hipSuccess;
+}
+
 // An empty batch: the parameters' gradients are 0.
 int norm_zero_gradients(const NormRequest &r) {
     JoinArgs j{};
@@ -631,13 +647,8 @@ int norm_zero_gradients(const NormRequest &r) {
     for (void *p : {r.d_post_w, r.d_post_b, r.d_pre_w, r.d_pre_b})
         if (p) j.out[sums++] = p;
     if (sums > 0) hipLaunchKernelGGL(ple_norm_join_kernel, dim3(j.colblocks * sums), dim3(kJoinWaves * kWave), 0, r.stream, j);
-    if (r.d_gate) {
-        j.out[0] = r.d_gate;
-        j.stacked = 1;
-        hipLaunchKernelGGL(ple_norm_join_kernel, dim3(static_cast<unsigned>(j.colblocks * r.groups)), dim3(kJoinWaves * kWave), 0,
-                           r.stream, j);
-    }
-    return static_cast<int>(hipGetLastError());
+    const hipError_t rc = hipGetLastError();
+    return static_cast<int>(rc == hipSuccess && r.d_gate ? join_gates(r, j) : rc);
 }
 
 }  // namespace
@@ -715,10 +726,7 @@ int norm_backward_run(const NormRequest &r) {
         j.part_stride = a.D;
         j.sum_stride = p.pieces * a.D;
         j.parts = static_cast<int>(p.pieces);
-        j.out[0] = r.d_gate;
-        j.stacked = 1;
-        hipLaunchKernelGGL(ple_norm_join_kernel, dim3(static_cast<unsigned>(j.colblocks * r.groups)), dim3(kJoinWaves * kWave), 0,
-                           r.stream, j);
+        return static_cast<int>(join_gates(r, j));
     }
     return static_cast<int>(hipGetLastError());
 }

@@ -304,6 +304,17 @@ def test_empty(ops):
     assert all(not bool(g.any()) for g in grads)
 
 
+def test_empty_with_many_gate_rows(ops):
+    """The gradients of more gate rows than one launch joins are cleared."""
+    g, d = 40_000, 8192
+    none = torch.zeros(0, d, dtype=BF16, device=DEV)
+    gate = torch.ones(g, d, dtype=BF16, device=DEV)
+    torch.ones(g, d, dtype=BF16, device=DEV)            # (the memory that the gradient gets is not clear)
+    stats = torch.zeros(0, 4, device=DEV)
+    grads = ops.residual_norm_backward(none, none, none, none, stats, None, None, gate, None, None, RMS, RMS, 0, 1.0, [True] * 7)
+    assert grads[4].shape == (g, d) and not bool(grads[4].any())
+
+
 def test_same_bits_every_time(ops):
     x = _inputs(7001, 136, BF16, BF16, BF16, gates=7, bias=True)
     x["residual"] = x["residual"][:7000]
