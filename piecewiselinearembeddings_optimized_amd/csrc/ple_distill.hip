@@ -55,7 +55,7 @@ struct DistillArgs {
     void *dz;
     float *loss;
     float *stats;                // a row: maximum, log2 of the sums at T and 1, l; m, factor outside, labelled, its base
-    float *partial;              // [N, splits, 4]
+    float *partial;              // [N, splits, 8]: maximum, sums at T and 1, whether classes occur twice and those alone
     int64_t N;
     int V, K, t_dtype, wide;     // wide: 64-bit classes
     int splits, part;            // classes a split takes
@@ -249,13 +249,28 @@ __device__ __forceinline__ void scan_row(Team<TEAM> &team, const DistillArgs &a,
     }
 }
 
-// The row's loss and stats from its lanes' sums.  mine: this lane's first entry.
-// With a given l the sums and their maximum leave out the K classes, which may
-// occur `twice`: the outside mass keeps its own scale, however far below the
-// row's maximum it is.
+// The marked classes alone, each once however many entries it has: by the bits,
+// since an entry that looks for its class among the others makes the work the
+// entries' square.
 template <int Z, int TEAM, int SUMS>
+__device__ __forceinline__ void scan_marked(Team<TEAM> &team, const DistillArgs &a, const Range<Z, true> &r, const uint32_t *bits,
+                                            float ct, Sums<SUMS> &s) {
+    for (int w = team.lane(); w < a.words; w += team.lanes())
+        for (uint32_t m = bits[w]; m != 0; m &= m - 1) {
+            Words<Z, 1> v[1];
+            v[0].load(a.z, r.base + r.c0 + 32 * w + __builtin_ctz(m) - r.shift);
+            const uint32_t in[1] = {0};
+            s.add(v, in, ct);
+        }
+}
+
+// The row's loss and stats from its lanes' sums.  mine: this lane's first entry.
+// With a given l the sums and their maximum leave out the K classes: the outside
+// mass keeps its own scale, however far below the row's maximum it is.  named(): this
+// lane's sums of the K classes where one of them occurs `twice`.
+template <int Z, int TEAM, int SUMS, typename Named>
 __device__ __forceinline__ void finish_row(Team<TEAM> &team, const DistillArgs &a, int64_t n, const Entry &mine,
-                                           const Entry &label, Sums<SUMS> &s, bool twice) {
+                                           const Entry &label, Sums<SUMS> &s, bool twice, Named named) {
     const bool on = n < a.N, tail = a.t_lse != nullptr;
     const float ct = a.inv_t * kLog2e;
     const auto each = [&](auto f) {
@@ -276,7 +291,7 @@ __device__ __forceinline__ void finish_row(Team<TEAM> &team, const DistillArgs &
     float v[kValues] = {s.at_t, s.at_1, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
     float lse = tail && on ? a.t_lse[n] : 0.0f;
     bool some = false, wrong = false;
-    each([&](int k, const Entry &e) {
+    each([&](int, const Entry &e) {
         if (e.c < 0) return;
         some = true;
         wrong = wrong || e.c >= a.V;
@@ -285,17 +300,18 @@ __device__ __forceinline__ void finish_row(Team<TEAM> &team, const DistillArgs &
             return;
         }
         if (!in_range(e)) return;
-        bool first = true;
-        if (twice)
-            for (int i = 0; i < k; ++i) first = first && class_of(a, n * a.K + i) != e.c;
-        if (first) {
-            v[kInT] += exp2_fast((e.z - peak) * ct);
-            v[kIn1] += exp2_fast((e.z - peak) * kLog2e);
-        }
+        v[kInT] += exp2_fast((e.z - peak) * ct);
+        v[kIn1] += exp2_fast((e.z - peak) * kLog2e);
         const float log_p = e.t - lse, p = exp2_fast(log_p * kLog2e);
         v[kMassP] += p;
         if (p != 0.0f) v[kCross] += p * (log_p - (e.z - peak) * a.inv_t);
     });
+    if (__builtin_expect(twice, 0)) {
+        Sums<SUMS> once = named();
+        once.rescale(peak, ct);
+        v[kInT] = once.at_t;
+        v[kIn1] = once.at_1;
+    }
     v[kCount] = (some ? 1.0f : 0.0f) + (wrong ? kWrong : 0.0f);      // (exact: at most 256 lanes)
     team.sums(v);
     bool taught = v[kCount] != 0.0f;
@@ -356,8 +372,8 @@ __global__ __launch_bounds__(Team<TEAM>::kThreads) void ple_distill_forward_kern
     __shared__ float s_sum[Team<TEAM>::kLdsFloats];
     __shared__ int s_twice[Team<TEAM>::kThreads / (TEAM < kBlock ? TEAM : kBlock)];
     Team<TEAM> team(s_sum);
-    const int split = blockIdx.x % a.splits;
-    const int64_t n = static_cast<int64_t>(blockIdx.x / a.splits) * team.per_block() + team.index();
+    const int splits = TEAM < kBlock ? 1 : a.splits, split = blockIdx.x % splits;    // (only workgroups' rows are split)
+    const int64_t n = static_cast<int64_t>(blockIdx.x / splits) * team.per_block() + team.index();
     const float ct = a.inv_t * kLog2e;
     uint32_t *bits = s_bits + team.index() * a.words;
     const Range<Z, true> r(a.z, n, a.V, split * a.part, min(a.V, (split + 1) * a.part));
@@ -365,16 +381,30 @@ __global__ __launch_bounds__(Team<TEAM>::kThreads) void ple_distill_forward_kern
     Sums<SUMS> s;
     const bool twice = a.t_lse && mark_classes(team, a, n, mine, r, bits, &s_twice[team.index()]);
     if (n < a.N) scan_row<Z, TEAM, SUMS>(team, a, r, bits, ct, s);
-    if (a.splits == 1) {
-        finish_row<Z>(team, a, n, mine, label, s, twice);
+    const auto marked = [&] {        // (none where n is past the rows)
+        Sums<SUMS> v;
+        scan_marked(team, a, r, bits, ct, v);
+        return v;
+    };
+    if (splits == 1) {
+        finish_row<Z>(team, a, n, mine, label, s, twice, marked);
         return;
     }
-    float top[1] = {s.m};
-    team.maxima(top);
-    s.rescale(top[0], ct);
-    team.sum2(s.at_t, s.at_1);
-    if (team.lane() == 0 && n < a.N)
-        reinterpret_cast<float4 *>(a.partial)[n * a.splits + split] = make_float4(s.m, s.at_t, s.at_1, twice ? 1.0f : 0.0f);
+    const auto join = [&](Sums<SUMS> &v) {
+        float top[1] = {v.m};
+        team.maxima(top);
+        v.rescale(top[0], ct);
+        team.sum2(v.at_t, v.at_1);
+    };
+    join(s);
+    const bool out = team.lane() == 0 && n < a.N;
+    float4 *part = reinterpret_cast<float4 *>(a.partial) + 2 * (n * splits + split);
+    if (out) part[0] = make_float4(s.m, s.at_t, s.at_1, twice ? 1.0f : 0.0f);
+    if (__builtin_expect(twice, 0)) {
+        Sums<SUMS> v = marked();
+        join(v);
+        if (out) part[1] = make_float4(v.m, v.at_t, v.at_1, 0.0f);
+    }
 }
 
 // A row's sums from its splits' (one wave a row), then its loss.
@@ -384,21 +414,77 @@ __global__ __launch_bounds__(kBlock) void ple_distill_join_kernel(DistillArgs a)
     const int64_t n = static_cast<int64_t>(blockIdx.x) * team.per_block() + team.index();
     const Entry mine = load_entry<Z>(a, n, team.lane()), label = load_label<Z>(a, n);
     Sums<SUMS> s;
-    bool twice = false;
-    for (int i = team.lane(); n < a.N && i < a.splits; i += kWave) {
-        const float4 v = reinterpret_cast<const float4 *>(a.partial)[n * a.splits + i];
+    const float4 *parts = reinterpret_cast<const float4 *>(a.partial) + 2 * n * a.splits;
+    const auto add = [&](Sums<SUMS> &to, const float4 &v) {
         Sums<SUMS> part;
         part.m = v.x;
         part.at_t = v.y;
         part.at_1 = v.z;
-        const float to = fmaxf(s.m, part.m);
-        s.rescale(to, a.inv_t * kLog2e);
-        part.rescale(to, a.inv_t * kLog2e);
-        s.at_t += part.at_t;
-        s.at_1 += part.at_1;
+        const float top = fmaxf(to.m, part.m);
+        to.rescale(top, a.inv_t * kLog2e);
+        part.rescale(top, a.inv_t * kLog2e);
+        to.at_t += part.at_t;
+        to.at_1 += part.at_1;
+    };
+    bool twice = false;
+    for (int i = team.lane(); n < a.N && i < a.splits; i += kWave) {
+        const float4 v = parts[2 * i];
+        add(s, v);
         twice = twice || v.w != 0.0f;
     }
-    finish_row<Z>(team, a, n, mine, label, s, __any(twice));
+    // the splits where a class occurs twice have their own sums, the others' entries are all there is
+    const auto named = [&] {
+        Sums<SUMS> v;
+        for (int i = team.lane(); i < a.splits; i += kWave)
+            if (parts[2 * i].w != 0.0f) add(v, parts[2 * i + 1]);
+        for (int k = team.lane(); k < a.K; k += kWave) {
+            const Entry e = load_entry<Z>(a, n, k);
+            if (e.c >= 0 && e.c < a.V && parts[2 * (static_cast<int>(e.c) / a.part)].w == 0.0f)
+                add(v, make_float4(e.z, 1.0f, 1.0f, 0.0f));
+        }
+        return v;
+    };
+    finish_row<Z>(team, a, n, mine, label, s, __any(twice), named);
+}
+
+// Entries of a row with repeats up to which each looks through them all for its class's
+// others; beyond, that is their square, and sum_repeats takes them (backwards of rows
+// with a repeat, searched / by sum_repeats: 512 x 50257 of 512 entries 230 / 307 us, of
+// 1024 800 / 546; 4096 x 2000 of 128 85 / 115, of 256 270 / 213; 16384 x 100 of 64 67 /
+// 103, of 128 314 / 240, of 2048 134 / 6.8 ms).
+template <int TEAM>
+constexpr int kSearched = 64 + 2 * TEAM;
+
+// put(entry, sum of its class's probabilities) for every entry in [c0, c1): as many
+// classes at a time as the team's bits have room for sums of (the bits are lost), to
+// which one wave adds the entries in their own order.
+template <int TEAM, int Z, bool VEC, typename Prob, typename Put>
+__device__ __forceinline__ void sum_repeats(Team<TEAM> &team, const DistillArgs &a, int64_t n, const Range<Z, VEC> &r,
+                                            uint32_t *bits, Prob prob, Put put) {
+    constexpr int kLanes = TEAM < kWave ? TEAM : kWave;
+    volatile float *sums = reinterpret_cast<volatile float *>(bits);
+    const int first = threadIdx.x % kWave / kLanes * kLanes;     // of the team in its wave
+    for (int lo = r.c0; lo < r.c1; lo += a.words) {
+        const int hi = min(lo + a.words, r.c1);
+        for (int w = team.lane(); w < a.words; w += team.lanes()) sums[w] = 0.0f;
+        team.sync();
+        for (int k0 = 0; team.lane() < kLanes && k0 < a.K; k0 += kLanes) {
+            const int k = k0 + team.lane();
+            const int64_t c = k < a.K ? class_of(a, n * a.K + k) : -1;
+            const bool on = c >= lo && c < hi;
+            const float p = on ? prob(load_any(a.t, n * a.K + k, a.t_dtype) * a.inv_t) : 0.0f;
+            for (uint64_t todo = __ballot(on) >> first & (~uint64_t{0} >> (kWave - kLanes)); todo != 0; todo &= todo - 1) {
+                if (team.lane() == __builtin_ctzll(todo)) sums[c - lo] = sums[c - lo] + p;
+                __builtin_amdgcn_wave_barrier();
+            }
+        }
+        team.sync();
+        for (int k = team.lane(); k < a.K; k += team.lanes()) {
+            const Entry e = load_entry<Z>(a, n, k);
+            if (e.c >= lo && e.c < hi) put(e, sums[e.c - lo]);
+        }
+        team.sync();
+    }
 }
 
 template <int Z, int TEAM, bool VEC, int SUMS, bool NT>
@@ -409,8 +495,8 @@ __global__ __launch_bounds__(Team<TEAM>::kThreads) void ple_distill_backward_ker
     Team<TEAM> team(nullptr);
     // the last rows first: the forward left them in the memory-side cache
     const unsigned block = gridDim.x - 1 - blockIdx.x;
-    const int split = block % a.splits;
-    const int64_t n = static_cast<int64_t>(block / a.splits) * team.per_block() + team.index();
+    const int splits = TEAM < kBlock ? 1 : a.splits, split = block % splits;
+    const int64_t n = static_cast<int64_t>(block / splits) * team.per_block() + team.index();
     const float ct = a.inv_t * kLog2e;
     uint32_t *bits = s_bits + team.index() * a.words;
     const Range<Z, VEC> r(a.z, n, a.V, split * a.part, min(a.V, (split + 1) * a.part));
@@ -471,6 +557,23 @@ __global__ __launch_bounds__(Team<TEAM>::kThreads) void ple_distill_backward_ker
     team.sync();
     if (n >= a.N) return;
     const auto prob = [&](float t) { return exp2_fast((t - lse) * kLog2e); };
+    const auto put = [&](const Entry &e, float p) {
+        float v = w_soft != 0.0f ? w_soft * (mass * soft(e.z) - p) : 0.0f;
+        if (w_hard != 0.0f) v += w_hard * (hard(e.z) - (e.c == label.c ? 1.0f : 0.0f));
+        store_vec<Z, 1>(a.dz, r.base + e.c, &v);
+    };
+    if (team.lane() == 0 && label.c >= r.c0 && label.c < r.c1) {
+        const int b = r.bit(static_cast<int>(label.c));
+        if (!(bits[b >> 5] >> (b & 31) & 1)) {
+            const float v = dense(label.z) - w_hard;
+            store_vec<Z, 1>(a.dz, r.base + label.c, &v);
+        }
+    }
+    if (__builtin_expect(twice && a.K > kSearched<TEAM>, 0)) {
+        team.sync();         // (the label's bit is read)
+        sum_repeats(team, a, n, r, bits, prob, put);
+        return;
+    }
     for (int k = team.lane(); k < a.K; k += team.lanes()) {
         const Entry e = k == team.lane() ? mine : load_entry<Z>(a, n, k);
         if (e.c < r.c0 || e.c >= r.c1) continue;
@@ -485,17 +588,7 @@ __global__ __launch_bounds__(Team<TEAM>::kThreads) void ple_distill_backward_ker
         } else {
             p = prob(e.t);
         }
-        if (!first) continue;
-        float v = w_soft != 0.0f ? w_soft * (mass * soft(e.z) - p) : 0.0f;
-        if (w_hard != 0.0f) v += w_hard * (hard(e.z) - (e.c == label.c ? 1.0f : 0.0f));
-        store_vec<Z, 1>(a.dz, r.base + e.c, &v);
-    }
-    if (team.lane() == 0 && label.c >= r.c0 && label.c < r.c1) {
-        const int b = r.bit(static_cast<int>(label.c));
-        if (!(bits[b >> 5] >> (b & 31) & 1)) {
-            const float v = dense(label.z) - w_hard;
-            store_vec<Z, 1>(a.dz, r.base + label.c, &v);
-        }
+        if (first) put(e, p);
     }
 }
 
@@ -533,7 +626,7 @@ DistillPlan plan_distill(int64_t N, int64_t V, int vec = 8) {
     }
     p.words = (p.part + 8 + 31) / 32;
     p.lds = static_cast<size_t>(p.words) * 4 * p.per_block;
-    p.bytes = p.splits > 1 ? align_up(static_cast<size_t>(N) * p.splits * 16, 256) : 0;
+    p.bytes = p.splits > 1 ? align_up(static_cast<size_t>(N) * p.splits * 32, 256) : 0;
     return p;
 }
 
@@ -595,7 +688,7 @@ hipError_t for_rows(const DistillRequest &r, const DistillPlan &p, const Distill
         skip(b.g, 1, 4);
         skip(b.loss, 1, 4);
         skip(b.stats, PLE_DISTILL_STATS, 4);
-        skip(b.partial, 4 * p.splits, 4);
+        skip(b.partial, 8 * p.splits, 4);
         const hipError_t rc = f(b, dim3(static_cast<unsigned>((b.N + p.per_block - 1) / p.per_block * p.splits)));
         if (rc != hipSuccess) return rc;
     }

@@ -10,6 +10,7 @@ it is made of, plus half a unit of the stored type.
 from __future__ import annotations
 
 import math
+import time
 
 import pytest
 import torch
@@ -289,6 +290,58 @@ def test_classes_and_labels_beyond_as_on_the_cpu(ops, alpha):
 def test_more_entries_than_classes(ops):
     _check(ops, _inputs(4, 5, 200, repeat=True))
     _check(ops, _inputs(2, 3000, 2500, tail=True))
+
+
+@pytest.mark.parametrize("k", [80, 81, 97, 193, 576, 577, 3000])
+@pytest.mark.parametrize("v", [40, 500, 3000, 9000, 40_000, 300_000])
+@pytest.mark.parametrize("tail", [False, True], ids=["top", "tail"])
+def test_many_entries_with_repeats(ops, v, k, tail):
+    """Rows whose entries repeat classes, some, none or all, beside each other.  A class of
+    m entries adds up m probabilities one after another: off by up to m 2^-24 of their sum."""
+    n = 5
+    x = _inputs(n, v, k, tail=tail, repeat=True)
+    gen = torch.Generator().manual_seed(k)
+    x["c"][0, :k // 2] = x["c"][0, 0]               # one class for half of the entries
+    x["c"][1, 7:] = -1                              # few entries
+    x["c"][2] = torch.arange(k) if k <= v else torch.arange(k) % v
+    x["c"][3] = x["labels"][3]                      # one class in all, the label's too
+    x["c"][4][torch.rand(k, generator=gen) < 0.5] = -3
+    if tail:
+        x["lse"] = torch.logsumexp(torch.where(x["c"] >= 0, x["t"] / 2, -INF), -1) + 0.4
+    loss, dz = _run(ops, x, 2.0, 0.6)
+    ref, size, rdz, dsize, eps = _reference(x, 2.0, 0.6)
+    most = torch.stack([c[c >= 0].bincount().max() for c in x["c"]])
+    eps = eps + 2.0 ** -24 * (most + k / 8)         # (and the row's sums of a lane's entries)
+    assert bool(((loss.double() - ref).abs() <= eps * size).all()), ((loss.double() - ref).abs() / (eps * size))
+    assert bool(((dz.double() - rdz).abs() <= eps[:, None] * dsize + UNIT[F32] * rdz.abs() + 1e-37).all())
+    again = _run(ops, x, 2.0, 0.6)
+    assert torch.equal(again[0], loss) and torch.equal(again[1], dz)
+
+
+def test_repeats_take_no_square_of_the_entries(ops):
+    """131072 entries a row, all of them twice: 2^34 comparisons if each looked for its class."""
+    n, v, k = 4, 70_000, 1 << 17
+    gen = torch.Generator().manual_seed(0)
+    half = torch.stack([torch.randperm(v, generator=gen)[:k // 2] for _ in range(n)])
+    x = {"z": torch.randn(n, v, generator=gen), "t": torch.randn(n, k, generator=gen), "c": torch.cat([half, half], 1),
+         "lse": None, "labels": None, "g": torch.ones(n)}
+    x["lse"] = torch.logsumexp(x["t"], -1) + 0.2
+    _run(ops, {key: None if t is None else t[:, :4].contiguous() if key in "tc" else t for key, t in x.items()}, 1.0, 1.0)
+    start = time.monotonic()
+    loss, dz = _run(ops, x, 1.0, 1.0)
+    assert time.monotonic() - start < 2.0
+    # each class once, with the sum of its two probabilities
+    p = torch.softmax(x["t"].double(), -1) * math.exp(-0.2)
+    target = torch.zeros(n, v, dtype=torch.float64).scatter_add_(1, x["c"], p)
+    log_q = torch.log_softmax(x["z"].double(), -1)
+    named = torch.zeros(n, v, dtype=torch.bool).scatter_(1, x["c"], True)
+    rho = 1 - math.exp(-0.2)
+    rest = torch.where(named, 0.0, log_q.exp()).sum(-1, keepdim=True)
+    want = (p * (p.log() - log_q.gather(1, x["c"]))).sum(-1) + rho * (math.log(rho) - rest.log())[:, 0]
+    grad = log_q.exp() - target - torch.where(named, 0.0, rho * log_q.exp() / rest)
+    # (a lane's 512 entries and the sums of 2^17 probabilities: some 2^-24 * 600 of the terms)
+    torch.testing.assert_close(loss.double(), want, rtol=4e-5 * 12, atol=0)
+    assert bool(((dz.double() - grad).abs() <= 4e-5 * (target + log_q.exp() * (1 + rho / rest))).all())
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
