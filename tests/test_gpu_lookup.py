@@ -107,6 +107,31 @@ def test_backward(ops, name, spread):
         _check_backward(ops, tokens.int(), g.bfloat16(), v, d ** 0.5, BF16)
 
 
+# tokens, rows, width; the sort's passes and bits a pass; whether one workgroup sorts
+SORTS = [
+    (5120, 1000, 24, 1, 10, True), (5121, 1000, 24, 1, 10, True), (8192, 1000, 24, 1, 10, True), (8193, 1000, 24, 1, 10, False),
+    (8191, 70_001, 16, 2, 9, True), (8192, 700_000, 8, 2, 10, True), (8193, 700_000, 8, 2, 10, False),
+    (8192, 200, 40, 1, 8, True), (8193, 200, 40, 1, 8, False), (8192, 1_100_003, 4, 3, 7, True),
+    (20_000, 70_001, 24, 2, 9, False), (20_000, 131_072, 9, 2, 9, False), (20_000, 60_000, 33, 2, 8, False),
+    (20_000, 1_100_003, 4, 3, 7, False), (70_001, 20_000_003, 2, 3, 9, False), (600_000, 900_001, 3, 2, 10, False),
+]
+
+
+@pytest.mark.parametrize("spread", ["even", "few_rows", "one_row"])
+@pytest.mark.parametrize("t,v,d,passes,bits,one", SORTS)
+def test_sorts(ops, t, v, d, passes, bits, one, spread):
+    """Both sorts at their borders, by every number of passes and both shapes of their workgroups."""
+    from piecewiselinearembeddings_optimized_amd import capi
+
+    plan = capi.lookup_backward_plan(t, v, d)
+    assert (plan["passes"], plan["digit_bits"], bool(plan["one_workgroup"])) == (passes, bits, one)
+    gen = torch.Generator().manual_seed(t + v)
+    high = {"even": v, "few_rows": min(v, 3), "one_row": 1}[spread]
+    tokens = torch.randint(0, high, (t,), generator=gen) + (v - high)
+    tokens = torch.where(torch.rand(t, generator=gen) < 0.05, -1, tokens)
+    _check_backward(ops, tokens, torch.randn(t, d, generator=gen), v, 1.0, F32)
+
+
 @pytest.mark.parametrize("w,o", PAIRS, ids=lambda d: str(d)[6:])
 @pytest.mark.parametrize("d", [1, 6, 15, 64, 520])
 def test_backward_types(ops, d, w, o):
@@ -140,6 +165,25 @@ def test_columns(ops, d, w):
     v = int(cards.sum())
     _check_forward(ops, tokens, torch.randn(v, d, generator=gen).to(w), 1.5, w, offsets)
     g = torch.randn(777, 5, d, generator=gen).to(w)
+    _check_backward(ops, tokens, g, v, 1.5, w, offsets)
+    _check_backward(ops, tokens.int(), g, v, 1.5, w, offsets, padding=1)
+
+
+@pytest.mark.parametrize("n,cards", [(1638, [2, 1, 300, 17, 5]), (1639, [2, 1, 300, 17, 5]), (9001, [3, 7000, 40]),
+                                     (5000, [70_000, 2, 1, 900]), (3000, [5] * 40), (2000, [400_000, 11, 700_000, 3, 9])])
+@pytest.mark.parametrize("d,w", [(32, F32), (10, BF16)])
+def test_many_rows_of_columns(ops, n, cards, d, w):
+    """Categorical columns beyond what one workgroup sorts."""
+    gen = torch.Generator().manual_seed(n + d)
+    cards = torch.tensor(cards)
+    offsets = torch.cat([torch.zeros(1, dtype=torch.int64), cards.cumsum(0)])
+    u = torch.rand(n, len(cards), generator=gen) ** 2
+    tokens = (u * (cards + 0.02)).long() - (torch.rand(n, len(cards), generator=gen) < 0.05).long()
+    tokens[7, -1] = int(cards[-1])                  # beyond its column, not beyond the table's others
+    tokens[8, 0] = int(cards[0])
+    v = int(cards.sum())
+    _check_forward(ops, tokens, torch.randn(v, d, generator=gen).to(w), 1.5, w, offsets)
+    g = torch.randn(n, len(cards), d, generator=gen).to(w)
     _check_backward(ops, tokens, g, v, 1.5, w, offsets)
     _check_backward(ops, tokens.int(), g, v, 1.5, w, offsets, padding=1)
 
