@@ -189,6 +189,17 @@ def test_many_rows(ops, n, d):
     _check(ops, _inputs(n, d, F32, BF16, F32, bias=True, post=LAYER, pre=LAYER), LAYER, LAYER, 1, 1.0)
 
 
+@pytest.mark.parametrize("types", [(F32, F32, F32), (BF16, BF16, BF16), (F32, BF16, F32)], ids=_ids)
+@pytest.mark.parametrize("n,d,gates", [(1100, 4104, 1), (1099, 4100, 7), (1100, 5120, 1), (1100, 5120, 5), (1033, 6001, 0),
+                                       (1100, 6144, 1), (1100, 6152, 1), (1100, 6152, 10), (1099, 8191, 1), (1100, 8192, 1),
+                                       (1100, 8192, 11), (600, 8192, 600)])
+def test_wide_rows_in_turn(ops, n, d, gates, types):
+    """Rows of 768 and 1024 threads, several to a workgroup: the next row's loads, the
+    joins' two buffers and the parameters' sums go from row to row."""
+    _check(ops, _inputs(n, d, *types, bias=True, post=LAYER, pre=LAYER, gates=gates), LAYER, LAYER, 2 if gates else 0, 0.75)
+    _check(ops, _inputs(n, d, *types, post=RMS, pre=RMS, gates=gates), RMS, RMS, 0, 1.0)
+
+
 def test_without_weights(ops):
     x = _inputs(40, 100, gates=0)
     x["post_weight"] = x["pre_weight"] = None
