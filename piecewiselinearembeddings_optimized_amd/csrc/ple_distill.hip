@@ -30,10 +30,12 @@
 // where there are few rows of many classes, to several workgroups, each a range
 // of the classes, whose sums a second kernel joins.
 //
-// Measured (one MI355X): 4096 x 131072 bf16 213 us forward (5.0 TB/s read) and
-// 410 backward (5.2 TB/s); 4096 x 50257 with labels at T = 2 91 and 156 us (4.5
-// and 5.3 TB/s; with two exponentials a class 125 forward); 24 x 32000 4.6 + 4.2
-// + 4.2 us and 4096 x 100 fp32 4.8 + 4.1 us, a chain of loads and joins each.
+// Measured (one MI355X, kernel trace): 4096 x 131072 bf16 212 us forward (5.1 TB/s
+// read) and 410 backward (5.2 TB/s); 4096 x 50257 with labels at T = 2 91 and 155 us
+// (4.5 and 5.3 TB/s; with two exponentials a class 125 forward); 24 x 32000 4.2 +
+// 4.3 + 4.3 us and 4096 x 100 fp32 4.5 + 4.0 us, a chain of loads and joins each.
+// Short rows: 262144 x 200 bf16 55 and 46 us (2.5 and 5.2 TB/s), of 100 entries a
+// row 202 and 212 (2.1 and 2.5): a lane's entries are loads that follow each other.
 
 #include <algorithm>
 #include <cfloat>
@@ -604,10 +606,10 @@ struct DistillPlan {
 constexpr int kMaxPart = 1 << 18;        // classes a workgroup has bits for, about (32 KB)
 
 DistillPlan plan_distill(int64_t N, int64_t V, int vec = 8) {
-    // Lanes a row: a few vectors for each, of `vec` classes (65536 rows bf16: 200
-    // classes by waves 82 us, by 16 lanes 40; 500 classes 101 and 80; 500 fp32, 125
-    // vectors, 54 and 63), a workgroup beyond 4096 classes (2100 classes by
-    // workgroups 104 us, by waves 63; 4096 60 and 55; 8192 48.5 and 51).
+    // Lanes a row: a few vectors for each, of `vec` classes (65536 rows, both ways: 200
+    // classes bf16 by waves 80 us, by 16 lanes 34; 500 87 and 72; 500 fp32, 125 vectors,
+    // 96 and 104), a workgroup beyond 4096 classes (bf16: 16384 x 2100 by workgroups 91
+    // us, by waves 50; x 4096 100 and 75; 8192 x 8192 76 and 74).
     // Splits: four workgroups a CU where the rows are fewer, 2048 classes each at
     // least.
     DistillPlan p{};
@@ -723,7 +725,9 @@ int distill_run(const DistillRequest &r) {
 
 int distill_backward_run(const DistillRequest &r) {
     const DistillPlan p = plan_distill(r.N, r.V, 16 / elem_bytes(r.dtype));
-    // one vector for z and dz: both addresses are the same way into 16 bytes
+    // One vector for z and dz: both addresses are the same way into 16 bytes.  Else an
+    // element at a time: most row slices of logits of odd widths (4096 x 50257 bf16
+    // 182 -> 218 us, 65536 x 2101 120 -> 145).
     const bool vec = (reinterpret_cast<uintptr_t>(r.logits) - reinterpret_cast<uintptr_t>(r.dz)) % 16 == 0;
     // Long rows' gradients of 64 MB on are stored past the caches, which the logits
     // need (50257 classes, both kernels: 2560 rows 178 -> 145 us, 1024 73 -> 62, 512

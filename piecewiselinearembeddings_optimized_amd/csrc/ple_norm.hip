@@ -21,13 +21,15 @@
 // registers; a workgroup adds its teams' sums and leaves them as partials in
 // 32 bits, which a second kernel adds in a fixed order.
 //
-// Measured (one MI355X; forward, backward and joins; the copy's rate is 5.2
-// TB/s): 16384 x 4096 bf16 112 + 166 + 6 us (4.8 and 4.9 TB/s), 51200 x 192 fp32
-// 34 + 42 + 5 us (4.7 and 5.7, the tensors partly in the memory-side cache),
-// 32800 x 1152 fp32 stream with a bf16 branch and a gate a sample 100 + 173 + 5
-// us (4.5 and 3.9: 144 of 192 lanes, and the biases' sums leave three waves a
-// SIMD).  Loads of the next row while this one is used: 445 -> 332 us for the
-// first, a second workgroup a CU 332 -> 281.
+// Measured (one MI355X, kernel trace; forward, backward and joins; the copy's rate
+// is 5.2 TB/s): 16384 x 4096 bf16 107 + 164 + 6 us (5.0 and 4.9 TB/s), 51200 x 192
+// fp32 34 + 41 + 5 us (4.6 and 5.7: tensors of 39 MB, several of which the
+// memory-side cache can hold), 32800 x 1152 fp32 stream with a bf16 branch and a
+// gate a sample 92 + 172 + 2 x 5 us (4.9 and 4.0: 144 of 192 lanes, and the biases'
+// sums leave three waves a SIMD).  Loads of the next row while this one is used:
+// 445 -> 332 us for the first, a second workgroup a CU 332 -> 281.
+// Not as near: rows that are not 16-byte vectors load an element at a time (16384 x
+// 4100 bf16 548 + 908 us, by vectors at 4096 107 + 164; 65536 x 1001 447 + 645).
 
 #include <algorithm>
 
@@ -308,7 +310,10 @@ struct Held {
 // Waves a SIMD the backward of wide rows is compiled for (its registers: 128, 168
 // or 256).  Workgroups of up to 768 threads have 168, of more than that 128, which
 // with biases are too few (9000 x 5120 layer norms with biases: 547 us with 128,
-// 232 with 168).
+// 232 with 168).  More than 768 threads can have no more, and spill there (8192 x
+// 8192 bf16, backward: 512 us with biases, 162 without).  fp32 rows without biases
+// spill up to 53 of 128 registers (16384 x 4096: 486 us of fp32, 3.3 TB/s; 267 of an
+// fp32 stream with a bf16 branch, 4.5).
 constexpr int backward_waves(bool vec, bool bias) { return !vec ? 2 : bias ? 3 : 4; }
 
 // Teams walk units of rows: a row each, or a piece of the rows of one gate, whose
