@@ -478,6 +478,96 @@ int ple_distill_backward_launch(const float *grad_loss, const void *logits, cons
                                 int dtype, int teacher_dtype, void *stream);
 
 /*
+ * Group norm with an activation, channels last; no counterpart in the
+ * reference.  A sample x [S, C] has G groups of C / G adjacent channels; a
+ * group's values over all S rows are standardised together:
+ *   y = act((x - mean) / sqrt(var + eps) * weight[c] + bias[c])
+ *   x, y         dtype [N, S, C]
+ *   weight, bias param_dtype [C], or NULL: 1, 0
+ *   stats        float32 [N, G, 2], 8-byte aligned: mean and 1 / sqrt(var + eps)
+ *   workspace    >= ple_group_norm_workspace_bytes() bytes (0 is possible),
+ *                256-byte aligned, need not be initialised
+ * Statistics and sums are 32-bit in a fixed order.  C <= 2^20, S < 2^31, N < 2^31,
+ * N * S * C < 2^44 (else PLE_E_TOO_LARGE); G divides C (else PLE_E_BAD_SHAPE).
+ */
+enum {
+    PLE_ACT_NONE = 0,
+    PLE_ACT_RELU = 1,
+    PLE_ACT_SILU = 2,
+    PLE_ACT_GELU = 3,    /* z times the standard normal distribution at z */
+};
+size_t ple_group_norm_workspace_bytes(int64_t N, int64_t S, int64_t C, int64_t G, int dtype);
+int ple_group_norm_launch(const void *x, const void *weight, const void *bias, void *y, float *stats, int64_t N,
+                          int64_t S, int64_t C, int64_t G, int activation, float eps, int dtype, int param_dtype,
+                          void *workspace, size_t workspace_bytes, void *stream);
+
+/* Backward of ple_group_norm_launch, from its x and stats.  grad_x (dtype),
+ * grad_weight and grad_bias (param_dtype [C]) may be NULL: not wanted. */
+size_t ple_group_norm_backward_workspace_bytes(int64_t N, int64_t S, int64_t C, int64_t G, int dtype);
+int ple_group_norm_backward_launch(const void *grad_y, const void *x, const float *stats, const void *weight,
+                                   const void *bias, void *grad_x, void *grad_weight, void *grad_bias, int64_t N,
+                                   int64_t S, int64_t C, int64_t G, int activation, int dtype, int param_dtype,
+                                   void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * Learned bias of attention scores by relative position; no counterpart in the
+ * reference.  With p = starts[b] (or offset) the position of a sample's first
+ * query:
+ *   out[b, h, i, j] = weight[buckets[clamp(j - p - i, -far, far) + far], h]
+ * A negative bucket has no bias (0, no gradient), one >= R gives NaN.  causal:
+ * -inf where j > p + i.
+ *   weight    weight_dtype [R, H]
+ *   buckets   int32 [2 far + 1]
+ *   starts    int64 [B], or NULL: offset for all (then B is 1)
+ *   out       out_dtype [B, H, q, k]
+ * 1 <= far <= 2^24; B, H, R, q, k < 2^31, B * H * q * k < 2^44, |offset| <= 2^60
+ * (else PLE_E_TOO_LARGE); positions beyond 2^60 count as 2^60.
+ */
+int ple_relative_bias_launch(const void *weight, const int32_t *buckets, const int64_t *starts, void *out, int64_t B,
+                             int64_t H, int64_t q, int64_t k, int64_t R, int64_t far, int64_t offset, int causal,
+                             int weight_dtype, int out_dtype, void *stream);
+
+/* Backward of ple_relative_bias_launch: grad_weight (weight_dtype [R, H]) from
+ * grad_output (out_dtype [B, H, q, k]), whose masked entries do not count.  Sums
+ * are 32-bit in a fixed order.  workspace: as above, >=
+ * ple_relative_bias_backward_workspace_bytes() bytes. */
+size_t ple_relative_bias_backward_workspace_bytes(int64_t B, int64_t H, int64_t q, int64_t k, int64_t R, int64_t far);
+int ple_relative_bias_backward_launch(const void *grad_output, const int32_t *buckets, const int64_t *starts,
+                                      void *grad_weight, int64_t B, int64_t H, int64_t q, int64_t k, int64_t R,
+                                      int64_t far, int64_t offset, int causal, int out_dtype, int weight_dtype,
+                                      void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * The norm of many gradients together, and their scaling to a limit; no
+ * counterpart in the reference.
+ *   norm = (sum |g|^p)^(1/p) over all elements of all tensors, p 1 or 2, or
+ *          max |g|; summed in 64 bits, in a fixed order, rounded to 32; NaN if
+ *          an element is
+ *   out = g * min(1, limit / (norm + 1e-6))
+ * The list lies in host memory and is read before the call returns; its
+ * addresses go into the kernels' arguments (and so into a captured graph).
+ */
+typedef struct ple_grad {
+    const void *grad;        /* numel elements of dtype */
+    void *out;               /* scaling: numel elements of out_dtype; grad itself
+                              * (and its dtype), or memory that no tensor of the
+                              * list shares */
+    int64_t numel;           /* 0 to 2^40 */
+    int dtype, out_dtype;    /* PLE_DTYPE_* (the norm does not look at out and out_dtype) */
+} ple_grad_t;
+enum { PLE_NORM_P1 = 1, PLE_NORM_P2 = 2, PLE_NORM_INF = 3 };
+
+/* norm: float32, one element; workspace >= ple_grad_norm_workspace_bytes()
+ * bytes, 256-byte aligned, need not be initialised. */
+size_t ple_grad_norm_workspace_bytes(const ple_grad_t *grads, int64_t count);
+int ple_grad_norm_launch(const ple_grad_t *grads, int64_t count, int kind, float *norm, void *workspace,
+                         size_t workspace_bytes, void *stream);
+
+/* out from the norm in device memory.  Gradients that stay in place are not
+ * touched where nothing is clipped; limit >= 0 (an infinite one clips nothing). */
+int ple_grad_scale_launch(const ple_grad_t *grads, int64_t count, const float *norm, float limit, void *stream);
+
+/*
  * Planner overrides, for tuning sweeps and for tests that run every kernel
  * form on the same inputs.  No counterpart in the reference (its launchers
  * have no knobs).  Each knob holds 0 -- the planner's own choice, the default

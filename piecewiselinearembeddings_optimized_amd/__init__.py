@@ -9,7 +9,10 @@ of ``include/ple_hip.h`` (``csrc/ple_capi.hip``).
 
 Around it, with no counterpart in the reference: embeddings of tokens and
 categorical columns, the norms of a residual trunk and a distillation loss
-(``trunk.py``; operators ``lookup``, ``residual_norm``, ``distillation_loss``).
+(``trunk.py``; operators ``lookup``, ``residual_norm``, ``distillation_loss``); a
+group norm with its activation and a learned relative position bias (``blocks.py``;
+``group_norm``, ``relative_bias``); the gradients' norm and clipping
+(``gradients.py``; ``gradient_norm``, ``clip_gradients_``, ``clip_gradients_into``).
 
 Import order follows the reference (``__init__.py:3-7`` there): the native
 registrations first, then the fake kernels, then autograd, then the module.
@@ -37,14 +40,22 @@ if not _running_build():
     from .module import CudaPiecewiseLinearEmbeddings, CudaPiecewiseLinearEncoding
     from .bins import bin_tables, compute_bins
     from .trunk import CudaCategoricalEmbeddings, CudaDistillationLoss, CudaResidualNorm, CudaTokenEmbeddings
+    from .blocks import CudaGroupNorm, CudaRelativeBias, relative_buckets
+    from .gradients import clip_grad_norm_, clip_gradients_, gradient_norm
 
 __all__ = [
     "CudaCategoricalEmbeddings",
     "CudaDistillationLoss",
+    "CudaGroupNorm",
     "CudaPiecewiseLinearEmbeddings",
     "CudaPiecewiseLinearEncoding",
+    "CudaRelativeBias",
     "CudaResidualNorm",
     "CudaTokenEmbeddings",
     "bin_tables",
+    "clip_grad_norm_",
+    "clip_gradients_",
     "compute_bins",
+    "gradient_norm",
+    "relative_buckets",
 ]

@@ -279,3 +279,73 @@ def _distillation_loss_backward_fake(grad_loss, logits, teacher_logits, teacher_
     _check_distillation(logits, teacher_logits, teacher_classes, labels, temperature, alpha)
     torch._check(grad_loss.ndim == 1 and grad_loss.dtype == torch.float32, lambda: "grad_loss must be float32 [N]")
     return torch.empty_like(logits)
+
+
+# ---------------------------------------------------------------------------
+# group norm, relative bias, gradients
+# ---------------------------------------------------------------------------
+
+def _check_group(x, weight, bias, num_groups) -> None:
+    torch._check(x.ndim >= 2, lambda: "x must have shape [N, ..., C]")
+    torch._check(x.dtype in SUPPORTED_OUTPUT_DTYPES, lambda: "x must be float32, float16, or bfloat16")
+    torch._check(num_groups > 0 and x.shape[-1] % num_groups == 0,
+                 lambda: f"num_groups must divide the number of channels, got {num_groups} and {x.shape[-1]}")
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None:
+            torch._check(t.ndim == 1 and t.shape[0] == x.shape[-1], lambda name=name: f"{name} must have shape [C]")
+
+
+@torch.library.register_fake("rtdl_num_embeddings_cuda::group_norm")
+def _group_norm_fake(x, weight, bias, num_groups, activation, eps):
+    _check_group(x, weight, bias, num_groups)
+    return torch.empty_like(x), x.new_empty((x.shape[0], num_groups, 2), dtype=torch.float32)
+
+
+@torch.library.register_fake("rtdl_num_embeddings_cuda::group_norm_backward")
+def _group_norm_backward_fake(grad_y, x, stats, weight, bias, num_groups, activation, output_mask):
+    _check_group(x, weight, bias, num_groups)
+    torch._check(grad_y.shape == x.shape and grad_y.dtype == x.dtype, lambda: "grad_y must have the shape and dtype of x")
+    return tuple(torch.empty_like(t) if wanted and t is not None else x.new_empty((0,))
+                 for t, wanted in zip((x, weight, bias), output_mask))
+
+
+def _check_bias(buckets, starts) -> None:
+    torch._check(buckets.ndim == 1 and buckets.dtype == torch.int32,
+                 lambda: "buckets must be int32 [2 * far + 1], far at least 1")
+    if starts is not None:
+        torch._check(starts.ndim == 1 and starts.dtype == torch.int64, lambda: "starts must be int64 [B]")
+
+
+@torch.library.register_fake("rtdl_num_embeddings_cuda::relative_bias")
+def _relative_bias_fake(weight, buckets, starts, q_len, k_len, offset, causal, output_dtype):
+    _check_bias(buckets, starts)
+    torch._check(weight.ndim == 2, lambda: "weight must have shape [R, H]")
+    torch._check(output_dtype in SUPPORTED_OUTPUT_DTYPES, lambda: "output_dtype must be float32, float16, or bfloat16")
+    lead = () if starts is None else (starts.shape[0],)
+    return weight.new_empty((*lead, weight.shape[1], q_len, k_len), dtype=output_dtype)
+
+
+@torch.library.register_fake("rtdl_num_embeddings_cuda::relative_bias_backward")
+def _relative_bias_backward_fake(grad_output, buckets, starts, num_rows, offset, causal, grad_dtype):
+    _check_bias(buckets, starts)
+    lead = 0 if starts is None else 1
+    torch._check(grad_output.ndim == 3 + lead,
+                 lambda: "grad_output must have shape [H, q, k], or [B, H, q, k] with starts")
+    return grad_output.new_empty((num_rows, grad_output.shape[lead]), dtype=grad_dtype)
+
+
+@torch.library.register_fake("rtdl_num_embeddings_cuda::gradient_norm")
+def _gradient_norm_fake(grads, norm_type):
+    torch._check(len(grads) > 0, lambda: "there has to be a gradient")
+    return grads[0].new_empty((), dtype=torch.float32)
+
+
+@torch.library.register_fake("rtdl_num_embeddings_cuda::clip_gradients_")
+def _clip_gradients_fake(grads, max_norm, norm_type, norm):
+    return _gradient_norm_fake(grads, norm_type)
+
+
+@torch.library.register_fake("rtdl_num_embeddings_cuda::clip_gradients_into")
+def _clip_gradients_into_fake(grads, out, max_norm, norm_type, norm):
+    torch._check(len(out) == len(grads), lambda: "out must have a tensor for every gradient")
+    return _gradient_norm_fake(grads, norm_type)

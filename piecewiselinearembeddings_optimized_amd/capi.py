@@ -77,6 +77,18 @@ class EncodePlanInfo(ctypes.Structure):
     ]
 
 
+class Grad(ctypes.Structure):
+    """``ple_grad_t``: a gradient of a list, and where it goes when scaled."""
+
+    _fields_ = [
+        ("grad", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("numel", ctypes.c_int64),
+        ("dtype", ctypes.c_int),
+        ("out_dtype", ctypes.c_int),
+    ]
+
+
 class LookupPlanInfo(ctypes.Structure):
     """``ple_lookup_plan_info_t``: the lookup backward's launch plan for a shape."""
 
@@ -188,6 +200,26 @@ def lib() -> ctypes.CDLL:
         L.ple_distill_launch.restype = i32
         L.ple_distill_backward_launch.argtypes = [p, p, p, p, i32, p, p, p, i64, i64, i64, f32, f32, i32, i32, p]
         L.ple_distill_backward_launch.restype = i32
+        L.ple_group_norm_workspace_bytes.argtypes = [i64, i64, i64, i64, i32]
+        L.ple_group_norm_workspace_bytes.restype = sz
+        L.ple_group_norm_launch.argtypes = [p, p, p, p, p, i64, i64, i64, i64, i32, f32, i32, i32, p, sz, p]
+        L.ple_group_norm_launch.restype = i32
+        L.ple_group_norm_backward_workspace_bytes.argtypes = [i64, i64, i64, i64, i32]
+        L.ple_group_norm_backward_workspace_bytes.restype = sz
+        L.ple_group_norm_backward_launch.argtypes = [p, p, p, p, p, p, p, p, i64, i64, i64, i64, i32, i32, i32, p, sz, p]
+        L.ple_group_norm_backward_launch.restype = i32
+        L.ple_relative_bias_launch.argtypes = [p, p, p, p, i64, i64, i64, i64, i64, i64, i64, i32, i32, i32, p]
+        L.ple_relative_bias_launch.restype = i32
+        L.ple_relative_bias_backward_workspace_bytes.argtypes = [i64, i64, i64, i64, i64, i64]
+        L.ple_relative_bias_backward_workspace_bytes.restype = sz
+        L.ple_relative_bias_backward_launch.argtypes = [p, p, p, p, i64, i64, i64, i64, i64, i64, i64, i32, i32, i32, p, sz, p]
+        L.ple_relative_bias_backward_launch.restype = i32
+        L.ple_grad_norm_workspace_bytes.argtypes = [ctypes.POINTER(Grad), i64]
+        L.ple_grad_norm_workspace_bytes.restype = sz
+        L.ple_grad_norm_launch.argtypes = [ctypes.POINTER(Grad), i64, i32, p, p, sz, p]
+        L.ple_grad_norm_launch.restype = i32
+        L.ple_grad_scale_launch.argtypes = [ctypes.POINTER(Grad), i64, p, f32, p]
+        L.ple_grad_scale_launch.restype = i32
         L.ple_timing_start.argtypes, L.ple_timing_start.restype = [i32], i32
         L.ple_timing_stop.argtypes, L.ple_timing_stop.restype = [], i32
         L.ple_timing_read.argtypes = [i32, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_int)]
@@ -437,3 +469,77 @@ def distill_backward(grad_loss, logits, teacher_logits, teacher_classes, stats, 
         _ptr(grad_loss), _ptr(logits), _ptr(teacher_logits), _ptr(teacher_classes), teacher_classes.element_size(),
         _ptr(labels), _ptr(stats), _ptr(grad_logits), n, v, teacher_logits.shape[1], temperature, alpha,
         dtype_code(logits.dtype), dtype_code(teacher_logits.dtype), _stream(stream)))
+
+
+def group_norm(x, weight, bias, y, stats, num_groups, activation=0, eps=1e-5, workspace=None, stream=None) -> None:
+    """``ple_group_norm_launch`` into caller-provided ``y`` (as ``x`` [N, S, C]) and ``stats`` [N, G, 2]."""
+    n, s, c = x.shape
+    param = next((t.dtype for t in (weight, bias) if t is not None), torch.float32)
+    if workspace is None:
+        workspace, need = _workspace(int(lib().ple_group_norm_workspace_bytes(n, s, c, num_groups, dtype_code(x.dtype))), x)
+    else:
+        need = workspace.numel() * workspace.element_size()
+    check(lib().ple_group_norm_launch(
+        _ptr(x), _ptr(weight), _ptr(bias), _ptr(y), _ptr(stats), n, s, c, num_groups, activation, eps, dtype_code(x.dtype),
+        dtype_code(param), _ptr(workspace), need, _stream(stream)))
+
+
+def group_norm_backward(grad_y, x, stats, weight, bias, grad_x, grad_weight, grad_bias, num_groups, activation=0,
+                        workspace=None, stream=None) -> None:
+    """``ple_group_norm_backward_launch``; gradients are caller-provided tensors or None."""
+    n, s, c = x.shape
+    param = next((t.dtype for t in (weight, bias) if t is not None), torch.float32)
+    if workspace is None:
+        workspace, need = _workspace(
+            int(lib().ple_group_norm_backward_workspace_bytes(n, s, c, num_groups, dtype_code(x.dtype))), x)
+    else:
+        need = workspace.numel() * workspace.element_size()
+    check(lib().ple_group_norm_backward_launch(
+        _ptr(grad_y), _ptr(x), _ptr(stats), _ptr(weight), _ptr(bias), _ptr(grad_x), _ptr(grad_weight), _ptr(grad_bias), n, s,
+        c, num_groups, activation, dtype_code(x.dtype), dtype_code(param), _ptr(workspace), need, _stream(stream)))
+
+
+def relative_bias(weight, buckets, out, starts=None, offset=0, causal=False, stream=None) -> None:
+    """``ple_relative_bias_launch`` into a caller-provided ``out`` [H, q, k] ([B, H, q, k] with ``starts``)."""
+    r, h = weight.shape
+    check(lib().ple_relative_bias_launch(
+        _ptr(weight), _ptr(buckets), _ptr(starts), _ptr(out), 1 if starts is None else starts.numel(), h, out.shape[-2],
+        out.shape[-1], r, buckets.numel() // 2, offset, int(causal), dtype_code(weight.dtype), dtype_code(out.dtype),
+        _stream(stream)))
+
+
+def relative_bias_backward(grad_output, buckets, grad_weight, starts=None, offset=0, causal=False, workspace=None,
+                           stream=None) -> None:
+    """``ple_relative_bias_backward_launch`` into a caller-provided ``grad_weight`` [R, H]."""
+    r, h = grad_weight.shape
+    b, q, k, far = 1 if starts is None else starts.numel(), *grad_output.shape[-2:], buckets.numel() // 2
+    if workspace is None:
+        workspace, need = _workspace(int(lib().ple_relative_bias_backward_workspace_bytes(b, h, q, k, r, far)), grad_output)
+    else:
+        need = workspace.numel() * workspace.element_size()
+    check(lib().ple_relative_bias_backward_launch(
+        _ptr(grad_output), _ptr(buckets), _ptr(starts), _ptr(grad_weight), b, h, q, k, r, far, offset, int(causal),
+        dtype_code(grad_output.dtype), dtype_code(grad_weight.dtype), _ptr(workspace), need, _stream(stream)))
+
+
+def gradient_list(grads, out=None):
+    """The host array of ``ple_grad_t`` of tensors that are contiguous (``out``: where they go; in place without)."""
+    pairs = list(zip(grads, grads if out is None else out))
+    return (Grad * len(pairs))(*(Grad(g.data_ptr(), o.data_ptr(), g.numel(), dtype_code(g.dtype), dtype_code(o.dtype))
+                                 for g, o in pairs)), len(pairs)
+
+
+def grad_norm(grads, norm, kind=2, workspace=None, stream=None) -> None:
+    """``ple_grad_norm_launch`` (``kind``: 1, 2, or 3 for the largest) into a caller-provided float32 ``norm``."""
+    listed, count = gradient_list(grads)
+    if workspace is None:
+        workspace, need = _workspace(int(lib().ple_grad_norm_workspace_bytes(listed, count)), norm)
+    else:
+        need = workspace.numel() * workspace.element_size()
+    check(lib().ple_grad_norm_launch(listed, count, kind, _ptr(norm), _ptr(workspace), need, _stream(stream)))
+
+
+def grad_scale(grads, norm, limit, out=None, stream=None) -> None:
+    """``ple_grad_scale_launch``: in place, or into ``out``."""
+    listed, count = gradient_list(grads, out)
+    check(lib().ple_grad_scale_launch(listed, count, _ptr(norm), limit, _stream(stream)))

@@ -1,0 +1,293 @@
+// The norm of many tensors together, and their scaling to a limit (gfx950).
+//
+//     norm = (sum |g|^p)^(1/p), p = 1 or 2, or max |g|
+//     factor = min(1, limit / (norm + 1e-6)),  out = g factor
+//
+// Bound by memory: a read for the norm; a read and a write for the scaling, which
+// does nothing where tensors stay where they are and the factor is 1.  Sums are
+// 64-bit: squares of 32-bit values neither overflow nor vanish there, and the
+// order of the additions is below the 32-bit result's rounding.
+//
+// The tensors' addresses and sizes are kernel arguments, kListed of them a launch,
+// so a captured graph holds them and nothing is copied to the device.
+
+#include <algorithm>
+
+#include "ple_internal.h"
+#include "ple_rows.h"
+
+namespace ple {
+namespace {
+
+constexpr int kListed = 100;             // tensors of a launch (its arguments stay below 4 KB)
+constexpr int64_t kChunk = 16384;        // elements that a workgroup takes at once
+constexpr int kNormThreads = 256;
+
+struct Listed {
+    const void *grad;
+    void *out;
+    int64_t numel;
+    int end;                             // chunks of the tensors up to and with this one
+    int8_t dtype, out_dtype;
+};
+
+struct GradsArgs {
+    Listed t[kListed];
+    int count, chunks;
+    double *partial;                     // of this launch's workgroups
+    const float *norm;
+    float limit;
+    int kind;
+    int in_place;
+};
+static_assert(sizeof(GradsArgs) <= 4096, "kernel arguments");
+
+// The tensor of a chunk.
+__device__ __forceinline__ int find_tensor(const GradsArgs &a, int chunk) {
+    int lo = 0, hi = a.count - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (chunk < a.t[mid].end) hi = mid;
+        else lo = mid + 1;
+    }
+    return lo;
+}
+
+// |v| as a value that grows with it, NaN the largest.
+__device__ __forceinline__ uint32_t size_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+// What a lane has of a norm: a 64-bit sum, or the bits of the largest.
+template <int KIND>
+struct Norm {
+    double sum = 0.0;
+    uint32_t most = 0;
+    __device__ __forceinline__ void add(float v) {
+        if constexpr (KIND == PLE_NORM_P2) sum = fma(static_cast<double>(v), static_cast<double>(v), sum);
+        else if constexpr (KIND == PLE_NORM_P1) sum += fabs(static_cast<double>(v));
+        else most = max(most, size_bits(v));
+    }
+    __device__ __forceinline__ void join(const Norm &o) {
+        sum += o.sum;
+        most = max(most, o.most);
+    }
+    __device__ __forceinline__ Norm moved(int mask) const {
+        Norm o;
+        if constexpr (KIND == PLE_NORM_INF) o.most = __shfl_xor(most, mask);
+        else o.sum = __shfl_xor(sum, mask);
+        return o;
+    }
+    // over the workgroup, on its first thread
+    __device__ __forceinline__ void join_block(double *lds) {
+#pragma unroll
+        for (int m = 1; m < kWave; m *= 2) join(moved(m));
+        if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = packed();
+        __syncthreads();
+        if (threadIdx.x == 0)
+            for (int w = 1; w < static_cast<int>(blockDim.x) / kWave; ++w) add_packed(lds[w]);
+    }
+    __device__ __forceinline__ double packed() const {
+        return KIND == PLE_NORM_INF ? static_cast<double>(__uint_as_float(most)) : sum;
+    }
+    __device__ __forceinline__ void add_packed(double v) {
+        if constexpr (KIND == PLE_NORM_INF) most = max(most, size_bits(static_cast<float>(v)));
+        else sum += v;
+    }
+};
+
+// f(element index, values) over elements [begin, end) of p: single elements up to a
+// 16-byte boundary, vectors, single elements.
+template <int T, typename FV, typename F1>
+__device__ __forceinline__ void walk(const void *p, int64_t begin, int64_t end, FV vec, F1 one) {
+    constexpr int E = T == PLE_DTYPE_F32 ? 4 : 8, kBytes = elem_bytes(T);
+    const uint64_t at = reinterpret_cast<uint64_t>(p) / kBytes + begin;
+    const int64_t head = min(end, begin + static_cast<int64_t>((E - at % E) % E));
+    const int64_t vecs = (end - head) / E, tail = head + vecs * E;
+    if (threadIdx.x < head - begin) one(begin + threadIdx.x);
+    if (threadIdx.x < end - tail) one(tail + threadIdx.x);
+#pragma unroll 4
+    for (int64_t i = threadIdx.x; i < vecs; i += kNormThreads) vec(head + i * E);
+}
+
+template <int T, int KIND>
+__device__ __forceinline__ void add_chunk(const void *p, int64_t begin, int64_t end, Norm<KIND> &n) {
+    constexpr int E = T == PLE_DTYPE_F32 ? 4 : 8;
+    walk<T>(p, begin, end,
+            [&](int64_t i) {
+                float v[E];
+                load_vec<T, E>(static_cast<const char *>(p) + i * elem_bytes(T), 0, v);
+#pragma unroll
+                for (int e = 0; e < E; ++e) n.add(v[e]);
+            },
+            [&](int64_t i) { n.add(load_grad<T>(p, i)); });
+}
+
+template <int KIND>
+__global__ __launch_bounds__(kNormThreads) void ple_grad_norm_kernel(GradsArgs a) {
+    __shared__ double s_norm[kNormThreads / kWave];
+    Norm<KIND> n;
+    for (int c = blockIdx.x; c < a.chunks; c += gridDim.x) {
+        const int i = find_tensor(a, c);
+        const int64_t begin = static_cast<int64_t>(c - (i > 0 ? a.t[i - 1].end : 0)) * kChunk;
+        const int64_t end = min(a.t[i].numel, begin + kChunk);
+        if (a.t[i].dtype == PLE_DTYPE_F32) add_chunk<PLE_DTYPE_F32>(a.t[i].grad, begin, end, n);
+        else if (a.t[i].dtype == PLE_DTYPE_BF16) add_chunk<PLE_DTYPE_BF16>(a.t[i].grad, begin, end, n);
+        else add_chunk<PLE_DTYPE_F16>(a.t[i].grad, begin, end, n);
+    }
+    n.join_block(s_norm);
+    if (threadIdx.x == 0) a.partial[blockIdx.x] = n.packed();
+}
+
+// The norm from the workgroups' partials, in a fixed order.
+template <int KIND>
+__global__ __launch_bounds__(1024) void ple_grad_norm_join_kernel(const double *partial, int count, float *norm) {
+    __shared__ double s_norm[1024 / kWave];
+    Norm<KIND> n;
+    for (int i = threadIdx.x; i < count; i += 1024) n.add_packed(partial[i]);
+    n.join_block(s_norm);
+    if (threadIdx.x != 0) return;
+    if constexpr (KIND == PLE_NORM_INF) *norm = __uint_as_float(n.most);
+    else *norm = static_cast<float>(KIND == PLE_NORM_P2 ? sqrt(n.sum) : n.sum);
+}
+
+template <int T, int O>
+__device__ __forceinline__ void scale_chunk(const void *p, void *out, int64_t begin, int64_t end, float factor) {
+    constexpr int E = O == PLE_DTYPE_F32 && T == PLE_DTYPE_F32 ? 4 : 8;
+    constexpr int kBytes = elem_bytes(T), kOut = elem_bytes(O);
+    const uint64_t at = reinterpret_cast<uint64_t>(out) / kOut + begin, in = reinterpret_cast<uint64_t>(p) / kBytes + begin;
+    // vectors where both sides have their boundaries at the same elements
+    constexpr int A = O == PLE_DTYPE_F32 ? 4 : 8, B = T == PLE_DTYPE_F32 ? 4 : 8;
+    constexpr int C = A > B ? A : B;
+    if ((at - in) % C != 0) {
+        for (int64_t i = begin + threadIdx.x; i < end; i += kNormThreads) {
+            const float v = load_grad<T>(p, i) * factor;
+            store_vec<O, 1>(out, i, &v);
+        }
+        return;
+    }
+    const int64_t head = min(end, begin + static_cast<int64_t>((C - at % C) % C));
+    const int64_t vecs = (end - head) / E, tail = head + vecs * E;
+    const auto one = [&](int64_t i) {
+        const float v = load_grad<T>(p, i) * factor;
+        store_vec<O, 1>(out, i, &v);
+    };
+    if (threadIdx.x < head - begin) one(begin + threadIdx.x);
+    if (threadIdx.x < end - tail) one(tail + threadIdx.x);
+#pragma unroll 4
+    for (int64_t i = threadIdx.x; i < vecs; i += kNormThreads) {
+        float v[E];
+        load_vec<T, E>(p, head + i * E, v);
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] *= factor;
+        store_vec<O, E>(out, head + i * E, v);
+    }
+}
+
+__global__ __launch_bounds__(kNormThreads) void ple_grad_scale_kernel(GradsArgs a) {
+    const float norm = *a.norm;
+    // (an infinite limit clips nothing; a norm of NaN makes everything NaN)
+    const double ratio = static_cast<double>(a.limit) / (static_cast<double>(norm) + 1e-6);
+    const float factor = a.limit == __builtin_inff() || ratio >= 1.0 ? 1.0f : static_cast<float>(ratio);
+    if (a.in_place && factor == 1.0f) return;
+    for (int b = blockIdx.x; b < a.chunks; b += gridDim.x) {
+        const int c = a.chunks - 1 - b;          // (the norm's last reads are the first that caches still have)
+        const int i = find_tensor(a, c);
+        const Listed &t = a.t[i];
+        const int64_t begin = static_cast<int64_t>(c - (i > 0 ? a.t[i - 1].end : 0)) * kChunk;
+        const int64_t end = min(t.numel, begin + kChunk);
+        const auto to = [&](auto from) {
+            constexpr int T = decltype(from)::value;
+            if (t.out_dtype == PLE_DTYPE_F32) scale_chunk<T, PLE_DTYPE_F32>(t.grad, t.out, begin, end, factor);
+            else if (t.out_dtype == PLE_DTYPE_BF16) scale_chunk<T, PLE_DTYPE_BF16>(t.grad, t.out, begin, end, factor);
+            else scale_chunk<T, PLE_DTYPE_F16>(t.grad, t.out, begin, end, factor);
+        };
+        if (t.dtype == PLE_DTYPE_F32) to(std::integral_constant<int, PLE_DTYPE_F32>{});
+        else if (t.dtype == PLE_DTYPE_BF16) to(std::integral_constant<int, PLE_DTYPE_BF16>{});
+        else to(std::integral_constant<int, PLE_DTYPE_F16>{});
+    }
+}
+
+// ---------------------------------------------------------------------------
+// launches
+// ---------------------------------------------------------------------------
+
+// The tensors of the list from `from` on that one launch takes; returns where the
+// next launch begins.  (A launch's chunks are counted in 32 bits.)
+int64_t fill(const ple_grad_t *grads, int64_t count, int64_t from, GradsArgs &a) {
+    a.count = 0;
+    a.chunks = 0;
+    a.in_place = 1;
+    int64_t i = from;
+    for (; i < count && a.count < kListed; ++i) {
+        if (grads[i].numel == 0) continue;
+        const int64_t chunks = (grads[i].numel + kChunk - 1) / kChunk;
+        if (a.chunks + chunks > INT32_MAX / 2) break;        // (numel is below 2^40: one tensor always fits)
+        Listed &t = a.t[a.count++];
+        t.grad = grads[i].grad;
+        t.out = grads[i].out;
+        t.numel = grads[i].numel;
+        t.dtype = static_cast<int8_t>(grads[i].dtype);
+        t.out_dtype = static_cast<int8_t>(grads[i].out_dtype);
+        a.chunks += static_cast<int>(chunks);
+        t.end = a.chunks;
+        if (t.out != t.grad) a.in_place = 0;
+    }
+    return i;
+}
+
+int grid_of(const GradsArgs &a) { return std::min(a.chunks, 8 * device_cu_count()); }
+
+template <int KIND>
+int norm_launches(const GradsRequest &r) {
+    GradsArgs a{};
+    int64_t used = 0;
+    for (int64_t from = 0; from < r.count;) {
+        from = fill(r.grads, r.count, from, a);
+        if (a.count == 0) break;
+        a.partial = static_cast<double *>(r.workspace) + used;
+        const int grid = grid_of(a);
+        used += grid;
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_grad_norm_kernel<KIND>), dim3(grid), dim3(kNormThreads), 0, r.stream, a);
+        const hipError_t rc = hipGetLastError();
+        if (rc != hipSuccess) return static_cast<int>(rc);
+    }
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_grad_norm_join_kernel<KIND>), dim3(1), dim3(1024), 0, r.stream,
+                       static_cast<const double *>(r.workspace), static_cast<int>(used), r.norm);
+    return static_cast<int>(hipGetLastError());
+}
+
+}  // namespace
+
+size_t grad_norm_workspace_bytes(const GradsRequest &r) {
+    GradsArgs a{};
+    int64_t used = 0;
+    for (int64_t from = 0; from < r.count;) {
+        from = fill(r.grads, r.count, from, a);
+        if (a.count == 0) break;
+        used += grid_of(a);
+    }
+    return align_up(static_cast<size_t>(std::max<int64_t>(used, 1)) * 8, 256);
+}
+
+int grad_norm_run(const GradsRequest &r) {
+    const size_t need = grad_norm_workspace_bytes(r);
+    if (!r.workspace || r.workspace_bytes < need || reinterpret_cast<uintptr_t>(r.workspace) % 256 != 0) return PLE_E_WORKSPACE;
+    if (r.kind == PLE_NORM_P2) return norm_launches<PLE_NORM_P2>(r);
+    if (r.kind == PLE_NORM_P1) return norm_launches<PLE_NORM_P1>(r);
+    return norm_launches<PLE_NORM_INF>(r);
+}
+
+int grad_scale_run(const GradsRequest &r) {
+    GradsArgs a{};
+    a.norm = r.norm;
+    a.limit = r.limit;
+    for (int64_t from = 0; from < r.count;) {
+        from = fill(r.grads, r.count, from, a);
+        if (a.count == 0) break;
+        hipLaunchKernelGGL(ple_grad_scale_kernel, dim3(grid_of(a)), dim3(kNormThreads), 0, r.stream, a);
+        const hipError_t rc = hipGetLastError();
+        if (rc != hipSuccess) return static_cast<int>(rc);
+    }
+    return PLE_OK;
+}
+
+}  // namespace ple

@@ -162,4 +162,56 @@ int distill_run(const DistillRequest &r);
 size_t distill_workspace_bytes(int64_t N, int64_t V);
 int distill_backward_run(const DistillRequest &r);
 
+struct GroupRequest {
+    const void *x, *weight, *bias;
+    const void *g = nullptr;             // backward: gradient of y
+    void *y = nullptr;                   // forward: y; backward: gradient of x
+    void *d_weight = nullptr, *d_bias = nullptr;
+    float *stats;                        // [N, G, 2]
+    int64_t N, S, C, G;
+    int dtype, param_dtype, act;
+    float eps;
+    void *workspace = nullptr;
+    size_t workspace_bytes = 0;
+    hipStream_t stream;
+};
+
+int group_run(const GroupRequest &r);
+size_t group_workspace_bytes(const GroupRequest &r);
+int group_backward_run(const GroupRequest &r);
+size_t group_backward_workspace_bytes(const GroupRequest &r);
+
+struct BiasRequest {
+    const void *weight = nullptr;        // [R, H], of weight_dtype
+    const void *grad = nullptr;          // backward: [B, H, q, k], of out_dtype
+    const int32_t *buckets;              // [2 far + 1]
+    const int64_t *starts = nullptr;     // [B], or NULL: offset (B is 1)
+    void *out = nullptr;                 // forward: [B, H, q, k], of out_dtype
+    void *dw = nullptr;                  // backward: [R, H], of weight_dtype
+    int64_t B, H, q, k, R, far, offset;
+    int causal, weight_dtype, out_dtype;
+    void *workspace = nullptr;
+    size_t workspace_bytes = 0;
+    hipStream_t stream;
+};
+
+int bias_run(const BiasRequest &r);
+size_t bias_backward_workspace_bytes(const BiasRequest &r);
+int bias_backward_run(const BiasRequest &r);
+
+struct GradsRequest {
+    const ple_grad_t *grads;
+    int64_t count;
+    int kind = PLE_NORM_P2;
+    float *norm;                         // written by the norm, read by the scaling
+    float limit = 0.0f;
+    void *workspace = nullptr;
+    size_t workspace_bytes = 0;
+    hipStream_t stream;
+};
+
+int grad_norm_run(const GradsRequest &r);
+size_t grad_norm_workspace_bytes(const GradsRequest &r);
+int grad_scale_run(const GradsRequest &r);
+
 }  // namespace ple
