@@ -520,7 +520,7 @@ int ple_group_norm_backward_launch(const void *grad_y, const void *x, const floa
  *   buckets   int32 [2 far + 1]
  *   starts    int64 [B], or NULL: offset for all (then B is 1)
  *   out       out_dtype [B, H, q, k]
- * 1 <= far <= 2^24; B, H, R, q, k < 2^31, B * H * q * k < 2^44, |offset| <= 2^60
+ * 1 <= far <= 2^24; q, k <= 2^23; B, H, R < 2^31, B * H * q * k < 2^44, |offset| <= 2^60
  * (else PLE_E_TOO_LARGE); positions beyond 2^60 count as 2^60.
  */
 int ple_relative_bias_launch(const void *weight, const int32_t *buckets, const int64_t *starts, void *out, int64_t B,

@@ -24,10 +24,12 @@ struct BiasArgs {
     const int64_t *starts;       // [B] or NULL: offset
     void *out;                   // forward: out; backward: the table's gradient
     float *partial;              // backward: [head, parts, stride]
+    float *total;                // backward: [head, 2 far + 1] sums of the parts, or NULL
     int64_t q, k, offset, tiles;
     int64_t rowblocks, colblocks;
     int B, H, R, far, causal;
-    int rows, cols;              // of a tile
+    int rows, cols;              // forward: of a tile; backward: diagonals of a unit ...
+    int reach;                   // ... and before them
     int stride;                  // floats of a partial
     int weight_dtype;
 };
@@ -144,129 +146,308 @@ __global__ __launch_bounds__(kBlock) void ple_bias_forward_kernel(BiasArgs a) {
 // backward
 // ---------------------------------------------------------------------------
 
-constexpr int kGradRows = 64, kGradCols = 2048;      // a backward tile
+constexpr int kGradRows = 64;            // rows of a wave's unit
+constexpr int kGradItems = 8;            // in so many steps of
+constexpr int kGradLoads = 8;            // loads a lane
 
-// A tile's distances, and the places of a partial that they reach: lo to hi, with
-// what lies beyond -far or far in the outermost.
-struct Window {
-    int64_t low;                 // distance of the window's first place
+// A wave's unit: kGradRows rows of a sample's head along 64 vectors of diagonals j - i
+// (a parallelogram of the matrix, so no unit has edges inside it), and the places of
+// its partial: distances lo to hi, with what lies beyond -far or far in the outermost.
+// Vectors begin up to reach diagonals before `first`, as the rows' addresses have it.
+// live: whether any distance counts.
+struct Unit {
+    int64_t first;               // diagonal
+    int64_t low;                 // distance of the first place, first - reach
     int size;
     int64_t lo, hi;
-    __device__ __forceinline__ Window(const BiasArgs &a, int64_t start, int64_t i0, int64_t c0) {
-        const int64_t i1 = min(a.q, i0 + a.rows), c1 = min(a.k, c0 + a.cols);
-        low = c0 - (start + i1 - 1);
-        size = static_cast<int>(c1 - c0 + i1 - i0 - 1);
-        const int64_t f = a.far;
-        lo = min(max(low, -f), f);
-        hi = min(max(low + size - 1, -f), f);
+    bool live;
+    __device__ __forceinline__ Unit(const BiasArgs &a, int64_t start, int64_t i0, int64_t chunk) {
+        const int64_t i1 = min(a.q, i0 + kGradRows);
+        first = chunk * a.cols - (i1 - 1);
+        low = first - a.reach - start;
+        size = a.cols + a.reach;
+        const int64_t f = a.far, top = a.causal ? 0 : f;
+        live = low <= top || !a.causal;
+        lo = min(max(low, -f), top);
+        hi = min(max(low + size - 1, -f), top);
     }
 };
 
-__device__ __forceinline__ float sum_block(float v, float *lds) {
-    v = group_sum<kWave>(v);
-    __syncthreads();
-    if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = v;
-    __syncthreads();
-    float s = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kWavesPerBlock; ++i) s += lds[i];
-    return s;
+// Elements of a vector as loaded.
+template <int T>
+__device__ __forceinline__ float vector_elem(const uint4 &raw, int e) {
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    return grad_elem<T>(w, e);
 }
 
-// Sums along a tile's diagonals.  Rows E apart (E: elements of 16 bytes) have their
-// vector boundaries on the same diagonals, whatever the row's length; so a lane
-// takes a vector of diagonals through every E-th row with aligned loads.
+// A vector without its elements before column 0 and from column k on; j: its first
+// element's column.
 template <int T>
-__global__ __launch_bounds__(kBlock) void ple_bias_backward_kernel(BiasArgs a) {
-    constexpr int E = vec_elems<T>(), kBytes = elem_bytes(T), kSteps = kGradRows / E;
-    constexpr int kPlaces = kGradCols + kGradRows + 2 * E;
-    __shared__ float s_diag[kWavesPerBlock][kPlaces];
-    __shared__ float s_sum[kWavesPerBlock];
-    const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-    for (int64_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
-        int64_t t = tile;
-        const int64_t c0 = t % a.colblocks * a.cols;
-        t /= a.colblocks;
-        const int64_t i0 = t % a.rowblocks * a.rows;
-        const int64_t z = t / a.rowblocks;
-        const int64_t start = start_of(a, z / a.H);
-        const int64_t c1 = min(a.k, c0 + a.cols), i1 = min(a.q, i0 + a.rows);
-        const Window win(a, start, i0, c0);
-        // diagonal u = j - i; its distance is u - start
-        const int64_t first = c0 - (i1 - 1), last = c1 - 1 - i0;
-        __syncthreads();
-        for (int i = threadIdx.x; i < kWavesPerBlock * kPlaces; i += kBlock) s_diag[0][i] = 0.0f;
-        __syncthreads();
-        const char *const grad = static_cast<const char *>(a.grad) + z * a.q * a.k * kBytes;
-        const uint64_t base = reinterpret_cast<uint64_t>(grad) / kBytes;
-        for (int c = wave; c < E && i0 + c < i1; c += kWavesPerBlock) {
-            const int64_t i = i0 + c;
-            // the first diagonal at or before `first` whose vectors are aligned in these rows
-            const int64_t back = static_cast<int64_t>((base + i * (a.k + 1) + first) & (E - 1));
-            for (int64_t u = first - back + lane * E; u <= last; u += kWave * E) {
-                if (a.causal && u > start) break;
-                float acc[E] = {};
+__device__ __forceinline__ uint4 within(const uint4 &raw, int64_t j, int64_t k) {
+    uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-                for (int s = 0; s < kSteps; ++s) {
-                    const int64_t r = i + s * E, j = u + r;
-                    if (r >= i1 || j >= c1 || j + E <= c0) continue;
-                    const char *const p = grad + (r * a.k + j) * kBytes;
-                    float v[E];
-                    if (j >= c0 && j + E <= c1) {
-                        load_vec<T, E>(p, 0, v);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < E; ++e) v[e] = j + e >= c0 && j + e < c1 ? load_grad<T>(p, e) : 0.0f;
-                    }
-#pragma unroll
-                    for (int e = 0; e < E; ++e) acc[e] += v[e];
-                }
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const int at = static_cast<int>(u + e - first) + E;
-                    s_diag[wave][at] += acc[e];
-                }
-            }
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (T == PLE_DTYPE_F32) {
+            w[i] = j + i >= 0 && j + i < k ? w[i] : 0u;
+        } else {
+            const uint32_t lo = j + 2 * i >= 0 && j + 2 * i < k ? 0xffffu : 0u;
+            const uint32_t hi = j + 2 * i + 1 >= 0 && j + 2 * i + 1 < k ? 0xffff0000u : 0u;
+            w[i] &= lo | hi;
         }
-        __syncthreads();
-        const int64_t parts = a.B * a.rowblocks * a.colblocks;
-        const int64_t part = ((z / a.H) * a.rowblocks + i0 / a.rows) * a.colblocks + c0 / a.cols;
-        float *const partial = a.partial + ((z % a.H) * parts + part) * a.stride;
-        float before = 0.0f, after = 0.0f;
-        for (int w = threadIdx.x; w < win.size; w += kBlock) {
-            const int64_t d = win.low + w;
-            if (a.causal && d > 0) break;
-            float s = 0.0f;
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Adds vectors that begin BACK diagonals before the lane's own to its sums
+// (sum[E - 1 + x]: x diagonals after its own first).
+template <int T, int BACK, int N>
+__device__ __forceinline__ void add_vectors(const uint4 (&raw)[N], float (&sum)[2 * vec_elems<T>() - 1]) {
+    constexpr int E = vec_elems<T>();
 #pragma unroll
-            for (int v = 0; v < kWavesPerBlock; ++v) s += s_diag[v][w + E];
-            if (d <= win.lo) before += s;
-            else if (d >= win.hi) after += s;
-            else partial[d - win.lo] = s;
+    for (int v = 0; v < N; ++v)
+#pragma unroll
+        for (int e = 0; e < E; ++e) sum[E - 1 - BACK + e] += vector_elem<T>(raw[v], e);
+}
+
+template <int T, int N>
+__device__ __forceinline__ void add_vectors(const uint4 (&raw)[N], int back, float (&sum)[2 * vec_elems<T>() - 1]) {
+    switch (back) {
+        case 0: return add_vectors<T, 0>(raw, sum);
+        case 1: return add_vectors<T, 1>(raw, sum);
+        case 2: return add_vectors<T, 2>(raw, sum);
+        case 3: return add_vectors<T, 3>(raw, sum);
+        default: break;
+    }
+    if constexpr (vec_elems<T>() == 8) {
+        switch (back) {
+            case 4: return add_vectors<T, 4>(raw, sum);
+            case 5: return add_vectors<T, 5>(raw, sum);
+            case 6: return add_vectors<T, 6>(raw, sum);
+            default: return add_vectors<T, 7>(raw, sum);
         }
-        before = sum_block(before, s_sum);
-        after = sum_block(after, s_sum);
-        if (threadIdx.x == 0) {
-            partial[0] = win.hi > win.lo ? before : before + after;
-            if (win.hi > win.lo) partial[win.hi - win.lo] = after;
-        }
-        // (masked distances between lo and hi have nothing)
-        if (a.causal)
-            for (int64_t e = max(win.lo + 1, static_cast<int64_t>(1)) + threadIdx.x; e < win.hi; e += kBlock) partial[e - win.lo] = 0.0f;
     }
 }
 
-// Sums of a head's distances over the tiles, then of each row's distances: a wave a
-// row.  Workgroups take a head and kJoinRows rows of the table.
-constexpr int kJoinRows = 64, kJoinPlaces = 4096, kJoinThreads = 1024;
+// The tensor's first elements that lie before its first 16-byte boundary, and its last
+// ones behind the last: the vectors that hold them are not all in its memory.
+// (apart_last of them end the last row, which has all of them: k >= E)
+template <int T>
+__device__ __forceinline__ int apart_first(const BiasArgs &a) {
+    constexpr int E = vec_elems<T>();
+    return (E - static_cast<int>(reinterpret_cast<uint64_t>(a.grad) / elem_bytes(T) % E)) % E;
+}
+
+template <int T>
+__device__ __forceinline__ int apart_last(const BiasArgs &a) {
+    constexpr int E = vec_elems<T>();
+    return static_cast<int>((reinterpret_cast<uint64_t>(a.grad) / elem_bytes(T) + a.B * a.H * a.q * a.k) % E);
+}
+
+// Sums along diagonals.  Rows E apart (E: elements of 16 bytes) have their vector
+// boundaries on the same diagonals, whatever the row's length; so a lane takes a vector
+// of diagonals through every E-th row with aligned loads, and the next rows with
+// another shift.  NARROW: rows of less than a vector, element by element.
+template <int T, bool NARROW>
+__global__ __launch_bounds__(kBlock, 4) void ple_bias_backward_kernel(BiasArgs a) {
+    constexpr int E = vec_elems<T>(), kBytes = elem_bytes(T);
+    constexpr int kEach = kGradItems / E;                    // steps of a class of rows
+    const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+    const int64_t parts = a.B * a.rowblocks * a.colblocks;
+    for (int64_t unit = static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + wave; unit < a.tiles;
+         unit += static_cast<int64_t>(gridDim.x) * kWavesPerBlock) {
+        const int64_t t = unit / a.colblocks, chunk = unit - t * a.colblocks;
+        const int64_t z = t / a.rowblocks, block = t - z * a.rowblocks, i0 = block * kGradRows;
+        const int64_t b = z / a.H, start = start_of(a, b);
+        const Unit win(a, start, i0, chunk);
+        if (!win.live) continue;
+        const int rows = static_cast<int>(min(a.q - i0, static_cast<int64_t>(kGradRows)));
+        const char *const row0 = static_cast<const char *>(a.grad) + (z * a.q + i0) * a.k * kBytes;
+        const int64_t own = win.first + lane * E;            // the lane's first diagonal
+        const int64_t col = own + i0;                        // ... its column in row i0
+        float mine[E], before_own[E - 1];
+        if constexpr (NARROW) {
+#pragma unroll
+            for (int d = 0; d < E; ++d) {
+                mine[d] = 0.0f;
+                if (d < E - 1) before_own[d] = 0.0f;
+                for (int j = 0; j < a.k; ++j) {
+                    const int64_t r = j - (col + d);
+                    if (r >= 0 && r < rows) mine[d] += load_grad<T>(row0, r * a.k + j);
+                }
+            }
+        } else {
+            const int64_t step = (a.k + 1) * kBytes;         // from row to row
+            const uint64_t place = reinterpret_cast<uint64_t>(row0) / kBytes + static_cast<uint64_t>(col);
+            const bool dead = a.causal && own - (E - 1) > start;
+            // vectors that leave the tensor are read by the join
+            const int skip_first = z == 0 && i0 == 0 ? 0 : -1;
+            const int skip_last = z + 1 == static_cast<int64_t>(a.B) * a.H && i0 + rows == a.q ? rows - 1 : -1;
+            // The lane's part of an address is the same in every row, the rows' is scalar;
+            // lanes outside of a row get zeros.
+            const __amdgpu_buffer_rsrc_t rs = make_rsrc(row0 + (win.first + i0 - (E - 1)) * kBytes, 0xfffffff0u);
+            const uint32_t at = static_cast<uint32_t>(lane) * 16;
+            float sum[2 * E - 1] = {};
+#pragma unroll 1
+            for (int item = 0; item < kGradItems; ++item) {
+                // the item's first row, and how far before the lane's diagonal its vectors begin
+                const int c = item / kEach + item % kEach * kGradLoads * E;
+                const int back = __builtin_amdgcn_readfirstlane(
+                    static_cast<int>(place + static_cast<uint64_t>(c) * static_cast<uint64_t>(a.k + 1)) & (E - 1));
+                if (c >= rows) continue;
+                const uint32_t from = static_cast<uint32_t>((E - 1 - back) * kBytes) + static_cast<uint32_t>(c * step);
+                // (columns E - 1 further than they are, so that all of a row's are positive)
+                const uint32_t j = static_cast<uint32_t>(col - back + c + (E - 1)), k = static_cast<uint32_t>(a.k + (E - 1));
+                uint4 raw[kGradLoads];
+                bool cut = false;
+#pragma unroll
+                for (int v = 0; v < kGradLoads; ++v) {
+                    const int r = c + v * E;
+                    const uint32_t jv = j + v * E;
+                    const bool part = jv < E - 1 || jv + E > k;
+                    const bool on = jv < k && r < rows && !dead &&
+                                    !(r == skip_first && jv < E - 1) && !(r == skip_last && jv + E > k);
+                    const auto w = __builtin_amdgcn_raw_buffer_load_b128(
+                        rs, on ? at : 0xffffffffu, __builtin_amdgcn_readfirstlane(from + static_cast<uint32_t>(v * E * step)), 0);
+                    raw[v] = make_uint4(w[0], w[1], w[2], w[3]);
+                    cut = cut || (on && part);
+                }
+                if (__any(cut)) {
+#pragma unroll
+                    for (int v = 0; v < kGradLoads; ++v) raw[v] = within<T>(raw[v], col - back + c + v * E, a.k);
+                }
+                add_vectors<T>(raw, back, sum);
+            }
+            // the lane's own diagonals: with what the next lane's vectors have of them
+            mine[0] = sum[E - 1];
+#pragma unroll
+            for (int d = 0; d < E - 1; ++d) {
+                before_own[d] = sum[d];
+                const float next = __shfl_down(sum[d], 1);
+                mine[d + 1] = sum[E + d] + (lane < kWave - 1 ? next : 0.0f);
+            }
+        }
+        float *const partial = a.partial + ((z - b * a.H) * parts + (b * a.rowblocks + block) * a.colblocks + chunk) * a.stride;
+        float before = 0.0f, after = 0.0f;
+        const auto leave = [&](int64_t d, float s) {
+            if (a.causal && d > 0) return;
+            if (d <= win.lo) before += s;
+            else if (d >= win.hi) after += s;
+            else partial[d - win.lo] = s;
+        };
+#pragma unroll
+        for (int d = 0; d < E; ++d) leave(own + d - start, mine[d]);
+        if (lane == 0)
+#pragma unroll
+            for (int d = 0; d < E - 1; ++d) leave(win.low + d, before_own[d]);
+        before = group_sum<kWave>(before);
+        after = group_sum<kWave>(after);
+        if (lane == 0) {
+            partial[0] = win.hi > win.lo ? before : before + after;
+            if (win.hi > win.lo) partial[win.hi - win.lo] = after;
+        }
+    }
+}
+
+// What of a head's sum at distance e lies in vectors that leave the tensor.
+template <int T>
+__device__ __forceinline__ float apart_sum(const BiasArgs &a, int h, int e) {
+    float s = 0.0f;
+    if (a.k < vec_elems<T>()) return s;
+    const int first = apart_first<T>(a), last = apart_last<T>(a);
+    const int64_t far = a.far, end = a.B * a.H * a.q * a.k;
+    const auto add = [&](int64_t at, int64_t b, int64_t i, int64_t j) {
+        const int64_t d = j - start_of(a, b) - i;
+        if (!(a.causal && d > 0) && min(max(d, -far), far) == e) s += load_grad<T>(a.grad, at);
+    };
+    if (h == 0)
+        for (int j = 0; j < first; ++j) add(j, 0, 0, j);
+    if (h == a.H - 1)
+        for (int64_t j = a.k - last; j < a.k; ++j)
+            if (end - a.k + j >= first) add(end - a.k + j, a.B - 1, a.q - 1, j);
+    return s;
+}
+
+// Sums of a head's distances over the units: 64 distances a workgroup.  It lists the
+// units that reach them, and its waves take one of these each in turn.
+constexpr int kJoinThreads = 1024;
+
+template <int T>
+__global__ __launch_bounds__(kJoinThreads) void ple_bias_total_kernel(BiasArgs a) {
+    __shared__ float s_sum[kJoinThreads];
+    __shared__ int64_t s_base[kJoinThreads];             // a unit's place of distance 0
+    __shared__ int s_lo[kJoinThreads], s_hi[kJoinThreads];
+    __shared__ int s_count[kJoinThreads / kWave];
+    const int64_t places = 2 * static_cast<int64_t>(a.far) + 1, blocks = (places + kWave - 1) / kWave;
+    const int64_t parts = a.B * a.rowblocks * a.colblocks;
+    const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+    for (int64_t unit = blockIdx.x; unit < a.H * blocks; unit += gridDim.x) {
+        const int h = static_cast<int>(unit / blocks);
+        const int64_t place = (unit - h * blocks) * kWave + lane;
+        const int e = static_cast<int>(place - a.far), e0 = e - lane;
+        const float *const head = a.partial + h * parts * a.stride;
+        // sums of units whose distances are all -far or less (fold[0]), or the most that
+        // counts and more: a thread a unit
+        const int top = a.causal ? 0 : a.far;
+        float s = 0.0f, fold[2] = {};
+        for (int64_t p0 = 0; p0 < parts && e0 <= top; p0 += kJoinThreads) {
+            const int64_t part = p0 + threadIdx.x;
+            bool hit = false;
+            int lo = 0, hi = 0;
+            if (part < parts) {
+                const int64_t by = part / a.colblocks, b = by / a.rowblocks;
+                const Unit win(a, start_of(a, b), (by - b * a.rowblocks) * kGradRows, part - by * a.colblocks);
+                lo = static_cast<int>(win.lo);
+                hi = static_cast<int>(win.hi);
+                hit = win.live && lo < e0 + kWave && hi >= e0;
+                if (hit && lo == hi) {
+                    fold[lo == top] += head[part * a.stride];
+                    hit = false;
+                }
+            }
+            const uint64_t hits = __ballot(hit);
+            __syncthreads();
+            if (lane == 0) s_count[wave] = __popcll(hits);
+            __syncthreads();
+            int at = __popcll(hits & ((uint64_t{1} << lane) - 1)), count = 0;
+#pragma unroll
+            for (int w = 0; w < kJoinThreads / kWave; ++w) {
+                if (w < wave) at += s_count[w];
+                count += s_count[w];
+            }
+            if (hit) {
+                s_base[at] = part * a.stride - lo;
+                s_lo[at] = lo;
+                s_hi[at] = hi;
+            }
+            __syncthreads();
+#pragma unroll 4
+            for (int i = wave; i < count; i += kJoinThreads / kWave)
+                if (e >= s_lo[i] && e <= s_hi[i]) s += head[s_base[i] + e];
+        }
+        fold[0] = group_sum<kWave>(fold[0]);
+        fold[1] = group_sum<kWave>(fold[1]);
+        if (e == -a.far) s += fold[0];
+        if (e == top) s += fold[1];
+        __syncthreads();
+        s_sum[threadIdx.x] = s;
+        __syncthreads();
+        if (wave == 0 && place < places) {
+            for (int w = 1; w < kJoinThreads / kWave; ++w) s += s_sum[w * kWave + lane];
+            if (parts > 0) s += apart_sum<T>(a, h, e);
+            a.total[h * places + place] = s;
+        }
+    }
+}
+
+// Sums of each row's distances: a wave a row.  Workgroups take a head and kJoinRows
+// rows of the table.
+constexpr int kJoinRows = 16, kJoinPlaces = 4096;
 
 __global__ __launch_bounds__(kJoinThreads) void ple_bias_join_kernel(BiasArgs a) {
     __shared__ float s_sum[kJoinPlaces];
+    __shared__ int s_bucket[kJoinPlaces];
     __shared__ float s_row[kJoinRows];
     const int64_t groups = (a.R + kJoinRows - 1) / kJoinRows;
-    const int64_t parts = a.B * a.rowblocks * a.colblocks;
     const int64_t places = 2 * static_cast<int64_t>(a.far) + 1;
     for (int64_t unit = blockIdx.x; unit < a.H * groups; unit += gridDim.x) {
         const int h = static_cast<int>(unit / groups);
@@ -277,24 +458,14 @@ __global__ __launch_bounds__(kJoinThreads) void ple_bias_join_kernel(BiasArgs a)
             const int count = static_cast<int>(min(places - p0, static_cast<int64_t>(kJoinPlaces)));
             __syncthreads();
             for (int i = threadIdx.x; i < count; i += kJoinThreads) {
-                const int64_t e = p0 + i - a.far;
-                float s = 0.0f;
-                for (int64_t b = 0; b < a.B; ++b) {
-                    const int64_t start = start_of(a, b);
-                    for (int64_t y = 0; y < a.rowblocks; ++y)
-                        for (int64_t x = 0; x < a.colblocks; ++x) {
-                            const Window win(a, start, y * a.rows, x * a.cols);
-                            if (e < win.lo || e > win.hi) continue;
-                            s += a.partial[(h * parts + (b * a.rowblocks + y) * a.colblocks + x) * a.stride + (e - win.lo)];
-                        }
-                }
-                s_sum[i] = s;
+                s_sum[i] = a.total[h * places + p0 + i];
+                s_bucket[i] = a.buckets[p0 + i];
             }
             __syncthreads();
             for (int r = threadIdx.x / kWave; r < rows; r += kJoinThreads / kWave) {
                 float s = 0.0f;
-                for (int i = threadIdx.x % kWave; i < count; i += kWave)
-                    if (a.buckets[p0 + i] == r0 + r) s += s_sum[i];
+#pragma unroll 4
+                for (int i = threadIdx.x % kWave; i < count; i += kWave) s += s_bucket[i] == r0 + r ? s_sum[i] : 0.0f;
                 s = group_sum<kWave>(s);
                 if (threadIdx.x % kWave == 0) s_row[r] += s;
             }
@@ -310,21 +481,41 @@ __global__ __launch_bounds__(kJoinThreads) void ple_bias_join_kernel(BiasArgs a)
 
 constexpr int64_t kMaxGrid = 1 << 20;
 
-BiasArgs bias_args(const BiasRequest &r, int rows, int cols) {
+BiasArgs bias_args(const BiasRequest &r) {
     BiasArgs a{};
     a.weight = r.weight; a.grad = r.grad; a.buckets = r.buckets; a.starts = r.starts;
     a.partial = static_cast<float *>(r.workspace);
     a.q = r.q; a.k = r.k; a.offset = r.offset;
     a.B = static_cast<int>(r.B); a.H = static_cast<int>(r.H); a.R = static_cast<int>(r.R); a.far = static_cast<int>(r.far);
     a.causal = r.causal;
-    a.rows = rows; a.cols = cols;
-    a.rowblocks = (r.q + rows - 1) / rows;
-    a.colblocks = (r.k + cols - 1) / cols;
-    a.tiles = r.B * r.H * a.rowblocks * a.colblocks;
-    a.stride = static_cast<int>(std::min<int64_t>(std::min<int64_t>(rows, r.q) + std::min<int64_t>(cols, r.k) - 1, 2 * r.far + 1));
     a.weight_dtype = r.weight_dtype;
     return a;
 }
+
+BiasArgs forward_args(const BiasRequest &r) {
+    BiasArgs a = bias_args(r);
+    a.out = r.out;
+    a.rows = kBiasRows; a.cols = kBiasCols;
+    a.rowblocks = (r.q + a.rows - 1) / a.rows;
+    a.colblocks = (r.k + a.cols - 1) / a.cols;
+    a.tiles = r.B * r.H * a.rowblocks * a.colblocks;
+    return a;
+}
+
+// elems: elements of 16 bytes of the gradient
+BiasArgs backward_args(const BiasRequest &r, int elems) {
+    BiasArgs a = bias_args(r);
+    a.out = r.dw;
+    a.rows = kGradRows; a.cols = kWave * elems; a.reach = elems - 1;
+    a.rowblocks = (r.q + kGradRows - 1) / kGradRows;
+    // a block's diagonals, and what vectors that begin before them miss at the end
+    a.colblocks = r.q > 0 && r.k > 0 ? (r.k + std::min<int64_t>(r.q, kGradRows) - 1 + a.reach + a.cols - 1) / a.cols : 0;
+    a.tiles = r.B * r.H * a.rowblocks * a.colblocks;
+    a.stride = static_cast<int>(std::min<int64_t>(a.cols + a.reach, 2 * r.far + 1));
+    return a;
+}
+
+size_t partial_bytes(const BiasArgs &a) { return align_up(static_cast<size_t>(a.tiles) * a.stride * 4, 256); }
 
 template <typename F>
 hipError_t with_type(int dtype, F f) {
@@ -336,8 +527,7 @@ hipError_t with_type(int dtype, F f) {
 }  // namespace
 
 int bias_run(const BiasRequest &r) {
-    BiasArgs a = bias_args(r, kBiasRows, kBiasCols);
-    a.out = r.out;
+    const BiasArgs a = forward_args(r);
     const dim3 grid(static_cast<unsigned>(std::min(a.tiles, kMaxGrid)));
     return static_cast<int>(with_type(r.out_dtype, [&](auto t) {
         hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_bias_forward_kernel<decltype(t)::value>), grid, dim3(kBlock), 0, r.stream, a);
@@ -345,25 +535,35 @@ int bias_run(const BiasRequest &r) {
     }));
 }
 
+// (of either type: 16-bit units have more places, 32-bit ones are more)
 size_t bias_backward_workspace_bytes(const BiasRequest &r) {
-    const BiasArgs a = bias_args(r, kGradRows, kGradCols);
-    return align_up(static_cast<size_t>(a.tiles) * a.stride * 4, 256);
+    return std::max(partial_bytes(backward_args(r, 4)), partial_bytes(backward_args(r, 8))) +
+           align_up(static_cast<size_t>(r.H) * (2 * r.far + 1) * 4, 256);
 }
 
 int bias_backward_run(const BiasRequest &r) {
     const size_t need = bias_backward_workspace_bytes(r);
     if (need > 0 && (!r.workspace || r.workspace_bytes < need || reinterpret_cast<uintptr_t>(r.workspace) % 256 != 0))
         return PLE_E_WORKSPACE;
-    BiasArgs a = bias_args(r, kGradRows, kGradCols);
-    a.out = r.dw;
-    if (a.tiles > 0) {
-        const dim3 grid(static_cast<unsigned>(std::min(a.tiles, kMaxGrid)));
-        const hipError_t rc = with_type(r.out_dtype, [&](auto t) {
-            hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_bias_backward_kernel<decltype(t)::value>), grid, dim3(kBlock), 0, r.stream, a);
-            return hipGetLastError();
-        });
-        if (rc != hipSuccess) return static_cast<int>(rc);
-    }
+    BiasArgs a = backward_args(r, r.out_dtype == PLE_DTYPE_F32 ? 4 : 8);
+    a.total = reinterpret_cast<float *>(static_cast<char *>(r.workspace) + partial_bytes(a));
+    const dim3 grid(static_cast<unsigned>(std::min((a.tiles + kWavesPerBlock - 1) / kWavesPerBlock, kMaxGrid)));
+    const int64_t blocks = r.H * ((2 * r.far + 1 + kWave - 1) / kWave);
+    const hipError_t rc = with_type(r.out_dtype, [&](auto t) {
+        constexpr int T = decltype(t)::value;
+        if (a.tiles > 0) {
+            if (a.k < vec_elems<T>())
+                hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_bias_backward_kernel<T, true>), grid, dim3(kBlock), 0, r.stream, a);
+            else
+                hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_bias_backward_kernel<T, false>), grid, dim3(kBlock), 0, r.stream, a);
+            const hipError_t e = hipGetLastError();
+            if (e != hipSuccess) return e;
+        }
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_bias_total_kernel<T>), dim3(static_cast<unsigned>(std::min(blocks, kMaxGrid))),
+                           dim3(kJoinThreads), 0, r.stream, a);
+        return hipGetLastError();
+    });
+    if (rc != hipSuccess) return static_cast<int>(rc);
     const int64_t units = r.H * ((r.R + kJoinRows - 1) / kJoinRows);
     hipLaunchKernelGGL(ple_bias_join_kernel, dim3(static_cast<unsigned>(std::min(units, kMaxGrid))), dim3(kJoinThreads), 0, r.stream, a);
     return static_cast<int>(hipGetLastError());

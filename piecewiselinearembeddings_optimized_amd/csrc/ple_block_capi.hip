@@ -14,6 +14,7 @@ constexpr int64_t kMaxCount = INT32_MAX;          // rows, samples, heads
 constexpr int64_t kMaxChannels = 1 << 20;
 constexpr int64_t kMaxFar = 1 << 24;
 constexpr int64_t kMaxOffset = int64_t{1} << 60;
+constexpr int64_t kMaxLength = 1 << 23;           // (a row block's offsets are 32-bit)
 
 bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
@@ -44,7 +45,7 @@ GroupRequest group_request(int64_t N, int64_t S, int64_t C, int64_t G, int dtype
 
 int check_bias(int64_t B, int64_t H, int64_t q, int64_t k, int64_t R, int64_t far, int64_t offset, bool starts) {
     if (B < 0 || H < 1 || q < 0 || k < 0 || R < 1 || far < 1 || (!starts && B != 1)) return PLE_E_BAD_SHAPE;
-    if (B > kMaxCount || H > kMaxCount || q > kMaxCount || k > kMaxCount || R > kMaxCount || far > kMaxFar ||
+    if (B > kMaxCount || H > kMaxCount || q > kMaxLength || k > kMaxLength || R > kMaxCount || far > kMaxFar ||
         offset > kMaxOffset || offset < -kMaxOffset || !product_fits({B, H, q, k}) || !product_fits({R, H}))
         return PLE_E_TOO_LARGE;
     return PLE_OK;
