@@ -590,6 +590,9 @@ int ple_grad_scale_launch(const ple_grad_t *grads, int64_t count, const float *n
  *                           for every shape it can take (also past 8 chunks)
  *   PLE_TUNE_BWD_STREAM     1: the matrix-core backward reads its gradient with
  *                           plain loads; 2: past the caches
+ *   PLE_TUNE_GROUP_POLLS    n: workgroups that share a sample of a group norm
+ *                           look n - 1 times for what another knows, before
+ *                           they compute it themselves
  * A forced value the shape cannot take is ignored.  Returns the knob's
  * previous value, or PLE_E_BAD_SHAPE for an unknown knob.  Not synchronised
  * with launches running on other threads.
@@ -608,7 +611,8 @@ enum {
     PLE_TUNE_BWD_WG_PER_CU = 10,
     PLE_TUNE_BWD_MFMA = 11,
     PLE_TUNE_BWD_STREAM = 12,
-    PLE_TUNE_COUNT = 13,
+    PLE_TUNE_GROUP_POLLS = 13,
+    PLE_TUNE_COUNT = 14,
 };
 int ple_set_tuning(int knob, int value);
 

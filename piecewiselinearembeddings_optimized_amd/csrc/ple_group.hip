@@ -17,9 +17,14 @@
 //
 // Held form: a workgroup holds a sample's groups (all, or a slab of them) in
 // registers: statistics in two passes over the registers, one read of memory.
-// Split form, for samples larger than that: sums of pieces of rows (per channel,
-// the squares about the piece's own mean), a join per group, and a second read
-// that applies it.
+// Shared form, for samples that several workgroups hold: each publishes what it knows
+// of a group and takes the others'.  A value is its own flag (a 64-bit word that is
+// not kUnknown), so nothing has to be ordered; and a workgroup that does not find
+// another's in time reads that one's rows and computes it, so no wait depends on what
+// else runs.
+// Split form, for samples larger still: sums of pieces of rows (per channel, the
+// squares about the piece's own mean), a join per group, and a second read that
+// applies it.
 
 #include <algorithm>
 
@@ -40,8 +45,8 @@ struct Piece {
 #pragma unroll
         for (int i = 0; i < kWords; ++i) w[i] = 0;
     }
-    __device__ __forceinline__ void load(const void *p, int64_t i) {
-        const char *q = static_cast<const char *>(p) + i * elem_bytes(T);
+    __device__ __forceinline__ void load(const void *p, int64_t i) { load_at(static_cast<const char *>(p) + i * elem_bytes(T)); }
+    __device__ __forceinline__ void load_at(const char *q) {
         if constexpr (W == 4) {
             const uint4 v = *reinterpret_cast<const uint4 *>(q);
             w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
@@ -52,6 +57,13 @@ struct Piece {
         }
     }
     __device__ __forceinline__ float operator[](int e) const { return grad_elem<T>(w, e); }
+    // Keeps the piece as it was loaded: without it the compiler widens 16-bit elements
+    // where they are loaded and keeps them all, twice the registers.
+    __device__ __forceinline__ void keep() {
+        if constexpr (T != PLE_DTYPE_F32)
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) asm volatile("" : "+v"(w[i]));
+    }
 };
 
 template <int T, int W>
@@ -72,8 +84,12 @@ struct GroupArgs {
     int L, slots, A, U;          // lanes of a row, rows at once of a sample, lanes of a sample, samples at once
     int slabs, Cs, Gs;           // slabs of a row, channels and groups of one
     int team;                    // lanes that join a group
-    int pieces, parts;
-    int act, param_dtype;
+    uint32_t wide_inverse;       // 2^32 / values of a group in a row, rounded up
+    int pieces;
+    uint64_t *exchange;          // shared: [units, members, Gs] what the members know of a group
+    int members, member_rows;    // shared: workgroups of a unit, rows of each
+    int polls;                   // shared: how often a member looks for another's
+    int act, param_dtype, param_vectors;
     float eps, inv;              // inv: 1 / (S P)
 };
 
@@ -81,13 +97,16 @@ struct GroupArgs {
 // activations
 // ---------------------------------------------------------------------------
 
-// Standard normal distribution and density at z.
+// Standard normal distribution and density at z.  Abramowitz and Stegun 26.2.17: the
+// tail is the density times a polynomial in 1 / (1 + p |z|), off by at most 7.5e-8.
 __device__ __forceinline__ void normal_cdf(float z, float &cdf, float &pdf) {
-    cdf = 0.5f * (1.0f + erff(z * 0.70710678118654752f));
-    pdf = 0.39894228040143268f * __expf(-0.5f * z * z);
+    pdf = 0.39894228f * __expf(-0.5f * z * z);
+    const float t = __builtin_amdgcn_rcpf(1.0f + 0.2316419f * fabsf(z));
+    const float tail = pdf * t * (0.319381530f + t * (-0.356563782f + t * (1.781477937f + t * (-1.821255978f + t * 1.330274429f))));
+    cdf = z > 0.0f ? 1.0f - tail : tail;
 }
 
-__device__ __forceinline__ float logistic(float z) { return 1.0f / (1.0f + __expf(-z)); }
+__device__ __forceinline__ float logistic(float z) { return __builtin_amdgcn_rcpf(1.0f + __expf(-z)); }
 
 template <int E>
 __device__ __forceinline__ void activate(float (&z)[E], int act) {
@@ -138,9 +157,16 @@ __device__ __forceinline__ void slopes(float (&z)[E], int act) {
 
 // A lane's place in its workgroup: sample, row slot and piece of the row.
 struct Place {
-    int unit, slot, lane;
+    int unit, slot, lane, thread;
     bool on;
-    __device__ __forceinline__ explicit Place(const GroupArgs &a) {
+    // The same, as values that the compiler takes for new ones in every turn of a loop:
+    // it would else compute the addresses of a turn before the loop, and hold them all.
+    __device__ __forceinline__ Place again() const {
+        Place q = *this;
+        asm volatile("" : "+v"(q.unit), "+v"(q.slot), "+v"(q.lane), "+v"(q.thread));
+        return q;
+    }
+    __device__ __forceinline__ explicit Place(const GroupArgs &a) : thread(threadIdx.x) {
         unit = threadIdx.x / a.A;
         const int r = threadIdx.x - unit * a.A;
         slot = r / a.L;
@@ -149,52 +175,99 @@ struct Place {
     }
 };
 
-// What a lane's channels are: their parameters, and each one's group (WHOLE: one
-// group for the whole piece).
-template <int E, bool WHOLE>
-struct Channels {
-    static constexpr int kGroups = WHOLE ? 1 : E;
-    float w[E], b[E];
-    int group[kGroups];
-    __device__ __forceinline__ Channels(const GroupArgs &a, int c0, int local) {
+// A lane's E values of a parameter from channel c0 on (`none` without one).
+template <int E>
+__device__ __forceinline__ void load_params(const GroupArgs &a, const void *p, int c0, float none, float (&v)[E]) {
+    if (!p) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const bool on = c0 + e < a.C;
-            w[e] = on && a.weight ? load_any(a.weight, c0 + e, a.param_dtype) : 1.0f;
-            b[e] = on && a.bias ? load_any(a.bias, c0 + e, a.param_dtype) : 0.0f;
-        }
+        for (int e = 0; e < E; ++e) v[e] = none;
+    } else if (E >= 4 && a.param_vectors) {
+        if (a.param_dtype == PLE_DTYPE_F32) load_vec<PLE_DTYPE_F32, E>(p, c0, v);
+        else if (a.param_dtype == PLE_DTYPE_BF16) load_vec<PLE_DTYPE_BF16, E>(p, c0, v);
+        else load_vec<PLE_DTYPE_F16, E>(p, c0, v);
+    } else {
 #pragma unroll
-        for (int e = 0; e < kGroups; ++e) group[e] = (local + e) / a.P;
+        for (int e = 0; e < E; ++e) v[e] = c0 + e < a.C ? load_any(p, c0 + e, a.param_dtype) : none;
     }
-    __device__ __forceinline__ int of(int e) const { return group[WHOLE ? 0 : e]; }
+}
+
+// The slab's parameters as 32-bit values in LDS, weights then biases.
+template <int THREADS>
+__device__ __forceinline__ void stage_params(const GroupArgs &a, int slab, float *s_params) {
+    for (int c = threadIdx.x; c < a.Cs; c += THREADS) {
+        s_params[c] = a.weight ? load_any(a.weight, slab * a.Cs + c, a.param_dtype) : 1.0f;
+        s_params[a.Cs + c] = a.bias ? load_any(a.bias, slab * a.Cs + c, a.param_dtype) : 0.0f;
+    }
+}
+
+template <int E>
+__device__ __forceinline__ void staged(const float *p, float (&v)[E]) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = p[e];
+}
+
+// A value that the compiler takes for another in every turn of a loop: it would else
+// make a copy of the loop for each activation, and hold what all of them need.
+__device__ __forceinline__ int unhoisted(int v) {
+    asm volatile("" : "+s"(v));
+    return v;
+}
+
+// The groups of a lane's channels (WHOLE: one group for the whole piece).
+template <int E, bool WHOLE>
+struct Groups {
+    static constexpr int kEach = WHOLE ? 1 : E;
+    int first;
+    uint32_t starts;             // bit e: channel e is the first of a group (e > 0)
+    __device__ __forceinline__ Groups again() const {
+        Groups q = *this;
+        asm volatile("" : "+v"(q.first), "+v"(q.starts));
+        return q;
+    }
+    __device__ __forceinline__ Groups(const GroupArgs &a, int channel) {
+        first = channel / a.P;
+        starts = 0;
+        if constexpr (!WHOLE) {
+            int r = channel - first * a.P;
+#pragma unroll
+            for (int e = 1; e < E; ++e)
+                if (++r == a.P) {
+                    r = 0;
+                    starts |= 1u << e;
+                }
+        }
+    }
+    __device__ __forceinline__ int of(int e) const { return WHOLE ? first : first + __popc(starts & ((2u << e) - 1)); }
 };
 
-// Joins the workgroup's per-lane values (WHOLE: one a lane, else one a channel)
-// over each group: the values of a group lie next to each other in LDS, a team of
-// lanes adds them, and `done(group, sum)` runs on the team's first lane.  K values
-// are joined at once.
+// A lane's values that are joined lie in LDS by value, its workgroup's lanes next to each
+// other (a few places more than lanes, so that a group's channels are in other banks).
+template <int THREADS>
+constexpr int kPlane = THREADS + 8;
+
+// Joins the workgroup's values in LDS (WHOLE: one a lane, else one a channel) over each
+// group: a team of lanes adds a group's, and `done(group, sums)` runs on the team's
+// first lane.  K values are joined at once.
 template <int K, int E, bool WHOLE, int THREADS, typename F>
-__device__ __forceinline__ void join_groups(const GroupArgs &a, const Place &p, float *lds, const float (&v)[K][WHOLE ? 1 : E],
-                                            F done) {
-    constexpr int kEach = WHOLE ? 1 : E;
-    const int per = (WHOLE ? a.P / E : a.P) * a.slots;           // values of a group
-    const int all = a.U * a.Gs;
-    const int plane = a.U * a.A * kEach;
-    if (p.on)
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-#pragma unroll
-            for (int e = 0; e < kEach; ++e)
-                lds[k * plane + p.unit * a.A * kEach + (p.lane * kEach + e) * a.slots + p.slot] = v[k][e];
+__device__ __forceinline__ void join_lds(const GroupArgs &a, const Place &p, const float *lds, F done) {
+    constexpr int kEach = WHOLE ? 1 : E, kStride = kPlane<THREADS>;
+    const int wide = WHOLE ? a.P / E : a.P;                      // values of a group in a row
+    const int per = wide * a.slots, all = a.U * a.Gs;
     __syncthreads();
-    const int lane = threadIdx.x & (a.team - 1), teams = THREADS / a.team;
+    const int lane = p.thread & (a.team - 1), teams = THREADS / a.team;
     for (int q0 = 0; q0 < all; q0 += teams) {
-        const int q = q0 + threadIdx.x / a.team;
+        const int q = q0 + p.thread / a.team;
         float s[K] = {};
-        if (q < all)
-            for (int i = lane; i < per; i += a.team)
+        if (q < all) {
+            const int unit = q / a.Gs, c0 = (q - unit * a.Gs) * wide, base = unit * a.A;
+            for (int i = lane; i < per; i += a.team) {
+                const int slot = wide == 1 ? i : static_cast<int>(__umulhi(static_cast<uint32_t>(i), a.wide_inverse));
+                const int c = c0 + i - slot * wide;
+                const int at = base + slot * a.L + c / kEach + c % kEach * kStride;
 #pragma unroll
-                for (int k = 0; k < K; ++k) s[k] += lds[k * plane + q * per + i];
+                for (int k = 0; k < K; ++k) s[k] += lds[k * kEach * kStride + at];
+            }
+        }
 #pragma unroll
         for (int k = 0; k < K; ++k) s[k] = group_sum_rt(s[k], a.team);
         if (q < all && lane == 0) done(q, s);
@@ -202,69 +275,298 @@ __device__ __forceinline__ void join_groups(const GroupArgs &a, const Place &p, 
     __syncthreads();
 }
 
-// LDS floats of the held form's workgroup.
-__host__ __device__ inline int held_floats(int threads, int each, int values, int groups) {
-    return threads * each * values + 2 * groups;
+template <int K, int E, bool WHOLE, int THREADS, typename F>
+__device__ __forceinline__ void join_groups(const GroupArgs &a, const Place &p, float *lds, const float (&v)[K][WHOLE ? 1 : E],
+                                            F done) {
+    constexpr int kEach = WHOLE ? 1 : E, kStride = kPlane<THREADS>;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) lds[(k * kEach + e) * kStride + p.thread] = v[k][e];
+    join_lds<K, E, WHOLE, THREADS>(a, p, lds, done);
 }
 
-template <int T, int W, bool WHOLE, int THREADS, int R>
-__global__ __launch_bounds__(THREADS) void ple_group_forward_kernel(GroupArgs a) {
+// The same for values that `lane_value(e, values)` computes one channel after the other: for
+// what is rarely done, in few registers.
+template <int K, int E, bool WHOLE, int THREADS, typename V, typename F>
+__device__ __forceinline__ void join_rarely(const GroupArgs &a, const Place &p, float *lds, V lane_value, F done) {
+    constexpr int kStride = kPlane<THREADS>;
+    float sum[K] = {};
+#pragma unroll 1
+    for (int e = 0; e < E; ++e) {
+        float v[K];
+        lane_value(e, v);
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            sum[k] += v[k];
+            if constexpr (!WHOLE) lds[(k * E + e) * kStride + p.thread] = v[k];
+        }
+    }
+    if constexpr (WHOLE)
+#pragma unroll
+        for (int k = 0; k < K; ++k) lds[k * kStride + p.thread] = sum[k];
+    join_lds<K, E, WHOLE, THREADS>(a, p, lds, done);
+}
+
+// What no group's values are (a computed NaN has another payload).
+constexpr uint64_t kUnknown = ~uint64_t{0};
+
+// A workgroup's rows: all of its samples' (held), or a member's share (shared).
+struct Rows {
+    int64_t n, first, count;     // sample; rows
+    __device__ __forceinline__ Rows(const GroupArgs &a, int64_t sample, int member, bool shared)
+        : n(sample), first(shared ? static_cast<int64_t>(member) * a.member_rows : 0),
+          count(shared ? min(a.S - first, static_cast<int64_t>(a.member_rows)) : a.S) {}
+};
+
+// A workgroup's slab, its first unit of work and the way to the next: held, every so
+// many samples of a slab; shared, one member of one unit, the members of a unit next to
+// each other in the grid's order.
+template <bool SHARED>
+struct Turn {
+    int slab, member;
+    int64_t block, step;
+    __device__ __forceinline__ explicit Turn(const GroupArgs &a) {
+        // (divisions leave vector registers: what follows from them is to be scalar)
+        const auto scalar = [](uint32_t v) { return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(v))); };
+        const uint32_t slabs = a.slabs;
+        if constexpr (SHARED) {
+            const uint32_t members = a.members, unit = scalar(blockIdx.x / members), at = scalar(unit / slabs);
+            member = static_cast<int>(blockIdx.x - unit * members);
+            slab = static_cast<int>(unit - at * slabs);
+            block = at;
+            step = a.blocks;
+        } else {
+            const uint32_t at = scalar(blockIdx.x / slabs);
+            member = 0;
+            slab = static_cast<int>(blockIdx.x - at * slabs);
+            block = at;
+            step = scalar(gridDim.x / slabs);
+        }
+    }
+};
+
+// Publishes a group's two values (on one lane of the workgroup).
+__device__ __forceinline__ void publish(uint64_t *to, float x, float y) {
+    uint64_t v = static_cast<uint64_t>(__float_as_uint(y)) << 32 | __float_as_uint(x);
+    if (v == kUnknown) v = 0x7fc000007fc00000u;
+    __hip_atomic_store(to, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// All members' values of the unit's groups into LDS (known[member, group]; the
+// workgroup's own are published already), and `missing(member)` -- run by the whole
+// workgroup, which then has its values there too -- for those that do not appear.
+template <int THREADS, typename F>
+__device__ __forceinline__ void collect(const GroupArgs &a, uint64_t *unit, float2 *known, int *s_late, F missing) {
+    if (threadIdx.x == 0) *s_late = 0;
+    __syncthreads();
+    const int all = a.members * a.Gs;
+    constexpr int kAtOnce = 4;
+    bool late = false;
+    for (int i0 = threadIdx.x; i0 < all; i0 += kAtOnce * THREADS) {
+        uint64_t v[kAtOnce];
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j) v[j] = i0 + j * THREADS < all ? kUnknown : 0;
+        for (int t = 0; t < a.polls; ++t) {
+            bool known_all = true;
+#pragma unroll
+            for (int j = 0; j < kAtOnce; ++j)
+                if (v[j] == kUnknown) v[j] = __hip_atomic_load(unit + i0 + j * THREADS, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+            for (int j = 0; j < kAtOnce; ++j) known_all = known_all && v[j] != kUnknown;
+            if (known_all) break;
+            __builtin_amdgcn_s_sleep(1);
+        }
+        // (kUnknown as it is: what a member computes in its place is none)
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j) {
+            if (i0 + j * THREADS >= all) continue;
+            late = late || v[j] == kUnknown;
+            known[i0 + j * THREADS] = make_float2(__uint_as_float(static_cast<uint32_t>(v[j])), __uint_as_float(static_cast<uint32_t>(v[j] >> 32)));
+        }
+    }
+    if (late) *s_late = 1;
+    __syncthreads();
+    if (*s_late == 0) return;
+    for (int m = 0; m < a.members; ++m) {
+        bool gone = false;
+        for (int g = 0; g < a.Gs; ++g)
+            gone = gone || (__float_as_uint(known[m * a.Gs + g].x) == ~0u && __float_as_uint(known[m * a.Gs + g].y) == ~0u);
+        __syncthreads();
+        if (gone) missing(m);
+        __syncthreads();
+    }
+}
+
+// Sums of a lane's values, by group where a piece is of one.
+template <int T, int W, bool WHOLE>
+__device__ __forceinline__ void add_piece(const Piece<T, W> &x, float (&v)[WHOLE ? 1 : Piece<T, W>::kElems]) {
+#pragma unroll
+    for (int e = 0; e < Piece<T, W>::kElems; ++e) v[WHOLE ? 0 : e] += x[e];
+}
+
+template <int T, int W, bool WHOLE>
+__device__ __forceinline__ void add_squares(const Piece<T, W> &x, const float (&mean)[WHOLE ? 1 : Piece<T, W>::kElems],
+                                            float (&v)[WHOLE ? 1 : Piece<T, W>::kElems]) {
+#pragma unroll
+    for (int e = 0; e < Piece<T, W>::kElems; ++e) {
+        const float d = x[e] - mean[WHOLE ? 0 : e];
+        v[WHOLE ? 0 : e] += d * d;
+    }
+}
+
+// LDS of the held and shared forms' workgroup, in floats: values to be joined, two a
+// group, two a member's group (shared), and two a channel.
+__host__ __device__ inline int held_floats(int threads, int values, int groups, int known, int channels) {
+    return (threads + 8) * values + 2 * groups + 2 * known + 4 + 2 * channels;
+}
+
+// Waves a SIMD that the held form is compiled for: registers for the pieces, and a
+// second workgroup a CU (a third, of 256 threads) to load while one computes.
+constexpr int held_waves(int threads) { return threads == 512 ? 4 : threads == 256 ? 3 : 2; }
+
+template <int T, int W, bool WHOLE, int THREADS, int R, bool SHARED>
+__global__ __launch_bounds__(THREADS, held_waves(THREADS)) void ple_group_forward_kernel(GroupArgs a) {
     constexpr int E = Piece<T, W>::kElems, kEach = WHOLE ? 1 : E;
-    extern __shared__ float s_lds[];
-    float *const s_mean = s_lds + a.U * a.A * kEach, *const s_rho = s_mean + a.U * a.Gs;
-    const Place p(a);
-    const int slab = blockIdx.x % a.slabs;
-    const int c0 = slab * a.Cs + p.lane * E;
-    const Channels<E, WHOLE> ch(a, c0, p.lane * E);
-    for (int64_t blk = blockIdx.x / a.slabs; blk < a.blocks; blk += gridDim.x / a.slabs) {
-        const int64_t n = blk * a.U + p.unit;
-        const bool on = p.on && n < a.N;
-        const int64_t first = (n * a.S + p.slot) * a.C + c0, step = static_cast<int64_t>(a.slots) * a.C;
+    extern __shared__ float4 s_all[];
+    float *const s_lds = reinterpret_cast<float *>(s_all);
+    float *const s_mean = s_lds + kPlane<THREADS> * kEach, *const s_rho = s_mean + a.U * a.Gs;
+    float2 *const s_known = reinterpret_cast<float2 *>(s_rho + a.U * a.Gs);
+    int *const s_late = reinterpret_cast<int *>(s_known + a.members * a.Gs);
+    float *const s_params = reinterpret_cast<float *>(s_late + 4);
+    const Place here(a);
+    const Turn<SHARED> turn(a);
+    const int slab = turn.slab, member = turn.member;
+    stage_params<THREADS>(a, slab, s_params);
+    const Groups<E, WHOLE> there(a, here.lane * E);
+    for (int64_t blk = turn.block; blk < a.blocks; blk += turn.step) {
+        const int64_t first_n = SHARED ? blk : blk * a.U;
+        const int act = unhoisted(a.act);
+        const Place p = here.again();
+        const Groups<E, WHOLE> groups = there.again();
+        const int own = !SHARED && p.on ? p.unit * a.Gs : 0;         // the sample's groups in LDS
+        const float *const own_params = s_params + (p.on ? p.lane * E : 0);
+        const uint32_t at = static_cast<uint32_t>((((SHARED ? 0 : p.unit * a.S) + p.slot) * a.C + p.lane * E) * elem_bytes(T));
+        const Rows rows(a, SHARED ? first_n : first_n + p.unit, member, SHARED);
+        // byte offsets: the workgroup's rows (the same for all lanes), the lane's place in them
+        const int64_t base = ((first_n * a.S + rows.first) * a.C + slab * a.Cs) * elem_bytes(T);
+        const int64_t step = static_cast<int64_t>(a.slots) * a.C * elem_bytes(T);
+        const char *const px = static_cast<const char *>(a.x) + base;
+        char *const py = static_cast<char *>(a.y) + base;
+        const int count = p.on && rows.n < a.N ? static_cast<int>(rows.count) - p.slot : 0;
+        const auto has = [&](int k) { return k * a.slots < count; };
         Piece<T, W> x[R];
 #pragma unroll
         for (int k = 0; k < R; ++k) {
             x[k].clear();
-            if (on && p.slot + k * a.slots < a.S) x[k].load(a.x, first + k * step);
+            if (has(k)) x[k].load_at(px + k * step + at);
         }
         float v[1][kEach] = {};
 #pragma unroll
-        for (int k = 0; k < R; ++k)
-#pragma unroll
-            for (int e = 0; e < E; ++e) v[0][WHOLE ? 0 : e] += x[k][e];
-        join_groups<1, E, WHOLE, THREADS>(a, p, s_lds, v, [&](int q, const float (&s)[1]) { s_mean[q] = s[0] * a.inv; });
+        for (int k = 0; k < R; ++k) {
+            x[k].keep();
+            add_piece<T, W, WHOLE>(x[k], v[0]);
+        }
+        const float inv = SHARED ? 1.0f / (static_cast<float>(rows.count) * static_cast<float>(a.P)) : a.inv;
+        join_groups<1, E, WHOLE, THREADS>(a, p, s_lds, v, [&](int q, const float (&s)[1]) {
+            s_rho[q] = s[0];
+            s_mean[q] = s[0] * inv;
+        });
         float mean[kEach];
 #pragma unroll
         for (int e = 0; e < kEach; ++e) {
-            mean[e] = p.on ? s_mean[p.unit * a.Gs + ch.group[e]] : 0.0f;
+            mean[e] = s_mean[own + groups.of(e)];
             v[0][e] = 0.0f;
         }
 #pragma unroll
-        for (int k = 0; k < R; ++k)
-            if (p.slot + k * a.slots < a.S)
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const float d = x[k][e] - mean[WHOLE ? 0 : e];
-                    v[0][WHOLE ? 0 : e] += d * d;
+        for (int k = 0; k < R; ++k) {
+            x[k].keep();
+            __builtin_amdgcn_sched_barrier(0);
+            if (has(k)) add_squares<T, W, WHOLE>(x[k], mean, v[0]);
+        }
+        if constexpr (!SHARED) {
+            join_groups<1, E, WHOLE, THREADS>(a, p, s_lds, v, [&](int q, const float (&s)[1]) {
+                const float rho = rsqrtf(s[0] * a.inv + a.eps);
+                s_rho[q] = rho;
+                const int u = q / a.Gs;
+                const int64_t sample = first_n + u;
+                if (sample < a.N) a.stats[sample * a.G + slab * a.Gs + (q - u * a.Gs)] = make_float2(s_mean[q], rho);
+            });
+        } else {
+            uint64_t *const unit = a.exchange + (rows.n * a.slabs + slab) * a.members * a.Gs;
+            join_groups<1, E, WHOLE, THREADS>(a, p, s_lds, v, [&](int q, const float (&s)[1]) {
+                publish(unit + member * a.Gs + q, s_rho[q], s[0]);
+            });
+            collect<THREADS>(a, unit, s_known, s_late, [&](int m) {
+                // the other member's rows
+                const Rows other(a, rows.n, m, true);
+                const char *const po = px + (other.first - rows.first) * a.C * elem_bytes(T) + at;
+                const int there = p.on ? static_cast<int>(other.count) - p.slot : 0;
+                const float share = 1.0f / (static_cast<float>(other.count) * static_cast<float>(a.P));
+                join_rarely<1, E, WHOLE, THREADS>(a, p, s_lds, [&](int e, float (&t)[1]) {
+                    t[0] = 0.0f;
+                    for (int k = 0; k * a.slots < there; ++k) t[0] += load_grad<T>(po + k * step, e);
+                }, [&](int q, const float (&s)[1]) {
+                    s_rho[q] = s[0];
+                    s_mean[q] = s[0] * share;
+                });
+                join_rarely<1, E, WHOLE, THREADS>(a, p, s_lds, [&](int e, float (&t)[1]) {
+                    t[0] = 0.0f;
+                    const float mu = s_mean[own + groups.of(e)];
+                    for (int k = 0; k * a.slots < there; ++k) {
+                        const float d = load_grad<T>(po + k * step, e) - mu;
+                        t[0] += d * d;
+                    }
+                }, [&](int q, const float (&s)[1]) { s_known[m * a.Gs + q] = make_float2(s_rho[q], s[0]); });
+            });
+            // the unit's mean, and its squares about it: the members' own, and their means' distance
+            const int lane = p.thread & (a.team - 1);
+            for (int q0 = 0; q0 < a.Gs; q0 += THREADS / a.team) {
+                const int q = q0 + p.thread / a.team;
+                float t = 0.0f;
+                if (q < a.Gs)
+                    for (int m = lane; m < a.members; m += a.team) t += s_known[m * a.Gs + q].x;
+                const float mu = group_sum_rt(t, a.team) * a.inv;
+                t = 0.0f;
+                if (q < a.Gs)
+                    for (int m = lane; m < a.members; m += a.team) {
+                        const float2 s = s_known[m * a.Gs + q];
+                        const float n = static_cast<float>(min(a.S - static_cast<int64_t>(m) * a.member_rows,
+                                                               static_cast<int64_t>(a.member_rows))) * static_cast<float>(a.P);
+                        const float d = s.x / n - mu;
+                        t += s.y + n * d * d;
+                    }
+                t = group_sum_rt(t, a.team);
+                if (q < a.Gs && lane == 0) {
+                    const float rho = rsqrtf(t * a.inv + a.eps);
+                    s_mean[q] = mu;
+                    s_rho[q] = rho;
+                    if (member == 0) a.stats[rows.n * a.G + slab * a.Gs + q] = make_float2(mu, rho);
                 }
-        join_groups<1, E, WHOLE, THREADS>(a, p, s_lds, v, [&](int q, const float (&s)[1]) {
-            const float rho = rsqrtf(s[0] * a.inv + a.eps);
-            s_rho[q] = rho;
-            const int u = q / a.Gs;
-            const int64_t sample = blk * a.U + u;
-            if (sample < a.N) a.stats[sample * a.G + slab * a.Gs + (q - u * a.Gs)] = make_float2(s_mean[q], rho);
-        });
-        float scale[E];
+            }
+            __syncthreads();
 #pragma unroll
-        for (int e = 0; e < E; ++e) scale[e] = (p.on ? s_rho[p.unit * a.Gs + ch.of(e)] : 0.0f) * ch.w[e];
+            for (int e = 0; e < kEach; ++e) mean[e] = s_mean[own + groups.of(e)];
+        }
+        float scale[E], bias[E];
+        staged(own_params, scale);
+        staged(own_params + a.Cs, bias);
 #pragma unroll
-        for (int k = 0; k < R; ++k)
-            if (on && p.slot + k * a.slots < a.S) {
+        for (int e = 0; e < E; ++e) scale[e] *= s_rho[own + groups.of(e)];
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+            x[k].keep();
+            __builtin_amdgcn_sched_barrier(0);
+            if (has(k)) {
                 float z[E];
 #pragma unroll
-                for (int e = 0; e < E; ++e) z[e] = (x[k][e] - mean[WHOLE ? 0 : e]) * scale[e] + ch.b[e];
-                activate(z, a.act);
-                store_piece<T, W>(a.y, first + k * step, z);
+                for (int e = 0; e < E; ++e) z[e] = (x[k][e] - mean[WHOLE ? 0 : e]) * scale[e] + bias[e];
+                activate(z, act);
+                store_piece<T, W>(py + k * step + at, 0, z);
             }
+        }
+        if constexpr (SHARED) break;
+        __syncthreads();             // (s_mean and s_rho are read before the next samples')
     }
 }
 
@@ -272,103 +574,234 @@ __global__ __launch_bounds__(THREADS) void ple_group_forward_kernel(GroupArgs a)
 template <int E, int THREADS>
 __device__ __forceinline__ void leave_sums(const GroupArgs &a, const Place &p, float *lds, const float (&v)[2][E], int slab,
                                            int64_t part) {
+    constexpr int kStride = kPlane<THREADS>;
     const int rows = a.U * a.slots;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
         __syncthreads();
-        if (p.on)
 #pragma unroll
-            for (int e = 0; e < E; ++e) lds[(p.lane * E + e) * rows + p.unit * a.slots + p.slot] = v[k][e];
+        for (int e = 0; e < E; ++e) lds[e * kStride + p.thread] = v[k][e];
         __syncthreads();
-        for (int c = threadIdx.x; c < a.Cs; c += THREADS) {
+        for (int c = p.thread; c < a.Cs; c += THREADS) {
             float s = 0.0f;
-            for (int i = 0; i < rows; ++i) s += lds[c * rows + i];
+            for (int i = 0; i < rows; ++i) s += lds[c % E * kStride + i * a.L + c / E];
             a.partial[(part * 2 + k) * a.C + slab * a.Cs + c] = s;
         }
     }
 }
 
-template <int T, int W, bool WHOLE, int THREADS, int R>
-__global__ __launch_bounds__(THREADS) void ple_group_backward_kernel(GroupArgs a) {
-    constexpr int E = Piece<T, W>::kElems, kEach = WHOLE ? 1 : E;
-    extern __shared__ float s_lds[];
-    float *const s_m1 = s_lds + 2 * a.U * a.A * kEach, *const s_m2 = s_m1 + a.U * a.Gs;
-    const Place p(a);
-    const int slab = blockIdx.x % a.slabs;
-    const int c0 = slab * a.Cs + p.lane * E;
-    const Channels<E, WHOLE> ch(a, c0, p.lane * E);
+// What a lane's channels are multiplied with: z = x scale + shift.  (Folded so that a
+// lane holds two values a channel; the products' roundings are of the size that the
+// mean's own has.)
+template <int E, bool WHOLE>
+struct Affine {
+    float scale[E], shift[E];
+    __device__ __forceinline__ Affine(const float *weight, const float *bias, const float2 *stats, const Groups<E, WHOLE> &groups) {
+        staged(weight, scale);
+        staged(bias, shift);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const float2 st = stats[groups.of(e)];
+            scale[e] *= st.y;
+            shift[e] -= st.x * scale[e];
+        }
+    }
+};
+
+// A piece's gradient before the activation.
+template <int T, int W, int E>
+__device__ __forceinline__ void piece_grad(int act, const Piece<T, W> &x, const Piece<T, W> &g, const float (&scale)[E],
+                                           const float (&shift)[E], float (&dz)[E]) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) dz[e] = x[e] * scale[e] + shift[e];
+    slopes(dz, act);
+#pragma unroll
+    for (int e = 0; e < E; ++e) dz[e] *= g[e];
+}
+
+// Sums of dz and dz x of a lane's channels -> of dz and dz xh.
+template <int E, bool WHOLE>
+__device__ __forceinline__ void standard_sums(const float2 *stats, const Groups<E, WHOLE> &groups, float (&sum)[2][E]) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const float2 st = stats[groups.of(e)];
+        sum[1][e] = st.y * (sum[1][e] - st.x * sum[0][e]);
+    }
+}
+
+// ... weighted, by group where a piece is of one.
+template <int E, bool WHOLE>
+__device__ __forceinline__ void weigh_sums(const float *weight, const float (&sum)[2][E], float (&v)[2][WHOLE ? 1 : E]) {
+    float w[E];
+    staged(weight, w);
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[j][WHOLE ? 0 : e] += sum[j][e] * w[e];
+}
+
+template <int T, int W, bool WHOLE, int THREADS, int R, bool SHARED>
+__global__ __launch_bounds__(THREADS, THREADS == 256 ? 3 : 2) void ple_group_backward_kernel(GroupArgs a) {
+    constexpr int E = Piece<T, W>::kElems, kEach = WHOLE ? 1 : E, kValues = 2 * kEach > E ? 2 * kEach : E;
+    extern __shared__ float4 s_all[];
+    float *const s_lds = reinterpret_cast<float *>(s_all);
+    float *const s_m1 = s_lds + kPlane<THREADS> * kValues, *const s_m2 = s_m1 + a.U * a.Gs;
+    float2 *const s_known = reinterpret_cast<float2 *>(s_m2 + a.U * a.Gs);
+    int *const s_late = reinterpret_cast<int *>(s_known + a.members * a.Gs);
+    float *const s_params = reinterpret_cast<float *>(s_late + 4);
+    const Place here(a);
+    const Turn<SHARED> turn(a);
+    const int slab = turn.slab, member = turn.member;
+    stage_params<THREADS>(a, slab, s_params);
+    __syncthreads();
+    const Groups<E, WHOLE> there(a, here.lane * E);
     float all[2][E] = {};
-    for (int64_t blk = blockIdx.x / a.slabs; blk < a.blocks; blk += gridDim.x / a.slabs) {
-        const int64_t n = blk * a.U + p.unit;
-        const bool on = p.on && n < a.N;
-        const int64_t first = (n * a.S + p.slot) * a.C + c0, step = static_cast<int64_t>(a.slots) * a.C;
+    for (int64_t blk = turn.block; blk < a.blocks; blk += turn.step) {
+        const int64_t first_n = SHARED ? blk : blk * a.U;
+        const int act = unhoisted(a.act);
+        const Place p = here.again();
+        const Groups<E, WHOLE> groups = there.again();
+        const int own = !SHARED && p.on ? p.unit * a.Gs : 0;         // the sample's groups in LDS
+        const float *const own_params = s_params + (p.on ? p.lane * E : 0);
+        const uint32_t at = static_cast<uint32_t>((((SHARED ? 0 : p.unit * a.S) + p.slot) * a.C + p.lane * E) * elem_bytes(T));
+        const Rows rows(a, SHARED ? first_n : first_n + p.unit, member, SHARED);
+        const int64_t base = ((first_n * a.S + rows.first) * a.C + slab * a.Cs) * elem_bytes(T);
+        const int64_t step = static_cast<int64_t>(a.slots) * a.C * elem_bytes(T);
+        const char *const px = static_cast<const char *>(a.x) + base;
+        const char *const pg = static_cast<const char *>(a.g) + base;
+        char *const py = static_cast<char *>(a.y) + base;
+        const int count = p.on && rows.n < a.N ? static_cast<int>(rows.count) - p.slot : 0;
+        const auto has = [&](int k) { return k * a.slots < count; };
+        // (lanes without rows read the statistics of the last sample's)
+        const float2 *const stats = a.stats + (SHARED ? first_n : min(p.on ? rows.n : first_n, a.N - 1)) * a.G + slab * a.Gs;
         Piece<T, W> x[R], g[R];
 #pragma unroll
         for (int k = 0; k < R; ++k) {
             x[k].clear();
             g[k].clear();
-            if (on && p.slot + k * a.slots < a.S) {
-                x[k].load(a.x, first + k * step);
-                g[k].load(a.g, first + k * step);
+            if (has(k)) {
+                x[k].load_at(px + k * step + at);
+                g[k].load_at(pg + k * step + at);
             }
         }
-        float2 st[kEach];
-#pragma unroll
-        for (int e = 0; e < kEach; ++e)
-            st[e] = on ? a.stats[n * a.G + slab * a.Gs + ch.group[e]] : make_float2(0.0f, 0.0f);
         float sum[2][E] = {};
-        float dz[R][E];
+        {
+            const Affine<E, WHOLE> f(own_params, own_params + a.Cs, stats, groups);
 #pragma unroll
-        for (int k = 0; k < R; ++k) {
-            float xh[E];
+            for (int k = 0; k < R; ++k) {
+                x[k].keep();
+                g[k].keep();
+                __builtin_amdgcn_sched_barrier(0);
+                // (a row that is not there has a gradient of 0)
+                float dz[E];
+                piece_grad<T, W>(act, x[k], g[k], f.scale, f.shift, dz);
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                xh[e] = (x[k][e] - st[WHOLE ? 0 : e].x) * st[WHOLE ? 0 : e].y;
-                dz[k][e] = xh[e] * ch.w[e] + ch.b[e];
-            }
-            slopes(dz[k], a.act);
-            const bool row = on && p.slot + k * a.slots < a.S;
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                dz[k][e] = row ? dz[k][e] * g[k][e] : 0.0f;
-                sum[0][e] += dz[k][e];
-                sum[1][e] += row ? dz[k][e] * xh[e] : 0.0f;
+                for (int e = 0; e < E; ++e) {
+                    sum[0][e] += dz[e];
+                    sum[1][e] += dz[e] * x[k][e];
+                    // (here, and not where the sums are used: the terms would all be held)
+                    asm volatile("" : "+v"(sum[0][e]), "+v"(sum[1][e]));
+                    // (a 32-bit gradient's place takes dz; a 16-bit one's is computed again)
+                    if constexpr (T == PLE_DTYPE_F32) g[k].w[e] = __float_as_uint(dz[e]);
+                }
             }
         }
-        float v[2][kEach] = {};
+        standard_sums<E, WHOLE>(stats, groups, sum);
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                all[j][e] += sum[j][e];
-                v[j][WHOLE ? 0 : e] += sum[j][e] * ch.w[e];
-            }
-        if (a.y) {
+            for (int e = 0; e < E; ++e) all[j][e] += sum[j][e];
+        if (!a.y) {
+            if constexpr (SHARED) break;
+            continue;
+        }
+        float v[2][kEach] = {};
+        weigh_sums<E, WHOLE>(own_params, sum, v);
+        if constexpr (!SHARED) {
             join_groups<2, E, WHOLE, THREADS>(a, p, s_lds, v, [&](int q, const float (&s)[2]) {
                 s_m1[q] = s[0] * a.inv;
                 s_m2[q] = s[1] * a.inv;
             });
-            float m1[kEach], m2[kEach];
+        } else {
+            uint64_t *const unit = a.exchange + (rows.n * a.slabs + slab) * a.members * a.Gs;
+            join_groups<2, E, WHOLE, THREADS>(a, p, s_lds, v, [&](int q, const float (&s)[2]) {
+                publish(unit + member * a.Gs + q, s[0], s[1]);
+            });
+            collect<THREADS>(a, unit, s_known, s_late, [&](int m) {
+                const Rows other(a, rows.n, m, true);
+                const int64_t away = (other.first - rows.first) * a.C * elem_bytes(T) + at;
+                const int there = p.on ? static_cast<int>(other.count) - p.slot : 0;
+                join_rarely<2, E, WHOLE, THREADS>(a, p, s_lds, [&](int e, float (&t)[2]) {
+                    const float2 st = stats[groups.of(e)];
+                    const float w = own_params[e], scale[1] = {w * st.y}, shift[1] = {own_params[a.Cs + e] - st.x * scale[0]};
+                    t[0] = t[1] = 0.0f;
+                    for (int k = 0; k * a.slots < there; ++k) {
+                        const float v = load_grad<T>(px + away + k * step, e);
+                        float dz[1] = {v * scale[0] + shift[0]};
+                        slopes(dz, act);
+                        dz[0] *= load_grad<T>(pg + away + k * step, e);
+                        t[0] += dz[0];
+                        t[1] += dz[0] * v;
+                    }
+                    t[1] = st.y * (t[1] - st.x * t[0]) * w;
+                    t[0] *= w;
+                }, [&](int q, const float (&r)[2]) { s_known[m * a.Gs + q] = make_float2(r[0], r[1]); });
+            });
+            const int lane = p.thread & (a.team - 1);
+            for (int q0 = 0; q0 < a.Gs; q0 += THREADS / a.team) {
+                const int q = q0 + p.thread / a.team;
+                float t = 0.0f, u = 0.0f;
+                if (q < a.Gs)
+                    for (int m = lane; m < a.members; m += a.team) {
+                        t += s_known[m * a.Gs + q].x;
+                        u += s_known[m * a.Gs + q].y;
+                    }
+                t = group_sum_rt(t, a.team);
+                u = group_sum_rt(u, a.team);
+                if (q < a.Gs && lane == 0) {
+                    s_m1[q] = t * a.inv;
+                    s_m2[q] = u * a.inv;
+                }
+            }
+            __syncthreads();
+        }
+        // dx = dz scale + x along + level
+        const Affine<E, WHOLE> f(own_params, own_params + a.Cs, stats, groups);
+        float along[kEach], level[kEach];
 #pragma unroll
-            for (int e = 0; e < kEach; ++e) {
-                m1[e] = p.on ? s_m1[p.unit * a.Gs + ch.group[e]] : 0.0f;
-                m2[e] = p.on ? s_m2[p.unit * a.Gs + ch.group[e]] : 0.0f;
+        for (int e = 0; e < kEach; ++e) {
+            const float2 st = stats[groups.of(e)];
+            const int q = own + groups.of(e);
+            along[e] = -st.y * st.y * s_m2[q];
+            level[e] = -st.y * s_m1[q] - along[e] * st.x;
+        }
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+            x[k].keep();
+            g[k].keep();
+            __builtin_amdgcn_sched_barrier(0);
+            float dz[E];
+            if constexpr (T == PLE_DTYPE_F32) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) dz[e] = g[k][e];
+            } else {
+                piece_grad<T, W>(act, x[k], g[k], f.scale, f.shift, dz);
             }
 #pragma unroll
-            for (int k = 0; k < R; ++k)
-                if (on && p.slot + k * a.slots < a.S) {
-                    float d[E];
-#pragma unroll
-                    for (int e = 0; e < E; ++e) {
-                        const float2 s = st[WHOLE ? 0 : e];
-                        const float xh = (x[k][e] - s.x) * s.y;
-                        d[e] = s.y * (dz[k][e] * ch.w[e] - m1[WHOLE ? 0 : e] - xh * m2[WHOLE ? 0 : e]);
-                    }
-                    store_piece<T, W>(a.y, first + k * step, d);
-                }
+            for (int e = 0; e < E; ++e)
+                dz[e] = dz[e] * f.scale[e] + (x[k][e] * along[WHOLE ? 0 : e] + level[WHOLE ? 0 : e]);
+            if (has(k)) store_piece<T, W>(py + k * step + at, 0, dz);
         }
+        if constexpr (SHARED) break;
+        __syncthreads();
     }
-    if (a.partial) leave_sums<E, THREADS>(a, p, s_lds, all, slab, blockIdx.x / a.slabs);
+    if (a.partial) leave_sums<E, THREADS>(a, here.again(), s_lds, all, slab, SHARED ? turn.block * a.members + member : turn.block);
+}
+
+// Clears the words that members exchange.
+__global__ __launch_bounds__(kBlock) void ple_group_unknown_kernel(uint64_t *p, int64_t n) {
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * kBlock)
+        p[i] = kUnknown;
 }
 
 // ---------------------------------------------------------------------------
@@ -395,6 +828,19 @@ struct Split {
         c0 = slab * a.Cs + lane * E;
         on = slot < a.slots && c0 < a.C;
     }
+};
+
+// A lane's channels of the split form: their parameters and groups.
+template <int E>
+struct SplitChannels {
+    float w[E], b[E];
+    Groups<E, false> groups;
+    int last;
+    __device__ __forceinline__ SplitChannels(const GroupArgs &a, int c0) : groups(a, c0), last(a.G - 1) {
+        load_params(a, a.weight, c0, 1.0f, w);
+        load_params(a, a.bias, c0, 0.0f, b);
+    }
+    __device__ __forceinline__ int of(int e) const { return min(groups.of(e), last); }
 };
 
 // Sums over the workgroup's row slots of a value a channel, to `done(channel, sum)`.
@@ -499,11 +945,11 @@ __global__ __launch_bounds__(kBlock) void ple_group_apply_kernel(GroupArgs a) {
     for (int64_t blk = blockIdx.x; blk < a.blocks; blk += gridDim.x) {
         const Split p(a, E, blk);
         if (!p.on) continue;
-        const Channels<E, false> ch(a, p.c0, p.c0);
+        const SplitChannels<E> ch(a, p.c0);
         float mean[E], scale[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const float2 s = a.stats[p.n * a.G + min(ch.of(e), a.G - 1)];
+            const float2 s = a.stats[p.n * a.G + ch.of(e)];
             mean[e] = s.x;
             scale[e] = s.y * ch.w[e];
         }
@@ -531,12 +977,12 @@ __global__ __launch_bounds__(kBlock) void ple_group_backward_sums_kernel(GroupAr
     float *const s_sum = s_lds + a.slots * a.Cs;
     for (int64_t blk = blockIdx.x; blk < a.blocks; blk += gridDim.x) {
         const Split p(a, E, blk);
-        const Channels<E, false> ch(a, p.c0, p.c0);
+        const SplitChannels<E> ch(a, p.c0);
         float v[E] = {}, u[E] = {};
         if (p.on) {
             float2 st[E];
 #pragma unroll
-            for (int e = 0; e < E; ++e) st[e] = a.stats[p.n * a.G + min(ch.of(e), a.G - 1)];
+            for (int e = 0; e < E; ++e) st[e] = a.stats[p.n * a.G + ch.of(e)];
             Piece<T, W> x[kSplitRows], g[kSplitRows];
 #pragma unroll
             for (int k = 0; k < kSplitRows; ++k)
@@ -617,12 +1063,12 @@ __global__ __launch_bounds__(kBlock) void ple_group_backward_apply_kernel(GroupA
     for (int64_t blk = blockIdx.x; blk < a.blocks; blk += gridDim.x) {
         const Split p(a, E, blk);
         if (!p.on) continue;
-        const Channels<E, false> ch(a, p.c0, p.c0);
+        const SplitChannels<E> ch(a, p.c0);
         float2 st[E], m[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            st[e] = a.stats[p.n * a.G + min(ch.of(e), a.G - 1)];
-            m[e] = a.means[p.n * a.G + min(ch.of(e), a.G - 1)];
+            st[e] = a.stats[p.n * a.G + ch.of(e)];
+            m[e] = a.means[p.n * a.G + ch.of(e)];
         }
         Piece<T, W> x[kSplitRows], g[kSplitRows];
 #pragma unroll
@@ -653,8 +1099,6 @@ __global__ __launch_bounds__(kBlock) void ple_group_backward_apply_kernel(GroupA
 // the parameters' gradients
 // ---------------------------------------------------------------------------
 
-constexpr int kJoinWaves = 16;
-
 struct ParamJoin {
     const float *sums;           // sum k (0: dz, 1: dz xh) of channel c of a part: sums[part * part_stride + k * sum_stride + c * step]
     void *bias, *weight;
@@ -662,21 +1106,25 @@ struct ParamJoin {
     int step, C, param_dtype;
 };
 
-// 64 channels a workgroup, its waves a part each in turn; blockIdx.y: which sum
-__global__ __launch_bounds__(kJoinWaves * kWave) void ple_group_param_kernel(ParamJoin a) {
-    __shared__ float s_sum[kJoinWaves * kWave];
-    const int wave = threadIdx.x / kWave, c = blockIdx.x * kWave + threadIdx.x % kWave, k = blockIdx.y;
+// 16 channels a workgroup, its 64 rows of lanes a part each in turn; blockIdx.y: which sum
+constexpr int kParamChannels = 16, kParamThreads = 1024;
+
+__global__ __launch_bounds__(kParamThreads) void ple_group_param_kernel(ParamJoin a) {
+    constexpr int kRows = kParamThreads / kParamChannels;
+    __shared__ float s_sum[kParamThreads];
+    const int row = threadIdx.x / kParamChannels, c = blockIdx.x * kParamChannels + threadIdx.x % kParamChannels, k = blockIdx.y;
     float v = 0.0f;
     if (c < a.C) {
 #pragma unroll 8
-        for (int64_t p = wave; p < a.parts; p += kJoinWaves)
+        for (int64_t p = row; p < a.parts; p += kRows)
             v += a.sums[p * a.part_stride + k * a.sum_stride + static_cast<int64_t>(c) * a.step];
     }
     s_sum[threadIdx.x] = v;
     __syncthreads();
     void *const out = k == 0 ? a.bias : a.weight;
-    if (wave == 0 && c < a.C && out) {
-        for (int w = 1; w < kJoinWaves; ++w) v += s_sum[w * kWave + threadIdx.x];
+    if (row == 0 && c < a.C && out) {
+#pragma unroll 8
+        for (int r = 1; r < kRows; ++r) v += s_sum[r * kParamChannels + threadIdx.x];
         store_any(out, c, v, a.param_dtype);
     }
 }
@@ -688,11 +1136,12 @@ __global__ __launch_bounds__(kJoinWaves * kWave) void ple_group_param_kernel(Par
 struct GroupPlan {
     int words;                   // a lane's piece: 4, 1 or 0 dwords
     int E;
-    bool whole, held;
+    bool whole, held, shared;    // held: also where it is shared
     int threads, rows;           // held: threads and rows a lane (both compile-time)
     int L, slots, U, slabs, Cs, Gs, team, pieces;
+    int members, member_rows;
     int64_t blocks, parts;
-    size_t lds, o_sums, o_channels, o_means, bytes;
+    size_t lds, o_exchange, o_channels, o_means, bytes;
 };
 
 // The widest piece that divides a row's slab and its address.
@@ -705,60 +1154,81 @@ int piece_words(int dtype, int64_t channels, bool aligned16, bool aligned4) {
 
 int piece_elems(int dtype, int words) { return words == 0 ? 1 : (dtype == PLE_DTYPE_F32 ? words : 2 * words); }
 
-// The workgroups and rows a lane of the held form.
+// The workgroups and pieces a lane of the held form, for pieces of 4 dwords (narrower
+// ones: four times as many of them).  The last is the shared form's.
 struct HeldShape {
     int threads, rows;
 };
-constexpr HeldShape kForwardShapes[] = {{64, 4}, {64, 16}, {256, 16}, {1024, 16}};
-constexpr HeldShape kBackwardShapes[] = {{64, 4}, {256, 4}, {256, 8}, {512, 8}};
+constexpr HeldShape kForwardShapes[] = {{64, 4}, {64, 16}, {256, 16}, {512, 16}};
+constexpr HeldShape kBackwardShapes[] = {{64, 4}, {64, 8}, {256, 4}, {256, 8}};
+constexpr int kShapes = 4;
+constexpr int kMaxMembers = 320;         // of a unit: fewer than workgroups run at once
+constexpr int kMaxKnown = 4096;          // groups of all members
 
-// The smallest workgroup that holds S rows of Cs channels, or false.
-bool held_shape(const HeldShape *shapes, int count, int64_t S, int L, HeldShape &out, int &slots) {
-    for (int i = 0; i < count; ++i) {
-        if (L > shapes[i].threads) continue;
-        const int64_t at_once = std::min<int64_t>(S, shapes[i].threads / L);
-        if (at_once * shapes[i].rows < S) continue;
-        out = shapes[i];
-        slots = static_cast<int>((S + shapes[i].rows - 1) / shapes[i].rows);      // as few as hold them ...
-        slots = static_cast<int>(std::max<int64_t>(slots, at_once));              // ... but as many as there are lanes for
-        return true;
+constexpr int rows_of(const HeldShape &s, int words) { return words == 4 ? s.rows : 4 * s.rows; }
+
+// The slab of gs groups as a workgroup's: false where its lanes or LDS do not fit.
+bool hold(const GroupRequest &r, bool backward, int64_t gs, bool aligned16, bool aligned4, const HeldShape &shape, bool share,
+          GroupPlan &p) {
+    const int64_t P = r.C / r.G, Cs = gs * P;
+    p.words = piece_words(r.dtype, gs < r.G ? Cs : r.C, aligned16 && (gs == r.G || r.C * elem_bytes(r.dtype) % 16 == 0),
+                          aligned4 && (gs == r.G || r.C * elem_bytes(r.dtype) % 4 == 0));
+    p.E = piece_elems(r.dtype, p.words);
+    const int64_t L = Cs / p.E;
+    if (L > shape.threads) return false;
+    p.whole = p.E != 2 && P % p.E == 0;          // (with_held's kernels)
+    p.threads = shape.threads;
+    p.rows = rows_of(shape, p.words);
+    p.L = static_cast<int>(L);
+    p.slots = static_cast<int>(std::min<int64_t>(r.S, shape.threads / L));
+    p.slabs = static_cast<int>(r.G / gs); p.Cs = static_cast<int>(Cs); p.Gs = static_cast<int>(gs);
+    if (!share && static_cast<int64_t>(p.slots) * p.rows < r.S) return false;
+    const int A = p.L * p.slots;
+    p.U = share ? 1 : static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(p.threads / A, r.N)));
+    p.blocks = (r.N + p.U - 1) / p.U;
+    p.members = 0;
+    if (share) {
+        // as many members as hold it, or as give every CU two workgroups, of 16 KB at least
+        const int64_t need = (r.S + static_cast<int64_t>(p.slots) * p.rows - 1) / (static_cast<int64_t>(p.slots) * p.rows);
+        const int64_t fill = 2 * device_cu_count() / (r.N * p.slabs), most = r.S * Cs * elem_bytes(r.dtype) / 16384;
+        const int64_t want = std::max(need, std::min({fill, most, static_cast<int64_t>(kMaxMembers)}));
+        p.member_rows = static_cast<int>(((r.S + want - 1) / want + p.slots - 1) / p.slots * p.slots);
+        const int64_t members = (r.S + p.member_rows - 1) / p.member_rows;
+        if (members > kMaxMembers || members * gs > kMaxKnown || r.N * p.slabs * members > (1 << 22)) return false;
+        p.members = static_cast<int>(members);
     }
-    return false;
+    const int each = p.whole ? 1 : p.E, values = static_cast<int>((p.whole ? P / p.E : P) * p.slots), groups = p.U * p.Gs;
+    p.team = 1;
+    while (p.team < kWave && 2 * p.team * groups <= p.threads && 2 * p.team <= values) p.team *= 2;
+    p.lds = 4 * static_cast<size_t>(held_floats(p.threads, backward ? std::max(2 * each, p.E) : each, groups, p.members * p.Gs, p.Cs));
+    return p.lds <= kLdsMax / 2;
 }
 
 GroupPlan plan_group(const GroupRequest &r, bool backward, bool aligned16, bool aligned4) {
     GroupPlan p{};
-    const int64_t P = r.C / r.G;
     const HeldShape *shapes = backward ? kBackwardShapes : kForwardShapes;
-    // held: as many groups a workgroup as fit; a slab's part of a row is a cache line or more
-    for (int64_t gs = r.G; gs >= 1 && !p.held; --gs) {
+    const int64_t P = r.C / r.G;
+    const auto lines = [&](int64_t gs) { return gs * P * elem_bytes(r.dtype) >= 128; };
+    // held: as many groups a workgroup as fit, the smallest workgroup that does; a slab's
+    // part of a row is a cache line or more
+    for (int64_t gs = r.G; gs >= 1 && !p.held && (gs == r.G || lines(gs)); --gs) {
         if (r.G % gs != 0) continue;
-        const int64_t Cs = gs * P;
-        if (gs < r.G && Cs * elem_bytes(r.dtype) < 128) break;
-        const int words = piece_words(r.dtype, gs < r.G ? Cs : r.C, aligned16, aligned4);
-        if (gs < r.G && words != 4) continue;
-        const int E = piece_elems(r.dtype, words);
-        const int64_t L = Cs / E;
-        HeldShape shape{};
-        int slots = 0;
-        if (L > 1024 || !held_shape(shapes, 4, r.S, static_cast<int>(L), shape, slots)) continue;
-        p.held = true;
-        p.words = words; p.E = E; p.whole = E != 2 && P % E == 0;      // (with_held's kernels)
-        p.threads = shape.threads; p.rows = shape.rows;
-        p.L = static_cast<int>(L); p.slots = slots;
-        p.slabs = static_cast<int>(r.G / gs); p.Cs = static_cast<int>(Cs); p.Gs = static_cast<int>(gs);
-        const int A = p.L * p.slots;
-        p.U = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(p.threads / A, r.N)));
-        p.blocks = (r.N + p.U - 1) / p.U;
-        const int each = p.whole ? 1 : E, values = static_cast<int>((p.whole ? P / E : P) * p.slots), groups = p.U * p.Gs;
-        p.team = 1;
-        while (p.team < kWave && 2 * p.team * groups <= p.threads && 2 * p.team <= values) p.team *= 2;
-        size_t floats = held_floats(p.threads, each, backward ? 2 : 1, groups);
-        if (backward) floats = std::max<size_t>(floats, static_cast<size_t>(p.U) * A * E);
-        p.lds = floats * 4;
-        if (p.lds > kLdsMax) p.held = false;
+        for (int i = 0; i < kShapes && !p.held; ++i) p.held = hold(r, backward, gs, aligned16, aligned4, shapes[i], false, p);
+    }
+    // shared: where a sample's slab is too large for that, or there are too few for half of
+    // the CUs.  The narrowest slab of whole cache lines, or the row.
+    if (!p.held || (r.N * p.slabs < device_cu_count() / 2 && static_cast<int64_t>(p.Cs) * r.S * elem_bytes(r.dtype) > 16384)) {
+        GroupPlan q{};
+        int64_t gs = r.G;
+        for (int64_t g = r.G; g >= 1; --g)
+            if (r.G % g == 0 && lines(g) && g * P * elem_bytes(r.dtype) % 128 == 0) gs = g;
+        if (hold(r, backward, gs, aligned16, aligned4, shapes[kShapes - 1], true, q)) {
+            p = q;
+            p.held = p.shared = true;
+        }
     }
     if (!p.held) {
+        p = GroupPlan{};
         p.words = piece_words(r.dtype, r.C, aligned16, aligned4);
         p.E = piece_elems(r.dtype, p.words);
         const int64_t lanes = (r.C + p.E - 1) / p.E;
@@ -775,9 +1245,12 @@ GroupPlan plan_group(const GroupRequest &r, bool backward, bool aligned16, bool 
         return p;
     }
     if (backward) {
-        p.parts = std::min<int64_t>(p.blocks, std::max<int64_t>(1, static_cast<int64_t>(device_cu_count()) * (1024 / p.threads) / p.slabs));
+        p.parts = p.shared ? r.N * p.members
+                           : std::min<int64_t>(p.blocks, std::max<int64_t>(1, static_cast<int64_t>(device_cu_count()) * (1024 / p.threads) / p.slabs));
         p.bytes = align_up(static_cast<size_t>(p.parts) * 2 * r.C * 4, 256);
     }
+    p.o_exchange = p.bytes;
+    if (p.shared) p.bytes += align_up(static_cast<size_t>(r.N) * p.slabs * p.members * p.Gs * 8, 256);
     return p;
 }
 
@@ -790,6 +1263,10 @@ GroupPlan plan_group(const GroupRequest &r, bool backward) {
     return plan_group(r, backward, a16, a4);
 }
 
+// How often a member looks for another's values (a microsecond each, about): more than
+// any start of workgroups takes that are not kept waiting by other work.
+constexpr int kPolls = 4000;
+
 GroupArgs group_args(const GroupRequest &r, const GroupPlan &p) {
     GroupArgs a{};
     a.x = r.x; a.g = r.g; a.weight = r.weight; a.bias = r.bias; a.y = r.y;
@@ -800,12 +1277,22 @@ GroupArgs group_args(const GroupRequest &r, const GroupPlan &p) {
         a.channels = reinterpret_cast<float2 *>(ws + p.o_channels);
         a.means = reinterpret_cast<float2 *>(ws + p.o_means);
     }
+    if (p.shared) {
+        a.exchange = reinterpret_cast<uint64_t *>(ws + p.o_exchange);
+        a.members = p.members;
+        a.member_rows = p.member_rows;
+        const int forced = tuning(PLE_TUNE_GROUP_POLLS);
+        a.polls = forced > 0 ? forced - 1 : kPolls;
+    }
     a.N = r.N; a.S = r.S; a.blocks = p.blocks;
     a.C = static_cast<int>(r.C); a.G = static_cast<int>(r.G); a.P = static_cast<int>(r.C / r.G);
     a.L = p.L; a.slots = p.slots; a.A = p.L * p.slots; a.U = p.U;
     a.slabs = p.slabs; a.Cs = p.Cs; a.Gs = p.Gs;
     a.team = p.team; a.pieces = p.pieces;
+    const int64_t wide = p.whole ? r.C / r.G / p.E : r.C / r.G;
+    a.wide_inverse = static_cast<uint32_t>(std::min<int64_t>(UINT32_MAX, ((int64_t{1} << 32) + wide - 1) / wide));
     a.act = r.act; a.param_dtype = r.param_dtype;
+    a.param_vectors = p.words == 4 && reinterpret_cast<uintptr_t>(r.weight) % 16 == 0 && reinterpret_cast<uintptr_t>(r.bias) % 16 == 0;
     a.eps = r.eps;
     a.inv = static_cast<float>(1.0 / (static_cast<double>(r.S) * static_cast<double>(r.C / r.G)));
     return a;
@@ -826,20 +1313,23 @@ hipError_t with_piece(int dtype, int words, F f) {
     return by_words(std::integral_constant<int, PLE_DTYPE_BF16>{});
 }
 
-// f(type, words, whole, threads, rows)
+// f(type, words, whole, threads, rows, shared)
 template <const HeldShape *SHAPES, typename F>
 hipError_t with_held(int dtype, const GroupPlan &p, F f) {
     return with_piece(dtype, p.words, [&](auto t, auto w) {
-        constexpr int E = Piece<decltype(t)::value, decltype(w)::value>::kElems;
+        constexpr int W = decltype(w)::value, E = Piece<decltype(t)::value, W>::kElems;
         const auto by_shape = [&](auto whole) {
-            const auto at = [&](auto i) {
+            const auto at = [&](auto i, auto shared) {
                 constexpr HeldShape s = SHAPES[decltype(i)::value];
-                return f(t, w, whole, std::integral_constant<int, s.threads>{}, std::integral_constant<int, s.rows>{});
+                return f(t, w, whole, std::integral_constant<int, s.threads>{}, std::integral_constant<int, rows_of(s, W)>{}, shared);
             };
-            if (p.threads == SHAPES[0].threads && p.rows == SHAPES[0].rows) return at(std::integral_constant<int, 0>{});
-            if (p.threads == SHAPES[1].threads && p.rows == SHAPES[1].rows) return at(std::integral_constant<int, 1>{});
-            if (p.threads == SHAPES[2].threads && p.rows == SHAPES[2].rows) return at(std::integral_constant<int, 2>{});
-            return at(std::integral_constant<int, 3>{});
+            using Last = std::integral_constant<int, kShapes - 1>;
+            if (p.shared) return at(Last{}, std::true_type{});
+            const auto is = [&](int i) { return p.threads == SHAPES[i].threads && p.rows == rows_of(SHAPES[i], W); };
+            if (is(0)) return at(std::integral_constant<int, 0>{}, std::false_type{});
+            if (is(1)) return at(std::integral_constant<int, 1>{}, std::false_type{});
+            if (is(2)) return at(std::integral_constant<int, 2>{}, std::false_type{});
+            return at(Last{}, std::false_type{});
         };
         if constexpr (E == 1) return by_shape(std::true_type{});
         else if constexpr (E == 2) return by_shape(std::false_type{});
@@ -854,6 +1344,15 @@ dim3 split_grid(const GroupPlan &p) { return dim3(static_cast<unsigned>(std::min
 
 bool bad_workspace(const GroupRequest &r, const GroupPlan &p) {
     return p.bytes > 0 && (!r.workspace || r.workspace_bytes < p.bytes || reinterpret_cast<uintptr_t>(r.workspace) % 256 != 0);
+}
+
+// (by a kernel: a captured graph holds no clearing of memory)
+hipError_t clear_exchange(const GroupRequest &r, const GroupPlan &p, const GroupArgs &a) {
+    if (!p.shared) return hipSuccess;
+    const int64_t n = r.N * p.slabs * p.members * p.Gs;
+    hipLaunchKernelGGL(ple_group_unknown_kernel, dim3(static_cast<unsigned>(std::min<int64_t>((n + kBlock - 1) / kBlock, 1024))),
+                       dim3(kBlock), 0, r.stream, a.exchange, n);
+    return hipGetLastError();
 }
 
 template <typename F>
@@ -877,11 +1376,14 @@ int group_run(const GroupRequest &r) {
     if (bad_workspace(r, p)) return PLE_E_WORKSPACE;
     const GroupArgs a = group_args(r, p);
     if (p.held) {
-        const int64_t grid = std::min<int64_t>(p.blocks, std::max<int64_t>(1, kMaxGrid / p.slabs)) * p.slabs;
-        return static_cast<int>(with_held<kForwardShapes>(r.dtype, p, [&](auto t, auto w, auto whole, auto threads, auto rows) {
+        const hipError_t rc = clear_exchange(r, p, a);
+        if (rc != hipSuccess) return static_cast<int>(rc);
+        const int64_t grid = p.shared ? r.N * p.slabs * p.members
+                                      : std::min<int64_t>(p.blocks, std::max<int64_t>(1, kMaxGrid / p.slabs)) * p.slabs;
+        return static_cast<int>(with_held<kForwardShapes>(r.dtype, p, [&](auto t, auto w, auto whole, auto threads, auto rows, auto shared) {
             hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_group_forward_kernel<decltype(t)::value, decltype(w)::value,
                                                                         decltype(whole)::value, decltype(threads)::value,
-                                                                        decltype(rows)::value>),
+                                                                        decltype(rows)::value, decltype(shared)::value>),
                                dim3(static_cast<unsigned>(grid)), dim3(decltype(threads)::value), p.lds, r.stream, a);
             return hipGetLastError();
         }));
@@ -911,11 +1413,14 @@ int group_backward_run(const GroupRequest &r) {
     hipError_t rc = hipSuccess;
     if (rows && p.held) {
         a.partial = params ? static_cast<float *>(r.workspace) : nullptr;
-        rc = with_held<kBackwardShapes>(r.dtype, p, [&](auto t, auto w, auto whole, auto threads, auto rows) {
+        rc = clear_exchange(r, p, a);
+        if (rc != hipSuccess) return static_cast<int>(rc);
+        const int64_t grid = p.shared ? r.N * p.slabs * p.members : p.parts * p.slabs;
+        rc = with_held<kBackwardShapes>(r.dtype, p, [&](auto t, auto w, auto whole, auto threads, auto rows, auto shared) {
             hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_group_backward_kernel<decltype(t)::value, decltype(w)::value,
                                                                          decltype(whole)::value, decltype(threads)::value,
-                                                                         decltype(rows)::value>),
-                               dim3(static_cast<unsigned>(p.parts * p.slabs)), dim3(decltype(threads)::value), p.lds, r.stream, a);
+                                                                         decltype(rows)::value, decltype(shared)::value>),
+                               dim3(static_cast<unsigned>(grid)), dim3(decltype(threads)::value), p.lds, r.stream, a);
             return hipGetLastError();
         });
         j.sums = a.partial;
@@ -937,8 +1442,8 @@ int group_backward_run(const GroupRequest &r) {
         j.parts = r.N; j.part_stride = 2 * r.C; j.sum_stride = 1; j.step = 2;
     }
     if (rc != hipSuccess || !params) return static_cast<int>(rc);
-    hipLaunchKernelGGL(ple_group_param_kernel, dim3(static_cast<unsigned>((j.C + kWave - 1) / kWave), 2), dim3(kJoinWaves * kWave), 0,
-                       r.stream, j);
+    hipLaunchKernelGGL(ple_group_param_kernel, dim3(static_cast<unsigned>((j.C + kParamChannels - 1) / kParamChannels), 2),
+                       dim3(kParamThreads), 0, r.stream, j);
     return static_cast<int>(hipGetLastError());
 }
 

@@ -181,6 +181,16 @@ def test_constant_and_bad_groups(ops, n, s, c, groups):
         assert bool(same[keep].all())
 
 
+@pytest.mark.parametrize("polls", [1, 2, 5])
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=lambda t: str(t)[6:])
+@pytest.mark.parametrize("n,s,c,groups", [(2, 4096, 40, 4), (3, 9001, 64, 8), (1, 3001, 250, 10), (2, 2100, 77, 7)])
+def test_members_that_do_not_find_the_others(ops, tune, n, s, c, groups, dtype, polls):
+    """Workgroups that share a sample look for each other's values no more than so often
+    (1: never): what they do not find they compute themselves."""
+    tune("GROUP_POLLS", polls)
+    _check(ops, _inputs(n, s, c, dtype, F32), groups, SILU)
+
+
 def test_repeatable(ops):
     for n, s, c, groups in [(900, 30, 48, 6), (2, 9000, 96, 8)]:
         x = _inputs(n, s, c, BF16, F32)
