@@ -85,7 +85,9 @@ struct GroupArgs {
     int slabs, Cs, Gs;           // slabs of a row, channels and groups of one
     int team;                    // lanes that join a group
     uint32_t wide_inverse;       // 2^32 / values of a group in a row, rounded up
-    int pieces;
+    int pieces, piece_rows;      // split: pieces of a sample, rows of one
+    int folded;                  // split: pieces after the fold
+    float2 *folds;               // split: [N, folded, C]
     uint64_t *exchange;          // shared: [units, members, Gs] what the members know of a group
     int members, member_rows;    // shared: workgroups of a unit, rows of each
     int polls;                   // shared: how often a member looks for another's
@@ -913,6 +915,49 @@ __device__ __forceinline__ float block_sum(float v, float *lds) {
     return s;
 }
 
+// Folds kFold pieces into one, channel by channel: the sums and the squares about the
+// mean (CENTRED), or two sums.  (A sample's groups are too few workgroups to read many
+// pieces: 1 x 60000 x 960 bf16 in 10 groups, 1875 pieces, fold and join of the backward
+// 19 us, the join alone 273.)
+constexpr int kFold = 32;
+
+template <bool CENTRED>
+__global__ __launch_bounds__(kBlock) void ple_group_fold_kernel(GroupArgs a) {
+    const int64_t all = a.N * a.folded * a.C;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; i < all; i += static_cast<int64_t>(gridDim.x) * kBlock) {
+        const int64_t t = i / a.C, n = t / a.folded;
+        const int c = static_cast<int>(i - t * a.C), first = static_cast<int>(t - n * a.folded) * kFold;
+        const int last = min(a.pieces, first + kFold);
+        const float2 *const p = a.sums + n * a.pieces * a.C + c;
+        float2 s = p[static_cast<int64_t>(first) * a.C];
+        float rows = static_cast<float>(min(static_cast<int64_t>(a.piece_rows), a.S - static_cast<int64_t>(first) * a.piece_rows));
+#pragma unroll 8
+        for (int j = first + 1; j < last; ++j) {
+            const float2 v = p[static_cast<int64_t>(j) * a.C];
+            if constexpr (CENTRED) {
+                const float m = static_cast<float>(min(static_cast<int64_t>(a.piece_rows), a.S - static_cast<int64_t>(j) * a.piece_rows));
+                const float d = v.x / m - s.x / rows;
+                s.y += v.y + d * d * (rows * m / (rows + m));
+                rows += m;
+            } else {
+                s.y += v.y;
+            }
+            s.x += v.x;
+        }
+        a.folds[i] = s;
+    }
+}
+
+// What the joins read after a fold.
+__host__ __device__ inline GroupArgs folded_args(GroupArgs a) {
+    if (a.folded > 0) {
+        a.sums = a.folds;
+        a.pieces = a.folded;
+        a.piece_rows *= kFold;
+    }
+    return a;
+}
+
 // Mean and factor of a sample's group from its pieces: the squares about a piece's
 // mean, and the mean's own distance.
 __global__ __launch_bounds__(kBlock) void ple_group_stats_kernel(GroupArgs a) {
@@ -926,7 +971,7 @@ __global__ __launch_bounds__(kBlock) void ple_group_stats_kernel(GroupArgs a) {
         for (int64_t i = threadIdx.x; i < all; i += kBlock) t += sums[i / a.P * a.C + i % a.P].x;
         const float mean = block_sum(t, s_lds) * a.inv;
         t = 0.0f;
-        const int64_t piece_rows = static_cast<int64_t>(a.slots) * kSplitRows;
+        const int64_t piece_rows = a.piece_rows;
         for (int64_t i = threadIdx.x; i < all; i += kBlock) {
             const int64_t piece = i / a.P;
             const float2 s = sums[piece * a.C + i % a.P];
@@ -1139,9 +1184,9 @@ struct GroupPlan {
     bool whole, held, shared;    // held: also where it is shared
     int threads, rows;           // held: threads and rows a lane (both compile-time)
     int L, slots, U, slabs, Cs, Gs, team, pieces;
-    int members, member_rows;
+    int members, member_rows, folded;
     int64_t blocks, parts;
-    size_t lds, o_exchange, o_channels, o_means, bytes;
+    size_t lds, o_exchange, o_channels, o_means, o_folds, bytes;
 };
 
 // The widest piece that divides a row's slab and its address.
@@ -1155,7 +1200,8 @@ int piece_words(int dtype, int64_t channels, bool aligned16, bool aligned4) {
 int piece_elems(int dtype, int words) { return words == 0 ? 1 : (dtype == PLE_DTYPE_F32 ? words : 2 * words); }
 
 // The workgroups and pieces a lane of the held form, for pieces of 4 dwords (narrower
-// ones: four times as many of them).  The last is the shared form's.
+// ones: four times as many of them).  The last is the shared form's, which rather has
+// more members.
 struct HeldShape {
     int threads, rows;
 };
@@ -1165,7 +1211,7 @@ constexpr int kShapes = 4;
 constexpr int kMaxMembers = 320;         // of a unit: fewer than workgroups run at once
 constexpr int kMaxKnown = 4096;          // groups of all members
 
-constexpr int rows_of(const HeldShape &s, int words) { return words == 4 ? s.rows : 4 * s.rows; }
+constexpr int rows_of(const HeldShape &s, int words, bool shared) { return words == 4 || shared ? s.rows : 4 * s.rows; }
 
 // The slab of gs groups as a workgroup's: false where its lanes or LDS do not fit.
 bool hold(const GroupRequest &r, bool backward, int64_t gs, bool aligned16, bool aligned4, const HeldShape &shape, bool share,
@@ -1178,9 +1224,13 @@ bool hold(const GroupRequest &r, bool backward, int64_t gs, bool aligned16, bool
     if (L > shape.threads) return false;
     p.whole = p.E != 2 && P % p.E == 0;          // (with_held's kernels)
     p.threads = shape.threads;
-    p.rows = rows_of(shape, p.words);
+    p.rows = rows_of(shape, p.words, share);
     p.L = static_cast<int>(L);
     p.slots = static_cast<int>(std::min<int64_t>(r.S, shape.threads / L));
+    // many samples: as few lanes each as hold them, so that more of them are loaded at once
+    // (65536 x 8 x 24 fp32 step: 147 us with all lanes that its rows have, 64 so)
+    const int64_t fewest = (r.S + p.rows - 1) / p.rows;
+    if (!share && fewest < p.slots && r.N * L * fewest >= 1024 * static_cast<int64_t>(device_cu_count())) p.slots = static_cast<int>(fewest);
     p.slabs = static_cast<int>(r.G / gs); p.Cs = static_cast<int>(Cs); p.Gs = static_cast<int>(gs);
     if (!share && static_cast<int64_t>(p.slots) * p.rows < r.S) return false;
     const int A = p.L * p.slots;
@@ -1191,7 +1241,7 @@ bool hold(const GroupRequest &r, bool backward, int64_t gs, bool aligned16, bool
         // as many members as hold it, or as give every CU two workgroups, of 16 KB at least
         const int64_t need = (r.S + static_cast<int64_t>(p.slots) * p.rows - 1) / (static_cast<int64_t>(p.slots) * p.rows);
         const int64_t fill = 2 * device_cu_count() / (r.N * p.slabs), most = r.S * Cs * elem_bytes(r.dtype) / 16384;
-        const int64_t want = std::max(need, std::min({fill, most, static_cast<int64_t>(kMaxMembers)}));
+        const int64_t want = std::max(need, std::min({fill, most, static_cast<int64_t>(kMaxMembers), kMaxKnown / gs}));
         p.member_rows = static_cast<int>(((r.S + want - 1) / want + p.slots - 1) / p.slots * p.slots);
         const int64_t members = (r.S + p.member_rows - 1) / p.member_rows;
         if (members > kMaxMembers || members * gs > kMaxKnown || r.N * p.slabs * members > (1 << 22)) return false;
@@ -1217,7 +1267,7 @@ GroupPlan plan_group(const GroupRequest &r, bool backward, bool aligned16, bool 
     }
     // shared: where a sample's slab is too large for that, or there are too few for half of
     // the CUs.  The narrowest slab of whole cache lines, or the row.
-    if (!p.held || (r.N * p.slabs < device_cu_count() / 2 && static_cast<int64_t>(p.Cs) * r.S * elem_bytes(r.dtype) > 16384)) {
+    if (!p.held || (r.N * p.slabs < device_cu_count() / 2 && static_cast<int64_t>(p.Cs) * r.S * elem_bytes(r.dtype) > 65536)) {
         GroupPlan q{};
         int64_t gs = r.G;
         for (int64_t g = r.G; g >= 1; --g)
@@ -1241,7 +1291,9 @@ GroupPlan plan_group(const GroupRequest &r, bool backward, bool aligned16, bool 
         p.lds = static_cast<size_t>(p.slots + 1) * p.Cs * 4;
         p.o_channels = align_up(static_cast<size_t>(r.N) * p.pieces * r.C * 8, 256);
         p.o_means = p.o_channels + (backward ? align_up(static_cast<size_t>(r.N) * r.C * 8, 256) : 0);
-        p.bytes = p.o_means + (backward ? align_up(static_cast<size_t>(r.N) * r.G * 8, 256) : 0);
+        p.o_folds = p.o_means + (backward ? align_up(static_cast<size_t>(r.N) * r.G * 8, 256) : 0);
+        p.folded = p.pieces > 2 * kFold ? (p.pieces + kFold - 1) / kFold : 0;
+        p.bytes = p.o_folds + align_up(static_cast<size_t>(r.N) * p.folded * r.C * 8, 256);
         return p;
     }
     if (backward) {
@@ -1276,6 +1328,9 @@ GroupArgs group_args(const GroupRequest &r, const GroupPlan &p) {
         a.sums = reinterpret_cast<float2 *>(ws);
         a.channels = reinterpret_cast<float2 *>(ws + p.o_channels);
         a.means = reinterpret_cast<float2 *>(ws + p.o_means);
+        a.folds = reinterpret_cast<float2 *>(ws + p.o_folds);
+        a.folded = p.folded;
+        a.piece_rows = p.slots * kSplitRows;
     }
     if (p.shared) {
         a.exchange = reinterpret_cast<uint64_t *>(ws + p.o_exchange);
@@ -1321,11 +1376,11 @@ hipError_t with_held(int dtype, const GroupPlan &p, F f) {
         const auto by_shape = [&](auto whole) {
             const auto at = [&](auto i, auto shared) {
                 constexpr HeldShape s = SHAPES[decltype(i)::value];
-                return f(t, w, whole, std::integral_constant<int, s.threads>{}, std::integral_constant<int, rows_of(s, W)>{}, shared);
+                return f(t, w, whole, std::integral_constant<int, s.threads>{}, std::integral_constant<int, rows_of(s, W, decltype(shared)::value)>{}, shared);
             };
             using Last = std::integral_constant<int, kShapes - 1>;
             if (p.shared) return at(Last{}, std::true_type{});
-            const auto is = [&](int i) { return p.threads == SHAPES[i].threads && p.rows == rows_of(SHAPES[i], W); };
+            const auto is = [&](int i) { return p.threads == SHAPES[i].threads && p.rows == rows_of(SHAPES[i], W, false); };
             if (is(0)) return at(std::integral_constant<int, 0>{}, std::false_type{});
             if (is(1)) return at(std::integral_constant<int, 1>{}, std::false_type{});
             if (is(2)) return at(std::integral_constant<int, 2>{}, std::false_type{});
@@ -1352,6 +1407,15 @@ hipError_t clear_exchange(const GroupRequest &r, const GroupPlan &p, const Group
     const int64_t n = r.N * p.slabs * p.members * p.Gs;
     hipLaunchKernelGGL(ple_group_unknown_kernel, dim3(static_cast<unsigned>(std::min<int64_t>((n + kBlock - 1) / kBlock, 1024))),
                        dim3(kBlock), 0, r.stream, a.exchange, n);
+    return hipGetLastError();
+}
+
+template <bool CENTRED>
+hipError_t fold(const GroupRequest &r, const GroupArgs &a) {
+    if (a.folded == 0) return hipSuccess;
+    const int64_t blocks = (a.N * a.folded * a.C + kBlock - 1) / kBlock;
+    hipLaunchKernelGGL(ple_group_fold_kernel<CENTRED>, dim3(static_cast<unsigned>(std::min(blocks, kMaxGrid))), dim3(kBlock), 0,
+                       r.stream, a);
     return hipGetLastError();
 }
 
@@ -1392,8 +1456,10 @@ int group_run(const GroupRequest &r) {
         hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_group_sums_kernel<decltype(t)::value, decltype(w)::value>), split_grid(p),
                            dim3(kBlock), p.lds, r.stream, a);
         hipError_t rc = hipGetLastError();
+        if (rc == hipSuccess) rc = fold<true>(r, a);
         if (rc != hipSuccess) return rc;
-        hipLaunchKernelGGL(ple_group_stats_kernel, dim3(static_cast<unsigned>(std::min<int64_t>(r.N * r.G, kMaxGrid))), dim3(kBlock), 0, r.stream, a);
+        hipLaunchKernelGGL(ple_group_stats_kernel, dim3(static_cast<unsigned>(std::min<int64_t>(r.N * r.G, kMaxGrid))),
+                           dim3(kBlock), 0, r.stream, folded_args(a));
         rc = hipGetLastError();
         if (rc != hipSuccess) return rc;
         hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_group_apply_kernel<decltype(t)::value, decltype(w)::value>), split_grid(p),
@@ -1430,8 +1496,10 @@ int group_backward_run(const GroupRequest &r) {
             hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_group_backward_sums_kernel<decltype(t)::value, decltype(w)::value>),
                                split_grid(p), dim3(kBlock), p.lds, r.stream, a);
             hipError_t e = hipGetLastError();
+            if (e == hipSuccess) e = fold<false>(r, a);
             if (e != hipSuccess) return e;
-            hipLaunchKernelGGL(ple_group_backward_join_kernel, dim3(static_cast<unsigned>(std::min<int64_t>(r.N * r.G, kMaxGrid))), dim3(kBlock), 0, r.stream, a);
+            hipLaunchKernelGGL(ple_group_backward_join_kernel, dim3(static_cast<unsigned>(std::min<int64_t>(r.N * r.G, kMaxGrid))),
+                               dim3(kBlock), 0, r.stream, folded_args(a));
             e = hipGetLastError();
             if (e != hipSuccess || !r.y) return e;
             hipLaunchKernelGGL(HIP_KERNEL_NAME(ple_group_backward_apply_kernel<decltype(t)::value, decltype(w)::value>),

@@ -157,6 +157,13 @@ def test_large_level(ops, n, s, c, groups):
     _check(ops, _inputs(n, s, c, level=3000.0), groups, NONE)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=lambda t: str(t)[6:])
+@pytest.mark.parametrize("n,s,c,groups", [(1, 60001, 100, 5), (2, 52000, 96, 1), (1, 9000, 960, 10)])
+def test_many_pieces(ops, n, s, c, groups, dtype):
+    """Samples of more pieces than their groups' workgroups should read."""
+    _check(ops, _inputs(n, s, c, dtype, level=10.0), groups, SILU)
+
+
 @pytest.mark.parametrize("n,s,c,groups", [(6, 40, 32, 4), (2, 9001, 40, 5), (2, 9001, 41, 1)])
 def test_constant_and_bad_groups(ops, n, s, c, groups):
     """A constant group has y = act(bias) and a finite gradient; NaN and infinities
