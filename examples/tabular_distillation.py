@@ -9,8 +9,9 @@ block, its gate, the residual and the next block's norm in one pass), and
 the labels.  Synthetic data; the teacher is a fixed random network, whose top
 logits and log-sum are stored as a real one's would be.
 
-    python examples/tabular_distillation.py [--device cuda] [--steps 60] [--autocast]
+    python examples/tabular_distillation.py [--device cuda] [--steps 60] [--autocast] [--clip 1.0]
 
+With ``--clip`` the gradients' norm is held to that limit (``clip_grad_norm_``).
 Prints the loss and the share of rows where the student agrees with the teacher.
 """
 
@@ -30,6 +31,7 @@ from piecewiselinearembeddings_optimized_amd import (  # noqa: E402
     CudaDistillationLoss,
     CudaPiecewiseLinearEmbeddings,
     CudaResidualNorm,
+    clip_grad_norm_,
     compute_bins,
 )
 
@@ -75,7 +77,7 @@ def make_data(n: int, n_numbers: int, cardinalities, n_classes: int, k: int, tem
 
 
 def train(device: str = "cuda", steps: int = 60, rows: int = 4096, batch: int = 512, autocast: bool = False,
-          temperature: float = 2.0, report=print) -> list[float]:
+          temperature: float = 2.0, report=print, clip: float | None = None) -> list[float]:
     torch.manual_seed(0)
     cardinalities = [3, 40, 500]
     data = make_data(rows, 8, cardinalities, 100, 10, temperature)
@@ -93,6 +95,8 @@ def train(device: str = "cuda", steps: int = 60, rows: int = 4096, batch: int = 
         loss = loss_fn(logits, top, classes, lse, labels)
         opt.zero_grad(set_to_none=True)
         loss.backward()
+        if clip is not None:
+            clip_grad_norm_(student.parameters(), clip)
         opt.step()
         losses.append(float(loss.detach()))
         if step % 10 == 0 or step == steps - 1:
@@ -106,5 +110,6 @@ if __name__ == "__main__":
     ap.add_argument("--device", default="cuda" if torch.cuda.is_available() else "cpu")
     ap.add_argument("--steps", type=int, default=60)
     ap.add_argument("--autocast", action="store_true")
+    ap.add_argument("--clip", type=float, default=None, help="the gradients' largest norm")
     args = ap.parse_args()
-    train(args.device, args.steps, autocast=args.autocast)
+    train(args.device, args.steps, autocast=args.autocast, clip=args.clip)

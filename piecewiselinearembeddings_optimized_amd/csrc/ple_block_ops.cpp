@@ -240,28 +240,78 @@ Listed describe(at::TensorList grads, const at::TensorList *out) {
 
 size_t bytes_of(int dtype) { return dtype == PLE_DTYPE_F32 ? 4 : 2; }
 
-// Every element is written once, and read by nothing but the one that writes it.
-void check_overlap(const std::vector<ple_grad_t> &list) {
-    struct Range {
-        uintptr_t begin, end;
-        bool written;
-    };
-    std::vector<Range> ranges;
-    ranges.reserve(2 * list.size());
-    for (const ple_grad_t &g : list) {
-        if (g.numel == 0) continue;
-        const auto o = reinterpret_cast<uintptr_t>(g.out), p = reinterpret_cast<uintptr_t>(g.grad);
-        ranges.push_back({o, o + g.numel * bytes_of(g.out_dtype), true});
-        if (o != p) ranges.push_back({p, p + g.numel * bytes_of(g.dtype), false});
-        TORCH_CHECK(o != p || g.dtype == g.out_dtype, "a gradient that is scaled in place keeps its dtype");
-    }
+struct Range {
+    uintptr_t begin, end;
+    bool written;
+};
+
+// Whether a range that is written has bytes of another.
+bool overlap(std::vector<Range> ranges) {
     std::sort(ranges.begin(), ranges.end(), [](const Range &a, const Range &b) { return a.begin < b.begin; });
     uintptr_t written = 0, read = 0;         // ends of what has been seen
     for (const Range &r : ranges) {
-        TORCH_CHECK(r.begin >= written && (!r.written || r.begin >= read),
-                    "gradients that are scaled must not share memory with each other or with out");
+        if (r.begin < written || (r.written && r.begin < read)) return true;
         (r.written ? written : read) = std::max(r.written ? written : read, r.end);
     }
+    return false;
+}
+
+// A tensor's elements as ranges of memory: all of it, gaps and all, or its runs.
+void add_ranges(const Tensor &t, bool runs, std::vector<Range> &ranges) {
+    const auto begin = reinterpret_cast<uintptr_t>(t.data_ptr());
+    std::vector<std::pair<int64_t, int64_t>> dims;          // stride, size
+    for (int64_t k = 0; k < t.dim(); ++k)
+        if (t.size(k) > 1) dims.emplace_back(t.stride(k), t.size(k));
+    std::sort(dims.begin(), dims.end());
+    int64_t run = 1, last = 0;
+    size_t inner = 0;
+    while (inner < dims.size() && dims[inner].first == run) run *= dims[inner++].second;
+    for (const auto &[stride, size] : dims) last += stride * (size - 1);
+    const auto push = [&](int64_t first, int64_t n) {
+        ranges.push_back({begin + first * t.element_size(), begin + (first + n) * t.element_size(), true});
+    };
+    if (!runs) return push(0, last + 1);
+    std::vector<int64_t> at(dims.size(), 0);
+    for (int64_t first = 0;;) {
+        push(first, run);
+        size_t k = inner;
+        for (; k < dims.size(); ++k) {
+            first += dims[k].first;
+            if (++at[k] < dims[k].second) break;
+            first -= dims[k].first * dims[k].second;
+            at[k] = 0;
+        }
+        if (k == dims.size()) return;
+    }
+}
+
+// Every element is written once, and read by nothing but the one that writes it.
+// Gradients with gaps that are scaled in place lie between others, often (columns of
+// one tensor): their runs are looked at if they do.
+void check_overlap(const Listed &list, at::TensorList grads, bool in_place) {
+    std::vector<Range> ranges;
+    ranges.reserve(2 * list.grads.size());
+    const auto dense = [&] {
+        ranges.clear();
+        for (const ple_grad_t &g : list.grads) {
+            if (g.numel == 0) continue;
+            const auto o = reinterpret_cast<uintptr_t>(g.out), p = reinterpret_cast<uintptr_t>(g.grad);
+            ranges.push_back({o, o + g.numel * bytes_of(g.out_dtype), true});
+            if (o != p) ranges.push_back({p, p + g.numel * bytes_of(g.dtype), false});
+            TORCH_CHECK(o != p || g.dtype == g.out_dtype, "a gradient that is scaled in place keeps its dtype");
+        }
+    };
+    const auto all = [&](bool runs) {
+        dense();
+        for (const auto &[i, copy] : list.copies) {
+            if (!in_place || grads[i].numel() == 0) continue;
+            at::assert_no_internal_overlap(grads[i]);
+            add_ranges(grads[i], runs, ranges);
+        }
+        return overlap(ranges);
+    };
+    TORCH_CHECK(!all(false) || (in_place && !list.copies.empty() && !all(true)),
+                "gradients that are scaled must not share memory with each other or with out");
 }
 
 void run_norm(const std::vector<ple_grad_t> &list, double norm_type, const Tensor &like, Tensor &norm) {
@@ -298,10 +348,8 @@ Tensor clip(at::TensorList grads, const at::TensorList *out, double max_norm, do
     check_limit(max_norm);
     (void)norm_kind(norm_type);
     const Listed list = describe(grads, out);
-    check_overlap(list.grads);
+    check_overlap(list, grads, !out);
     if (has(given)) check_norm(*given, grads[0]);
-    if (!out)
-        for (const auto &[i, copy] : list.copies) at::assert_no_internal_overlap(grads[i]);
     DeviceScope scope(grads[0].device().index());
     Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat));
     if (has(given)) norm.copy_(given->reshape({}));

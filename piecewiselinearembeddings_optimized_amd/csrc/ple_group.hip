@@ -1397,8 +1397,8 @@ constexpr int64_t kMaxGrid = 1 << 20;
 
 dim3 split_grid(const GroupPlan &p) { return dim3(static_cast<unsigned>(std::min<int64_t>(p.blocks, kMaxGrid))); }
 
-bool bad_workspace(const GroupRequest &r, const GroupPlan &p) {
-    return p.bytes > 0 && (!r.workspace || r.workspace_bytes < p.bytes || reinterpret_cast<uintptr_t>(r.workspace) % 256 != 0);
+bool bad_workspace(const GroupRequest &r, size_t need) {
+    return need > 0 && (!r.workspace || r.workspace_bytes < need || reinterpret_cast<uintptr_t>(r.workspace) % 256 != 0);
 }
 
 // (by a kernel: a captured graph holds no clearing of memory)
@@ -1436,8 +1436,8 @@ size_t group_backward_workspace_bytes(const GroupRequest &r) {
 }
 
 int group_run(const GroupRequest &r) {
+    if (bad_workspace(r, group_workspace_bytes(r))) return PLE_E_WORKSPACE;
     const GroupPlan p = plan_group(r, false);
-    if (bad_workspace(r, p)) return PLE_E_WORKSPACE;
     const GroupArgs a = group_args(r, p);
     if (p.held) {
         const hipError_t rc = clear_exchange(r, p, a);
@@ -1470,8 +1470,8 @@ int group_run(const GroupRequest &r) {
 
 int group_backward_run(const GroupRequest &r) {
     const bool params = r.d_bias || r.d_weight, rows = r.N > 0 && r.S > 0;
+    if (rows && bad_workspace(r, group_backward_workspace_bytes(r))) return PLE_E_WORKSPACE;
     const GroupPlan p = rows ? plan_group(r, true) : GroupPlan{};
-    if (bad_workspace(r, p)) return PLE_E_WORKSPACE;
     GroupArgs a = rows ? group_args(r, p) : GroupArgs{};
     ParamJoin j{};                   // (without rows of no parts: the gradients are 0)
     j.bias = r.d_bias; j.weight = r.d_weight;

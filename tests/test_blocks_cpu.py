@@ -289,3 +289,12 @@ def test_clip_grad_norm_as_torch_has_it():
 def test_refusals(call, match):
     with pytest.raises(ValueError, match=match):
         call()
+
+
+def test_example_with_clipping():
+    """Runs with a limit; without one that is ever reached nothing changes."""
+    from tests.test_example import _example
+
+    run = lambda **kw: _example().train("cpu", steps=3, rows=512, batch=256, report=lambda s: None, **kw)  # noqa: E731
+    assert run(clip=float("inf")) == run()
+    assert all(map(torch.isfinite, map(torch.tensor, run(clip=0.1))))
