@@ -643,7 +643,7 @@ __device__ __forceinline__ void weigh_sums(const float *weight, const float (&su
 }
 
 template <int T, int W, bool WHOLE, int THREADS, int R, bool SHARED>
-__global__ __launch_bounds__(THREADS, THREADS == 256 ? 3 : 2) void ple_group_backward_kernel(GroupArgs a) {
+__global__ __launch_bounds__(THREADS, SHARED ? 3 : 2) void ple_group_backward_kernel(GroupArgs a) {
     constexpr int E = Piece<T, W>::kElems, kEach = WHOLE ? 1 : E, kValues = 2 * kEach > E ? 2 * kEach : E;
     extern __shared__ float4 s_all[];
     float *const s_lds = reinterpret_cast<float *>(s_all);
@@ -686,7 +686,11 @@ __global__ __launch_bounds__(THREADS, THREADS == 256 ? 3 : 2) void ple_group_bac
                 g[k].load_at(pg + k * step + at);
             }
         }
-        float sum[2][E] = {};
+        // dz is kept until the groups' sums are known (8 x 65536 x 256 bf16 in groups of 8:
+        // 233 us, computed again 277), where three workgroups have the registers for it (16 x
+        // 4096 x 320 in groups of 10: 50 us either way, kept in part in scratch memory)
+        constexpr bool kKept = WHOLE || !SHARED || E < 8;
+        float sum[2][E] = {}, grad[kKept ? R : 1][E];
         {
             const Affine<E, WHOLE> f(own_params, own_params + a.Cs, stats, groups);
 #pragma unroll
@@ -695,40 +699,39 @@ __global__ __launch_bounds__(THREADS, THREADS == 256 ? 3 : 2) void ple_group_bac
                 g[k].keep();
                 __builtin_amdgcn_sched_barrier(0);
                 // (a row that is not there has a gradient of 0)
-                float dz[E];
+                float (&dz)[E] = grad[kKept ? k : 0];
                 piece_grad<T, W>(act, x[k], g[k], f.scale, f.shift, dz);
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     sum[0][e] += dz[e];
                     sum[1][e] += dz[e] * x[k][e];
                     // (here, and not where the sums are used: the terms would all be held)
-                    asm volatile("" : "+v"(sum[0][e]), "+v"(sum[1][e]));
-                    // (a 32-bit gradient's place takes dz; a 16-bit one's is computed again)
-                    if constexpr (T == PLE_DTYPE_F32) g[k].w[e] = __float_as_uint(dz[e]);
+                    asm volatile("" : "+v"(sum[0][e]), "+v"(sum[1][e]), "+v"(dz[e]));
                 }
             }
         }
         standard_sums<E, WHOLE>(stats, groups, sum);
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int e = 0; e < E; ++e) all[j][e] += sum[j][e];
-        if (!a.y) {
-            if constexpr (SHARED) break;
-            continue;
-        }
         float v[2][kEach] = {};
         weigh_sums<E, WHOLE>(own_params, sum, v);
         if constexpr (!SHARED) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < E; ++e) all[j][e] += sum[j][e];
+            if (!a.y) continue;
             join_groups<2, E, WHOLE, THREADS>(a, p, s_lds, v, [&](int q, const float (&s)[2]) {
                 s_m1[q] = s[0] * a.inv;
                 s_m2[q] = s[1] * a.inv;
             });
         } else {
             uint64_t *const unit = a.exchange + (rows.n * a.slabs + slab) * a.members * a.Gs;
-            join_groups<2, E, WHOLE, THREADS>(a, p, s_lds, v, [&](int q, const float (&s)[2]) {
-                publish(unit + member * a.Gs + q, s[0], s[1]);
-            });
+            if (a.y)
+                join_groups<2, E, WHOLE, THREADS>(a, p, s_lds, v, [&](int q, const float (&s)[2]) {
+                    publish(unit + member * a.Gs + q, s[0], s[1]);
+                });
+            // (while the others' are on their way)
+            if (a.partial) leave_sums<E, THREADS>(a, p, s_lds, sum, slab, blk * a.members + member);
+            if (!a.y) break;
             collect<THREADS>(a, unit, s_known, s_late, [&](int m) {
                 const Rows other(a, rows.n, m, true);
                 const int64_t away = (other.first - rows.first) * a.C * elem_bytes(T) + at;
@@ -780,15 +783,10 @@ __global__ __launch_bounds__(THREADS, THREADS == 256 ? 3 : 2) void ple_group_bac
 #pragma unroll
         for (int k = 0; k < R; ++k) {
             x[k].keep();
-            g[k].keep();
+            if constexpr (!kKept) g[k].keep();
             __builtin_amdgcn_sched_barrier(0);
-            float dz[E];
-            if constexpr (T == PLE_DTYPE_F32) {
-#pragma unroll
-                for (int e = 0; e < E; ++e) dz[e] = g[k][e];
-            } else {
-                piece_grad<T, W>(act, x[k], g[k], f.scale, f.shift, dz);
-            }
+            float (&dz)[E] = grad[kKept ? k : 0];
+            if constexpr (!kKept) piece_grad<T, W>(act, x[k], g[k], f.scale, f.shift, dz);
 #pragma unroll
             for (int e = 0; e < E; ++e)
                 dz[e] = dz[e] * f.scale[e] + (x[k][e] * along[WHOLE ? 0 : e] + level[WHOLE ? 0 : e]);
@@ -797,7 +795,8 @@ __global__ __launch_bounds__(THREADS, THREADS == 256 ? 3 : 2) void ple_group_bac
         if constexpr (SHARED) break;
         __syncthreads();
     }
-    if (a.partial) leave_sums<E, THREADS>(a, here.again(), s_lds, all, slab, SHARED ? turn.block * a.members + member : turn.block);
+    if constexpr (!SHARED)
+        if (a.partial) leave_sums<E, THREADS>(a, here.again(), s_lds, all, slab, turn.block);
 }
 
 // Clears the words that members exchange.
