@@ -567,6 +567,10 @@ int ple_grad_norm_launch(const ple_grad_t *grads, int64_t count, int kind, float
  * touched where nothing is clipped; limit >= 0 (an infinite one clips nothing). */
 int ple_grad_scale_launch(const ple_grad_t *grads, int64_t count, const float *norm, float limit, void *stream);
 
+/* Both: the norm of ple_grad_norm_launch, and out scaled with it. */
+int ple_grad_clip_launch(const ple_grad_t *grads, int64_t count, int kind, float limit, float *norm, void *workspace,
+                         size_t workspace_bytes, void *stream);
+
 /*
  * Planner overrides, for tuning sweeps and for tests that run every kernel
  * form on the same inputs.  No counterpart in the reference (its launchers

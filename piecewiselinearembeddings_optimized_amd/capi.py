@@ -220,6 +220,8 @@ def lib() -> ctypes.CDLL:
         L.ple_grad_norm_launch.restype = i32
         L.ple_grad_scale_launch.argtypes = [ctypes.POINTER(Grad), i64, p, f32, p]
         L.ple_grad_scale_launch.restype = i32
+        L.ple_grad_clip_launch.argtypes = [ctypes.POINTER(Grad), i64, i32, f32, p, p, sz, p]
+        L.ple_grad_clip_launch.restype = i32
         L.ple_timing_start.argtypes, L.ple_timing_start.restype = [i32], i32
         L.ple_timing_stop.argtypes, L.ple_timing_stop.restype = [], i32
         L.ple_timing_read.argtypes = [i32, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_int)]
@@ -543,3 +545,13 @@ def grad_scale(grads, norm, limit, out=None, stream=None) -> None:
     """``ple_grad_scale_launch``: in place, or into ``out``."""
     listed, count = gradient_list(grads, out)
     check(lib().ple_grad_scale_launch(listed, count, _ptr(norm), limit, _stream(stream)))
+
+
+def grad_clip(grads, norm, limit, kind=2, out=None, workspace=None, stream=None) -> None:
+    """``ple_grad_clip_launch``: :func:`grad_norm` into ``norm``, and :func:`grad_scale` with it."""
+    listed, count = gradient_list(grads, out)
+    if workspace is None:
+        workspace, need = _workspace(int(lib().ple_grad_norm_workspace_bytes(listed, count)), norm)
+    else:
+        need = workspace.numel() * workspace.element_size()
+    check(lib().ple_grad_clip_launch(listed, count, kind, limit, _ptr(norm), _ptr(workspace), need, _stream(stream)))

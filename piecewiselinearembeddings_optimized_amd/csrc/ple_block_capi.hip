@@ -206,4 +206,19 @@ int ple_grad_scale_launch(const ple_grad_t *grads, int64_t count, const float *n
     return ple::grad_scale_run(r);
 }
 
+int ple_grad_clip_launch(const ple_grad_t *grads, int64_t count, int kind, float limit, float *norm, void *workspace,
+                         size_t workspace_bytes, void *stream) {
+    const int rc = ple::check_grads(grads, count, true);
+    if (rc != PLE_OK) return rc;
+    if (kind != PLE_NORM_P1 && kind != PLE_NORM_P2 && kind != PLE_NORM_INF) return PLE_E_UNSUPPORTED;
+    if (!(limit >= 0.0f)) return PLE_E_UNSUPPORTED;
+    if (!norm) return PLE_E_NULL_POINTER;
+    if (!ple::aligned(norm, 4)) return PLE_E_MISALIGNED;
+    ple::GradsRequest r{};
+    r.grads = grads; r.count = count; r.kind = kind; r.norm = norm; r.limit = limit;
+    r.workspace = workspace; r.workspace_bytes = workspace_bytes;
+    r.stream = static_cast<hipStream_t>(stream);
+    return ple::grad_clip_run(r);
+}
+
 }  // extern "C"

@@ -314,20 +314,6 @@ void check_overlap(const Listed &list, at::TensorList grads, bool in_place) {
                 "gradients that are scaled must not share memory with each other or with out");
 }
 
-void run_norm(const std::vector<ple_grad_t> &list, double norm_type, const Tensor &like, Tensor &norm) {
-    const size_t bytes = ple_grad_norm_workspace_bytes(list.data(), static_cast<int64_t>(list.size()));
-    Tensor ws = scratch(bytes, like);
-    check_rc(ple_grad_norm_launch(list.data(), static_cast<int64_t>(list.size()), norm_kind(norm_type), norm.data_ptr<float>(),
-                                  ws.data_ptr(), bytes, current_stream(like)),
-             "ple_grad_norm_launch");
-}
-
-void run_scale(const std::vector<ple_grad_t> &list, const Tensor &norm, double max_norm, const Tensor &like) {
-    check_rc(ple_grad_scale_launch(list.data(), static_cast<int64_t>(list.size()), norm.data_ptr<float>(),
-                                   static_cast<float>(max_norm), current_stream(like)),
-             "ple_grad_scale_launch");
-}
-
 void check_limit(double max_norm) { TORCH_CHECK(max_norm >= 0, "max_norm must not be negative, got ", max_norm); }
 
 void check_norm(const Tensor &norm, const Tensor &like) {
@@ -337,24 +323,39 @@ void check_norm(const Tensor &norm, const Tensor &like) {
 
 Tensor ple_gradient_norm(at::TensorList grads, double norm_type) {
     const Listed list = describe(grads, nullptr);
-    (void)norm_kind(norm_type);
+    const int kind = norm_kind(norm_type);
     DeviceScope scope(grads[0].device().index());
     Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat));
-    run_norm(list.grads, norm_type, grads[0], norm);
+    const int64_t count = static_cast<int64_t>(list.grads.size());
+    const size_t bytes = ple_grad_norm_workspace_bytes(list.grads.data(), count);
+    Tensor ws = scratch(bytes, grads[0]);
+    check_rc(ple_grad_norm_launch(list.grads.data(), count, kind, norm.data_ptr<float>(), ws.data_ptr(), bytes,
+                                  current_stream(grads[0])),
+             "ple_grad_norm_launch");
     return norm;
 }
 
 Tensor clip(at::TensorList grads, const at::TensorList *out, double max_norm, double norm_type, const OptTensor &given) {
     check_limit(max_norm);
-    (void)norm_kind(norm_type);
+    const int kind = norm_kind(norm_type);
     const Listed list = describe(grads, out);
     check_overlap(list, grads, !out);
     if (has(given)) check_norm(*given, grads[0]);
     DeviceScope scope(grads[0].device().index());
     Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat));
-    if (has(given)) norm.copy_(given->reshape({}));
-    else run_norm(list.grads, norm_type, grads[0], norm);
-    run_scale(list.grads, norm, max_norm, grads[0]);
+    const int64_t count = static_cast<int64_t>(list.grads.size());
+    const float limit = static_cast<float>(max_norm);
+    if (has(given)) {
+        norm.copy_(given->reshape({}));
+        check_rc(ple_grad_scale_launch(list.grads.data(), count, norm.data_ptr<float>(), limit, current_stream(grads[0])),
+                 "ple_grad_scale_launch");
+    } else {
+        const size_t bytes = ple_grad_norm_workspace_bytes(list.grads.data(), count);
+        Tensor ws = scratch(bytes, grads[0]);
+        check_rc(ple_grad_clip_launch(list.grads.data(), count, kind, limit, norm.data_ptr<float>(), ws.data_ptr(), bytes,
+                                      current_stream(grads[0])),
+                 "ple_grad_clip_launch");
+    }
     if (!out)
         for (const auto &[i, copy] : list.copies) grads[i].copy_(copy);
     return norm;

@@ -213,5 +213,6 @@ struct GradsRequest {
 int grad_norm_run(const GradsRequest &r);
 size_t grad_norm_workspace_bytes(const GradsRequest &r);
 int grad_scale_run(const GradsRequest &r);
+int grad_clip_run(const GradsRequest &r);          // both
 
 }  // namespace ple

@@ -93,6 +93,21 @@ def test_c_abi_refuses_gradients():
     assert lib.ple_grad_norm_workspace_bytes(listed(), 1) >= 8
 
 
+def test_c_abi_refuses_clipping():
+    lib = capi.lib()
+
+    def clip(count=1, kind=2, limit=1.0, out=P, ws=P, size=1 << 20, **kw):
+        g = (capi.Grad * 1)(capi.Grad(**({"grad": 256, "out": 256, "numel": 4, "dtype": 0, "out_dtype": 0} | kw)))
+        return lib.ple_grad_clip_launch(g, count, kind, limit, out, ws, size, None)
+
+    assert clip(count=-1) == clip(numel=-1) == -2 and clip(numel=(1 << 40) + 1) == -5
+    assert clip(dtype=4) == clip(out_dtype=-1) == -3
+    assert clip(grad=None) == clip(out=None) == lib.ple_grad_clip_launch(None, 1, 2, 1.0, P, P, 1 << 20, None) == -1
+    assert clip(grad=258) == clip(out=ODD) == -8
+    assert clip(ws=None) == clip(size=7) == clip(ws=ctypes.c_void_p(264)) == -6
+    assert clip(kind=0) == clip(kind=4) == clip(limit=-1.0) == clip(limit=math.nan) == clip(out_dtype=1) == -7
+
+
 def _meta(*shape, dtype=F32):
     return torch.empty(*shape, dtype=dtype, device="meta")
 

@@ -323,9 +323,14 @@ def test_c_abi_gradients(package, kind, p):
     want = [torch.empty_like(o) for o in out]
     assert torch.equal(norm, package.clip_gradients_(grads, 0.5, p, out=want))
     assert _same(out, want)
+    both, into = torch.empty((), device=DEV), [torch.empty_like(o) for o in out]
+    capi.grad_clip(grads, both, 0.5, kind, into)
+    assert torch.equal(both, norm) and _same(into, want)
     size = capi.lib().ple_grad_norm_workspace_bytes(*capi.gradient_list(grads))
     with pytest.raises(capi.PleError, match="workspace"):
         capi.grad_norm(grads, norm, kind, workspace=torch.empty(size - 1, dtype=torch.uint8, device=DEV))
+    with pytest.raises(capi.PleError, match="workspace"):
+        capi.grad_clip(grads, norm, 0.5, kind, into, workspace=torch.empty(size - 1, dtype=torch.uint8, device=DEV))
 
 
 def test_gradients_with_gaps_that_share_memory(package):
