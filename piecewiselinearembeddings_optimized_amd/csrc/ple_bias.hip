@@ -587,8 +587,8 @@ void split_columns(BiasArgs &a, int most) {
     a.cols = static_cast<int>(((a.k + a.colblocks - 1) / a.colblocks + 7) / 8 * 8);
 }
 
-// Tiles of fewer rows where there are not four for every CU.  (12 x 1023 x 1301 fp32:
-// 64 rows 17.3 us)
+// Tiles of fewer rows where there are not four for every CU.  (12 x 1023 x 1301 fp32: of
+// 16 rows 14.8 us, of 64 17.3)
 BiasArgs forward_args(const BiasRequest &r) {
     BiasArgs a = bias_args(r);
     a.out = r.out;
