@@ -487,6 +487,7 @@ int ple_distill_backward_launch(const float *grad_loss, const void *logits, cons
  *   stats        float32 [N, G, 2], 8-byte aligned: mean and 1 / sqrt(var + eps)
  *   workspace    >= ple_group_norm_workspace_bytes() bytes (0 is possible),
  *                256-byte aligned, need not be initialised
+ * Results share no memory with anything that is read.
  * Statistics and sums are 32-bit in a fixed order.  C <= 2^20, S < 2^31, N < 2^31,
  * N * S * C < 2^44 (else PLE_E_TOO_LARGE); G divides C (else PLE_E_BAD_SHAPE).
  */

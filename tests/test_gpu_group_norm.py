@@ -316,3 +316,47 @@ def test_refusals(ops):
     for call, text in bad:
         with pytest.raises(RuntimeError, match=text):
             call()
+
+
+@pytest.mark.parametrize("n,s,c,groups", [(2, 9000, 30000, 30), (3, 3001, 20000, 10)])
+def test_statistics_of_wide_samples(ops, n, s, c, groups):
+    """Many pieces of many channels, where the kernels that join them fill the device; the
+    first sample is constant."""
+    x = torch.empty(n, s, c, dtype=BF16, device=DEV).normal_(generator=torch.Generator(DEV).manual_seed(1))
+    x[0] = 3.0
+    stats = ops.group_norm(x, None, None, groups, NONE, EPS)[1]
+    for i in range(n):
+        for g in range(groups):
+            v = x[i, :, g * (c // groups):(g + 1) * (c // groups)].double()
+            m = v.mean()
+            rho = ((v - m).square().mean() + EPS).rsqrt()
+            size = float(rho * v.abs().mean())
+            assert abs(float(stats[i, g, 0] - m)) <= E * float(v.abs().mean()), (i, g)
+            assert abs(float(stats[i, g, 1] / rho - 1)) <= E * (1 + size) ** 2, (i, g)
+
+
+@pytest.mark.parametrize("n,s,c,groups,last", [(33000, 256, 256, 32, 2), (9, 9000, 30000, 30, 1)])
+def test_more_than_32_bits_of_elements(ops, n, s, c, groups, last):
+    """The last samples behind 2^31 elements, against the same samples alone (whose
+    workgroups may take other rows: sums of 2^16 or 2^20 values in another order), and the
+    parameters' gradients, which are theirs alone."""
+    x = torch.empty(n, s, c, dtype=BF16, device=DEV)
+    x[:-last].fill_(1.0)
+    x[-last:].normal_(generator=torch.Generator(DEV).manual_seed(1))
+    g = torch.zeros_like(x)
+    g[-last:].normal_(generator=torch.Generator(DEV).manual_seed(2))
+    w, b = torch.linspace(0.5, 1.5, c, device=DEV), torch.linspace(-1, 1, c, device=DEV)
+    y, stats = ops.group_norm(x, w, b, groups, SILU, EPS)
+    gx, gw, gb = ops.group_norm_backward(g, x, stats, w, b, groups, SILU, [True] * 3)
+    xs, gs = x[-last:].clone(), g[-last:].clone()
+    del x, g
+    ys, ss = ops.group_norm(xs, w, b, groups, SILU, EPS)
+    gxs, gws, gbs = ops.group_norm_backward(gs, xs, ss, w, b, groups, SILU, [True] * 3)
+    # 32-bit values differ by some 2^-20 of their size, 16-bit ones by one step where that
+    # crosses a rounding border; sums of 512 to 9000 terms of about 1
+    torch.testing.assert_close(stats[-last:], ss, rtol=2.0 ** -18, atol=2.0 ** -18)
+    torch.testing.assert_close(y[-last:], ys, rtol=2.0 ** -7, atol=2.0 ** -16)
+    torch.testing.assert_close(gx[-last:], gxs, rtol=2.0 ** -7, atol=2.0 ** -16)
+    torch.testing.assert_close(gw, gws, rtol=2.0 ** -14, atol=2.0 ** -10)
+    torch.testing.assert_close(gb, gbs, rtol=2.0 ** -14, atol=2.0 ** -10)
+    assert torch.isfinite(y[:2]).all() and float(gx[:2].abs().max()) == 0
