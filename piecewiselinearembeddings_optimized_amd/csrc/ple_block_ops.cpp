@@ -358,6 +358,9 @@ Tensor clip(at::TensorList grads, const at::TensorList *out, double max_norm, do
     }
     if (!out)
         for (const auto &[i, copy] : list.copies) grads[i].copy_(copy);
+    // (what autograd has saved of them is no longer there)
+    for (const Tensor &t : out ? *out : grads)
+        if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
     return norm;
 }
 

@@ -248,3 +248,18 @@ def test_refusals(package):
     assert math.isclose(float(package.gradient_norm([a, a])), math.sqrt(2) * float(a.double().norm()), rel_tol=1e-6)
     package.clip_gradients_([a], 1.0, out=[a])
     assert math.isclose(float(a.double().norm()), 1.0, rel_tol=1e-5)
+
+
+def test_autograd_sees_the_writes(package):
+    """A tensor that a graph has saved is scaled: its backward must not use the new values."""
+    for into in (False, True):
+        x = torch.randn(20, device=DEV, requires_grad=True)
+        s = x.exp()                                  # (its backward reads s)
+        target = s.detach()
+        package.clip_gradients_([torch.ones_like(target)] if into else [target], 0.1, out=[target] if into else None)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            s.sum().backward()
+    with torch.inference_mode():
+        g = torch.ones(4, device=DEV)
+        package.clip_gradients_([g], 1.0)
+    assert torch.allclose(g, torch.full_like(g, 0.5))
