@@ -513,6 +513,34 @@ int ple_group_norm_backward_launch(const void *grad_y, const void *x, const floa
                                    void *workspace, size_t workspace_bytes, void *stream);
 
 /*
+ * The launch plan of ple_group_norm_launch (backward != 0: of its backward) for a
+ * shape, without launching.  `x` may be NULL; its alignment stands for that of all
+ * [N, S, C] tensors.  Returns the error the launch would return for the sizes,
+ * else fills `info` (all 0 without rows).
+ *   form             PLE_GROUP_*
+ *   lane_channels    channels a lane takes of a row
+ *   slabs            of a row's channels, a workgroup each
+ *   members          PLE_GROUP_SHARED: workgroups that share a sample's slab
+ *   params_end       one past the last channel whose weight and bias a lane reads
+ *   workspace_bytes  as ple_group_norm[_backward]_workspace_bytes
+ */
+enum {
+    PLE_GROUP_HELD = 0,    /* a workgroup holds a sample's slab */
+    PLE_GROUP_SHARED = 1,  /* several do, and exchange what they know */
+    PLE_GROUP_SPLIT = 2,   /* pieces of samples, read twice */
+};
+typedef struct ple_group_norm_plan_info {
+    int form;
+    int lane_channels;
+    int slabs;
+    int members;
+    int64_t params_end;
+    size_t workspace_bytes;
+} ple_group_norm_plan_info_t;
+int ple_group_norm_plan_query(const void *x, int64_t N, int64_t S, int64_t C, int64_t G, int dtype, int backward,
+                              ple_group_norm_plan_info_t *info);
+
+/*
  * Learned bias of attention scores by relative position; no counterpart in the
  * reference.  With p = starts[b] (or offset) the position of a sample's first
  * query:

@@ -104,6 +104,19 @@ class LookupPlanInfo(ctypes.Structure):
     ]
 
 
+class GroupNormPlanInfo(ctypes.Structure):
+    """``ple_group_norm_plan_info_t``: the group norm's launch plan for a shape."""
+
+    _fields_ = [
+        ("form", ctypes.c_int),
+        ("lane_channels", ctypes.c_int),
+        ("slabs", ctypes.c_int),
+        ("members", ctypes.c_int),
+        ("params_end", ctypes.c_int64),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 class Norm(ctypes.Structure):
     """``ple_norm_t``: the norms, gate and residual scale around a block."""
 
@@ -208,6 +221,8 @@ def lib() -> ctypes.CDLL:
         L.ple_group_norm_backward_workspace_bytes.restype = sz
         L.ple_group_norm_backward_launch.argtypes = [p, p, p, p, p, p, p, p, i64, i64, i64, i64, i32, i32, i32, p, sz, p]
         L.ple_group_norm_backward_launch.restype = i32
+        L.ple_group_norm_plan_query.argtypes = [p, i64, i64, i64, i64, i32, i32, ctypes.POINTER(GroupNormPlanInfo)]
+        L.ple_group_norm_plan_query.restype = i32
         L.ple_relative_bias_launch.argtypes = [p, p, p, p, i64, i64, i64, i64, i64, i64, i64, i32, i32, i32, p]
         L.ple_relative_bias_launch.restype = i32
         L.ple_relative_bias_backward_workspace_bytes.argtypes = [i64, i64, i64, i64, i64, i64]
@@ -499,6 +514,14 @@ def group_norm_backward(grad_y, x, stats, weight, bias, grad_x, grad_weight, gra
     check(lib().ple_group_norm_backward_launch(
         _ptr(grad_y), _ptr(x), _ptr(stats), _ptr(weight), _ptr(bias), _ptr(grad_x), _ptr(grad_weight), _ptr(grad_bias), n, s,
         c, num_groups, activation, dtype_code(x.dtype), dtype_code(param), _ptr(workspace), need, _stream(stream)))
+
+
+def group_norm_plan(n, s, c, num_groups, dtype=torch.float32, backward=False, x=None) -> dict:
+    """The launch plan for samples [n, s, c] (``x``: a tensor whose alignment counts), as a dict of
+    :class:`GroupNormPlanInfo`'s fields."""
+    info = GroupNormPlanInfo()
+    check(lib().ple_group_norm_plan_query(_ptr(x), n, s, c, num_groups, dtype_code(dtype), int(backward), ctypes.byref(info)))
+    return {name: getattr(info, name) for name, _ in GroupNormPlanInfo._fields_}
 
 
 def relative_bias(weight, buckets, out, starts=None, offset=0, causal=False, stream=None) -> None:

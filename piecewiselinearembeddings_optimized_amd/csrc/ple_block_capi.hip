@@ -127,6 +127,16 @@ int ple_group_norm_backward_launch(const void *grad_y, const void *x, const floa
     return ple::group_backward_run(r);
 }
 
+int ple_group_norm_plan_query(const void *x, int64_t N, int64_t S, int64_t C, int64_t G, int dtype, int backward,
+                              ple_group_norm_plan_info_t *info) {
+    const int rc = ple::check_group(N, S, C, G, dtype);
+    if (rc != PLE_OK) return rc;
+    if (!info) return PLE_E_NULL_POINTER;
+    ple::GroupRequest r = ple::group_request(N, S, C, G, dtype);
+    r.x = x;
+    return ple::group_plan_info(r, backward != 0, info);
+}
+
 int ple_relative_bias_launch(const void *weight, const int32_t *buckets, const int64_t *starts, void *out, int64_t B,
                              int64_t H, int64_t q, int64_t k, int64_t R, int64_t far, int64_t offset, int causal,
                              int weight_dtype, int out_dtype, void *stream) {

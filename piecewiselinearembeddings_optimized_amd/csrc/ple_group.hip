@@ -823,9 +823,10 @@ struct Split {
     int64_t n, row;
     int piece, c0;
     bool on;
-    __device__ __forceinline__ Split(const GroupArgs &a, int E, int64_t blk) {
-        slot = threadIdx.x / a.L;
-        lane = threadIdx.x - slot * a.L;
+    __device__ __forceinline__ Split(const GroupArgs &a, int E, int64_t blk) : Split(a, E, blk, static_cast<int>(threadIdx.x)) {}
+    __host__ __device__ __forceinline__ Split(const GroupArgs &a, int E, int64_t blk, int thread) {
+        slot = thread / a.L;
+        lane = thread - slot * a.L;
         const int64_t u = blk / a.slabs;
         slab = static_cast<int>(blk - u * a.slabs);
         n = u / a.pieces;
@@ -843,9 +844,12 @@ struct SplitChannels {
     Groups<E, false> groups;
     int last;
     __device__ __forceinline__ SplitChannels(const GroupArgs &a, int c0) : groups(a, c0), last(a.G - 1) {
-        load_params(a, a.weight, c0, 1.0f, w);
-        load_params(a, a.bias, c0, 0.0f, b);
+        load_params(a, a.weight, first_param(a, c0), 1.0f, w);
+        load_params(a, a.bias, first_param(a, c0), 0.0f, b);
     }
+    // Where a lane reads its E parameters (the last slab may be narrower: its lanes without
+    // channels read the last ones).
+    __host__ __device__ static __forceinline__ int first_param(const GroupArgs &a, int c0) { return min(c0, a.C - E); }
     __device__ __forceinline__ int of(int e) const { return min(groups.of(e), last); }
 };
 
@@ -1468,6 +1472,32 @@ hipError_t fold(const GroupRequest &r, const GroupArgs &a) {
 size_t group_workspace_bytes(const GroupRequest &r) { return plans_of(r, false).most; }
 
 size_t group_backward_workspace_bytes(const GroupRequest &r) { return plans_of(r, true).most; }
+
+int group_plan_info(const GroupRequest &r, bool backward, ple_group_norm_plan_info_t *info) {
+    *info = ple_group_norm_plan_info_t{};
+    if (r.N == 0 || r.S == 0) return PLE_OK;
+    const GroupPlan &p = plan_group(r, backward);
+    info->form = p.shared ? PLE_GROUP_SHARED : p.held ? PLE_GROUP_HELD : PLE_GROUP_SPLIT;
+    info->lane_channels = p.E;
+    info->slabs = p.slabs;
+    info->members = p.members;
+    info->workspace_bytes = backward ? group_backward_workspace_bytes(r) : group_workspace_bytes(r);
+    info->params_end = r.C;                      // (held and shared: slabs are of one width)
+    if (!p.held) {
+        const GroupArgs a = group_args(r, p);
+        const auto reach = [&](auto e) {
+            constexpr int E = decltype(e)::value;
+            for (int slab = 0; slab < p.slabs; ++slab)
+                for (int t = 0; t < kBlock; ++t)
+                    info->params_end = std::max<int64_t>(info->params_end, SplitChannels<E>::first_param(a, Split(a, E, slab, t).c0) + E);
+        };
+        if (p.E == 8) reach(std::integral_constant<int, 8>{});
+        else if (p.E == 4) reach(std::integral_constant<int, 4>{});
+        else if (p.E == 2) reach(std::integral_constant<int, 2>{});
+        else reach(std::integral_constant<int, 1>{});
+    }
+    return PLE_OK;
+}
 
 int group_run(const GroupRequest &r) {
     if (bad_workspace(r, group_workspace_bytes(r))) return PLE_E_WORKSPACE;

@@ -180,6 +180,7 @@ int group_run(const GroupRequest &r);
 size_t group_workspace_bytes(const GroupRequest &r);
 int group_backward_run(const GroupRequest &r);
 size_t group_backward_workspace_bytes(const GroupRequest &r);
+int group_plan_info(const GroupRequest &r, bool backward, ple_group_norm_plan_info_t *info);
 
 struct BiasRequest {
     const void *weight = nullptr;        // [R, H], of weight_dtype

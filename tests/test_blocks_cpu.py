@@ -313,3 +313,21 @@ def test_example_with_clipping():
     run = lambda **kw: _example().train("cpu", steps=3, rows=512, batch=256, report=lambda s: None, **kw)  # noqa: E731
     assert run(clip=float("inf")) == run()
     assert all(map(torch.isfinite, map(torch.tensor, run(clip=0.1))))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=lambda t: str(t)[6:])
+@pytest.mark.parametrize("s", [1, 4096, 40_000])
+@pytest.mark.parametrize("c,groups", [(1, 1), (60, 5), (77, 7), (520, 1), (960, 10), (1000, 10), (1280, 32), (4098, 2), (9000, 3),
+                                      (20_001, 1), (30_000, 30), (1 << 20, 1)])
+def test_group_norm_parameters_are_read_in_range(c, groups, s, dtype):
+    """Every lane of a row's slabs, the last of which may be narrower than the others:
+    the weight and bias have no channel behind the last."""
+    forms = set()
+    for n in (1, 300):
+        for backward in (False, True):
+            for x in (None, torch.empty(4)[1:], torch.empty(8, dtype=BF16)[1:]):
+                plan = capi.group_norm_plan(n, s, c, groups, dtype, backward, x)
+                assert plan["params_end"] == c, plan
+                forms.add(plan["form"])
+    assert 2 in forms if c >= 1000 and s > 4096 else True
+    assert capi.group_norm_plan(0, s, c, groups)["params_end"] == 0

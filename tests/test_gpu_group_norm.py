@@ -360,3 +360,10 @@ def test_more_than_32_bits_of_elements(ops, n, s, c, groups, last):
     torch.testing.assert_close(gw, gws, rtol=2.0 ** -14, atol=2.0 ** -10)
     torch.testing.assert_close(gb, gbs, rtol=2.0 ** -14, atol=2.0 ** -10)
     assert torch.isfinite(y[:2]).all() and float(gx[:2].abs().max()) == 0
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=lambda t: str(t)[6:])
+@pytest.mark.parametrize("n,s,c,groups", [(2, 300, 520, 1), (1, 800, 1000, 1), (1, 20_000, 1280, 32), (1, 9000, 9000, 3)])
+def test_narrow_last_slab(ops, n, s, c, groups, dtype):
+    """Rows whose slabs are not of one width: lanes without channels in the last."""
+    _check(ops, _inputs(n, s, c, dtype, dtype), groups, SILU)
