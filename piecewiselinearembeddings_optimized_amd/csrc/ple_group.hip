@@ -76,6 +76,23 @@ __device__ __forceinline__ void store_piece(void *p, int64_t i, const float *v) 
     store_out<T, Piece<T, W>::kElems, false>(p, i, v);
 }
 
+// A sample's rows (or its groups' values in them) in shares of one size, the last one
+// smaller.  The host makes the inverses: kernels here divide no floats.  (With divisions in
+// the fold's loop its squares were wrong, other ones each time, wherever two of its waves
+// shared a SIMD.  Seen in its code: several divisions interleaved, a v_div_fmas with its VCC
+// from an s_mov right before it.  That this was the cause is not shown; with the inverses
+// the squares are right.)
+struct Shares {
+    float count, count_last, inv, inv_last;
+    int last;                    // the last share
+    __device__ __forceinline__ float inverse(int share) const { return share == last ? inv_last : inv; }
+    // the squared distance of a share's mean (its sum's), for each of its values
+    __device__ __forceinline__ float distance(float sum, int share, float mean) const {
+        const float d = sum * inverse(share) - mean;
+        return (share == last ? count_last : count) * d * d;
+    }
+};
+
 struct GroupArgs {
     const void *x, *g, *weight, *bias;
     void *y;                     // forward: y; backward: dx
@@ -90,8 +107,9 @@ struct GroupArgs {
     int slabs, Cs, Gs;           // slabs of a row, channels and groups of one
     int team;                    // lanes that join a group
     uint32_t wide_inverse;       // 2^32 / values of a group in a row, rounded up
-    int pieces, piece_rows;      // split: pieces of a sample, rows of one
+    int pieces;                  // split: pieces of a sample
     int folded;                  // split: pieces after the fold
+    Shares share, fold;          // shared: values of a member; split: rows of a piece, of folded ones
     float2 *folds;               // split: [N, folded, C]
     uint64_t *exchange;          // shared: [units, members, Gs] what the members know of a group
     int members, member_rows;    // shared: workgroups of a unit, rows of each
@@ -474,7 +492,7 @@ __global__ __launch_bounds__(THREADS, held_waves(THREADS)) void ple_group_forwar
             x[k].keep();
             add_piece<T, W, WHOLE>(x[k], v[0]);
         }
-        const float inv = SHARED ? 1.0f / (static_cast<float>(rows.count) * static_cast<float>(a.P)) : a.inv;
+        const float inv = SHARED ? a.share.inverse(member) : a.inv;
         join_groups<1, E, WHOLE, THREADS>(a, p, s_lds, v, [&](int q, const float (&s)[1]) {
             s_rho[q] = s[0];
             s_mean[q] = s[0] * inv;
@@ -509,7 +527,7 @@ __global__ __launch_bounds__(THREADS, held_waves(THREADS)) void ple_group_forwar
                 const Rows other(a, rows.n, m, true);
                 const char *const po = px + (other.first - rows.first) * a.C * elem_bytes(T) + at;
                 const int there = p.on ? static_cast<int>(other.count) - p.slot : 0;
-                const float share = 1.0f / (static_cast<float>(other.count) * static_cast<float>(a.P));
+                const float share = a.share.inverse(m);
                 join_rarely<1, E, WHOLE, THREADS>(a, p, s_lds, [&](int e, float (&t)[1]) {
                     t[0] = 0.0f;
                     for (int k = 0; k * a.slots < there; ++k) t[0] += load_grad<T>(po + k * step, e);
@@ -538,10 +556,7 @@ __global__ __launch_bounds__(THREADS, held_waves(THREADS)) void ple_group_forwar
                 if (q < a.Gs)
                     for (int m = lane; m < a.members; m += a.team) {
                         const float2 s = s_known[m * a.Gs + q];
-                        const float n = static_cast<float>(min(a.S - static_cast<int64_t>(m) * a.member_rows,
-                                                               static_cast<int64_t>(a.member_rows))) * static_cast<float>(a.P);
-                        const float d = s.x / n - mu;
-                        t += s.y + n * d * d;
+                        t += s.y + a.share.distance(s.x, m, mu);
                     }
                 t = group_sum_rt(t, a.team);
                 if (q < a.Gs && lane == 0) {
@@ -882,8 +897,7 @@ __global__ __launch_bounds__(kBlock) void ple_group_sums_kernel(GroupArgs a) {
             x[k].clear();
             if (p.on && p.row + k * a.slots < a.S) x[k].load(a.x, (p.n * a.S + p.row + k * a.slots) * a.C + p.c0);
         }
-        const int64_t rows = min(static_cast<int64_t>(a.slots) * kSplitRows, a.S - static_cast<int64_t>(p.piece) * a.slots * kSplitRows);
-        const float inv = 1.0f / static_cast<float>(rows);
+        const float inv = a.share.inverse(p.piece);
         float v[E] = {};
 #pragma unroll
         for (int k = 0; k < kSplitRows; ++k)
@@ -923,24 +937,6 @@ __device__ __forceinline__ float block_sum(float v, float *lds) {
     return s;
 }
 
-// Rows of a piece, and of the last one, as factors.  (With divisions in the fold's loop
-// its squares were wrong, other ones each time, wherever two of its waves shared a SIMD:
-// seen where several divisions interleave, so that a v_div_fmas has its VCC from an s_mov
-// right before it.  No kernel here has such code.)
-struct PieceRows {
-    float count, count_last, inv, inv_last;
-    __device__ __forceinline__ explicit PieceRows(const GroupArgs &a)
-        : count(static_cast<float>(a.piece_rows)),
-          count_last(static_cast<float>(static_cast<int>(a.S - static_cast<int64_t>(a.pieces - 1) * a.piece_rows))),
-          inv(__builtin_amdgcn_rcpf(count)), inv_last(__builtin_amdgcn_rcpf(count_last)) {}
-    // the squared distance of a piece's mean, for each of its rows
-    __device__ __forceinline__ float distance(const GroupArgs &a, float sum, int piece, float mean) const {
-        const bool end = piece == a.pieces - 1;
-        const float d = sum * (end ? inv_last : inv) - mean;
-        return (end ? count_last : count) * d * d;
-    }
-};
-
 // Folds kFold pieces into one, channel by channel: the sums and the squares about the
 // mean (CENTRED), or two sums.  (A sample's groups are too few workgroups to read many
 // pieces: 1 x 60000 x 960 bf16 in 10 groups, 1875 pieces, fold and join of the backward
@@ -955,7 +951,6 @@ __global__ __launch_bounds__(kBlock) void ple_group_fold_kernel(GroupArgs a) {
         const int c = static_cast<int>(i - t * a.C), first = static_cast<int>(t - n * a.folded) * kFold;
         const int last = min(a.pieces, first + kFold);
         const float2 *const p = a.sums + n * a.pieces * a.C + c;
-        const PieceRows rows(a);
         float2 s = make_float2(0.0f, 0.0f);
 #pragma unroll 8
         for (int j = first; j < last; ++j) {
@@ -964,10 +959,10 @@ __global__ __launch_bounds__(kBlock) void ple_group_fold_kernel(GroupArgs a) {
             s.y += v.y;
         }
         if constexpr (CENTRED) {
-            const float mean = s.x * (last < a.pieces ? rows.inv * (1.0f / kFold) : 1.0f / ((last - first - 1) * rows.count + rows.count_last));
+            const float mean = s.x * a.fold.inverse(first / kFold);
             float t = 0.0f;
 #pragma unroll 8
-            for (int j = first; j < last; ++j) t += rows.distance(a, p[static_cast<int64_t>(j) * a.C].x, j, mean);
+            for (int j = first; j < last; ++j) t += a.share.distance(p[static_cast<int64_t>(j) * a.C].x, j, mean);
             s.y += t;
         }
         a.folds[i] = s;
@@ -975,11 +970,11 @@ __global__ __launch_bounds__(kBlock) void ple_group_fold_kernel(GroupArgs a) {
 }
 
 // What the joins read after a fold.
-__host__ __device__ inline GroupArgs folded_args(GroupArgs a) {
+inline GroupArgs folded_args(GroupArgs a) {
     if (a.folded > 0) {
         a.sums = a.folds;
         a.pieces = a.folded;
-        a.piece_rows *= kFold;
+        a.share = a.fold;
     }
     return a;
 }
@@ -997,11 +992,10 @@ __global__ __launch_bounds__(kBlock) void ple_group_stats_kernel(GroupArgs a) {
         for (int64_t i = threadIdx.x; i < all; i += kBlock) t += sums[i / a.P * a.C + i % a.P].x;
         const float mean = block_sum(t, s_lds) * a.inv;
         t = 0.0f;
-        const PieceRows rows(a);
         for (int64_t i = threadIdx.x; i < all; i += kBlock) {
             const int64_t piece = i / a.P;
             const float2 s = sums[piece * a.C + i % a.P];
-            t += s.y + rows.distance(a, s.x, static_cast<int>(piece), mean);
+            t += s.y + a.share.distance(s.x, static_cast<int>(piece), mean);
         }
         t = block_sum(t, s_lds);
         if (threadIdx.x == 0) a.stats[ng] = make_float2(mean, rsqrtf(t * a.inv + a.eps));
@@ -1366,6 +1360,14 @@ const GroupPlan &plan_group(const GroupRequest &r, bool backward) {
 // any start of workgroups takes that are not kept waiting by other work.
 constexpr int kPolls = 4000;
 
+// S rows of P values in shares of `rows` rows
+Shares shares_of(int64_t S, int64_t P, int64_t rows) {
+    const int64_t last = (S - 1) / rows;
+    const double count = static_cast<double>(rows) * P, count_last = static_cast<double>(S - last * rows) * P;
+    return {static_cast<float>(count), static_cast<float>(count_last), static_cast<float>(1 / count),
+            static_cast<float>(1 / count_last), static_cast<int>(last)};
+}
+
 GroupArgs group_args(const GroupRequest &r, const GroupPlan &p) {
     GroupArgs a{};
     a.x = r.x; a.g = r.g; a.weight = r.weight; a.bias = r.bias; a.y = r.y;
@@ -1377,12 +1379,15 @@ GroupArgs group_args(const GroupRequest &r, const GroupPlan &p) {
         a.means = reinterpret_cast<float2 *>(ws + p.o_means);
         a.folds = reinterpret_cast<float2 *>(ws + p.o_folds);
         a.folded = p.folded;
-        a.piece_rows = p.slots * kSplitRows;
+        const int64_t piece_rows = static_cast<int64_t>(p.slots) * kSplitRows;
+        a.share = shares_of(r.S, 1, piece_rows);
+        a.fold = shares_of(r.S, 1, piece_rows * kFold);
     }
     if (p.shared) {
         a.exchange = reinterpret_cast<uint64_t *>(ws + p.o_exchange);
         a.members = p.members;
         a.member_rows = p.member_rows;
+        a.share = shares_of(r.S, r.C / r.G, p.member_rows);
         const int forced = tuning(PLE_TUNE_GROUP_POLLS);
         a.polls = forced > 0 ? forced - 1 : kPolls;
     }
