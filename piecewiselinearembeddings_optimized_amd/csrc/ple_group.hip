@@ -612,30 +612,30 @@ __device__ __forceinline__ void leave_sums(const GroupArgs &a, const Place &p, f
     }
 }
 
-// What a lane's channels are multiplied with: z = x scale + shift.  (Folded so that a
-// lane holds two values a channel; the products' roundings are of the size that the
-// mean's own has.)
+// A lane's channels before the activation: z = (x - mean) scale + bias, in the order and with
+// the roundings of the forward, so that a relu's gradient passes where its output is above 0.
 template <int E, bool WHOLE>
 struct Affine {
-    float scale[E], shift[E];
-    __device__ __forceinline__ Affine(const float *weight, const float *bias, const float2 *stats, const Groups<E, WHOLE> &groups) {
+    float scale[E], bias[E], mean[WHOLE ? 1 : E];
+    __device__ __forceinline__ Affine(const float *weight, const float *biases, const float2 *stats, const Groups<E, WHOLE> &groups) {
         staged(weight, scale);
-        staged(bias, shift);
+        staged(biases, bias);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const float2 st = stats[groups.of(e)];
             scale[e] *= st.y;
-            shift[e] -= st.x * scale[e];
+            mean[WHOLE ? 0 : e] = st.x;
         }
     }
+    __device__ __forceinline__ float operator()(float x, int e) const { return (x - mean[WHOLE ? 0 : e]) * scale[e] + bias[e]; }
 };
 
 // A piece's gradient before the activation.
-template <int T, int W, int E>
-__device__ __forceinline__ void piece_grad(int act, const Piece<T, W> &x, const Piece<T, W> &g, const float (&scale)[E],
-                                           const float (&shift)[E], float (&dz)[E]) {
+template <int T, int W, int E, bool WHOLE>
+__device__ __forceinline__ void piece_grad(int act, const Piece<T, W> &x, const Piece<T, W> &g, const Affine<E, WHOLE> &f,
+                                           float (&dz)[E]) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) dz[e] = x[e] * scale[e] + shift[e];
+    for (int e = 0; e < E; ++e) dz[e] = f(x[e], e);
     slopes(dz, act);
 #pragma unroll
     for (int e = 0; e < E; ++e) dz[e] *= g[e];
@@ -720,7 +720,7 @@ __global__ __launch_bounds__(THREADS, SHARED ? 3 : 2) void ple_group_backward_ke
                 __builtin_amdgcn_sched_barrier(0);
                 // (a row that is not there has a gradient of 0)
                 float (&dz)[E] = grad[kKept ? k : 0];
-                piece_grad<T, W>(act, x[k], g[k], f.scale, f.shift, dz);
+                piece_grad<T, W>(act, x[k], g[k], f, dz);
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     sum[0][e] += dz[e];
@@ -758,11 +758,11 @@ __global__ __launch_bounds__(THREADS, SHARED ? 3 : 2) void ple_group_backward_ke
                 const int there = p.on ? static_cast<int>(other.count) - p.slot : 0;
                 join_rarely<2, E, WHOLE, THREADS>(a, p, s_lds, [&](int e, float (&t)[2]) {
                     const float2 st = stats[groups.of(e)];
-                    const float w = own_params[e], scale[1] = {w * st.y}, shift[1] = {own_params[a.Cs + e] - st.x * scale[0]};
+                    const float w = own_params[e], scale = w * st.y, bias = own_params[a.Cs + e];
                     t[0] = t[1] = 0.0f;
                     for (int k = 0; k * a.slots < there; ++k) {
                         const float v = load_grad<T>(px + away + k * step, e);
-                        float dz[1] = {v * scale[0] + shift[0]};
+                        float dz[1] = {(v - st.x) * scale + bias};
                         slopes(dz, act);
                         dz[0] *= load_grad<T>(pg + away + k * step, e);
                         t[0] += dz[0];
@@ -806,7 +806,7 @@ __global__ __launch_bounds__(THREADS, SHARED ? 3 : 2) void ple_group_backward_ke
             if constexpr (!kKept) g[k].keep();
             __builtin_amdgcn_sched_barrier(0);
             float (&dz)[E] = grad[kKept ? k : 0];
-            if constexpr (!kKept) piece_grad<T, W>(act, x[k], g[k], f.scale, f.shift, dz);
+            if constexpr (!kKept) piece_grad<T, W>(act, x[k], g[k], f, dz);
 #pragma unroll
             for (int e = 0; e < E; ++e)
                 dz[e] = dz[e] * f.scale[e] + (x[k][e] * along[WHOLE ? 0 : e] + level[WHOLE ? 0 : e]);
@@ -1060,8 +1060,9 @@ __global__ __launch_bounds__(kBlock) void ple_group_backward_sums_kernel(GroupAr
                     float xh[E], dz[E];
 #pragma unroll
                     for (int e = 0; e < E; ++e) {
-                        xh[e] = (x[k][e] - st[e].x) * st[e].y;
-                        dz[e] = xh[e] * ch.w[e] + ch.b[e];
+                        const float d = x[k][e] - st[e].x;
+                        xh[e] = d * st[e].y;
+                        dz[e] = d * (st[e].y * ch.w[e]) + ch.b[e];       // (as the forward)
                     }
                     slopes(dz, a.act);
 #pragma unroll
@@ -1147,8 +1148,9 @@ __global__ __launch_bounds__(kBlock) void ple_group_backward_apply_kernel(GroupA
                 float xh[E], dz[E];
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
-                    xh[e] = (x[k][e] - st[e].x) * st[e].y;
-                    dz[e] = xh[e] * ch.w[e] + ch.b[e];
+                    const float d = x[k][e] - st[e].x;
+                    xh[e] = d * st[e].y;
+                    dz[e] = d * (st[e].y * ch.w[e]) + ch.b[e];
                 }
                 slopes(dz, a.act);
 #pragma unroll

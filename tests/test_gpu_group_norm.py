@@ -367,3 +367,24 @@ def test_more_than_32_bits_of_elements(ops, n, s, c, groups, last):
 def test_narrow_last_slab(ops, n, s, c, groups, dtype):
     """Rows whose slabs are not of one width: lanes without channels in the last."""
     _check(ops, _inputs(n, s, c, dtype, dtype), groups, SILU)
+
+
+# held in one workgroup and several a slab, shared, split
+FORMS = [(6, 40, 32, 4), (300, 64, 64, 8), (40, 30, 250, 10), (2, 9001, 40, 5), (2, 9001, 41, 1), (8, 4096, 64, 8), (2, 3, 9000, 3),
+         (1, 90_001, 1000, 10)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=lambda t: str(t)[6:])
+@pytest.mark.parametrize("level", [1.0, 3000.0])
+@pytest.mark.parametrize("n,s,c,groups", FORMS)
+def test_relu_passes_where_its_output_is_positive(ops, n, s, c, groups, level, dtype):
+    """The backward's value before the activation is the forward's, bit for bit: a gradient
+    of ones gives the bias as many as outputs are above 0 (whole numbers below 2^24), in
+    constant groups too, where that is rounding alone."""
+    x = _inputs(n, s, c, dtype, F32, level=level)
+    x["x"][0, :, :c // groups] = 2.7
+    x["g"] = torch.ones_like(x["g"])
+    for bias in (torch.zeros(c), x["bias"]):
+        got, _ = _run(ops, x | {"bias": bias}, groups, RELU)
+        assert torch.equal(got[3], (got[0] > 0).sum((0, 1)).float())
+        assert not bool(got[1][:, :, -(c // groups):][(got[0] > 0).any((1, 2)).logical_not()].any())
