@@ -627,7 +627,8 @@ struct Affine {
             mean[WHOLE ? 0 : e] = st.x;
         }
     }
-    __device__ __forceinline__ float operator()(float x, int e) const { return (x - mean[WHOLE ? 0 : e]) * scale[e] + bias[e]; }
+    __device__ __forceinline__ float distance(float x, int e) const { return x - mean[WHOLE ? 0 : e]; }
+    __device__ __forceinline__ float operator()(float x, int e) const { return distance(x, e) * scale[e] + bias[e]; }
 };
 
 // A piece's gradient before the activation.
@@ -641,14 +642,12 @@ __device__ __forceinline__ void piece_grad(int act, const Piece<T, W> &x, const 
     for (int e = 0; e < E; ++e) dz[e] *= g[e];
 }
 
-// Sums of dz and dz x of a lane's channels -> of dz and dz xh.
+// Sums of dz and dz (x - mean) of a lane's channels -> of dz and dz xh.  (Of dz x, less mean
+// times the sum of dz, they lost what the mean is larger than the deviation.)
 template <int E, bool WHOLE>
 __device__ __forceinline__ void standard_sums(const float2 *stats, const Groups<E, WHOLE> &groups, float (&sum)[2][E]) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const float2 st = stats[groups.of(e)];
-        sum[1][e] = st.y * (sum[1][e] - st.x * sum[0][e]);
-    }
+    for (int e = 0; e < E; ++e) sum[1][e] *= stats[groups.of(e)].y;
 }
 
 // ... weighted, by group where a piece is of one.
@@ -724,7 +723,7 @@ __global__ __launch_bounds__(THREADS, SHARED ? 3 : 2) void ple_group_backward_ke
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     sum[0][e] += dz[e];
-                    sum[1][e] += dz[e] * x[k][e];
+                    sum[1][e] += dz[e] * f.distance(x[k][e], e);
                     // (here, and not where the sums are used: the terms would all be held)
                     asm volatile("" : "+v"(sum[0][e]), "+v"(sum[1][e]), "+v"(dz[e]));
                 }
@@ -761,14 +760,14 @@ __global__ __launch_bounds__(THREADS, SHARED ? 3 : 2) void ple_group_backward_ke
                     const float w = own_params[e], scale = w * st.y, bias = own_params[a.Cs + e];
                     t[0] = t[1] = 0.0f;
                     for (int k = 0; k * a.slots < there; ++k) {
-                        const float v = load_grad<T>(px + away + k * step, e);
-                        float dz[1] = {(v - st.x) * scale + bias};
+                        const float d = load_grad<T>(px + away + k * step, e) - st.x;
+                        float dz[1] = {d * scale + bias};
                         slopes(dz, act);
                         dz[0] *= load_grad<T>(pg + away + k * step, e);
                         t[0] += dz[0];
-                        t[1] += dz[0] * v;
+                        t[1] += dz[0] * d;
                     }
-                    t[1] = st.y * (t[1] - st.x * t[0]) * w;
+                    t[1] *= st.y * w;
                     t[0] *= w;
                 }, [&](int q, const float (&r)[2]) { s_known[m * a.Gs + q] = make_float2(r[0], r[1]); });
             });
@@ -790,7 +789,7 @@ __global__ __launch_bounds__(THREADS, SHARED ? 3 : 2) void ple_group_backward_ke
             }
             __syncthreads();
         }
-        // dx = dz scale + x along + level
+        // dx = dz scale + (x - mean) along + level
         const Affine<E, WHOLE> f(own_params, own_params + a.Cs, stats, groups);
         float along[kEach], level[kEach];
 #pragma unroll
@@ -798,7 +797,7 @@ __global__ __launch_bounds__(THREADS, SHARED ? 3 : 2) void ple_group_backward_ke
             const float2 st = stats[groups.of(e)];
             const int q = own + groups.of(e);
             along[e] = -st.y * st.y * s_m2[q];
-            level[e] = -st.y * s_m1[q] - along[e] * st.x;
+            level[e] = -st.y * s_m1[q];
         }
 #pragma unroll
         for (int k = 0; k < R; ++k) {
@@ -809,7 +808,7 @@ __global__ __launch_bounds__(THREADS, SHARED ? 3 : 2) void ple_group_backward_ke
             if constexpr (!kKept) piece_grad<T, W>(act, x[k], g[k], f, dz);
 #pragma unroll
             for (int e = 0; e < E; ++e)
-                dz[e] = dz[e] * f.scale[e] + (x[k][e] * along[WHOLE ? 0 : e] + level[WHOLE ? 0 : e]);
+                dz[e] = dz[e] * f.scale[e] + (f.distance(x[k][e], e) * along[WHOLE ? 0 : e] + level[WHOLE ? 0 : e]);
             if (has(k)) store_piece<T, W>(py + k * step + at, 0, dz);
         }
         if constexpr (SHARED) break;

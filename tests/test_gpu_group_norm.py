@@ -388,3 +388,32 @@ def test_relu_passes_where_its_output_is_positive(ops, n, s, c, groups, level, d
         got, _ = _run(ops, x | {"bias": bias}, groups, RELU)
         assert torch.equal(got[3], (got[0] > 0).sum((0, 1)).float())
         assert not bool(got[1][:, :, -(c // groups):][(got[0] > 0).any((1, 2)).logical_not()].any())
+
+
+@pytest.mark.parametrize("n,s,c,groups", [(6, 40, 32, 4), (300, 64, 64, 8), (40, 30, 250, 10), (2, 9000, 40, 5), (2, 9002, 41, 1),
+                                          (8, 4096, 64, 8), (2, 4, 9000, 3), (1, 90_000, 1000, 10)])
+def test_sums_are_about_the_mean(ops, n, s, c, groups):
+    """Groups whose mean is tens of thousands of deviations: the gradients lose nothing by it.
+    x - mean is exact here (the mean a power of 2, deviations in pairs), the statistics are
+    given; so a sum of terms is off by 64 roundings of their sizes, as one without a mean."""
+    gen = torch.Generator().manual_seed(n + s + c)
+    p, level = c // groups, 2.0 ** 15
+    d = (torch.randn(n, s // 2, c, generator=gen) * 2 ** 7).round() / 2 ** 7
+    d = torch.cat([d, -d], 1)
+    x, g = level + d, torch.randn(n, s, c, generator=gen)
+    w = 1 + 0.3 * torch.randn(c, generator=gen)
+    assert torch.equal(x.double() - level, d.double())
+    grouped = lambda t: t.reshape(n, s, groups, p)  # noqa: E731
+    rho = (grouped(d.double()).square().mean((1, 3)) + EPS).rsqrt().float()
+    stats = torch.stack([torch.full_like(rho, level), rho], -1)
+    got = ops.group_norm_backward(g.to(DEV), x.to(DEV), stats.to(DEV), w.to(DEV), torch.zeros(c, device=DEV), groups, NONE,
+                                  [True] * 3)
+    r = rho.double().repeat_interleave(p, 1)[:, None]
+    xh, gw = d.double() * r, g.double() * w.double()
+    mean = lambda t: grouped(t).mean((1, 3)).repeat_interleave(p, 1)[:, None]  # noqa: E731
+    want = [r * (gw - mean(gw) - xh * mean(gw * xh)), (g * xh).sum((0, 1)), g.double().sum((0, 1))]
+    err = [r * (gw.abs() + mean(gw.abs()) + xh.abs() * mean((gw * xh).abs())), (g * xh).abs().sum((0, 1)),
+           g.double().abs().sum((0, 1))]
+    for name, a, b, e in zip(("dx", "dw", "db"), got, want, err):
+        off = (a.cpu().double() - b).abs() / (E * e + TINY[F32])
+        assert bool((off <= 1).all()), (name, float(off.max()))
