@@ -10,6 +10,7 @@
 
 namespace {
 
+using c10::SymInt;
 using Tensors2 = std::tuple<Tensor, Tensor>;
 using Tensors3 = std::tuple<Tensor, Tensor, Tensor>;
 
@@ -18,9 +19,9 @@ PLE_OP(op_group_norm_backward, "group_norm_backward",
        Tensors3(const Tensor &, const Tensor &, const Tensor &, const OptTensor &, const OptTensor &, int64_t, int64_t,
                 std::array<bool, 3>))
 PLE_OP(op_relative_bias, "relative_bias",
-       Tensor(const Tensor &, const Tensor &, const OptTensor &, int64_t, int64_t, int64_t, bool, at::ScalarType))
+       Tensor(const Tensor &, const Tensor &, const OptTensor &, SymInt, SymInt, SymInt, bool, at::ScalarType))
 PLE_OP(op_relative_bias_backward, "relative_bias_backward",
-       Tensor(const Tensor &, const Tensor &, const OptTensor &, int64_t, int64_t, bool, at::ScalarType))
+       Tensor(const Tensor &, const Tensor &, const OptTensor &, SymInt, SymInt, bool, at::ScalarType))
 
 OptTensor maybe(const Tensor &t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 
@@ -66,13 +67,13 @@ Tensors2 group_norm(DispatchKeySet ks, const Tensor &x, const OptTensor &weight,
 struct RelativeBias : torch::autograd::Function<RelativeBias> {
     static constexpr bool is_traceable = true;
     static Tensor forward(AutogradContext *ctx, DispatchKeySet ks, const Tensor &weight, const Tensor &buckets,
-                          const OptTensor &starts, int64_t q_len, int64_t k_len, int64_t offset, bool causal,
+                          const OptTensor &starts, SymInt q_len, SymInt k_len, SymInt offset, bool causal,
                           at::ScalarType output_dtype) {
         at::AutoDispatchBelowAutograd guard;
         Tensor out = op_relative_bias().redispatch(below(ks), weight, buckets, starts, q_len, k_len, offset, causal,
                                                    output_dtype);
         ctx->save_for_backward({buckets, starts.value_or(Tensor())});
-        ctx->saved_data["rows"] = weight.size(0);
+        ctx->saved_data["rows"] = weight.sym_size(0);
         ctx->saved_data["offset"] = offset;
         ctx->saved_data["causal"] = causal;
         ctx->saved_data["dtype"] = static_cast<int64_t>(weight.scalar_type());
@@ -83,15 +84,16 @@ struct RelativeBias : torch::autograd::Function<RelativeBias> {
         variable_list r(9);
         if (!grads[0].defined()) return r;
         const auto s = ctx->get_saved_variables();
-        r[1] = op_relative_bias_backward().call(grads[0].contiguous(), s[0], maybe(s[1]), ctx->saved_data["rows"].toInt(),
-                                                ctx->saved_data["offset"].toInt(), ctx->saved_data["causal"].toBool(),
+        r[1] = op_relative_bias_backward().call(grads[0].contiguous(), s[0], maybe(s[1]), ctx->saved_data["rows"].toSymInt(),
+                                                ctx->saved_data["offset"].toSymInt(), ctx->saved_data["causal"].toBool(),
                                                 static_cast<at::ScalarType>(ctx->saved_data["dtype"].toInt()));
         return r;
     }
 };
 
-Tensor relative_bias(DispatchKeySet ks, const Tensor &weight, const Tensor &buckets, const OptTensor &starts, int64_t q_len,
-                     int64_t k_len, int64_t offset, bool causal, at::ScalarType output_dtype) {
+// (lengths, the offset and the table's rows are symbols where a graph is made for all of them)
+Tensor relative_bias(DispatchKeySet ks, const Tensor &weight, const Tensor &buckets, const OptTensor &starts, SymInt q_len,
+                     SymInt k_len, SymInt offset, bool causal, at::ScalarType output_dtype) {
     if (!recorded(weight)) {
         at::AutoDispatchBelowAutograd guard;
         return op_relative_bias().redispatch(below(ks), weight, buckets, starts, q_len, k_len, offset, causal, output_dtype);

@@ -383,10 +383,10 @@ TORCH_LIBRARY_FRAGMENT(rtdl_num_embeddings_cuda, m) {
         "group_norm_backward(Tensor grad_y, Tensor x, Tensor stats, Tensor? weight, Tensor? bias, int num_groups, "
         "int activation, bool[3] output_mask) -> (Tensor grad_x, Tensor grad_weight, Tensor grad_bias)");
     m.def(
-        "relative_bias(Tensor weight, Tensor buckets, Tensor? starts, int q_len, int k_len, int offset, bool causal, "
+        "relative_bias(Tensor weight, Tensor buckets, Tensor? starts, SymInt q_len, SymInt k_len, SymInt offset, bool causal, "
         "ScalarType output_dtype) -> Tensor");
     m.def(
-        "relative_bias_backward(Tensor grad_output, Tensor buckets, Tensor? starts, int num_rows, int offset, "
+        "relative_bias_backward(Tensor grad_output, Tensor buckets, Tensor? starts, SymInt num_rows, SymInt offset, "
         "bool causal, ScalarType grad_dtype) -> Tensor");
     m.def("gradient_norm(Tensor[] grads, float norm_type) -> Tensor");
     m.def("clip_gradients_(Tensor(a!)[] grads, float max_norm, float norm_type, Tensor? norm) -> Tensor");

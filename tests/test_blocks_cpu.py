@@ -331,3 +331,52 @@ def test_group_norm_parameters_are_read_in_range(c, groups, s, dtype):
                 forms.add(plan["form"])
     assert 2 in forms if c >= 1000 and s > 4096 else True
     assert capi.group_norm_plan(0, s, c, groups)["params_end"] == 0
+
+
+@pytest.mark.parametrize("train", [False, True])
+@pytest.mark.parametrize("with_starts", [False, True])
+@pytest.mark.parametrize("queries", [1, 4, None])
+def test_relative_bias_compiles_once_for_all_lengths(queries, with_starts, train):
+    """A decoding loop: a key more each time (queries None: as many queries as keys).  The
+    first length and the lengths' symbol are the two graphs."""
+    graphs = []
+
+    def count(gm, inputs):
+        graphs.append(gm)
+        return gm.forward
+
+    from torch._dynamo.backends.common import aot_autograd
+
+    torch._dynamo.reset()
+    starts = _meta(3, dtype=torch.int64) if with_starts else None
+    buckets = _meta(9, dtype=torch.int32)
+
+    def step(weight, k_len):
+        q_len = k_len if queries is None else queries
+        return _ops.relative_bias(weight, buckets, starts, q_len, k_len, k_len - q_len, True, F32) * 2
+
+    compiled = torch.compile(step, backend=aot_autograd(fw_compiler=count, bw_compiler=lambda gm, _: gm.forward), fullgraph=True)
+    for k_len in range(10, 30):
+        weight = _meta(6, 4).requires_grad_(train)
+        out = compiled(weight, k_len)
+        assert out.shape[-2:] == (queries or k_len, k_len)
+        if train:
+            assert torch.autograd.grad(out.sum(), weight)[0].shape == (6, 4)
+    torch._dynamo.reset()
+    assert len(graphs) == 2
+
+
+def test_relative_bias_compiles_with_symbolic_tables():
+    """Every size a symbol, the table's rows and heads too."""
+    torch._dynamo.reset()
+
+    def step(weight, buckets, x):
+        return _ops.relative_bias(weight, buckets, None, x.shape[0], x.shape[1], x.shape[1] - x.shape[0], False, F32).sum()
+
+    compiled = torch.compile(step, backend="aot_eager", fullgraph=True, dynamic=True)
+    for r, h, q, k in ((6, 4, 3, 5), (7, 5, 4, 8), (9, 2, 2, 3)):
+        weight = _meta(r, h).requires_grad_()
+        with torch._dynamo.config.patch(error_on_recompile=r > 6):
+            (grad,) = torch.autograd.grad(compiled(weight, _meta(2 * r + 1, dtype=torch.int32), _meta(q, k)), weight)
+        assert grad.shape == (r, h)
+    torch._dynamo.reset()

@@ -350,3 +350,29 @@ def test_example_with_clipping():
     run = lambda **kw: _example().train("cuda", steps=3, rows=512, batch=256, report=lambda s: None, **kw)  # noqa: E731
     assert run(clip=float("inf")) == run()
     assert all(map(torch.isfinite, map(torch.tensor, run(clip=0.1))))
+
+
+@pytest.mark.parametrize("train", [False, True])
+@pytest.mark.parametrize("with_starts", [False, True])
+def test_compiled_decoding(package, with_starts, train):
+    """A compiled module that gets a key more each time is compiled for the first length, and
+    once for all others."""
+    bias = package.CudaRelativeBias(8, 2, max_distance=16, bidirectional=False, causal=True).to(DEV)
+    starts = torch.tensor([3, 9], device=DEV) if with_starts else None
+    graphs = []
+
+    def backend(gm, inputs):
+        graphs.append(gm)
+        return torch._dynamo.backends.registry.lookup_backend("aot_eager")(gm, inputs)
+
+    torch._dynamo.reset()
+    compiled = torch.compile(lambda q, k: bias(q, k, starts=starts) * 2, backend=backend, fullgraph=True)
+    for k in range(10, 30):
+        with torch.set_grad_enabled(train):
+            want, got = bias(1, k, starts=starts) * 2, compiled(1, k)
+        assert torch.equal(got, want)
+        if train:
+            g = _rand(*want.shape)
+            assert torch.equal(*(torch.autograd.grad(out, bias.weight, g)[0] for out in (got, want)))
+    torch._dynamo.reset()
+    assert len(graphs) == 2
