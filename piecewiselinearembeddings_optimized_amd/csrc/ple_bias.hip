@@ -322,6 +322,9 @@ __device__ __forceinline__ void add_vectors(const uint4 (&raw)[N], int back, flo
     }
 }
 
+// Elements of the gradient (samples times heads alone may pass 32 bits).
+__device__ __forceinline__ int64_t elements(const BiasArgs &a) { return static_cast<int64_t>(a.B) * a.H * a.q * a.k; }
+
 // The tensor's first elements that lie before its first 16-byte boundary, and its last
 // ones behind the last: the vectors that hold them are not all in its memory.
 // (apart_last of them end the last row, which has all of them: k >= E)
@@ -334,7 +337,7 @@ __device__ __forceinline__ int apart_first(const BiasArgs &a) {
 template <int T>
 __device__ __forceinline__ int apart_last(const BiasArgs &a) {
     constexpr int E = vec_elems<T>();
-    return static_cast<int>((reinterpret_cast<uint64_t>(a.grad) / elem_bytes(T) + a.B * a.H * a.q * a.k) % E);
+    return static_cast<int>((reinterpret_cast<uint64_t>(a.grad) / elem_bytes(T) + elements(a)) % E);
 }
 
 // Sums along diagonals.  Rows E apart (E: elements of 16 bytes) have their vector
@@ -448,7 +451,7 @@ __device__ __forceinline__ float apart_sum(const BiasArgs &a, int h, int e) {
     float s = 0.0f;
     if (a.k < vec_elems<T>()) return s;
     const int first = apart_first<T>(a), last = apart_last<T>(a);
-    const int64_t far = a.far, end = a.B * a.H * a.q * a.k;
+    const int64_t far = a.far, end = elements(a);
     const auto add = [&](int64_t at, int64_t b, int64_t i, int64_t j) {
         const int64_t d = j - start_of(a, b) - i;
         if (!(a.causal && d > 0) && min(max(d, -far), far) == e) s += load_grad<T>(a.grad, at);

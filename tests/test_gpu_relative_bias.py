@@ -217,3 +217,23 @@ def test_refusals(ops):
     for call, text in bad:
         with pytest.raises(RuntimeError, match=text):
             call()
+
+
+def test_gradient_of_more_than_32_bits_of_heads(ops):
+    """Samples and heads whose product passes 32 bits, behind which the tensor's last
+    elements lie that no whole vector holds."""
+    if torch.cuda.mem_get_info()[0] < 80 << 30:
+        pytest.skip("needs 80 GB")
+    n, k = 46_341, 9                                             # n * n * k = 8 * vectors + 1
+    g = torch.zeros(n, n, 1, k, dtype=torch.bfloat16, device=DEV)
+    g[-1, -1, 0] = torch.arange(1, k + 1)
+    g[0, 0, 0] = 1
+    buckets = torch.tensor([0, 1, 2], dtype=torch.int32, device=DEV)
+    starts = torch.full((n,), 4, device=DEV)
+    got = ops.relative_bias_backward(g, buckets, starts, 3, 0, False, torch.float32)
+    del g
+    torch.cuda.empty_cache()
+    want = torch.zeros(3, n)
+    want[:, 0] = torch.tensor([4.0, 1.0, 4.0])
+    want[:, -1] = torch.tensor([1.0 + 2 + 3 + 4, 5, 6 + 7 + 8 + 9])
+    assert torch.equal(got.cpu(), want)
