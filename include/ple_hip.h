@@ -488,9 +488,9 @@ int ple_distill_backward_launch(const float *grad_loss, const void *logits, cons
  *   workspace    >= ple_group_norm_workspace_bytes() bytes (0 is possible),
  *                256-byte aligned, need not be initialised
  * Results share no memory with anything that is read.
- * Statistics and sums are 32-bit in a fixed order (where workgroups that share a
- * sample wait in vain for each other, milliseconds, they compute what is missing
- * themselves, which may round otherwise).  C <= 2^20, S < 2^31, N < 2^31,
+ * Statistics and sums are 32-bit in a fixed order (workgroups that share a sample
+ * and wait in vain for each other, milliseconds, compute what is missing
+ * themselves, to the same bits).  C <= 2^20, S < 2^31, N < 2^31,
  * N * S * C < 2^44 (else PLE_E_TOO_LARGE); G divides C (else PLE_E_BAD_SHAPE).
  */
 enum {

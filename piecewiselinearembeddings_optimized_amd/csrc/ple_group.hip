@@ -122,12 +122,17 @@ struct GroupArgs {
 // activations
 // ---------------------------------------------------------------------------
 
+// (What workgroups compute in each other's place, and what the backward repeats of the
+// forward, has to have the same bits wherever it is compiled: such products and sums are
+// fused by fmaf, or not at all.)
+
 // Standard normal distribution and density at z.  Abramowitz and Stegun 26.2.17: the
 // tail is the density times a polynomial in 1 / (1 + p |z|), off by at most 7.5e-8.
 __device__ __forceinline__ void normal_cdf(float z, float &cdf, float &pdf) {
+#pragma clang fp contract(off)
     pdf = 0.39894228f * __expf(-0.5f * z * z);
-    const float t = __builtin_amdgcn_rcpf(1.0f + 0.2316419f * fabsf(z));
-    const float tail = pdf * t * (0.319381530f + t * (-0.356563782f + t * (1.781477937f + t * (-1.821255978f + t * 1.330274429f))));
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.2316419f, fabsf(z), 1.0f));
+    const float tail = pdf * t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.330274429f, -1.821255978f), 1.781477937f), -0.356563782f), 0.319381530f);
     cdf = z > 0.0f ? 1.0f - tail : tail;
 }
 
@@ -161,14 +166,14 @@ __device__ __forceinline__ void slopes(float (&z)[E], int act) {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const float s = logistic(z[e]);
-            z[e] = s + z[e] * s * (1.0f - s);
+            z[e] = fmaf(z[e] * s, 1.0f - s, s);
         }
     } else if (act == PLE_ACT_GELU) {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             float cdf, pdf;
             normal_cdf(z[e], cdf, pdf);
-            z[e] = cdf + z[e] * pdf;
+            z[e] = fmaf(z[e], pdf, cdf);
         }
     } else {
 #pragma unroll
@@ -311,25 +316,27 @@ __device__ __forceinline__ void join_groups(const GroupArgs &a, const Place &p, 
     join_lds<K, E, WHOLE, THREADS>(a, p, lds, done);
 }
 
-// The same for values that `lane_value(e, values)` computes one channel after the other: for
-// what is rarely done, in few registers.
-template <int K, int E, bool WHOLE, int THREADS, typename V, typename F>
-__device__ __forceinline__ void join_rarely(const GroupArgs &a, const Place &p, float *lds, V lane_value, F done) {
+// The same for values that `add(e, values)` adds up: for what is rarely done, in few
+// registers.  CALLS: 1, for all of a lane's channels at once (WHOLE), or E, one after the
+// other, as the lanes that do it ordinarily add them.
+template <int K, int CALLS, int E, bool WHOLE, int THREADS, typename V, typename F>
+__device__ __forceinline__ void join_rarely(const GroupArgs &a, const Place &p, float *lds, V add, F done) {
     constexpr int kStride = kPlane<THREADS>;
-    float sum[K] = {};
+    static_assert(CALLS == E || (WHOLE && CALLS == 1));
+    float v[K] = {};
 #pragma unroll 1
-    for (int e = 0; e < E; ++e) {
-        float v[K];
-        lane_value(e, v);
+    for (int e = 0; e < CALLS; ++e) {
+        add(e, v);
+        if constexpr (!WHOLE)
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            sum[k] += v[k];
-            if constexpr (!WHOLE) lds[(k * E + e) * kStride + p.thread] = v[k];
-        }
+            for (int k = 0; k < K; ++k) {
+                lds[(k * E + e) * kStride + p.thread] = v[k];
+                v[k] = 0.0f;
+            }
     }
     if constexpr (WHOLE)
 #pragma unroll
-        for (int k = 0; k < K; ++k) lds[k * kStride + p.thread] = sum[k];
+        for (int k = 0; k < K; ++k) lds[k * kStride + p.thread] = v[k];
     join_lds<K, E, WHOLE, THREADS>(a, p, lds, done);
 }
 
@@ -436,7 +443,7 @@ __device__ __forceinline__ void add_squares(const Piece<T, W> &x, const float (&
 #pragma unroll
     for (int e = 0; e < Piece<T, W>::kElems; ++e) {
         const float d = x[e] - mean[WHOLE ? 0 : e];
-        v[WHOLE ? 0 : e] += d * d;
+        v[WHOLE ? 0 : e] = fmaf(d, d, v[WHOLE ? 0 : e]);
     }
 }
 
@@ -528,20 +535,21 @@ __global__ __launch_bounds__(THREADS, held_waves(THREADS)) void ple_group_forwar
                 const char *const po = px + (other.first - rows.first) * a.C * elem_bytes(T) + at;
                 const int there = p.on ? static_cast<int>(other.count) - p.slot : 0;
                 const float share = a.share.inverse(m);
-                join_rarely<1, E, WHOLE, THREADS>(a, p, s_lds, [&](int e, float (&t)[1]) {
-                    t[0] = 0.0f;
-                    for (int k = 0; k * a.slots < there; ++k) t[0] += load_grad<T>(po + k * step, e);
+                constexpr int kCalls = WHOLE ? 1 : E;
+                join_rarely<1, kCalls, E, WHOLE, THREADS>(a, p, s_lds, [&](int e0, float (&t)[1]) {
+                    for (int k = 0; k * a.slots < there; ++k)
+                        for (int e = e0; e < e0 + E / kCalls; ++e) t[0] += load_grad<T>(po + k * step, e);
                 }, [&](int q, const float (&s)[1]) {
                     s_rho[q] = s[0];
                     s_mean[q] = s[0] * share;
                 });
-                join_rarely<1, E, WHOLE, THREADS>(a, p, s_lds, [&](int e, float (&t)[1]) {
-                    t[0] = 0.0f;
-                    const float mu = s_mean[own + groups.of(e)];
-                    for (int k = 0; k * a.slots < there; ++k) {
-                        const float d = load_grad<T>(po + k * step, e) - mu;
-                        t[0] += d * d;
-                    }
+                join_rarely<1, kCalls, E, WHOLE, THREADS>(a, p, s_lds, [&](int e0, float (&t)[1]) {
+                    const float mu = s_mean[own + groups.of(e0)];
+                    for (int k = 0; k * a.slots < there; ++k)
+                        for (int e = e0; e < e0 + E / kCalls; ++e) {
+                            const float d = load_grad<T>(po + k * step, e) - mu;
+                            t[0] = fmaf(d, d, t[0]);
+                        }
                 }, [&](int q, const float (&s)[1]) { s_known[m * a.Gs + q] = make_float2(s_rho[q], s[0]); });
             });
             // the unit's mean, and its squares about it: the members' own, and their means' distance
@@ -582,7 +590,7 @@ __global__ __launch_bounds__(THREADS, held_waves(THREADS)) void ple_group_forwar
             if (has(k)) {
                 float z[E];
 #pragma unroll
-                for (int e = 0; e < E; ++e) z[e] = (x[k][e] - mean[WHOLE ? 0 : e]) * scale[e] + bias[e];
+                for (int e = 0; e < E; ++e) z[e] = fmaf(x[k][e] - mean[WHOLE ? 0 : e], scale[e], bias[e]);
                 activate(z, act);
                 store_piece<T, W>(py + k * step + at, 0, z);
             }
@@ -628,13 +636,14 @@ struct Affine {
         }
     }
     __device__ __forceinline__ float distance(float x, int e) const { return x - mean[WHOLE ? 0 : e]; }
-    __device__ __forceinline__ float operator()(float x, int e) const { return distance(x, e) * scale[e] + bias[e]; }
+    __device__ __forceinline__ float operator()(float x, int e) const { return fmaf(distance(x, e), scale[e], bias[e]); }
 };
 
 // A piece's gradient before the activation.
 template <int T, int W, int E, bool WHOLE>
 __device__ __forceinline__ void piece_grad(int act, const Piece<T, W> &x, const Piece<T, W> &g, const Affine<E, WHOLE> &f,
                                            float (&dz)[E]) {
+#pragma clang fp contract(off)
 #pragma unroll
     for (int e = 0; e < E; ++e) dz[e] = f(x[e], e);
     slopes(dz, act);
@@ -658,7 +667,7 @@ __device__ __forceinline__ void weigh_sums(const float *weight, const float (&su
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int e = 0; e < E; ++e) v[j][WHOLE ? 0 : e] += sum[j][e] * w[e];
+        for (int e = 0; e < E; ++e) v[j][WHOLE ? 0 : e] = fmaf(sum[j][e], w[e], v[j][WHOLE ? 0 : e]);
 }
 
 template <int T, int W, bool WHOLE, int THREADS, int R, bool SHARED>
@@ -723,7 +732,7 @@ __global__ __launch_bounds__(THREADS, SHARED ? 3 : 2) void ple_group_backward_ke
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     sum[0][e] += dz[e];
-                    sum[1][e] += dz[e] * f.distance(x[k][e], e);
+                    sum[1][e] = fmaf(dz[e], f.distance(x[k][e], e), sum[1][e]);
                     // (here, and not where the sums are used: the terms would all be held)
                     asm volatile("" : "+v"(sum[0][e]), "+v"(sum[1][e]), "+v"(dz[e]));
                 }
@@ -755,20 +764,21 @@ __global__ __launch_bounds__(THREADS, SHARED ? 3 : 2) void ple_group_backward_ke
                 const Rows other(a, rows.n, m, true);
                 const int64_t away = (other.first - rows.first) * a.C * elem_bytes(T) + at;
                 const int there = p.on ? static_cast<int>(other.count) - p.slot : 0;
-                join_rarely<2, E, WHOLE, THREADS>(a, p, s_lds, [&](int e, float (&t)[2]) {
+                join_rarely<2, E, E, WHOLE, THREADS>(a, p, s_lds, [&](int e, float (&v)[2]) {
+#pragma clang fp contract(off)
                     const float2 st = stats[groups.of(e)];
                     const float w = own_params[e], scale = w * st.y, bias = own_params[a.Cs + e];
-                    t[0] = t[1] = 0.0f;
+                    float t[2] = {};
                     for (int k = 0; k * a.slots < there; ++k) {
                         const float d = load_grad<T>(px + away + k * step, e) - st.x;
-                        float dz[1] = {d * scale + bias};
+                        float dz[1] = {fmaf(d, scale, bias)};
                         slopes(dz, act);
                         dz[0] *= load_grad<T>(pg + away + k * step, e);
                         t[0] += dz[0];
-                        t[1] += dz[0] * d;
+                        t[1] = fmaf(dz[0], d, t[1]);
                     }
-                    t[1] *= st.y * w;
-                    t[0] *= w;
+                    v[0] = fmaf(t[0], w, v[0]);
+                    v[1] = fmaf(t[1] * st.y, w, v[1]);
                 }, [&](int q, const float (&r)[2]) { s_known[m * a.Gs + q] = make_float2(r[0], r[1]); });
             });
             const int lane = p.thread & (a.team - 1);
@@ -1024,7 +1034,7 @@ __global__ __launch_bounds__(kBlock) void ple_group_apply_kernel(GroupArgs a) {
             if (p.row + k * a.slots < a.S) {
                 float z[E];
 #pragma unroll
-                for (int e = 0; e < E; ++e) z[e] = (x[k][e] - mean[e]) * scale[e] + ch.b[e];
+                for (int e = 0; e < E; ++e) z[e] = fmaf(x[k][e] - mean[e], scale[e], ch.b[e]);
                 activate(z, a.act);
                 store_piece<T, W>(a.y, (p.n * a.S + p.row + k * a.slots) * a.C + p.c0, z);
             }
@@ -1061,7 +1071,7 @@ __global__ __launch_bounds__(kBlock) void ple_group_backward_sums_kernel(GroupAr
                     for (int e = 0; e < E; ++e) {
                         const float d = x[k][e] - st[e].x;
                         xh[e] = d * st[e].y;
-                        dz[e] = d * (st[e].y * ch.w[e]) + ch.b[e];       // (as the forward)
+                        dz[e] = fmaf(d, st[e].y * ch.w[e], ch.b[e]);     // (as the forward)
                     }
                     slopes(dz, a.act);
 #pragma unroll
@@ -1149,7 +1159,7 @@ __global__ __launch_bounds__(kBlock) void ple_group_backward_apply_kernel(GroupA
                 for (int e = 0; e < E; ++e) {
                     const float d = x[k][e] - st[e].x;
                     xh[e] = d * st[e].y;
-                    dz[e] = d * (st[e].y * ch.w[e]) + ch.b[e];
+                    dz[e] = fmaf(d, st[e].y * ch.w[e], ch.b[e]);
                 }
                 slopes(dz, a.act);
 #pragma unroll

@@ -417,3 +417,22 @@ def test_sums_are_about_the_mean(ops, n, s, c, groups):
     for name, a, b, e in zip(("dx", "dw", "db"), got, want, err):
         off = (a.cpu().double() - b).abs() / (E * e + TINY[F32])
         assert bool((off <= 1).all()), (name, float(off.max()))
+
+
+@pytest.mark.parametrize("act", [NONE, RELU, SILU, GELU], ids=["none", "relu", "silu", "gelu"])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=lambda t: str(t)[6:])
+@pytest.mark.parametrize("n,s,c,groups", [(2, 4096, 40, 4), (3, 9001, 64, 8), (1, 3001, 250, 10), (2, 2100, 77, 7), (1, 5000, 64, 64),
+                                          (2, 20_011, 256, 32)])
+def test_members_compute_the_same_for_each_other(ops, tune, n, s, c, groups, dtype, act):
+    """What a member computes in another's place has the bits that the other publishes, so a
+    call's results do not depend on who ran when."""
+    from piecewiselinearembeddings_optimized_amd import capi
+
+    assert capi.group_norm_plan(n, s, c, groups, dtype)["form"] == 1
+    x = _inputs(n, s, c, dtype, F32, level=3.0)
+    want, stats = _run(ops, x, groups, act)
+    for polls in (1, 2):
+        tune("GROUP_POLLS", polls)
+        got, again = _run(ops, x, groups, act)
+        for name, a, b in zip(("stats", "y", "dx", "dw", "db"), (again, *got), (stats, *want)):
+            assert torch.equal(a, b), (polls, name, float((a.double() - b.double()).abs().max()))
