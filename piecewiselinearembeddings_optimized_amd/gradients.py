@@ -90,11 +90,12 @@ def clip_gradients_(grads: Sequence[Tensor], max_norm: float, norm_type: float =
 
 
 def clip_grad_norm_(parameters: Tensor | Iterable[Tensor], max_norm: float, norm_type: float = 2.0,
-                    error_if_nonfinite: bool = False) -> Tensor:
+                    error_if_nonfinite: bool = False, foreach: bool | None = None) -> Tensor:
     """:func:`clip_gradients_` of the parameters' gradients, with the arguments of
-    ``torch.nn.utils.clip_grad_norm_``.  A parameter that is given twice counts
-    once.  ``error_if_nonfinite`` waits for the norm and raises where it is not
-    finite, before anything is scaled."""
+    ``torch.nn.utils.clip_grad_norm_`` (``norm_type`` 1, 2 or infinity).  A parameter
+    that is given twice counts once.  ``error_if_nonfinite`` waits for the norm and
+    raises where it is not finite, before anything is scaled.  ``foreach`` changes
+    nothing: a device takes all gradients together in any case."""
     parameters = [parameters] if isinstance(parameters, Tensor) else list(parameters)
     grads = list({id(p): p.grad for p in parameters if p.grad is not None}.values())
     norm = None

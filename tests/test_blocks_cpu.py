@@ -380,3 +380,17 @@ def test_relative_bias_compiles_with_symbolic_tables():
             (grad,) = torch.autograd.grad(compiled(weight, _meta(2 * r + 1, dtype=torch.int32), _meta(q, k)), weight)
         assert grad.shape == (r, h)
     torch._dynamo.reset()
+
+
+def test_clip_grad_norm_takes_the_arguments_of_torch():
+    """Called as torch's, with every argument by name and in its place."""
+    import inspect
+
+    theirs = list(inspect.signature(torch.nn.utils.clip_grad_norm_).parameters)
+    assert list(inspect.signature(pkg.clip_grad_norm_).parameters)[:len(theirs)] == theirs
+    p = torch.nn.Parameter(torch.ones(4))
+    for foreach in (None, True, False):
+        p.grad = torch.full((4,), 3.0)
+        assert float(pkg.clip_grad_norm_([p], 1.5, 2.0, False, foreach)) == 6.0
+        torch.testing.assert_close(p.grad, torch.full((4,), 0.75))
+        assert float(pkg.clip_grad_norm_(p, max_norm=9.0, norm_type=2.0, error_if_nonfinite=True, foreach=foreach)) == pytest.approx(1.5)
