@@ -31,9 +31,11 @@ _ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3}
 
 def _group_norm_cpu(x: Tensor, weight: Tensor | None, bias: Tensor | None, groups: int, activation: str | None,
                     eps: float) -> Tensor:
-    z = _wide(x).reshape(x.shape[0], -1, groups, x.shape[-1] // groups)
-    z = z - z.mean((1, 3), keepdim=True)
-    z = (z * torch.rsqrt(z.square().mean((1, 3), keepdim=True) + eps)).reshape(x.shape)
+    z = _wide(x)
+    if x.numel() > 0:
+        z = z.reshape(x.shape[0], -1, groups, x.shape[-1] // groups)
+        z = z - z.mean((1, 3), keepdim=True)
+        z = (z * torch.rsqrt(z.square().mean((1, 3), keepdim=True) + eps)).reshape(x.shape)
     if weight is not None:
         z = z * _wide(weight)
     if bias is not None:
@@ -77,8 +79,6 @@ class CudaGroupNorm(nn.Module):
         if x.ndim < 2 or x.shape[-1] != self.num_channels:
             raise ValueError(f"Expected [N, ..., {self.num_channels}], got shape {tuple(x.shape)}")
         if x.device.type != "cuda":
-            if x.numel() == 0:
-                return x * 1.0
             return _group_norm_cpu(x, self.weight, self.bias, self.num_groups, self.activation, self.eps)
         return _ops.group_norm(x.contiguous(), self.weight, self.bias, self.num_groups, _ACTIVATIONS[self.activation],
                                self.eps)[0]

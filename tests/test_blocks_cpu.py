@@ -394,3 +394,17 @@ def test_clip_grad_norm_takes_the_arguments_of_torch():
         assert float(pkg.clip_grad_norm_([p], 1.5, 2.0, False, foreach)) == 6.0
         torch.testing.assert_close(p.grad, torch.full((4,), 0.75))
         assert float(pkg.clip_grad_norm_(p, max_norm=9.0, norm_type=2.0, error_if_nonfinite=True, foreach=foreach)) == pytest.approx(1.5)
+
+
+@pytest.mark.parametrize("shape", [(0, 5, 12), (2, 0, 12), (0, 12)])
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=lambda t: str(t)[6:])
+def test_module_group_norm_without_rows_on_cpu(shape, dtype):
+    """As on a device: parameters have gradients, of zeros."""
+    m = pkg.CudaGroupNorm(3, 12, activation="silu")
+    x = torch.empty(shape, dtype=dtype, requires_grad=True)
+    y = m(x)
+    assert y.shape == shape and y.dtype == dtype
+    y.sum().backward()
+    assert x.grad.shape == shape
+    assert torch.equal(m.weight.grad, torch.zeros(12)) and torch.equal(m.bias.grad, torch.zeros(12))
+    assert pkg.CudaGroupNorm(3, 12, affine=False)(x).shape == shape
