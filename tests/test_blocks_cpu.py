@@ -408,3 +408,13 @@ def test_module_group_norm_without_rows_on_cpu(shape, dtype):
     assert x.grad.shape == shape
     assert torch.equal(m.weight.grad, torch.zeros(12)) and torch.equal(m.bias.grad, torch.zeros(12))
     assert pkg.CudaGroupNorm(3, 12, affine=False)(x).shape == shape
+
+
+def test_relative_bias_of_far_positions_on_cpu():
+    """Positions beyond 2^60 count as 2^60, at either end of what 64 bits hold."""
+    m = pkg.CudaRelativeBias(8, 2, max_distance=20, causal=True)
+    starts = torch.tensor([2 ** 63 - 1, 2 ** 60, -2 ** 63, -2 ** 60])
+    out = m(2, 3, starts=starts)
+    past = m.weight[m.buckets[0].long()]
+    assert torch.equal(out[:2], past[:, None, None].expand(2, 2, 2, 3))
+    assert bool(torch.isneginf(out[2:]).all())
