@@ -124,7 +124,7 @@ def relative_buckets(num_buckets: int, max_distance: int, bidirectional: bool = 
 def _relative_bias_cpu(weight: Tensor, buckets: Tensor, starts: Tensor | None, q_len: int, k_len: int, offset: int,
                        causal: bool, dtype: torch.dtype) -> Tensor:
     far = buckets.shape[0] // 2
-    first = torch.tensor([offset]) if starts is None else starts.clamp(-2 ** 60, 2 ** 60)    # (so that no difference overflows)
+    first = torch.tensor([offset]) if starts is None else starts.long().clamp(-2 ** 60, 2 ** 60)    # (so that no difference overflows)
     d = torch.arange(k_len) - (first[:, None, None] + torch.arange(q_len)[:, None])          # [B, q, k]
     row = buckets[d.clamp(-far, far) + far].long()
     none, beyond = row < 0, row >= weight.shape[0]

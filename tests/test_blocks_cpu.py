@@ -418,3 +418,9 @@ def test_relative_bias_of_far_positions_on_cpu():
     past = m.weight[m.buckets[0].long()]
     assert torch.equal(out[:2], past[:, None, None].expand(2, 2, 2, 3))
     assert bool(torch.isneginf(out[2:]).all())
+
+
+def test_relative_bias_starts_of_32_bits_on_cpu():
+    m = pkg.CudaRelativeBias(8, 2, max_distance=20)
+    starts = torch.tensor([5, 0, 90])
+    assert torch.equal(m(4, 9, starts=starts.int()), m(4, 9, starts=starts))
