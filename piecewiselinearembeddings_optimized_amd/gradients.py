@@ -80,6 +80,12 @@ def clip_gradients_(grads: Sequence[Tensor], max_norm: float, norm_type: float =
     out = grads if out is None else list(out)
     if len(out) != len(grads):
         raise ValueError("out must have a tensor for every gradient")
+    if any(o.shape != g.shape for g, o in zip(grads, out)):
+        raise ValueError("out must have the shape of its gradient")
+    # (of those that overlap in part, a device finds all)
+    begins = [o.data_ptr() for o in out if o.numel() > 0]
+    if len(set(begins)) < len(begins):
+        raise ValueError("gradients that are scaled must not share memory with each other or with out")
     norm = _norm_cpu(grads, norm_type) if norm is None else norm.reshape(()).clone()
     factor = torch.ones(()) if max_norm == float("inf") else (max_norm / (norm.double() + 1e-6)).clamp_max(1.0).float()
     for g, o in zip(grads, out):

@@ -424,3 +424,19 @@ def test_relative_bias_starts_of_32_bits_on_cpu():
     m = pkg.CudaRelativeBias(8, 2, max_distance=20)
     starts = torch.tensor([5, 0, 90])
     assert torch.equal(m(4, 9, starts=starts.int()), m(4, 9, starts=starts))
+
+
+@pytest.mark.parametrize("call,match", [
+    (lambda g: pkg.clip_gradients_(g, 0.5, out=[torch.zeros(3, 4), torch.zeros(5)]), "shape"),
+    (lambda g: pkg.clip_gradients_(g, 0.5, out=[torch.zeros(2, 3, 4), torch.zeros(4)]), "shape"),
+    (lambda g: pkg.clip_gradients_(g, 0.5, out=[torch.zeros(1), torch.zeros(4)]), "shape"),
+    (lambda g: pkg.clip_gradients_([*g, g[0]], 0.5), "share memory"),
+    (lambda g: pkg.clip_gradients_([*g, g[0][:, :2]], 0.5), "share memory"),
+    (lambda g: pkg.clip_gradients_([g[1], g[1].clone()], 0.5, out=[g[0][0], g[0][0]]), "share memory"),
+])
+def test_clipping_refusals_on_cpu(call, match):
+    """As on a device; nothing is scaled."""
+    grads = [torch.ones(3, 4), torch.ones(4)]
+    with pytest.raises(ValueError, match=match):
+        call(grads)
+    assert all(bool((g == 1).all()) for g in grads)
