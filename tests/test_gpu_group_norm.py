@@ -436,3 +436,33 @@ def test_members_compute_the_same_for_each_other(ops, tune, n, s, c, groups, dty
         got, again = _run(ops, x, groups, act)
         for name, a, b in zip(("stats", "y", "dx", "dw", "db"), (again, *got), (stats, *want)):
             assert torch.equal(a, b), (polls, name, float((a.double() - b.double()).abs().max()))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=lambda t: str(t)[6:])
+@pytest.mark.parametrize("shift", [0, 1, 2, 3, 8])
+@pytest.mark.parametrize("n,s,c,groups", [(7, 20, 32, 4), (5, 3, 7, 7), (2, 9000, 32, 4), (3, 3001, 77, 7), (1, 300, 1000, 10), (2, 3, 9001, 1)])
+def test_nothing_beside_the_results_is_written(n, s, c, groups, shift, dtype):
+    """Results at any element of a buffer (held, shared and split): what lies before and
+    behind each stays, and the values are right."""
+    from piecewiselinearembeddings_optimized_amd import capi
+
+    x, mark, edge = _inputs(n, s, c, dtype, dtype), 7.0, 64
+
+    def placed(shape, kind, at=shift, fill=None):
+        size = math.prod(shape)
+        buf = torch.full((edge + size + edge,), mark, dtype=kind, device=DEV)
+        t = buf[edge + at:edge + at + size].view(shape)
+        if fill is not None:
+            t.copy_(fill)
+        return buf, t, at
+
+    inputs = {k: placed(v.shape, dtype, fill=v)[1] for k, v in x.items()}
+    y, gx = placed((n, s, c), dtype), placed((n, s, c), dtype)
+    gw, gb, stats = placed((c,), dtype), placed((c,), dtype), placed((n, groups, 2), F32, shift // 2 * 2)
+    capi.group_norm(inputs["x"], inputs["weight"], inputs["bias"], y[1], stats[1], groups, SILU, EPS)
+    capi.group_norm_backward(inputs["g"], inputs["x"], stats[1], inputs["weight"], inputs["bias"], gx[1], gw[1], gb[1], groups, SILU)
+    for buf, t, at in (y, gx, gw, gb, stats):
+        assert bool((buf[:edge + at] == mark).all()) and bool((buf[edge + at + t.numel():] == mark).all())
+    ref, err = _reference(x, groups, SILU)
+    for (_, a, _), r, e in zip((y, gx, gw, gb), ref, err):
+        assert bool(((a.cpu().double() - r).abs() <= e + UNIT[dtype] * (r.abs() + e) + TINY[dtype]).all())
