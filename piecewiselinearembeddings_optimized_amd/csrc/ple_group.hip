@@ -635,17 +635,33 @@ struct Affine {
             mean[WHOLE ? 0 : e] = st.x;
         }
     }
-    __device__ __forceinline__ float distance(float x, int e) const { return x - mean[WHOLE ? 0 : e]; }
-    __device__ __forceinline__ float operator()(float x, int e) const { return fmaf(distance(x, e), scale[e], bias[e]); }
 };
 
-// A piece's gradient before the activation.
+// x - mean of a piece.  Pieces of 32-bit values hold it in the place of x (centre), which
+// saves the registers of the means.
 template <int T, int W, int E, bool WHOLE>
-__device__ __forceinline__ void piece_grad(int act, const Piece<T, W> &x, const Piece<T, W> &g, const Affine<E, WHOLE> &f,
+__device__ __forceinline__ void centre(Piece<T, W> &x, const Affine<E, WHOLE> &f) {
+    if constexpr (T == PLE_DTYPE_F32)
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            x.w[e] = __float_as_uint(x[e] - f.mean[WHOLE ? 0 : e]);
+            asm volatile("" : "+v"(x.w[e]));         // (here, and not where it is used)
+        }
+}
+
+template <int T, int W, int E, bool WHOLE>
+__device__ __forceinline__ void distances(const Piece<T, W> &x, const Affine<E, WHOLE> &f, float (&d)[E]) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) d[e] = T == PLE_DTYPE_F32 ? x[e] : x[e] - f.mean[WHOLE ? 0 : e];
+}
+
+// A piece's gradient before the activation, from its distances.
+template <int T, int W, int E, bool WHOLE>
+__device__ __forceinline__ void piece_grad(int act, const float (&d)[E], const Piece<T, W> &g, const Affine<E, WHOLE> &f,
                                            float (&dz)[E]) {
 #pragma clang fp contract(off)
 #pragma unroll
-    for (int e = 0; e < E; ++e) dz[e] = f(x[e], e);
+    for (int e = 0; e < E; ++e) dz[e] = fmaf(d[e], f.scale[e], f.bias[e]);
     slopes(dz, act);
 #pragma unroll
     for (int e = 0; e < E; ++e) dz[e] *= g[e];
@@ -670,8 +686,14 @@ __device__ __forceinline__ void weigh_sums(const float *weight, const float (&su
         for (int e = 0; e < E; ++e) v[j][WHOLE ? 0 : e] = fmaf(sum[j][e], w[e], v[j][WHOLE ? 0 : e]);
 }
 
+// Waves a SIMD that the backward is compiled for (its largest 32-bit pieces just fit four:
+// 8192 x 64 x 96 in groups of 3 119 us, with three 131).
+constexpr int backward_waves(int type, int words, bool shared) {
+    return shared ? 3 : type == PLE_DTYPE_F32 && words == 4 ? 4 : 2;
+}
+
 template <int T, int W, bool WHOLE, int THREADS, int R, bool SHARED>
-__global__ __launch_bounds__(THREADS, SHARED ? 3 : 2) void ple_group_backward_kernel(GroupArgs a) {
+__global__ __launch_bounds__(THREADS, backward_waves(T, W, SHARED)) void ple_group_backward_kernel(GroupArgs a) {
     constexpr int E = Piece<T, W>::kElems, kEach = WHOLE ? 1 : E, kValues = 2 * kEach > E ? 2 * kEach : E;
     extern __shared__ float4 s_all[];
     float *const s_lds = reinterpret_cast<float *>(s_all);
@@ -722,17 +744,21 @@ __global__ __launch_bounds__(THREADS, SHARED ? 3 : 2) void ple_group_backward_ke
         {
             const Affine<E, WHOLE> f(own_params, own_params + a.Cs, stats, groups);
 #pragma unroll
+            for (int k = 0; k < R; ++k) centre(x[k], f);
+#pragma unroll
             for (int k = 0; k < R; ++k) {
                 x[k].keep();
                 g[k].keep();
                 __builtin_amdgcn_sched_barrier(0);
                 // (a row that is not there has a gradient of 0)
+                float d[E];
                 float (&dz)[E] = grad[kKept ? k : 0];
-                piece_grad<T, W>(act, x[k], g[k], f, dz);
+                distances(x[k], f, d);
+                piece_grad<T, W>(act, d, g[k], f, dz);
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     sum[0][e] += dz[e];
-                    sum[1][e] = fmaf(dz[e], f.distance(x[k][e], e), sum[1][e]);
+                    sum[1][e] = fmaf(dz[e], d[e], sum[1][e]);
                     // (here, and not where the sums are used: the terms would all be held)
                     asm volatile("" : "+v"(sum[0][e]), "+v"(sum[1][e]), "+v"(dz[e]));
                 }
@@ -814,11 +840,13 @@ __global__ __launch_bounds__(THREADS, SHARED ? 3 : 2) void ple_group_backward_ke
             x[k].keep();
             if constexpr (!kKept) g[k].keep();
             __builtin_amdgcn_sched_barrier(0);
+            float d[E];
             float (&dz)[E] = grad[kKept ? k : 0];
-            if constexpr (!kKept) piece_grad<T, W>(act, x[k], g[k], f, dz);
+            distances(x[k], f, d);
+            if constexpr (!kKept) piece_grad<T, W>(act, d, g[k], f, dz);
 #pragma unroll
             for (int e = 0; e < E; ++e)
-                dz[e] = dz[e] * f.scale[e] + (f.distance(x[k][e], e) * along[WHOLE ? 0 : e] + level[WHOLE ? 0 : e]);
+                dz[e] = dz[e] * f.scale[e] + (d[e] * along[WHOLE ? 0 : e] + level[WHOLE ? 0 : e]);
             if (has(k)) store_piece<T, W>(py + k * step + at, 0, dz);
         }
         if constexpr (SHARED) break;
