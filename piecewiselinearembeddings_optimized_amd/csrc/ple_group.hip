@@ -26,10 +26,10 @@
 // squares about the piece's own mean), a join per group, and a second read that
 // applies it.
 //
-// Measured, forward / backward: held, 16384 x 64 x 64 fp32 97 / 157 us (5.5 / 5.1 TB/s);
-// shared, 8 x 65536 x 256 bf16 139 / 233 us (3.9 / 3.4 TB/s: three workgroups a CU load,
-// wait for each other and store in step) and 16 x 4096 x 320 28 / 50 us; split, 1 x
-// 60000 x 960 backward 157 us (2.2 TB/s: x and the gradient are read twice).
+// Measured, forward / backward: held, 16384 x 64 x 64 fp32 100 / 155 us (5.4 / 5.2 TB/s);
+// shared, 8 x 65536 x 256 bf16 140 / 241 us (3.8 / 3.3 TB/s: three workgroups a CU load,
+// wait for each other and store in step) and 16 x 4096 x 320 27 / 49 us; split, 1 x
+// 60000 x 960 76 / 154 us (3.0 / 2.3 TB/s: x, and the gradient, are read twice).
 
 #include <algorithm>
 
@@ -736,9 +736,10 @@ __global__ __launch_bounds__(THREADS, backward_waves(T, W, SHARED)) void ple_gro
                 g[k].load_at(pg + k * step + at);
             }
         }
-        // dz is kept until the groups' sums are known (8 x 65536 x 256 bf16 in groups of 8:
-        // 233 us, computed again 277), where three workgroups have the registers for it (16 x
-        // 4096 x 320 in groups of 10: 50 us either way, kept in part in scratch memory)
+        // dz is kept until the groups' sums are known (8 x 65536 x 256 bf16 in groups of 8,
+        // when this was chosen: 233 us, computed again 277), where three workgroups have the
+        // registers for it (16 x 4096 x 320 in groups of 10: 50 us either way, kept in part in
+        // scratch memory)
         constexpr bool kKept = WHOLE || !SHARED || E < 8;
         float sum[2][E] = {}, grad[kKept ? R : 1][E];
         {
