@@ -29,7 +29,7 @@
 // Measured, forward / backward: held, 16384 x 64 x 64 fp32 100 / 155 us (5.4 / 5.2 TB/s);
 // shared, 8 x 65536 x 256 bf16 140 / 241 us (3.8 / 3.3 TB/s: three workgroups a CU load,
 // wait for each other and store in step) and 16 x 4096 x 320 27 / 49 us; split, 1 x
-// 60000 x 960 76 / 154 us (3.0 / 2.3 TB/s: x, and the gradient, are read twice).
+// 200000 x 960 288 / 440 us (2.7 / 2.6 TB/s: x, and the gradient, are read twice).
 
 #include <algorithm>
 
