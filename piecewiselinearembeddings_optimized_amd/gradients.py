@@ -82,8 +82,8 @@ def clip_gradients_(grads: Sequence[Tensor], max_norm: float, norm_type: float =
         raise ValueError("out must have a tensor for every gradient")
     if any(o.shape != g.shape for g, o in zip(grads, out)):
         raise ValueError("out must have the shape of its gradient")
-    # (of those that overlap in part, a device finds all)
-    begins = [o.data_ptr() for o in out if o.numel() > 0]
+    # (of those that overlap in part, a device finds all; in a graph tensors have no addresses yet)
+    begins = [] if torch.compiler.is_compiling() else [o.data_ptr() for o in out if o.numel() > 0 and not o.is_meta]
     if len(set(begins)) < len(begins):
         raise ValueError("gradients that are scaled must not share memory with each other or with out")
     norm = _norm_cpu(grads, norm_type) if norm is None else norm.reshape(()).clone()

@@ -440,3 +440,16 @@ def test_clipping_refusals_on_cpu(call, match):
     with pytest.raises(ValueError, match=match):
         call(grads)
     assert all(bool((g == 1).all()) for g in grads)
+
+
+def test_clipping_into_others_compiles_and_has_shapes():
+    """On the CPU in one graph, and on meta tensors, which have no memory to share."""
+    torch._dynamo.reset()
+    grads = [torch.ones(3, 4), torch.ones(4)]
+    want, got = ([torch.empty_like(g) for g in grads] for _ in range(2))
+    norm = pkg.clip_gradients_(grads, 0.5, out=want)
+    compiled = torch.compile(lambda g, o: pkg.clip_gradients_(g, 0.5, out=o), backend="eager", fullgraph=True)
+    assert torch.equal(compiled(grads, got), norm) and all(map(torch.equal, got, want))
+    torch._dynamo.reset()
+    metas = [_meta(3, 4), _meta(4)]
+    assert pkg.clip_gradients_(metas, 0.5, out=[_meta(3, 4), _meta(4)]).shape == ()
